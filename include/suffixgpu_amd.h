@@ -32,7 +32,7 @@ extern "C" {
 
 #define SFX_EINVAL (-1)
 #define SFX_MAX_CANDIDATES 32
-#define SFX_ABI_VERSION 15
+#define SFX_ABI_VERSION 16
 
 /* Drafter configuration shared by the local and global paths.
  * Mirrors the constructor arguments of SuffixGPUDrafter
@@ -504,6 +504,126 @@ int sfx_ingest_active(void* state, const int32_t* corpus, int64_t capacity,
 /* The staged build is live (after sfx_index_swap): the rebuild is no
  * longer running. */
 int sfx_ingest_swapped(void* state, hipStream_t stream);
+
+/* ---- the target model's side of a step (no reference counterpart) ------ */
+
+/* Element types of the operators below. */
+#define SFX_BF16 0
+#define SFX_F16 1
+#define SFX_F32 2
+
+/* A paged key/value cache held in 4 bits.  pages: [num_pages, heads,
+ * page_size / 32] blocks of 32 tokens of one KV head, 16-byte aligned, each
+ * sfx_kv4_block_bytes(head_dim) bytes, D = head_dim:
+ *   32 x D/2 bytes   keys, token by token; channel 2i in the low half of
+ *                    byte i
+ *   32 x D/32 bytes  key scales 2^(byte - 127), one per 32 channels
+ *   D/64 x 64 x 16   values: the 32-bit word [c / 64][2 s + h][c % 16]
+ *                    [c / 16 % 4] holds in its j-th 4 bits channel c of
+ *                    token 16 s + 8 (j / 4) + 4 h + j % 4 of the block
+ *   32 x 4 bytes     value scales (float), one per token
+ * Four bits are a sign and one of 0, .5, 1, 1.5, 2, 3, 4, 6.  A byte of 255
+ * as a key scale makes its 32 channels NaN.
+ * table: [rows, table_width] page ids with a row stride (elements); position
+ * p of row b lies in page table[b][p / page_size].  Ids outside
+ * [0, num_pages) and positions past the table hold nothing: nothing is
+ * written there and no query sees them. */
+typedef struct sfx_kv4 {
+    void* pages;
+    int64_t num_pages;
+    int64_t heads;        /* KV heads                                     */
+    int64_t head_dim;     /* 64, 128 or 256                               */
+    int64_t page_size;    /* a power of two, 32 .. 65536                  */
+    int32_t dtype;        /* SFX_BF16 or SFX_F16: of keys, values, queries */
+    const int32_t* table;
+    int64_t table_width;
+    int64_t table_stride;
+} sfx_kv4;
+
+/* Rows of new keys, values or queries: element strides of batch row, token
+ * and head; the head_dim channels of a head are contiguous. */
+typedef struct sfx_heads {
+    const void* data;
+    int64_t stride_b, stride_t, stride_h;
+} sfx_heads;
+
+int64_t sfx_kv4_block_bytes(int64_t head_dim);
+
+/* Writes tokens 0 .. min(count[b], tokens) of row b of k and v (heads KV
+ * heads each) at positions start[b], start[b] + 1, ...  Keys: per group of 32
+ * channels the power of two 2^e that puts the largest magnitude in (3.5, 7]
+ * (-126 <= e <= 125; at most 13 in an SFX_F16 cache, whose values end below
+ * 2^16); values: per token and head a sixth of the largest magnitude, at
+ * least 2^-100.  Both round to the nearest, ties to the even code.  An
+ * infinity or NaN makes its group of keys, or its token's values, NaN.
+ * count == NULL: all `tokens`.  Rows of one call must not share pages that
+ * they write. */
+int sfx_kv4_append(const sfx_kv4* cache, const sfx_heads* k,
+                   const sfx_heads* v, int64_t batch, int64_t tokens,
+                   const void* start, int32_t start_is64, const void* count,
+                   int32_t count_is64, hipStream_t stream);
+
+/* k_out, v_out [batch, tokens, heads, head_dim] in the cache's type: what the
+ * cache holds at positions start[b] + i for i < count[b], zeros elsewhere. */
+int sfx_kv4_read(const sfx_kv4* cache, int64_t batch, int64_t tokens,
+                 const void* start, int32_t start_is64, const void* count,
+                 int32_t count_is64, void* k_out, void* v_out,
+                 hipStream_t stream);
+
+/* Attention of the newest tokens over the cache.  Row b holds kv_len[b]
+ * tokens, the last q_len[b] of which (q_len == NULL: `tokens`) are q's tokens
+ * 0 .. q_len[b] - 1; query i sees the positions up to its own,
+ * kv_len - q_len + i.  out [batch, tokens, q_heads, head_dim], contiguous, in
+ * the cache's type: softmax(scale q k) v over what it sees, zeros for a query
+ * that sees nothing and for tokens from q_len on.  Query head g uses KV head
+ * g / (q_heads / heads).  workspace: sfx_kv4_attend_workspace_size bytes,
+ * 16-byte aligned, of any content. */
+size_t sfx_kv4_attend_workspace_size(const sfx_kv4* cache, int64_t batch,
+                                     int64_t tokens, int64_t q_heads);
+int sfx_kv4_attend(const sfx_kv4* cache, const sfx_heads* q, int64_t batch,
+                   int64_t tokens, int64_t q_heads, const void* kv_len,
+                   int32_t kv_len_is64, const void* q_len,
+                   int32_t q_len_is64, float scale, void* out,
+                   void* workspace, size_t workspace_bytes,
+                   hipStream_t stream);
+
+/* Verification of drafted tokens.  logits [batch, K + 1, vocab] with element
+ * strides of row and position: position j holds the target's logits for the
+ * token after j drafted ones.  p_j = softmax(logits / temperature); a NaN
+ * counts as -inf, equal +inf share.  Temperature 0 (or below, or NaN): p_j is
+ * one at the first of the largest logits.  temperature == NULL: 1.
+ * Draft j < min(num_valid[b], K) (and before the first id outside
+ * [0, vocab)) is accepted iff uniform[b][j] q(draft) < p_j(draft), q =
+ * draft_probs[b][j] or, with draft_probs == NULL, one at the draft.  At the
+ * first draft not accepted a token is drawn from max(p_j - q, 0) (from p_j
+ * where that is empty), after num_valid accepted ones from p_j: the one with
+ * the largest probability / noise[b][token], the lowest on ties; noise is
+ * exponentially distributed, every value > 0.  A position without any logit
+ * above -inf accepts and draws nothing.
+ * sampled [batch, K + 1]: the accepted drafts, the drawn token, -1 after
+ * them; count [batch] their number.  uniform [batch, K] and noise
+ * [batch, vocab] may be NULL only with all_greedy != 0, which takes every
+ * row's temperature as 0.  workspace: sfx_verify_workspace_size bytes,
+ * 16-byte aligned, of any content. */
+typedef struct sfx_verify {
+    const void* logits;
+    int32_t dtype;             /* SFX_BF16, SFX_F16 or SFX_F32            */
+    int32_t all_greedy;
+    int64_t batch, k, vocab;
+    int64_t stride_b, stride_j;
+    const int32_t* draft;      /* [batch, K]                              */
+    const int32_t* num_valid;  /* [batch]                                 */
+    const float* uniform;      /* [batch, K]                              */
+    const float* noise;        /* [batch, vocab]                          */
+    const float* temperature;  /* [batch] or NULL                         */
+    const float* draft_probs;  /* [batch, K, vocab] or NULL               */
+    int32_t* sampled;          /* [batch, K + 1]                          */
+    int32_t* count;            /* [batch]                                 */
+} sfx_verify;
+
+size_t sfx_verify_workspace_size(int64_t batch, int64_t k, int64_t vocab);
+int sfx_verify_draft(const sfx_verify* args, void* workspace,
+                     size_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -18,7 +18,7 @@ import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libsuffixgpu_amd.so"
 MAX_CANDIDATES = 32
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 c_i32 = ctypes.c_int32
 c_i64 = ctypes.c_int64
@@ -70,7 +70,33 @@ class SfxAppendDoc(ctypes.Structure):
     _fields_ = [("src", c_p), ("n", c_i64), ("dst", c_i64)]
 
 
+class SfxKv4(ctypes.Structure):
+    _fields_ = [
+        ("pages", c_p), ("num_pages", c_i64), ("heads", c_i64),
+        ("head_dim", c_i64), ("page_size", c_i64), ("dtype", c_i32),
+        ("table", c_p), ("table_width", c_i64), ("table_stride", c_i64),
+    ]
+
+
+class SfxHeads(ctypes.Structure):
+    _fields_ = [("data", c_p), ("stride_b", c_i64), ("stride_t", c_i64),
+                ("stride_h", c_i64)]
+
+
+class SfxVerify(ctypes.Structure):
+    _fields_ = [
+        ("logits", c_p), ("dtype", c_i32), ("all_greedy", c_i32),
+        ("batch", c_i64), ("k", c_i64), ("vocab", c_i64),
+        ("stride_b", c_i64), ("stride_j", c_i64),
+        ("draft", c_p), ("num_valid", c_p), ("uniform", c_p), ("noise", c_p),
+        ("temperature", c_p), ("draft_probs", c_p),
+        ("sampled", c_p), ("count", c_p),
+    ]
+
+
 APPEND_MAX_DOCS = 64
+# element types of the target-side operators
+DTYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -148,6 +174,23 @@ SIGNATURES = {
                                       ctypes.c_size_t, c_p]),
     "sfx_sa_build": (c_i32, [c_p, c_i64, c_i64, c_p, c_i32, c_p,
                              ctypes.c_size_t, c_p]),
+    "sfx_kv4_block_bytes": (c_i64, [c_i64]),
+    "sfx_kv4_append": (c_i32, [ctypes.POINTER(SfxKv4),
+                               ctypes.POINTER(SfxHeads),
+                               ctypes.POINTER(SfxHeads), c_i64, c_i64, c_p,
+                               c_i32, c_p, c_i32, c_p]),
+    "sfx_kv4_read": (c_i32, [ctypes.POINTER(SfxKv4), c_i64, c_i64, c_p,
+                             c_i32, c_p, c_i32, c_p, c_p, c_p]),
+    "sfx_kv4_attend_workspace_size": (ctypes.c_size_t,
+                                      [ctypes.POINTER(SfxKv4), c_i64, c_i64,
+                                       c_i64]),
+    "sfx_kv4_attend": (c_i32, [ctypes.POINTER(SfxKv4),
+                               ctypes.POINTER(SfxHeads), c_i64, c_i64, c_i64,
+                               c_p, c_i32, c_p, c_i32, ctypes.c_float, c_p,
+                               c_p, ctypes.c_size_t, c_p]),
+    "sfx_verify_workspace_size": (ctypes.c_size_t, [c_i64, c_i64, c_i64]),
+    "sfx_verify_draft": (c_i32, [ctypes.POINTER(SfxVerify), c_p,
+                                 ctypes.c_size_t, c_p]),
 }
 
 _lib = None

@@ -1,0 +1,197 @@
+"""KV4Cache: a paged key/value cache held in 4 bits, and attention over it.
+
+What the target model of a speculative step keeps per request, at 27% of the
+size of 16-bit types (136 bytes a token and KV head of width 128, not 512): keys
+as e2m1 with a power-of-two scale per 32 channels, values as e2m1 with a float32
+scale per token.  ``append`` writes the newest tokens'
+keys and values, drafts among them; ``attend`` is the attention of those tokens'
+queries, each over everything up to itself; a rejected draft's entries are
+simply overwritten by the next ``append``.  No counterpart in the reference.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from suffixgpu_amd import _lib
+from suffixgpu_amd._lib import (SuffixGPUError, check, count_arg, lib, ptr,
+                                require_gpu, stream_of)
+
+BLOCK = 32  # tokens
+
+
+def block_bytes(head_dim: int) -> int:
+    """Bytes of 32 tokens of one KV head: 32 (D + D/32 + 4)."""
+    return BLOCK * (head_dim + head_dim // 32 + 4)
+
+
+class KV4Cache:
+    """``num_pages`` pages of ``page_size`` tokens (a power of two, 32 to
+    65536) for ``num_kv_heads`` heads of width ``head_dim`` (64, 128 or 256),
+    for keys, values and queries of type ``dtype`` (bfloat16 or float16).
+
+    ``pages`` [num_pages, num_kv_heads, page_size / 32, block_bytes] uint8 is
+    the pool (its layout is in include/suffixgpu_amd.h); an existing one may be
+    passed.  Which pages a request holds is the caller's: every call takes
+    ``page_table`` [B, W] int32, position p of row b lying in page
+    ``page_table[b, p // page_size]``.  Page ids outside [0, num_pages) hold
+    nothing: nothing is written there and no query sees them.
+    """
+
+    def __init__(self, num_pages: int, num_kv_heads: int, head_dim: int,
+                 page_size: int = 64, dtype: torch.dtype = torch.bfloat16,
+                 device: torch.device | str = "cuda",
+                 pages: torch.Tensor | None = None):
+        if head_dim not in (64, 128, 256):
+            raise ValueError("head_dim must be 64, 128 or 256")
+        if not 32 <= page_size <= 65536 or page_size & (page_size - 1):
+            raise ValueError("page_size must be a power of two in 32..65536")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("dtype must be bfloat16 or float16")
+        if num_pages < 0 or not 1 <= num_kv_heads <= 65535:
+            raise ValueError("num_pages >= 0 and 1..65535 KV heads")
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise SuffixGPUError("KV4Cache needs a ROCm GPU device; there is "
+                                 "no CPU path")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.num_pages = int(num_pages)
+        self.num_kv_heads = int(num_kv_heads)
+        self.head_dim = int(head_dim)
+        self.page_size = int(page_size)
+        self.dtype = dtype
+        shape = (self.num_pages, self.num_kv_heads, self.page_size // BLOCK,
+                 block_bytes(self.head_dim))
+        if pages is None:
+            pages = torch.zeros(shape, dtype=torch.uint8, device=self.device)
+        elif (pages.shape != shape or pages.dtype != torch.uint8
+              or pages.device != self.device or not pages.is_contiguous()):
+            raise ValueError(f"pages must be a contiguous uint8 {list(shape)} "
+                             f"tensor on {self.device}")
+        elif pages.data_ptr() % 16:
+            raise ValueError("pages must be 16-byte aligned")
+        self.pages = pages
+
+    # ------------------------------------------------------------------
+    def _view(self, page_table: torch.Tensor, rows: int) -> _lib.SfxKv4:
+        if (page_table.dim() != 2 or page_table.dtype != torch.int32
+                or page_table.shape[0] != rows
+                or page_table.device != self.device
+                or (page_table.shape[1] > 1 and page_table.stride(1) != 1)):
+            raise ValueError(f"page_table must be an int32 [{rows}, W] tensor "
+                             f"on {self.device} with contiguous rows")
+        return _lib.SfxKv4(self.pages.data_ptr(), self.num_pages,
+                           self.num_kv_heads, self.head_dim, self.page_size,
+                           _lib.DTYPE_CODES[self.dtype],
+                           page_table.data_ptr(), page_table.shape[1],
+                           page_table.stride(0))
+
+    def _heads(self, name: str, x: torch.Tensor, heads: int | None = None):
+        if (x.dim() != 4 or x.shape[3] != self.head_dim
+                or x.dtype != self.dtype or x.device != self.device
+                or x.stride(3) != 1
+                or (heads is not None and x.shape[2] != heads)):
+            raise ValueError(
+                f"{name} must be a {self.dtype} [B, T, heads, "
+                f"{self.head_dim}] tensor on {self.device}, contiguous along "
+                "the last dimension"
+                + (f", with {heads} heads" if heads is not None else ""))
+        return _lib.SfxHeads(x.data_ptr(), x.stride(0), x.stride(1),
+                             x.stride(2))
+
+    def _counts(self, name: str, t: torch.Tensor | None, rows: int):
+        if t is None:
+            return None, 0
+        if t.dim() != 1 or t.shape[0] != rows or t.device != self.device:
+            raise ValueError(f"{name} must hold {rows} integers on "
+                             f"{self.device}")
+        return count_arg(t)
+
+    def append(self, k: torch.Tensor, v: torch.Tensor,
+               page_table: torch.Tensor, start: torch.Tensor,
+               count: torch.Tensor | None = None) -> None:
+        """Write tokens i < ``count[b]`` (all without it) of ``k`` and ``v``
+        [B, T, num_kv_heads, head_dim] at positions ``start[b] + i``.
+
+        A page that one row of a call writes must not be written by another
+        row of it.  Infinities and NaN make their 32 channels of a key, or
+        their token's values, NaN."""
+        require_gpu(k, v, page_table, start, count)
+        kh = self._heads("k", k, self.num_kv_heads)
+        vh = self._heads("v", v, self.num_kv_heads)
+        if k.shape != v.shape:
+            raise ValueError("k and v differ in shape")
+        b, t = k.shape[:2]
+        view = self._view(page_table, b)
+        st, st64 = self._counts("start", start, b)
+        if st is None:
+            raise ValueError("start is needed")
+        ct, ct64 = self._counts("count", count, b)
+        if b == 0 or t == 0:
+            return
+        check(lib().sfx_kv4_append(view, kh, vh, b, t, st.data_ptr(), st64,
+                                   ptr(ct), ct64, stream_of(self.device)),
+              "KV4Cache.append")
+
+    def read(self, page_table: torch.Tensor, start: torch.Tensor,
+             tokens: int, count: torch.Tensor | None = None):
+        """The keys and values [B, tokens, num_kv_heads, head_dim] that the
+        cache holds at positions ``start[b] + i``, i < ``count[b]``; zeros
+        elsewhere."""
+        require_gpu(page_table, start, count)
+        b = page_table.shape[0]
+        view = self._view(page_table, b)
+        st, st64 = self._counts("start", start, b)
+        if st is None:
+            raise ValueError("start is needed")
+        ct, ct64 = self._counts("count", count, b)
+        shape = (b, int(tokens), self.num_kv_heads, self.head_dim)
+        k = torch.empty(shape, dtype=self.dtype, device=self.device)
+        v = torch.empty(shape, dtype=self.dtype, device=self.device)
+        if k.numel() == 0:
+            return k, v
+        check(lib().sfx_kv4_read(view, b, int(tokens), st.data_ptr(), st64,
+                                 ptr(ct), ct64, k.data_ptr(), v.data_ptr(),
+                                 stream_of(self.device)), "KV4Cache.read")
+        return k, v
+
+    def attend(self, q: torch.Tensor, page_table: torch.Tensor,
+               kv_len: torch.Tensor, q_len: torch.Tensor | None = None,
+               scale: float | None = None) -> torch.Tensor:
+        """Attention of the newest tokens' queries ``q`` [B, T, q_heads,
+        head_dim] over the cache.
+
+        Row b holds ``kv_len[b]`` tokens (as appended, the new ones included);
+        its last ``q_len[b]`` (T without it) are q's tokens 0 .. q_len - 1, and
+        query i sees the positions up to its own, kv_len - q_len + i.  q_heads
+        is a multiple of num_kv_heads, consecutive query heads sharing a KV
+        head.  ``scale`` defaults to head_dim ** -0.5.  Returns [B, T, q_heads,
+        head_dim] in the cache's type: zeros for a query that sees nothing and
+        for tokens from q_len on.  T = 1 is a decode step, T = k + 1 a
+        verification step, a long T a chunk of a prompt."""
+        require_gpu(q, page_table, kv_len, q_len)
+        qh = self._heads("q", q)
+        b, t, heads = q.shape[:3]
+        if heads < 1 or heads % self.num_kv_heads:
+            raise ValueError(f"{heads} query heads do not share "
+                             f"{self.num_kv_heads} KV heads evenly")
+        view = self._view(page_table, b)
+        ln, ln64 = self._counts("kv_len", kv_len, b)
+        if ln is None:
+            raise ValueError("kv_len is needed")
+        ql, ql64 = self._counts("q_len", q_len, b)
+        if scale is None:
+            scale = self.head_dim ** -0.5
+        out = torch.empty(q.shape, dtype=self.dtype, device=self.device)
+        if out.numel() == 0:
+            return out
+        L = lib()
+        nbytes = L.sfx_kv4_attend_workspace_size(view, b, t, heads)
+        ws = (torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+              if nbytes else None)
+        check(L.sfx_kv4_attend(view, qh, b, t, heads, ln.data_ptr(), ln64,
+                               ptr(ql), ql64, float(scale), out.data_ptr(),
+                               ptr(ws), nbytes, stream_of(self.device)),
+              "KV4Cache.attend")
+        return out

@@ -1,0 +1,378 @@
+"""KV4Cache (append, read, attend) against the definitions in 64 bits
+(oracle/target.py)."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import target
+
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+
+
+def make(gpu, b, positions, heads, d, page, dtype, seed, garbage=True):
+    """A cache whose pages start as garbage (every float a NaN, every key scale
+    a NaN) and a shuffled page table."""
+    from suffixgpu_amd import KV4Cache
+    width = -(-positions // page)
+    c = KV4Cache(b * width, heads, d, page_size=page, dtype=dtype, device=gpu)
+    if garbage:
+        c.pages.fill_(255)
+    g = torch.Generator().manual_seed(seed)
+    table = torch.randperm(b * width, generator=g).to(torch.int32)
+    return c, table.view(b, width).to(gpu)
+
+
+def ints(x, gpu, dtype=torch.int32):
+    return torch.tensor(x, dtype=dtype, device=gpu)
+
+
+def np64(t):
+    return t.detach().to("cpu", torch.float64).numpy()
+
+
+def data(gpu, b, t, heads, d, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(b, t, heads, d, generator=g)
+    x[..., ::17] *= 6.0
+    return x.to(dtype).to(gpu)
+
+
+def filled(gpu, b, lens, heads, d, page, dtype, seed, cap=None):
+    """A cache holding lens[i] random tokens in row i, and what it stands
+    for."""
+    n = max(max(lens), 1)
+    c, table = make(gpu, b, cap or n, heads, d, page, dtype, seed)
+    k = data(gpu, b, n, heads, d, dtype, seed + 1)
+    v = data(gpu, b, n, heads, d, dtype, seed + 2)
+    c.append(k, v, table, ints([0] * b, gpu), ints(lens, gpu))
+    half = dtype == HF
+    kq = target.quantize_k(np64(k), half)
+    vq, vs = target.quantize_v(np64(v))
+    return c, table, kq, vq, vs
+
+
+def check_attend(out, q, kq, vq, vs, kv_len, q_len, dtype, scale=None):
+    exp, bound = target.attend(np64(q), kq, vq, vs, kv_len, q_len, scale)
+    rel, tiny = target.ulp16(dtype == HF)
+    err = np.abs(np64(out) - exp)
+    tol = bound + rel * (np.abs(exp) + bound) + tiny
+    tol = np.where(bound == 0, 0.0, tol)     # rows that see nothing are zeros
+    bad = err > tol
+    assert not bad.any(), (np.argwhere(bad)[:5], err[bad][:5], tol[bad][:5])
+
+
+# ------------------------------------------------------------ append, read
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("page,t", [(32, 1), (64, 17), (32, 70), (128, 300)])
+def test_append_holds_the_rounded_values(gpu, dtype, d, page, t):
+    b, heads, cap = 3, 2, 400
+    c, table = make(gpu, b, cap, heads, d, page, dtype, 5)
+    k = data(gpu, b, t, heads, d, dtype, 6)
+    v = data(gpu, b, t, heads, d, dtype, 7)
+    start, count = [0, 31, 77], [t, max(0, t - 2), t]
+    c.append(k, v, table, ints(start, gpu), ints(count, gpu))
+    gk, gv = c.read(table, ints(start, gpu), t, ints(count, gpu))
+    ek = target.quantize_k(np64(k), dtype == HF)
+    ev, _ = target.quantize_v(np64(v))
+    rel, tiny = target.ulp16(dtype == HF)
+    for i in range(b):
+        n = count[i]
+        np.testing.assert_array_equal(np64(gk)[i, :n], ek[i, :n])
+        err = np.abs(np64(gv)[i, :n] - ev[i, :n])
+        assert (err <= np.abs(ev[i, :n]) * (rel + 2.0 ** -22) + tiny).all()
+        assert not np64(gk)[i, n:].any() and not np64(gv)[i, n:].any()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_append_rounds_ties_and_extremes(gpu, dtype):
+    """Every magnitude of the type's upper bits in one token or another: ties of
+    both scales, subnormals, the largest values, zeros of both signs."""
+    d, heads = 128, 1
+    top = 65504.0 if dtype == HF else 3.38e38
+    rows = []
+    for amax in (6.0, 7.0, 7.03125, 8.0, 3.5, 12.0, 1.5, 1e-7, 1e-40, top, 0.0):
+        base = torch.arange(d, dtype=torch.float64) / 24.0 * (amax / 5.25)
+        base[::2] *= -1
+        base[7] = amax
+        base[40] = -amax
+        rows.append(base.clamp(-amax, amax) if amax else base * 0.0)
+    x = torch.stack(rows).to(dtype)[None, :, None].to(gpu)
+    t = x.shape[1]
+    c, table = make(gpu, 1, t, heads, d, 32, dtype, 8)
+    c.append(x, x, table, ints([0], gpu))
+    gk, gv = c.read(table, ints([0], gpu), t)
+    np.testing.assert_array_equal(np64(gk),
+                                  target.quantize_k(np64(x), dtype == HF))
+    ev, _ = target.quantize_v(np64(x))
+    rel, tiny = target.ulp16(dtype == HF)
+    assert (np.abs(np64(gv) - ev)
+            <= np.abs(ev) * (rel + 2.0 ** -22) + tiny).all()
+
+
+def test_append_infinities_and_nan(gpu):
+    """They make their group of a key, or their token's values, NaN, and the
+    queries that see them; no other group, token or row."""
+    d, heads = 128, 2
+    c, table = make(gpu, 1, 64, heads, d, 32, BF, 9)
+    k = data(gpu, 1, 40, heads, d, BF, 10)
+    v = data(gpu, 1, 40, heads, d, BF, 11)
+    k[0, 35, 0, 40] = float("inf")
+    v[0, 38, 1, 3] = float("nan")
+    c.append(k, v, table, ints([0], gpu))
+    gk, gv = c.read(table, ints([0], gpu), 40)
+    nk, nv = torch.isnan(gk), torch.isnan(gv)
+    assert nk[0, 35, 0, 32:64].all() and int(nk.sum()) == 32
+    assert nv[0, 38, 1].all() and int(nv.sum()) == d
+    q = data(gpu, 1, 40, heads, d, BF, 12)
+    out = c.attend(q, table, ints([40], gpu))
+    bad = torch.isnan(out).any(dim=-1)[0]
+    assert bad[35:, 0].all() and not bad[:35, 0].any()
+    assert bad[38:, 1].all() and not bad[:38, 1].any()
+
+
+def test_append_keeps_other_tokens_and_overwrites(gpu):
+    """Token by token, overlapping and out of order: what is held at the end is
+    each position's last write."""
+    d, heads, n = 64, 3, 100
+    c, table = make(gpu, 2, n, heads, d, 32, BF, 13)
+    rng = np.random.default_rng(1)
+    want_k = np.zeros((2, n, heads, d))
+    want_v = np.zeros((2, n, heads, d))
+    c.pages.zero_()
+    for step in range(40):
+        t = int(rng.integers(1, 9))
+        k = data(gpu, 2, t, heads, d, BF, 100 + step)
+        v = data(gpu, 2, t, heads, d, BF, 200 + step)
+        start = [int(rng.integers(0, n - t + 1)) for _ in range(2)]
+        count = [int(rng.integers(0, t + 1)) for _ in range(2)]
+        c.append(k, v, table, ints(start, gpu, torch.int64),
+                 ints(count, gpu, torch.int64))
+        ek = target.quantize_k(np64(k), False)
+        ev, _ = target.quantize_v(np64(v))
+        for i in range(2):
+            want_k[i, start[i]:start[i] + count[i]] = ek[i, :count[i]]
+            want_v[i, start[i]:start[i] + count[i]] = ev[i, :count[i]]
+    gk, gv = c.read(table, ints([0, 0], gpu), n)
+    np.testing.assert_array_equal(np64(gk), want_k)
+    err = np.abs(np64(gv) - want_v)
+    assert (err <= np.abs(want_v) * (2.0 ** -8 + 2.0 ** -22)).all()
+
+
+def test_append_outside_the_table_writes_nothing(gpu):
+    d, heads = 64, 1
+    c, table = make(gpu, 3, 64, heads, d, 32, BF, 14)
+    before = c.pages.clone()
+    k = data(gpu, 3, 8, heads, d, BF, 15)
+    table[1, 1] = -1
+    table[2, 1] = c.num_pages
+    # past the end, into a page id that is none, and before position 0
+    c.append(k, k, table, ints([64, 32, 40], gpu))
+    c.append(k, k, table, ints([-1, 1 << 20, -8], gpu))
+    assert torch.equal(before, c.pages)
+    # only the part inside the table is written and read
+    c.append(k, k, table, ints([60, 28, 28], gpu))
+    gk, _ = c.read(table, ints([60, 28, 28], gpu), 8)
+    ek = target.quantize_k(np64(k), False)
+    np.testing.assert_array_equal(np64(gk)[:, :4], ek[:, :4])
+    assert not np64(gk)[:, 4:].any()
+
+
+# ---------------------------------------------------------------- attend
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("hq,heads", [(4, 4), (6, 2), (8, 1)])
+@pytest.mark.parametrize("t", [1, 5, 17])
+def test_attend_shapes(gpu, dtype, d, hq, heads, t):
+    lens = [t, 33, 64, 200]
+    lens = [max(x, t) for x in lens]
+    c, table, kq, vq, vs = filled(gpu, 4, lens, heads, d, 32, dtype, 20)
+    q = data(gpu, 4, t, hq, d, dtype, 21)
+    out = c.attend(q, table, ints(lens, gpu))
+    check_attend(out, q, kq, vq, vs, lens, [t] * 4, dtype)
+
+
+@pytest.mark.parametrize("page", [32, 64, 256])
+@pytest.mark.parametrize("t", [1, 17])
+def test_attend_lengths(gpu, page, t):
+    """Rows of no token, one, and around blocks and pages; fewer queries than
+    T, none, and more queries than tokens."""
+    lens = [0, 1, 2, 31, 32, 33, 63, 65, 257, 700]
+    qn = [min(t, max(1, n)) for n in lens]
+    qn[4] = 0
+    qn[2] = t        # queries before position 0 see nothing
+    b = len(lens)
+    c, table, kq, vq, vs = filled(gpu, b, lens, 2, 128, page, BF, 30, cap=800)
+    q = data(gpu, b, t, 4, 128, BF, 31)
+    out = c.attend(q, table, ints(lens, gpu, torch.int64),
+                   ints(qn, gpu, torch.int64))
+    check_attend(out, q, kq, vq, vs, lens, qn, BF)
+    assert not np64(out)[0].any() and not np64(out)[4].any()
+
+
+@pytest.mark.parametrize("dtype,d,hq,heads", [(BF, 128, 8, 2), (HF, 64, 3, 3),
+                                              (HF, 256, 4, 1)])
+def test_attend_prompt(gpu, dtype, d, hq, heads):
+    """A prompt's chunk of many rows, ragged, after a context."""
+    t, lens, qn = 150, [150, 411], [150, 133]
+    c, table, kq, vq, vs = filled(gpu, 2, lens, heads, d, 64, dtype, 40)
+    q = data(gpu, 2, t, hq, d, dtype, 41)
+    out = c.attend(q, table, ints(lens, gpu), ints(qn, gpu))
+    check_attend(out, q, kq, vq, vs, lens, qn, dtype)
+
+
+@pytest.mark.parametrize("t", [1, 3])
+def test_attend_long_row_is_split_and_joined(gpu, t):
+    lens = [5000, 1300]
+    c, table, kq, vq, vs = filled(gpu, 2, lens, 1, 128, 64, BF, 50)
+    q = data(gpu, 2, t, 4, 128, BF, 51)
+    out = c.attend(q, table, ints(lens, gpu))
+    check_attend(out, q, kq, vq, vs, lens, [t] * 2, BF)
+
+
+def test_attend_scales_far_apart(gpu):
+    """Values whose scales differ by 2^40 and more, tokens of zero values, a
+    large softmax scale: weights stay in range."""
+    n, d = 300, 128
+    c, table = make(gpu, 1, n, 1, d, 64, BF, 60)
+    k = data(gpu, 1, n, 1, d, BF, 61)
+    v = data(gpu, 1, n, 1, d, BF, 62)
+    g = torch.Generator().manual_seed(63)
+    e = torch.randint(-60, 20, (n, 1, 1), generator=g).to(gpu)
+    v = torch.ldexp(v[0].float(), e).to(BF)[None]
+    v[0, ::13] = 0
+    c.append(k, v, table, ints([0], gpu))
+    q = data(gpu, 1, 4, 2, d, BF, 64)
+    kq = target.quantize_k(np64(k), False)
+    vq, vs = target.quantize_v(np64(v))
+    for scale in (0.02, 1.0):
+        out = c.attend(q, table, ints([n], gpu), scale=scale)
+        check_attend(out, q, kq, vq, vs, [n], [4], BF, scale)
+
+
+def test_attend_strides_and_alignment(gpu):
+    """Queries as slices of a fused projection, of misaligned rows, and of
+    transposed storage."""
+    b, t, hq, d, lens = 2, 7, 4, 64, [90, 40]
+    c, table, kq, vq, vs = filled(gpu, b, lens, 2, d, 32, BF, 70)
+    fused = data(gpu, b, t, hq + 5, d, BF, 71)
+    odd = torch.zeros(b * t * hq * d + 1, dtype=BF, device=gpu)
+    odd[1:] = fused[:, :, :hq].reshape(-1)
+    qs = [fused[:, :, 1:1 + hq], odd[1:].view(b, t, hq, d),
+          fused[:, :, :hq].transpose(1, 2).contiguous().transpose(1, 2)]
+    wide = torch.full((b, table.shape[1] + 3), -7, dtype=torch.int32,
+                      device=gpu)
+    wide[:, :table.shape[1]] = table
+    for q in qs:
+        out = c.attend(q, wide[:, :table.shape[1]], ints(lens, gpu))
+        check_attend(out, q, kq, vq, vs, lens, [t] * b, BF)
+    k = data(gpu, b, t, 4, d, BF, 72)
+    for src in (k[:, :, 1:3], k[:, :, ::2]):
+        c.append(src, src, table, ints([0, 3], gpu))
+        gk, _ = c.read(table, ints([0, 3], gpu), t)
+        np.testing.assert_array_equal(np64(gk),
+                                      target.quantize_k(np64(src), False))
+    flat = torch.zeros(k.numel() + 3, dtype=BF, device=gpu)
+    flat[3:] = k.reshape(-1)
+    src = flat[3:].view(k.shape)[:, :, :2]
+    c.append(src, src, table, ints([1, 2], gpu))
+    gk, _ = c.read(table, ints([1, 2], gpu), t)
+    np.testing.assert_array_equal(np64(gk),
+                                  target.quantize_k(np64(src), False))
+
+
+def test_attend_skips_pages_that_are_none(gpu):
+    """A page id that is none hides its positions."""
+    c, table, kq, vq, vs = filled(gpu, 2, [96, 96], 1, 64, 32, BF, 80)
+    q = data(gpu, 2, 1, 2, 64, BF, 81)
+    cut = table.clone()
+    cut[0, 1] = -1
+    cut[1, 1] = 1 << 30
+    out = c.attend(q, cut, ints([96, 96], gpu))
+    keep = np.r_[0:32, 64:96]
+    check_attend(out, q, kq[:, keep], vq[:, keep], vs[:, keep], [64, 64],
+                 [1, 1], BF)
+    cut[:] = -1
+    assert not np64(c.attend(q, cut, ints([96, 96], gpu))).any()
+
+
+def test_attend_is_repeatable_and_independent_of_the_batch(gpu):
+    lens = [900, 77]
+    c, table, *_ = filled(gpu, 2, lens, 2, 128, 64, BF, 90)
+    q = data(gpu, 2, 3, 8, 128, BF, 91)
+    a = c.attend(q, table, ints(lens, gpu))
+    for _ in range(5):
+        assert torch.equal(a, c.attend(q, table, ints(lens, gpu)))
+
+
+def test_cache_under_graph_and_on_another_stream(gpu):
+    """append + attend captured and replayed with other data in between, and on
+    a side stream."""
+    lens = [130, 40]
+    c, table, *_ = filled(gpu, 2, lens, 2, 128, 64, BF, 95, cap=200)
+    k = data(gpu, 2, 3, 2, 128, BF, 96)
+    q = data(gpu, 2, 3, 4, 128, BF, 97)
+    start, ln = ints(lens, gpu), ints([n + 3 for n in lens], gpu)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        c.append(k, k, table, start)
+        c.attend(q, table, ln)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c.append(k, k, table, start)
+        out = c.attend(q, table, ln)
+    for seed in (1, 2, 3):
+        k.copy_(data(gpu, 2, 3, 2, 128, BF, seed))
+        q.copy_(data(gpu, 2, 3, 4, 128, BF, seed + 10))
+        g.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        c.append(k, k, table, start)
+        assert torch.equal(got, c.attend(q, table, ln))
+
+
+def test_cache_refusals(gpu):
+    from suffixgpu_amd import KV4Cache
+    from suffixgpu_amd._lib import SuffixGPUError
+    for bad in (dict(head_dim=96), dict(page_size=48), dict(page_size=16),
+                dict(dtype=torch.float32), dict(num_kv_heads=0),
+                dict(num_pages=-1)):
+        with pytest.raises(ValueError):
+            KV4Cache(**{**dict(num_pages=4, num_kv_heads=2, head_dim=64,
+                               device=gpu), **bad})
+    with pytest.raises(SuffixGPUError):
+        KV4Cache(4, 2, 64, device="cpu")
+    c = KV4Cache(4, 2, 64, page_size=32, device=gpu)
+    with pytest.raises(ValueError):
+        KV4Cache(4, 2, 64, page_size=32, device=gpu, pages=c.pages[:3])
+    table = ints([[0, 1], [2, 3]], gpu)
+    k = data(gpu, 2, 3, 2, 64, BF, 1)
+    q = data(gpu, 2, 3, 4, 64, BF, 1)
+    n = ints([3, 3], gpu)
+    for args in ((k.half(), k, table, n), (k, k[:, :2], table, n),
+                 (k[..., ::2], k, table, n), (k, k, table.long(), n),
+                 (k, k, table[:1], n), (k, k, table, n[:1]),
+                 (k, k, table.t(), n), (k[:, :, :1], k, table, n),
+                 (k, k, table, None)):
+        with pytest.raises(ValueError):
+            c.append(*args)
+    for args in ((q.half(), table, n), (q[:, :, :3], table, n),
+                 (q, table, n[:1]), (q, table, None), (q[0], table, n),
+                 (q, table, n, n[:1])):
+        with pytest.raises(ValueError):
+            c.attend(*args)
+    with pytest.raises(SuffixGPUError):
+        c.attend(q.cpu(), table, n)
+    # nothing to do is no error
+    assert c.attend(q[:0], table[:0], n[:0]).shape == (0, 3, 4, 64)
+    assert c.attend(q[:, :0], table, n).shape == (2, 0, 4, 64)
+    c.append(k[:0], k[:0], table[:0], n[:0])
+    empty = torch.empty(2, 0, dtype=torch.int32, device=gpu)
+    assert not c.attend(q, empty, n).any()
