@@ -603,8 +603,10 @@ int sfx_kv4_attend(const sfx_kv4* cache, const sfx_heads* q, int64_t batch,
  * sampled [batch, K + 1]: the accepted drafts, the drawn token, -1 after
  * them; count [batch] their number.  uniform [batch, K] and noise
  * [batch, vocab] may be NULL only with all_greedy != 0, which takes every
- * row's temperature as 0.  workspace: sfx_verify_workspace_size bytes,
- * 16-byte aligned, of any content. */
+ * row's temperature as 0.  counters: sfx_verify_counter_bytes bytes,
+ * zero-filled once; every call leaves them zero, whatever its sizes.
+ * workspace: sfx_verify_workspace_size bytes of any content.  Both 16-byte
+ * aligned; calls that share either must not overlap. */
 typedef struct sfx_verify {
     const void* logits;
     int32_t dtype;             /* SFX_BF16, SFX_F16 or SFX_F32            */
@@ -622,7 +624,9 @@ typedef struct sfx_verify {
 } sfx_verify;
 
 size_t sfx_verify_workspace_size(int64_t batch, int64_t k, int64_t vocab);
-int sfx_verify_draft(const sfx_verify* args, void* workspace,
+size_t sfx_verify_counter_bytes(int64_t batch, int64_t k, int64_t vocab);
+int sfx_verify_draft(const sfx_verify* args, void* counters,
+                     size_t counter_bytes, void* workspace,
                      size_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus

@@ -189,8 +189,10 @@ SIGNATURES = {
                                c_p, c_i32, c_p, c_i32, ctypes.c_float, c_p,
                                c_p, ctypes.c_size_t, c_p]),
     "sfx_verify_workspace_size": (ctypes.c_size_t, [c_i64, c_i64, c_i64]),
+    "sfx_verify_counter_bytes": (ctypes.c_size_t, [c_i64, c_i64, c_i64]),
     "sfx_verify_draft": (c_i32, [ctypes.POINTER(SfxVerify), c_p,
-                                 ctypes.c_size_t, c_p]),
+                                 ctypes.c_size_t, c_p, ctypes.c_size_t,
+                                 c_p]),
 }
 
 _lib = None

@@ -15,6 +15,35 @@ from suffixgpu_amd import _lib
 from suffixgpu_amd._lib import check, lib, ptr, require_gpu, stream_of
 
 
+# (device, stream) -> (counters, scratch).  The counters are zero between calls
+# (every call leaves them so), the scratch is anything; two calls that share
+# them are ordered by their stream.  Calls recorded into a HIP graph share a
+# pair of their own per device (replays must not overlap each other): eager
+# calls see to its size, so that a capture after a first eager call of that size
+# records no fill.  Outgrown pairs of graphs are kept, a graph may hold them.
+_workspaces: dict[tuple, tuple[torch.Tensor, torch.Tensor]] = {}
+_outgrown: list[tuple[torch.Tensor, torch.Tensor]] = []
+
+
+def _workspace(dev: torch.device, stream: int, nc: int, ns: int):
+    capturing = torch.cuda.is_current_stream_capturing()
+    for key in (((dev, "graph"),) if capturing
+                else ((dev, "graph"), (dev, stream))):
+        ws = _workspaces.get(key)
+        if ws is None or ws[0].numel() < nc or ws[1].numel() < ns:
+            if ws is not None:
+                if key[1] == "graph":
+                    _outgrown.append(ws)
+                nc2 = max(nc, 2 * ws[0].numel())
+                ns2 = max(ns, 2 * ws[1].numel())
+            else:
+                nc2, ns2 = max(nc, 1 << 16), max(ns, 1 << 18)
+            ws = (torch.zeros(nc2, dtype=torch.uint8, device=dev),
+                  torch.empty(ns2, dtype=torch.uint8, device=dev))
+            _workspaces[key] = ws
+    return ws
+
+
 def verify_draft(logits: torch.Tensor, draft: torch.Tensor,
                  num_valid: torch.Tensor,
                  uniform: torch.Tensor | None = None,
@@ -80,8 +109,10 @@ def verify_draft(logits: torch.Tensor, draft: torch.Tensor,
     if b == 0:
         return sampled, count
     L = lib()
-    nbytes = L.sfx_verify_workspace_size(b, k1 - 1, v)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    stream = stream_of(dev)
+    counters, scratch = _workspace(dev, stream,
+                                   L.sfx_verify_counter_bytes(b, k1 - 1, v),
+                                   L.sfx_verify_workspace_size(b, k1 - 1, v))
     args = _lib.SfxVerify(
         logits.data_ptr(), code, int(greedy), b, k1 - 1, v,
         logits.stride(0), logits.stride(1), draft.data_ptr(),
@@ -91,6 +122,7 @@ def verify_draft(logits: torch.Tensor, draft: torch.Tensor,
         None if greedy else ptr(temperature),
         None if greedy else ptr(draft_probs),
         sampled.data_ptr(), count.data_ptr())
-    check(L.sfx_verify_draft(args, ws.data_ptr(), nbytes, stream_of(dev)),
+    check(L.sfx_verify_draft(args, counters.data_ptr(), counters.numel(),
+                             scratch.data_ptr(), scratch.numel(), stream),
           "verify_draft")
     return sampled, count

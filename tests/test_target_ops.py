@@ -99,11 +99,18 @@ def test_verify_is_checked_on_the_host():
                 dict(draft=None), dict(num_valid=None), dict(uniform=None),
                 dict(noise=None), dict(sampled=None), dict(count=None),
                 dict(batch=1 << 24)):
-        assert lib.sfx_verify_draft(args(**bad), 0x7000, 1 << 30, None) == -1
-    assert lib.sfx_verify_draft(args(), 0x7000, need - 1, None) == -1
-    assert lib.sfx_verify_draft(args(), 0x7008, 1 << 30, None) == -1
-    assert lib.sfx_verify_draft(args(), None, 1 << 30, None) == -1
-    assert lib.sfx_verify_draft(args(batch=0), None, 0, None) == 0
+        assert lib.sfx_verify_draft(args(**bad), 0x7000, 1 << 30, 0x8000,
+                                    1 << 30, None) == -1
+    zeros = lib.sfx_verify_counter_bytes(2, 3, 100)
+    assert zeros > 0
+    for c, nc, w, nw in ((0x7000, zeros, 0x8000, need - 1),
+                         (0x7000, zeros - 1, 0x8000, need),
+                         (0x7008, zeros, 0x8000, need),
+                         (0x7000, zeros, 0x8008, need),
+                         (None, zeros, 0x8000, need),
+                         (0x7000, zeros, None, need)):
+        assert lib.sfx_verify_draft(args(), c, nc, w, nw, None) == -1
+    assert lib.sfx_verify_draft(args(batch=0), None, 0, None, 0, None) == 0
     assert lib.sfx_verify_workspace_size(0, 3, 100) == 0
 
 
