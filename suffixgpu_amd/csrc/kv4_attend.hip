@@ -26,6 +26,7 @@ namespace sfx {
 namespace {
 
 typedef float F4 __attribute__((ext_vector_type(4)));
+typedef float F16 __attribute__((ext_vector_type(16)));
 typedef _Float16 H2 __attribute__((ext_vector_type(2)));
 typedef _Float16 H8 __attribute__((ext_vector_type(8)));
 typedef __bf16 B2 __attribute__((ext_vector_type(2)));
@@ -35,7 +36,6 @@ typedef uint32_t U4 __attribute__((ext_vector_type(4)));
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kSlack = 8.0f;
 constexpr int kWaves = 4;
-constexpr int kTile = 16;  // query rows of a matrix instruction
 
 struct AttendArgs {
   KvView c;
@@ -44,15 +44,16 @@ struct AttendArgs {
   int group;       // query heads per KV head
   int q_heads;
   int rows;        // tokens * group
-  int q_tiles;     // of 16 * NQ rows
+  int q_tiles;     // row groups of a workgroup
   int splits;
+  int64_t batch;
   int vec;
   const void* kv_len;
   const void* q_len;
   int kv64, q64;
   float scale;     // times log2(e)
   uint16_t* out;
-  float* part;     // [batch, heads, q_tiles, splits, 16 NQ, D + 2]
+  float* part;     // [batch, heads, q_tiles, splits, rows of a group, D + 2]
 };
 
 // Eight 4-bit values of a word as 16-bit ones, times `scale` (a power of two,
@@ -83,7 +84,16 @@ __device__ __forceinline__ U4 widen(uint32_t w, float scale) {
 }
 
 template <bool kHalf>
-__device__ __forceinline__ F4 mma(U4 a, U4 b, F4 c) {
+__device__ __forceinline__ F16 mma32(U4 a, U4 b, F16 c) {
+  if (kHalf)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(
+        __builtin_bit_cast(H8, a), __builtin_bit_cast(H8, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+      __builtin_bit_cast(B8, a), __builtin_bit_cast(B8, b), c, 0, 0, 0);
+}
+
+template <bool kHalf>
+__device__ __forceinline__ F4 mma16(U4 a, U4 b, F4 c) {
   if (kHalf)
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(
         __builtin_bit_cast(H8, a), __builtin_bit_cast(H8, b), c, 0, 0, 0);
@@ -98,65 +108,113 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b) {
   return __builtin_bit_cast(uint32_t, h);
 }
 
-// A block of the cache as a lane holds it: row i = lane % 16 of tile a is
-// token 16 (i / 8) + 8 a + i % 8, which makes result row 4 quad + r of tile a
-// the (4 a + r)-th token of the lane's words of values.
+// Both forms of the kernel keep, per query row (a lane's column), M, l and O,
+// and take a block in the same steps; they differ in the matrix instruction.
+// kTile = 16: 16x16x32, a lane holds 8 tokens' scores of a row, four lanes
+// share it.  kTile = 32: 32x32x16, 16 tokens' scores, two lanes share a row.
+
+// A block of the cache as a lane holds it.
+// kTile = 16: row i = lane % 16 of score tile a is token 16 (i / 8) + 8 a +
+// i % 8, which makes result row 4 quad + r of tile a the (4 a + r)-th token of
+// the lane's words of values.
+// kTile = 32: row lane % 32 is that token; result row 8 (r / 4) + 4 (lane / 32)
+// + r % 4 is token r % 8 of the lane's word of step r / 8.
+template <int D, int kTile>
+struct Block;
+
 template <int D>
-struct Block {
+struct Block<D, 16> {
   uint32_t k[2][D / 32];  // 8 channels a word
   uint32_t ks[2];         // scale bytes of the lane's channels
   uint32_t v[D / 16];     // a word of tokens for each 16 channels
-  float vs[8];
+  float vs;               // scale of token lane % 32's values
+
+  __device__ __forceinline__ void load(const char* base) {
+    using L = KvLayout<D>;
+    const int lane = lane_id();
+    const int i = lane % 16, quad = lane / 16;
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const int t = 16 * (i / 8) + 8 * a + i % 8;
+      const char* p = base + t * (D / 2) + quad * (D / 8);
+      if (D == 64) {
+        const uint2 w = *(const uint2*)p;
+        k[a][0] = w.x;
+        k[a][1] = w.y;
+      } else {
+#pragma unroll
+        for (int u = 0; u < D / 128; ++u) {
+          const uint4 w = ((const uint4*)p)[u];
+          k[a][4 * u] = w.x;
+          k[a][4 * u + 1] = w.y;
+          k[a][4 * u + 2] = w.z;
+          k[a][4 * u + 3] = w.w;
+        }
+      }
+      const uint8_t* s = (const uint8_t*)(base + L::kScale) + t * (D / 32);
+      if (D == 256)
+        ks[a] = *(const uint16_t*)(s + 2 * quad);
+      else
+        ks[a] = s[D == 64 ? quad / 2 : quad];
+    }
+#pragma unroll
+    for (int g = 0; g < D / 64; ++g) {
+      const uint4 w = *(const uint4*)(base + L::kValue + (g * 64 + lane) * 16);
+      v[4 * g] = w.x;
+      v[4 * g + 1] = w.y;
+      v[4 * g + 2] = w.z;
+      v[4 * g + 3] = w.w;
+    }
+    vs = ((const float*)(base + L::kVScale))[lane % 32];
+  }
+  // Scale of the channels of matrix step i in tile a.  The conversion takes
+  // its exponent alone, all ones is a NaN.
+  __device__ __forceinline__ float scale(int a, int i) const {
+    uint32_t b = ks[a];
+    if (D == 256) b = i < D / 64 ? b & 255u : b >> 8;
+    return __uint_as_float(b << 23);
+  }
 };
 
 template <int D>
-__device__ __forceinline__ void load_block(const char* base, Block<D>& b) {
-  using L = KvLayout<D>;
-  const int lane = lane_id();
-  const int i = lane % 16, quad = lane / 16;
+struct Block<D, 32> {
+  uint32_t k[D / 16];
+  uint32_t ks;
+  uint32_t v[2][D / 32];  // by step of 16 tokens, then 16 channels
+  float vs;
+
+  __device__ __forceinline__ void load(const char* base) {
+    using L = KvLayout<D>;
+    const int lane = lane_id();
+    const int t = lane % 32, h = lane / 32;
+    const uint4* p = (const uint4*)(base + t * (D / 2) + h * (D / 4));
 #pragma unroll
-  for (int a = 0; a < 2; ++a) {
-    const int t = 16 * (i / 8) + 8 * a + i % 8;
-    const char* p = base + t * (D / 2) + quad * (D / 8);
-    if (D == 64) {
-      const uint2 w = *(const uint2*)p;
-      b.k[a][0] = w.x;
-      b.k[a][1] = w.y;
-    } else {
-#pragma unroll
-      for (int u = 0; u < D / 128; ++u) {
-        const uint4 w = ((const uint4*)p)[u];
-        b.k[a][4 * u] = w.x;
-        b.k[a][4 * u + 1] = w.y;
-        b.k[a][4 * u + 2] = w.z;
-        b.k[a][4 * u + 3] = w.w;
-      }
+    for (int u = 0; u < D / 64; ++u) {
+      const uint4 w = p[u];
+      k[4 * u] = w.x;
+      k[4 * u + 1] = w.y;
+      k[4 * u + 2] = w.z;
+      k[4 * u + 3] = w.w;
     }
     const uint8_t* s = (const uint8_t*)(base + L::kScale) + t * (D / 32);
-    if (D == 256)
-      b.ks[a] = *(const uint16_t*)(s + 2 * quad);
-    else
-      b.ks[a] = s[D == 64 ? quad / 2 : quad];
-  }
+    ks = D == 64 ? s[h]
+                 : (D == 128 ? ((const uint16_t*)s)[h] : ((const uint32_t*)s)[h]);
 #pragma unroll
-  for (int g = 0; g < D / 64; ++g) {
-    const uint4 w = *(const uint4*)(base + L::kValue + (g * 64 + lane) * 16);
-    b.v[4 * g] = w.x;
-    b.v[4 * g + 1] = w.y;
-    b.v[4 * g + 2] = w.z;
-    b.v[4 * g + 3] = w.w;
-  }
-  const float* vs = (const float*)(base + L::kVScale) + 16 * (quad / 2) +
-                    4 * (quad % 2);
+    for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
-  for (int a = 0; a < 2; ++a) {
-    const float4 w = *(const float4*)(vs + 8 * a);
-    b.vs[4 * a] = w.x;
-    b.vs[4 * a + 1] = w.y;
-    b.vs[4 * a + 2] = w.z;
-    b.vs[4 * a + 3] = w.w;
+      for (int g = 0; g < D / 64; ++g) {
+        const uint2 w = *(const uint2*)(base + L::kValue +
+                                        ((g * 4 + 2 * s2 + h) * 16 + lane % 16) *
+                                            16 + lane / 16 % 2 * 8);
+        v[s2][2 * g] = w.x;
+        v[s2][2 * g + 1] = w.y;
+      }
+    vs = ((const float*)(base + L::kVScale))[t];
   }
-}
+  __device__ __forceinline__ float scale(int i) const {
+    return __uint_as_float((ks >> (8 * (i / 4)) & 255u) << 23);
+  }
+};
 
 // A lane's 8 channels of a query row, as bits.
 __device__ __forceinline__ U4 load_q8(const uint16_t* p, bool vec, bool live) {
@@ -169,48 +227,180 @@ __device__ __forceinline__ U4 load_q8(const uint16_t* p, bool vec, bool live) {
   return r;
 }
 
-// One workgroup: a tile of 16 NQ query rows of one KV head and batch row over
-// one split of the row's visible blocks, its waves taking every fourth block.
-template <int D, bool kHalf, int NQ>
-__global__ __launch_bounds__(64 * kWaves) void k_kv4_attend(AttendArgs a) {
-  constexpr int kRows = kTile * NQ;
+// What a workgroup works on: rows [row0, row0 + rows of a group) of KV head h
+// of batch row b, one split of the row's blocks.  Workgroups go round the eight
+// XCDs in turn: those of the same blocks and other query rows follow each other
+// on one XCD, whose L2 then holds the blocks.
+struct Work {
+  int64_t b;
+  int h, qt, split;
+  bool any;
+};
+
+__device__ __forceinline__ Work work_of(const AttendArgs& a) {
+  Work w;
+  const int id = (int)blockIdx.x;
+  const int k = id >> 3;
+  w.qt = k % a.q_tiles;
+  const int64_t item = (int64_t)(k / a.q_tiles) * 8 + (id & 7);
+  w.split = (int)(item % a.splits);
+  const int64_t bh = item / a.splits;
+  w.h = (int)(bh % a.c.heads);
+  w.b = bh / a.c.heads;
+  w.any = w.b < a.batch;
+  return w;
+}
+
+__device__ __forceinline__ int64_t kv_len_of(const AttendArgs& a, int64_t b) {
+  const int64_t n = load_count(a.kv_len, a.kv64, b);
+  return n < 0 ? 0 : (n > a.c.positions ? a.c.positions : n);
+}
+
+__device__ __forceinline__ int64_t q_len_of(const AttendArgs& a, int64_t b) {
+  if (!a.q_len) return a.tokens;
+  const int64_t n = load_count(a.q_len, a.q64, b);
+  return n < 0 ? 0 : (n > a.tokens ? a.tokens : n);
+}
+
+// Positions that row r sees; 0: none.
+__device__ __forceinline__ int visible(const AttendArgs& a, int64_t len,
+                                       int64_t nq, int r) {
+  const int t = r / a.group;
+  const int64_t v = len - nq + t + 1;
+  return r < a.rows && t < nq && v > 0 ? (int)v : 0;
+}
+
+__device__ __forceinline__ const uint16_t* q_row(const AttendArgs& a,
+                                                 int64_t b, int h, int r) {
+  return (const uint16_t*)a.q.data + b * a.q.stride_b +
+         (int64_t)(r / a.group) * a.q.stride_t +
+         (int64_t)(h * a.group + r % a.group) * a.q.stride_h;
+}
+
+// Scale of a block's values in base 2, and one over it, of the tokens that a
+// lane's scores belong to: each lane works out one token's, and they cross in
+// the wave's own 64 floats of LDS, in order as its accesses are.
+// 1 / s is finite whatever the scale: a row that does not see a token (of a
+// NaN, or past the end, where a block holds anything) multiplies it by zero,
+// and one that sees a NaN has it from the logarithm.
+__device__ __forceinline__ void share_scales(float vs, float* lds) {
+  const int t = lane_id() % 32;
+  const float x =
+      lane_id() < 32
+          ? __builtin_amdgcn_logf(vs)
+          : fminf(fmaxf(__builtin_amdgcn_rcpf(vs), 0.0f), 0x1p101f);
+  lds[lane_id() / 32 * 32 + t] = x;
+  asm volatile("" ::: "memory");
+}
+
+// body(block, index) for blocks first, first + kWaves, ... below last of row b
+// and KV head h, by one wave for which all of these are the same.  A block's
+// loads are under way while the one before is worked on (two sets of registers
+// in turn: a copy from one to the other would wait for the loads), and its page
+// id while the one before that is.  Blocks without a page are left out.
+template <class B, class F>
+__device__ __forceinline__ void each_block(const KvView& c, int64_t b, int h,
+                                           int bytes, int first, int last,
+                                           F body) {
+  if (first >= last || c.num_pages == 0) return;
+  typedef const __attribute__((address_space(4))) int32_t* Ids;
+  const Ids ids = (Ids)(uintptr_t)(c.table + b * c.table_stride);
+  const int in_page = (1 << c.page_shift) - 1;
+  auto page = [&](int blk) { return blk < last ? ids[blk >> c.page_shift] : -1; };
+  auto good = [&](int32_t id) { return id >= 0 && id < c.num_pages; };
+  auto at = [&](int32_t id, int blk) {
+    return good(id) ? c.pages + ((((int64_t)id * c.heads + h) << c.page_shift) +
+                                 (blk & in_page)) * bytes
+                    : c.pages;
+  };
+  B x, y;
+  int32_t idx = page(first), idy = page(first + kWaves);
+  x.load(at(idx, first));
+  for (int blk = first;; blk += 2 * kWaves) {
+    const int n1 = blk + kWaves, n2 = blk + 2 * kWaves;
+    if (n1 < last) y.load(at(idy, n1));
+    const int32_t id2 = page(n2);
+    if (good(idx)) body(x, blk);
+    if (n1 >= last) break;
+    if (n2 < last) x.load(at(id2, n2));
+    const int32_t id3 = page(n2 + kWaves);
+    if (good(idy)) body(y, n1);
+    if (n2 >= last) break;
+    idx = id2;
+    idy = id3;
+  }
+}
+
+// Follows the maximum of a row's scores when it has grown by more than kSlack:
+// then O and l shrink by the factor returned, else it is 1.  kLanes: distance
+// of the lanes that share a row.
+template <int kLanes>
+__device__ __forceinline__ float follow(float top, float* m) {
+  if (kLanes == 16) top = fmaxf(top, __shfl_xor(top, 16));
+  top = fmaxf(top, __shfl_xor(top, 32));
+  const float mn = fmaxf(*m, top);
+  const float f = mn == *m ? 1.0f : __builtin_amdgcn_exp2f(*m - mn);
+  *m = mn;
+  return f;
+}
+
+// Writes a row's joined channels c0 .. c0 + N of the workgroup's waves: to the
+// result, or to this split's part.  x: the sum, lt: l, mx: M.
+template <bool kHalf, int N>
+__device__ __forceinline__ void put_row(const AttendArgs& a, const Work& w,
+                                        int d, int rows_tile, int row, int r,
+                                        bool see, float mx, float lt, int c0,
+                                        const float (&x)[N]) {
+  if (a.splits == 1) {
+    if (r >= a.rows) return;
+    const float inv = see ? 1.0f / lt : 0.0f;
+    uint32_t* out = (uint32_t*)(a.out + ((w.b * a.tokens + r / a.group) *
+                                             a.q_heads +
+                                         w.h * a.group + r % a.group) * d + c0);
+#pragma unroll
+    for (int c = 0; c < N; c += 2)
+      out[c / 2] = see ? from_float16b<kHalf>(x[c] * inv) |
+                             from_float16b<kHalf>(x[c + 1] * inv) << 16
+                       : 0u;
+  } else {
+    float* p = a.part + ((((w.b * a.c.heads + w.h) * a.q_tiles + w.qt) *
+                              a.splits + w.split) * rows_tile + row) * (d + 2);
+#pragma unroll
+    for (int c = 0; c < N; ++c) p[2 + c0 + c] = x[c];
+    if (c0 == 0) {
+      p[0] = see ? mx : kNegInf;
+      p[1] = lt;
+    }
+  }
+}
+
+// Up to 16 query rows a workgroup: single tokens, and small groups of drafts.
+template <int D, bool kHalf>
+__global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : (D == 128 ? 3 : 4))
+void k_kv4_attend16(AttendArgs a) {
   constexpr int kStep = D / 32;   // matrix instructions a score tile
   constexpr int kDt = D / 16;     // channel tiles
-  const int64_t b = blockIdx.z;
-  const int h = blockIdx.y;
-  const int qt = blockIdx.x / a.splits;
-  const int split = blockIdx.x % a.splits;
+  const Work wk = work_of(a);
+  if (!wk.any) return;
   const int lane = lane_id();
-  const int wave = threadIdx.x / kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int col = lane % 16, quad = lane / 16;
+  __shared__ float so[kWaves][16][D + 4];
+  __shared__ float sm[kWaves][16], sl[kWaves][16];
+  __shared__ float sc[kWaves][64];
 
-  int64_t len = load_count(a.kv_len, a.kv64, b);
-  len = len < 0 ? 0 : (len > a.c.positions ? a.c.positions : len);
-  int64_t nq = a.q_len ? load_count(a.q_len, a.q64, b) : a.tokens;
-  nq = nq < 0 ? 0 : (nq > a.tokens ? a.tokens : nq);
-
-  // Positions that each of the lane's rows sees; 0: none.
-  int vis[NQ];
-  U4 qf[NQ][kStep];
-  int most = 0, least = 0x7fffffff;
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int r = (qt * NQ + n) * kTile + col;
-    const int t = r / a.group;
-    const int64_t v = len - nq + t + 1;
-    vis[n] = (r < a.rows && t < nq && v > 0) ? (int)v : 0;
+  const int64_t len = kv_len_of(a, wk.b);
+  const int64_t nq = q_len_of(a, wk.b);
+  const int row0 = wk.qt * 16;
+  const int vis = visible(a, len, nq, row0 + col);
+  U4 qf[kStep];
+  {
     const uint16_t* p =
-        (const uint16_t*)a.q.data +
-        (vis[n] ? b * a.q.stride_b + (int64_t)t * a.q.stride_t +
-                      (int64_t)(h * a.group + r % a.group) * a.q.stride_h +
-                      quad * (D / 4)
-                : 0);
+        q_row(a, wk.b, wk.h, vis ? row0 + col : 0) + quad * (D / 4);
 #pragma unroll
-    for (int i = 0; i < kStep; ++i)
-      qf[n][i] = load_q8(p + 8 * i, a.vec, vis[n] > 0);
-    most = max(most, vis[n]);
-    if (vis[n]) least = min(least, vis[n]);
+    for (int i = 0; i < kStep; ++i) qf[i] = load_q8(p + 8 * i, a.vec, vis > 0);
   }
+  int most = vis, least = vis ? vis : 0x7fffffff;
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) {
     most = max(most, __shfl_xor(most, o));
@@ -218,183 +408,293 @@ __global__ __launch_bounds__(64 * kWaves) void k_kv4_attend(AttendArgs a) {
   }
   most = __builtin_amdgcn_readfirstlane(most);
   least = __builtin_amdgcn_readfirstlane(least);
-
-  // This split's blocks.
   const int blocks = (most + kKvBlock - 1) / kKvBlock;
   const int per = (blocks + a.splits - 1) / a.splits;
-  const int first = split * per;
-  const int last = min(blocks, first + per);
+  const int first = wk.split * per + wave;
+  const int last = min(blocks, wk.split * per + per);
+
+  float m = kNegInf, l = 0.0f;
+  F4 o[kDt];
+#pragma unroll
+  for (int d = 0; d < kDt; ++d) o[d] = F4{0, 0, 0, 0};
+
+  each_block<Block<D, 16>>(a.c, wk.b, wk.h, KvLayout<D>::kBytes, first, last,
+                           [&](const Block<D, 16>& kb, int blk) {
+    share_scales(kb.vs, sc[wave]);
+    const int p0 = blk * kKvBlock + 16 * (quad / 2) + 4 * (quad % 2);
+    const bool edge = blk * kKvBlock + kKvBlock > least;
+    F4 s[2] = {F4{0, 0, 0, 0}, F4{0, 0, 0, 0}};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < kStep; ++i)
+        s[t] = mma16<kHalf>(widen<kHalf>(kb.k[t][i], kb.scale(t, i)), qf[i],
+                            s[t]);
+    F4 ls[2], rs[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int at = 16 * (quad / 2) + 4 * (quad % 2) + 8 * t;
+      ls[t] = *(const F4*)&sc[wave][at];
+      rs[t] = *(const F4*)&sc[wave][32 + at];
+    }
+    float y[8];
+    float top = kNegInf;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      y[j] = __builtin_fmaf(s[j / 4][j % 4], a.scale, ls[j / 4][j % 4]);
+      if (edge && p0 + 8 * (j / 4) + j % 4 >= vis) y[j] = kNegInf;
+      top = fmaxf(top, y[j]);
+    }
+    if (__any(top > m + kSlack)) {
+      const float f = follow<16>(top, &m);
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < kDt; ++d) o[d] *= f;
+    }
+    const float mu = m == kNegInf ? 0.0f : m;
+    float w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      w[j] = __builtin_amdgcn_exp2f(y[j] - mu);
+      l = __builtin_fmaf(w[j], rs[j / 4][j % 4], l);
+    }
+    const U4 pf = {pack_half(w[0], w[1]), pack_half(w[2], w[3]),
+                   pack_half(w[4], w[5]), pack_half(w[6], w[7])};
+#pragma unroll
+    for (int d = 0; d < kDt; ++d)
+      o[d] = mma16<true>(widen<true>(kb.v[d], 1.0f), pf, o[d]);
+  });
+
+  // Join the waves in LDS; 16 threads a row, D / 16 channels each.
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+#pragma unroll
+  for (int d = 0; d < kDt; ++d) *(F4*)&so[wave][col][d * 16 + quad * 4] = o[d];
+  if (quad == 0) {
+    sm[wave][col] = m;
+    sl[wave][col] = l;
+  }
+  __syncthreads();
+  const int row = threadIdx.x / 16, c0 = threadIdx.x % 16 * (D / 16);
+  float mx = kNegInf;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, sm[w][row]);
+  float f[kWaves], lt = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    f[w] = sm[w][row] == kNegInf ? 0.0f
+                                 : __builtin_amdgcn_exp2f(sm[w][row] - mx);
+    lt = __builtin_fmaf(f[w], sl[w][row], lt);
+  }
+  float x[D / 16];
+#pragma unroll
+  for (int c = 0; c < D / 16; ++c) {
+    x[c] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w)
+      x[c] = __builtin_fmaf(f[w], so[w][row][c0 + c], x[c]);
+  }
+  const bool see = visible(a, len, nq, row0 + row) > 0 && lt != 0.0f;
+  put_row<kHalf>(a, wk, D, 16, row, row0 + row, see, mx, lt, c0, x);
+}
+
+// 32 NQ query rows a workgroup: verification steps and prompts.  The query rows
+// lie in LDS in the order of the matrix instruction's operand; every wave holds
+// O of all of them.
+template <int D, bool kHalf, int NQ>
+__global__ __launch_bounds__(64 * kWaves, D * NQ >= 256 ? 1 : 2)
+void k_kv4_attend32(AttendArgs a) {
+  constexpr int kRows = 32 * NQ;
+  constexpr int kStep = D / 16;
+  constexpr int kDt = D / 32;
+  const Work wk = work_of(a);
+  if (!wk.any) return;
+  const int lane = lane_id();
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int col = lane % 32, h2 = lane / 32;
+  constexpr int kJoin = kWaves * 32 * (64 + 4) * 4;
+  constexpr int kQ = kRows * D * 2;
+  __shared__ __align__(16) char pool[kJoin > kQ ? kJoin : kQ];
+  __shared__ float sm[kWaves][32], sl[kWaves][32];
+  __shared__ float sc[kWaves][64];
+  U4* sq = (U4*)pool;
+
+  const int64_t len = kv_len_of(a, wk.b);
+  const int64_t nq = q_len_of(a, wk.b);
+  const int row0 = wk.qt * kRows;
+  for (int e = threadIdx.x; e < kRows * (D / 8); e += 64 * kWaves) {
+    // operand (tile, step, lane): channels (lane / 32) D / 2 + 8 step
+    const int n = e / (kStep * 64), i = e / 64 % kStep, ln = e % 64;
+    const int r = row0 + 32 * n + ln % 32;
+    const bool live = visible(a, len, nq, r) > 0;
+    sq[e] = load_q8(q_row(a, wk.b, wk.h, live ? r : 0) + ln / 32 * (D / 2) +
+                        8 * i,
+                    a.vec, live);
+  }
+  int vis[NQ];
+  int most = 0, least = 0x7fffffff;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    vis[n] = visible(a, len, nq, row0 + 32 * n + col);
+    most = max(most, vis[n]);
+    if (vis[n]) least = min(least, vis[n]);
+  }
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    most = max(most, __shfl_xor(most, o));
+    least = min(least, __shfl_xor(least, o));
+  }
+  most = __builtin_amdgcn_readfirstlane(most);
+  least = __builtin_amdgcn_readfirstlane(least);
+  const int blocks = (most + kKvBlock - 1) / kKvBlock;
+  const int per = (blocks + a.splits - 1) / a.splits;
+  const int first = wk.split * per + wave;
+  const int last = min(blocks, wk.split * per + per);
+  __syncthreads();
 
   float m[NQ], l[NQ];
-  F4 o[NQ][kDt];
+  F16 o[NQ][kDt];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     m[n] = kNegInf;
     l[n] = 0.0f;
 #pragma unroll
-    for (int d = 0; d < kDt; ++d) o[n][d] = F4{0, 0, 0, 0};
+    for (int d = 0; d < kDt; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[n][d][r] = 0.0f;
   }
 
-  for (int blk = first + wave; blk < last; blk += kWaves) {
-    const char* base = kv_block<D>(a.c, b, h, blk);
-    if (!base) continue;
-    Block<D> kb;
-    load_block<D>(base, kb);
-    const int p0 = blk * kKvBlock + 16 * (quad / 2) + 4 * (quad % 2);
+  each_block<Block<D, 32>>(a.c, wk.b, wk.h, KvLayout<D>::kBytes, first, last,
+                           [&](const Block<D, 32>& kb, int blk) {
+    share_scales(kb.vs, sc[wave]);
+    const int p0 = blk * kKvBlock + 4 * h2;
     const bool edge = blk * kKvBlock + kKvBlock > least;
-    F4 s[NQ][2];
+    F16 s[NQ];
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) s[n][0] = s[n][1] = F4{0, 0, 0, 0};
+    for (int n = 0; n < NQ; ++n)
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+      for (int r = 0; r < 16; ++r) s[n][r] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kStep; ++i) {
-        uint32_t sb = kb.ks[t];
-        if (D == 256) sb = i < kStep / 2 ? sb & 255u : sb >> 8;
-        // the conversion takes the exponent alone: 255 is NaN
-        const U4 kf = widen<kHalf>(kb.k[t][i], __uint_as_float(sb << 23));
+    for (int i = 0; i < kStep; ++i) {
+      const U4 kf = widen<kHalf>(kb.k[i], kb.scale(i));
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) s[n][t] = mma<kHalf>(kf, qf[n][i], s[n][t]);
-      }
+      for (int n = 0; n < NQ; ++n)
+        s[n] = mma32<kHalf>(kf, sq[(n * kStep + i) * 64 + lane], s[n]);
     }
-    float ls[8], rs[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      ls[j] = __builtin_amdgcn_logf(kb.vs[j]);
-      // Finite whatever the scale: a row that does not see a token (of a NaN,
-      // or past the end, where a block holds anything) multiplies it by zero,
-      // and one that sees a NaN has it from ls.
-      rs[j] = fminf(fmaxf(__builtin_amdgcn_rcpf(kb.vs[j]), 0.0f), 0x1p101f);
-    }
-    U4 pf[NQ];
+    U4 pf[NQ][2];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      float y[8];
       float top = kNegInf;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        y[j] = __builtin_fmaf(s[n][j / 4][j % 4], a.scale, ls[j]);
-        if (edge && p0 + 8 * (j / 4) + j % 4 >= vis[n]) y[j] = kNegInf;
-        top = fmaxf(top, y[j]);
+      for (int g = 0; g < 4; ++g) {
+        const F4 ls = *(const F4*)&sc[wave][8 * g + 4 * h2];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float y = __builtin_fmaf(s[n][4 * g + r], a.scale, ls[r]);
+          if (edge && p0 + 8 * g + r >= vis[n]) y = kNegInf;
+          s[n][4 * g + r] = y;
+          top = fmaxf(top, y);
+        }
       }
       if (__any(top > m[n] + kSlack)) {
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float mn = fmaxf(m[n], top);
-        const float f = mn == m[n] ? 1.0f : __builtin_amdgcn_exp2f(m[n] - mn);
-        m[n] = mn;
+        const float f = follow<32>(top, &m[n]);
         l[n] *= f;
 #pragma unroll
         for (int d = 0; d < kDt; ++d) o[n][d] *= f;
       }
       const float mu = m[n] == kNegInf ? 0.0f : m[n];
-      float w[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        w[j] = __builtin_amdgcn_exp2f(y[j] - mu);
-        l[n] = __builtin_fmaf(w[j], rs[j], l[n]);
+      for (int g = 0; g < 4; ++g) {
+        const F4 rs = *(const F4*)&sc[wave][32 + 8 * g + 4 * h2];
+        float w[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          w[r] = __builtin_amdgcn_exp2f(s[n][4 * g + r] - mu);
+          l[n] = __builtin_fmaf(w[r], rs[r], l[n]);
+        }
+        pf[n][g / 2][g % 2 * 2] = pack_half(w[0], w[1]);
+        pf[n][g / 2][g % 2 * 2 + 1] = pack_half(w[2], w[3]);
       }
-      pf[n] = U4{pack_half(w[0], w[1]), pack_half(w[2], w[3]),
-                 pack_half(w[4], w[5]), pack_half(w[6], w[7])};
     }
 #pragma unroll
-    for (int d = 0; d < kDt; ++d) {
-      const U4 vf = widen<true>(kb.v[d], 1.0f);
+    for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) o[n][d] = mma<true>(vf, pf[n], o[n][d]);
-    }
-  }
+      for (int d = 0; d < kDt; ++d) {
+        const U4 vf = widen<true>(kb.v[s2][d], 1.0f);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) o[n][d] = mma32<true>(vf, pf[n][s2], o[n][d]);
+      }
+  });
 
-  // Join the waves in LDS, one tile of rows at a time.
-  __shared__ float so[kWaves][kTile][D + 4];
-  __shared__ float sm[kWaves][kTile], sl[kWaves][kTile];
+  // Join the waves in LDS, 32 rows and 64 channels at a time: 8 threads a row.
+  float(*so)[32][64 + 4] = (float(*)[32][64 + 4])pool;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    l[n] += __shfl_xor(l[n], 16);
     l[n] += __shfl_xor(l[n], 32);
-    if (n) __syncthreads();
 #pragma unroll
-    for (int d = 0; d < kDt; ++d)
-      *(F4*)&so[wave][col][d * 16 + quad * 4] = o[n][d];
-    if (quad == 0) {
-      sm[wave][col] = m[n];
-      sl[wave][col] = l[n];
-    }
-    __syncthreads();
-    // 16 threads a row, D / 16 channels each
-    const int row = threadIdx.x / 16, c0 = threadIdx.x % 16 * (D / 16);
-    const int r = (qt * NQ + n) * kTile + row;
-    float mx = kNegInf;
+    for (int g = 0; g < D / 64; ++g) {
+      __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, sm[w][row]);
-    float f[kWaves], lt = 0.0f;
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      f[w] = sm[w][row] == kNegInf
-                 ? 0.0f
-                 : __builtin_amdgcn_exp2f(sm[w][row] - mx);
-      lt = __builtin_fmaf(f[w], sl[w][row], lt);
-    }
-    float x[D / 16];
-#pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
-      x[c] = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w)
-        x[c] = __builtin_fmaf(f[w], so[w][row][c0 + c], x[c]);
-    }
-    // What a row without visible positions gathered counts for nothing.
-    const int t = r / a.group;
-    const bool see = r < a.rows && t < nq && len - nq + t + 1 > 0 && lt != 0.0f;
-    if (a.splits == 1) {
-      if (r < a.rows) {
-        const float inv = see ? 1.0f / lt : 0.0f;
-        uint32_t* out =
-            (uint32_t*)(a.out +
-                        ((b * a.tokens + t) * a.q_heads + h * a.group +
-                         r % a.group) * D + c0);
-#pragma unroll
-        for (int c = 0; c < D / 16; c += 2)
-          out[c / 2] = see ? from_float16b<kHalf>(x[c] * inv) |
-                                 from_float16b<kHalf>(x[c + 1] * inv) << 16
-                           : 0u;
+        for (int r = 0; r < 4; ++r)
+          // result rows 8 r + 4 h2 ..: channel tile 2 (r / 2) + t of the 64
+          *(F4*)&so[wave][col][(2 * (r / 2) + t) * 16 + r % 2 * 8 + 4 * h2] =
+              F4{o[n][2 * g + t][4 * r], o[n][2 * g + t][4 * r + 1],
+                 o[n][2 * g + t][4 * r + 2], o[n][2 * g + t][4 * r + 3]};
+      if (h2 == 0) {
+        sm[wave][col] = m[n];
+        sl[wave][col] = l[n];
       }
-    } else {
-      float* p = a.part +
-                 ((((b * a.c.heads + h) * a.q_tiles + qt) * a.splits + split) *
-                      kRows + n * kTile + row) * (D + 2);
+      __syncthreads();
+      const int row = threadIdx.x / 8, c0 = threadIdx.x % 8 * 8;
+      float mx = kNegInf;
 #pragma unroll
-      for (int c = 0; c < D / 16; ++c) p[2 + c0 + c] = x[c];
-      if (threadIdx.x % 16 == 0) {
-        p[0] = see ? mx : kNegInf;
-        p[1] = lt;
+      for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, sm[w][row]);
+      float f[kWaves], lt = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        f[w] = sm[w][row] == kNegInf
+                   ? 0.0f
+                   : __builtin_amdgcn_exp2f(sm[w][row] - mx);
+        lt = __builtin_fmaf(f[w], sl[w][row], lt);
       }
+      float x[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        x[c] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w)
+          x[c] = __builtin_fmaf(f[w], so[w][row][c0 + c], x[c]);
+      }
+      const int r = row0 + 32 * n + row;
+      const bool see = visible(a, len, nq, r) > 0 && lt != 0.0f;
+      put_row<kHalf>(a, wk, D, kRows, 32 * n + row, r, see, mx, lt, 64 * g + c0,
+                     x);
     }
   }
 }
 
 // Joins the splits of one query row and head: one workgroup of D threads.
-template <int D, bool kHalf, int NQ>
-__global__ __launch_bounds__(D) void k_kv4_join(AttendArgs a) {
-  constexpr int kRows = kTile * NQ;
+template <int D, bool kHalf>
+__global__ __launch_bounds__(D) void k_kv4_join(AttendArgs a, int rows_tile) {
   const int64_t b = blockIdx.z;
   const int h = blockIdx.y;
   const int r = blockIdx.x;
-  const int qt = r / kRows;
   const int c = threadIdx.x;
-  const float* p = a.part +
-                   (((b * a.c.heads + h) * a.q_tiles + qt) * a.splits * kRows +
-                    r % kRows) * (D + 2);
-  constexpr int64_t kNext = (int64_t)kRows * (D + 2);
+  const float* p =
+      a.part + (((b * a.c.heads + h) * a.q_tiles + r / rows_tile) * a.splits *
+                    rows_tile + r % rows_tile) * (D + 2);
+  const int64_t next = (int64_t)rows_tile * (D + 2);
   float mx = kNegInf;
-  for (int s = 0; s < a.splits; ++s) mx = fmaxf(mx, p[s * kNext]);
+  for (int s = 0; s < a.splits; ++s) mx = fmaxf(mx, p[s * next]);
   float lt = 0.0f, x = 0.0f;
   for (int s = 0; s < a.splits; ++s) {
-    const float m = p[s * kNext];
+    const float m = p[s * next];
     if (m == kNegInf) continue;
     const float f = __builtin_amdgcn_exp2f(m - mx);
-    lt = __builtin_fmaf(f, p[s * kNext + 1], lt);
-    x = __builtin_fmaf(f, p[s * kNext + 2 + c], x);
+    lt = __builtin_fmaf(f, p[s * next + 1], lt);
+    x = __builtin_fmaf(f, p[s * next + 2 + c], x);
   }
   const int t = r / a.group;
   a.out[((b * a.tokens + t) * a.q_heads + h * a.group + r % a.group) * D + c] =
@@ -402,7 +702,8 @@ __global__ __launch_bounds__(D) void k_kv4_join(AttendArgs a) {
 }
 
 struct Plan {
-  int nq, q_tiles, splits;
+  int rows_tile;  // query rows of a workgroup
+  int q_tiles, splits;
   size_t bytes;
 };
 
@@ -410,37 +711,40 @@ Plan plan_for(const sfx_kv4* c, int64_t batch, int64_t tokens,
               int64_t q_heads) {
   Plan p;
   const int64_t rows = tokens * (q_heads / c->heads);
-  p.nq = rows > kTile ? 2 : 1;
-  p.q_tiles = (int)((rows + kTile * p.nq - 1) / (kTile * p.nq));
+  p.rows_tile = rows <= 16 ? 16 : 32;
+  p.q_tiles = (int)((rows + p.rows_tile - 1) / p.rows_tile);
   const int64_t wgs = batch * c->heads * p.q_tiles;
   const int64_t blocks = c->table_width * c->page_size / kKvBlock;
   int64_t s = wgs > 0 ? 1024 / wgs : 1;
   s = std::min<int64_t>(s, (blocks + 15) / 16);
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(s, 128));
   p.bytes = p.splits == 1 ? 0
-                          : (size_t)wgs * p.splits * kTile * p.nq *
+                          : (size_t)wgs * p.splits * p.rows_tile *
                                 (c->head_dim + 2) * 4;
   return p;
 }
 
-template <int D, bool kHalf, int NQ>
-int launch(AttendArgs& a, int64_t batch, hipStream_t stream) {
-  hipLaunchKernelGGL((k_kv4_attend<D, kHalf, NQ>),
-                     dim3((unsigned)(a.splits * a.q_tiles),
-                          (unsigned)a.c.heads, (unsigned)batch),
-                     dim3(64 * kWaves), 0, stream, a);
-  if (a.splits > 1)
-    hipLaunchKernelGGL((k_kv4_join<D, kHalf, NQ>),
-                       dim3((unsigned)a.rows, (unsigned)a.c.heads,
-                            (unsigned)batch),
-                       dim3(D), 0, stream, a);
-  return (int)hipGetLastError();
-}
-
 template <int D, bool kHalf>
-int launch_nq(AttendArgs& a, int nq, int64_t batch, hipStream_t stream) {
-  return nq == 1 ? launch<D, kHalf, 1>(a, batch, stream)
-                 : launch<D, kHalf, 2>(a, batch, stream);
+int launch(AttendArgs& a, int rows_tile, hipStream_t stream) {
+  const int64_t items = (a.batch * a.c.heads * a.splits + 7) / 8 * 8;
+  if (items * a.q_tiles >= (int64_t(1) << 32) / (64 * kWaves))
+    return SFX_EINVAL;  // more threads than a grid takes
+  const dim3 grid((unsigned)(items * a.q_tiles));
+  const dim3 block(64 * kWaves);
+  if (rows_tile == 16)
+    hipLaunchKernelGGL((k_kv4_attend16<D, kHalf>), grid, block, 0, stream, a);
+  else if (rows_tile == 32)
+    hipLaunchKernelGGL((k_kv4_attend32<D, kHalf, 1>), grid, block, 0, stream,
+                       a);
+  else
+    hipLaunchKernelGGL((k_kv4_attend32<D, kHalf, D == 256 ? 1 : 2>), grid,
+                       block, 0, stream, a);
+  if (a.splits > 1)
+    hipLaunchKernelGGL((k_kv4_join<D, kHalf>),
+                       dim3((unsigned)a.rows, (unsigned)a.c.heads,
+                            (unsigned)a.batch),
+                       dim3(D), 0, stream, a, rows_tile);
+  return (int)hipGetLastError();
 }
 
 bool shapes_ok(const sfx_kv4* c, int64_t batch, int64_t tokens,
@@ -496,16 +800,17 @@ extern "C" int sfx_kv4_attend(const sfx_kv4* cache, const sfx_heads* q,
   a.scale = scale * 1.44269504088896340736f;
   a.out = (uint16_t*)out;
   a.part = (float*)workspace;
+  a.batch = batch;
   const bool half = cache->dtype == SFX_F16;
   switch (cache->head_dim) {
     case 64:
-      return half ? launch_nq<64, true>(a, p.nq, batch, stream)
-                  : launch_nq<64, false>(a, p.nq, batch, stream);
+      return half ? launch<64, true>(a, p.rows_tile, stream)
+                  : launch<64, false>(a, p.rows_tile, stream);
     case 128:
-      return half ? launch_nq<128, true>(a, p.nq, batch, stream)
-                  : launch_nq<128, false>(a, p.nq, batch, stream);
+      return half ? launch<128, true>(a, p.rows_tile, stream)
+                  : launch<128, false>(a, p.rows_tile, stream);
     default:
-      return half ? launch_nq<256, true>(a, p.nq, batch, stream)
-                  : launch_nq<256, false>(a, p.nq, batch, stream);
+      return half ? launch<256, true>(a, p.rows_tile, stream)
+                  : launch<256, false>(a, p.rows_tile, stream);
   }
 }
