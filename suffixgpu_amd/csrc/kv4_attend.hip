@@ -129,14 +129,14 @@ struct Block<D, 16> {
   uint32_t v[D / 16];     // a word of tokens for each 16 channels
   float vs;               // scale of token lane % 32's values
 
-  __device__ __forceinline__ void load(const char* base) {
+  __device__ __forceinline__ void load_k(const char* base) {
     using L = KvLayout<D>;
     const int lane = lane_id();
     const int i = lane % 16, quad = lane / 16;
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
       const int t = 16 * (i / 8) + 8 * a + i % 8;
-      const char* p = base + t * (D / 2) + quad * (D / 8);
+      const char* p = base + (uint32_t)(t * (D / 2) + quad * (D / 8));
       if (D == 64) {
         const uint2 w = *(const uint2*)p;
         k[a][0] = w.x;
@@ -151,21 +151,25 @@ struct Block<D, 16> {
           k[a][4 * u + 3] = w.w;
         }
       }
-      const uint8_t* s = (const uint8_t*)(base + L::kScale) + t * (D / 32);
-      if (D == 256)
-        ks[a] = *(const uint16_t*)(s + 2 * quad);
-      else
-        ks[a] = s[D == 64 ? quad / 2 : quad];
+      const char* s = base + (uint32_t)(L::kScale + t * (D / 32) +
+                                        (D == 256 ? 2 * quad
+                                                  : (D == 64 ? quad / 2 : quad)));
+      ks[a] = D == 256 ? *(const uint16_t*)s : *(const uint8_t*)s;
     }
+    vs = *(const float*)(base + (uint32_t)(L::kVScale + lane % 32 * 4));
+  }
+  __device__ __forceinline__ void load_v(const char* base) {
+    using L = KvLayout<D>;
+    const int lane = lane_id();
 #pragma unroll
     for (int g = 0; g < D / 64; ++g) {
-      const uint4 w = *(const uint4*)(base + L::kValue + (g * 64 + lane) * 16);
+      const uint4 w = *(const uint4*)(
+          base + (uint32_t)(L::kValue + (g * 64 + lane) * 16));
       v[4 * g] = w.x;
       v[4 * g + 1] = w.y;
       v[4 * g + 2] = w.z;
       v[4 * g + 3] = w.w;
     }
-    vs = ((const float*)(base + L::kVScale))[lane % 32];
   }
   // Scale of the channels of matrix step i in tile a.  The conversion takes
   // its exponent alone, all ones is a NaN.
@@ -183,11 +187,12 @@ struct Block<D, 32> {
   uint32_t v[2][D / 32];  // by step of 16 tokens, then 16 channels
   float vs;
 
-  __device__ __forceinline__ void load(const char* base) {
+  __device__ __forceinline__ void load_k(const char* base) {
     using L = KvLayout<D>;
     const int lane = lane_id();
     const int t = lane % 32, h = lane / 32;
-    const uint4* p = (const uint4*)(base + t * (D / 2) + h * (D / 4));
+    const uint4* p =
+        (const uint4*)(base + (uint32_t)(t * (D / 2) + h * (D / 4)));
 #pragma unroll
     for (int u = 0; u < D / 64; ++u) {
       const uint4 w = p[u];
@@ -196,20 +201,26 @@ struct Block<D, 32> {
       k[4 * u + 2] = w.z;
       k[4 * u + 3] = w.w;
     }
-    const uint8_t* s = (const uint8_t*)(base + L::kScale) + t * (D / 32);
-    ks = D == 64 ? s[h]
-                 : (D == 128 ? ((const uint16_t*)s)[h] : ((const uint32_t*)s)[h]);
+    const char* s =
+        base + (uint32_t)(L::kScale + t * (D / 32) + h * (D / 64));
+    ks = D == 64 ? *(const uint8_t*)s
+                 : (D == 128 ? *(const uint16_t*)s : *(const uint32_t*)s);
+    vs = *(const float*)(base + (uint32_t)(L::kVScale + t * 4));
+  }
+  __device__ __forceinline__ void load_v(const char* base) {
+    using L = KvLayout<D>;
+    const int lane = lane_id(), h = lane / 32;
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
       for (int g = 0; g < D / 64; ++g) {
-        const uint2 w = *(const uint2*)(base + L::kValue +
-                                        ((g * 4 + 2 * s2 + h) * 16 + lane % 16) *
-                                            16 + lane / 16 % 2 * 8);
+        const uint2 w = *(const uint2*)(
+            base + (uint32_t)(L::kValue +
+                              ((g * 4 + 2 * s2 + h) * 16 + lane % 16) * 16 +
+                              lane / 16 % 2 * 8));
         v[s2][2 * g] = w.x;
         v[s2][2 * g + 1] = w.y;
       }
-    vs = ((const float*)(base + L::kVScale))[t];
   }
   __device__ __forceinline__ float scale(int i) const {
     return __uint_as_float((ks >> (8 * (i / 4)) & 255u) << 23);
@@ -293,11 +304,13 @@ __device__ __forceinline__ void share_scales(float vs, float* lds) {
   asm volatile("" ::: "memory");
 }
 
-// body(block, index) for blocks first, first + kWaves, ... below last of row b
-// and KV head h, by one wave for which all of these are the same.  A block's
-// loads are under way while the one before is worked on (two sets of registers
-// in turn: a copy from one to the other would wait for the loads), and its page
-// id while the one before that is.  Blocks without a page are left out.
+// Goes through blocks first, first + kWaves, ... below last of row b and KV head
+// h, by one wave for which all of these are the same: body(block, index, kdone,
+// vdone) calls kdone() when it has used the keys and vdone() when it has used
+// the values, which load the next block's into the same registers.  A second
+// set for the loads under way would cost a wave in three; issued this early
+// they are as well hidden.  A block's page id is read (as a scalar) one block
+// ahead of that.  Blocks without a page are left out.
 template <class B, class F>
 __device__ __forceinline__ void each_block(const KvView& c, int64_t b, int h,
                                            int bytes, int first, int last,
@@ -306,28 +319,29 @@ __device__ __forceinline__ void each_block(const KvView& c, int64_t b, int h,
   typedef const __attribute__((address_space(4))) int32_t* Ids;
   const Ids ids = (Ids)(uintptr_t)(c.table + b * c.table_stride);
   const int in_page = (1 << c.page_shift) - 1;
-  auto page = [&](int blk) { return blk < last ? ids[blk >> c.page_shift] : -1; };
+  auto page = [&](int blk) { return ids[min(blk, last - 1) >> c.page_shift]; };
   auto good = [&](int32_t id) { return id >= 0 && id < c.num_pages; };
+  // past the last block, and without a page: memory that is there
   auto at = [&](int32_t id, int blk) {
     return good(id) ? c.pages + ((((int64_t)id * c.heads + h) << c.page_shift) +
                                  (blk & in_page)) * bytes
                     : c.pages;
   };
-  B x, y;
-  int32_t idx = page(first), idy = page(first + kWaves);
-  x.load(at(idx, first));
-  for (int blk = first;; blk += 2 * kWaves) {
-    const int n1 = blk + kWaves, n2 = blk + 2 * kWaves;
-    if (n1 < last) y.load(at(idy, n1));
-    const int32_t id2 = page(n2);
-    if (good(idx)) body(x, blk);
-    if (n1 >= last) break;
-    if (n2 < last) x.load(at(id2, n2));
-    const int32_t id3 = page(n2 + kWaves);
-    if (good(idy)) body(y, n1);
-    if (n2 >= last) break;
-    idx = id2;
-    idy = id3;
+  B x;
+  int32_t id = page(first), id1 = page(first + kWaves);
+  x.load_k(at(id, first));
+  x.load_v(at(id, first));
+  for (int blk = first; blk < last; blk += kWaves) {
+    const char* next = at(id1, blk + kWaves);
+    const int32_t id2 = page(blk + 2 * kWaves);
+    if (good(id)) {
+      body(x, blk, [&]() { x.load_k(next); }, [&]() { x.load_v(next); });
+    } else {
+      x.load_k(next);
+      x.load_v(next);
+    }
+    id = id1;
+    id1 = id2;
   }
 }
 
@@ -376,7 +390,7 @@ __device__ __forceinline__ void put_row(const AttendArgs& a, const Work& w,
 
 // Up to 16 query rows a workgroup: single tokens, and small groups of drafts.
 template <int D, bool kHalf>
-__global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : (D == 128 ? 3 : 4))
+__global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 4)
 void k_kv4_attend16(AttendArgs a) {
   constexpr int kStep = D / 32;   // matrix instructions a score tile
   constexpr int kDt = D / 16;     // channel tiles
@@ -419,7 +433,8 @@ void k_kv4_attend16(AttendArgs a) {
   for (int d = 0; d < kDt; ++d) o[d] = F4{0, 0, 0, 0};
 
   each_block<Block<D, 16>>(a.c, wk.b, wk.h, KvLayout<D>::kBytes, first, last,
-                           [&](const Block<D, 16>& kb, int blk) {
+                           [&](Block<D, 16>& kb, int blk, auto kdone,
+                               auto vdone) {
     share_scales(kb.vs, sc[wave]);
     const int p0 = blk * kKvBlock + 16 * (quad / 2) + 4 * (quad % 2);
     const bool edge = blk * kKvBlock + kKvBlock > least;
@@ -430,6 +445,7 @@ void k_kv4_attend16(AttendArgs a) {
       for (int i = 0; i < kStep; ++i)
         s[t] = mma16<kHalf>(widen<kHalf>(kb.k[t][i], kb.scale(t, i)), qf[i],
                             s[t]);
+    kdone();
     F4 ls[2], rs[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -442,9 +458,15 @@ void k_kv4_attend16(AttendArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       y[j] = __builtin_fmaf(s[j / 4][j % 4], a.scale, ls[j / 4][j % 4]);
-      if (edge && p0 + 8 * (j / 4) + j % 4 >= vis) y[j] = kNegInf;
-      top = fmaxf(top, y[j]);
     }
+    if (edge) {
+      asm volatile("");  // a branch: most blocks have no edge
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (p0 + 8 * (j / 4) + j % 4 >= vis) y[j] = kNegInf;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, y[j]);
     if (__any(top > m + kSlack)) {
       const float f = follow<16>(top, &m);
       l *= f;
@@ -463,6 +485,7 @@ void k_kv4_attend16(AttendArgs a) {
 #pragma unroll
     for (int d = 0; d < kDt; ++d)
       o[d] = mma16<true>(widen<true>(kb.v[d], 1.0f), pf, o[d]);
+    vdone();
   });
 
   // Join the waves in LDS; 16 threads a row, D / 16 channels each.
@@ -502,7 +525,7 @@ void k_kv4_attend16(AttendArgs a) {
 // lie in LDS in the order of the matrix instruction's operand; every wave holds
 // O of all of them.
 template <int D, bool kHalf, int NQ>
-__global__ __launch_bounds__(64 * kWaves, D * NQ >= 256 ? 1 : 2)
+__global__ __launch_bounds__(64 * kWaves, D * NQ >= 256 ? 2 : 3)
 void k_kv4_attend32(AttendArgs a) {
   constexpr int kRows = 32 * NQ;
   constexpr int kStep = D / 16;
@@ -565,7 +588,8 @@ void k_kv4_attend32(AttendArgs a) {
   }
 
   each_block<Block<D, 32>>(a.c, wk.b, wk.h, KvLayout<D>::kBytes, first, last,
-                           [&](const Block<D, 32>& kb, int blk) {
+                           [&](Block<D, 32>& kb, int blk, auto kdone,
+                               auto vdone) {
     share_scales(kb.vs, sc[wave]);
     const int p0 = blk * kKvBlock + 4 * h2;
     const bool edge = blk * kKvBlock + kKvBlock > least;
@@ -581,6 +605,7 @@ void k_kv4_attend32(AttendArgs a) {
       for (int n = 0; n < NQ; ++n)
         s[n] = mma32<kHalf>(kf, sq[(n * kStep + i) * 64 + lane], s[n]);
     }
+    kdone();
     U4 pf[NQ][2];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
@@ -589,13 +614,17 @@ void k_kv4_attend32(AttendArgs a) {
       for (int g = 0; g < 4; ++g) {
         const F4 ls = *(const F4*)&sc[wave][8 * g + 4 * h2];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float y = __builtin_fmaf(s[n][4 * g + r], a.scale, ls[r]);
-          if (edge && p0 + 8 * g + r >= vis[n]) y = kNegInf;
-          s[n][4 * g + r] = y;
-          top = fmaxf(top, y);
-        }
+        for (int r = 0; r < 4; ++r)
+          s[n][4 * g + r] = __builtin_fmaf(s[n][4 * g + r], a.scale, ls[r]);
       }
+      if (edge) {
+        asm volatile("");  // a branch: most blocks have no edge
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (p0 + r / 4 * 8 + r % 4 >= vis[n]) s[n][r] = kNegInf;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
       if (__any(top > m[n] + kSlack)) {
         const float f = follow<32>(top, &m[n]);
         l[n] *= f;
@@ -624,6 +653,7 @@ void k_kv4_attend32(AttendArgs a) {
 #pragma unroll
         for (int n = 0; n < NQ; ++n) o[n][d] = mma32<true>(vf, pf[n][s2], o[n][d]);
       }
+    vdone();
   });
 
   // Join the waves in LDS, 32 rows and 64 channels at a time: 8 threads a row.
