@@ -45,7 +45,8 @@ struct AttendArgs {
   int q_heads;
   int rows;        // tokens * group
   int q_tiles;     // row groups of a workgroup
-  int splits;
+  int splits;      // of the longest row that the table can hold
+  int chunk;       // blocks of a split
   int64_t batch;
   int vec;
   const void* kv_len;
@@ -122,21 +123,29 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b) {
 template <int D, int kTile>
 struct Block;
 
+// A lane's place in a block is a register, what is the same for all lanes an
+// immediate of the load.
 template <int D>
 struct Block<D, 16> {
   uint32_t k[2][D / 32];  // 8 channels a word
   uint32_t ks[2];         // scale bytes of the lane's channels
   uint32_t v[D / 16];     // a word of tokens for each 16 channels
   float vs;               // scale of token lane % 32's values
+  uint32_t at_k, at_ks, at_v, at_vs;
 
+  using L = KvLayout<D>;
+  __device__ __forceinline__ Block() {
+    const int lane = lane_id(), i = lane % 16, quad = lane / 16;
+    const int t = 16 * (i / 8) + i % 8;
+    at_k = t * (D / 2) + quad * (D / 8);
+    at_ks = t * (D / 32) + (D == 256 ? 2 * quad : (D == 64 ? quad / 2 : quad));
+    at_v = lane * 16;
+    at_vs = lane % 32 * 4;
+  }
   __device__ __forceinline__ void load_k(const char* base) {
-    using L = KvLayout<D>;
-    const int lane = lane_id();
-    const int i = lane % 16, quad = lane / 16;
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
-      const int t = 16 * (i / 8) + 8 * a + i % 8;
-      const char* p = base + (uint32_t)(t * (D / 2) + quad * (D / 8));
+      const char* p = base + at_k + 8 * a * (D / 2);
       if (D == 64) {
         const uint2 w = *(const uint2*)p;
         k[a][0] = w.x;
@@ -151,20 +160,16 @@ struct Block<D, 16> {
           k[a][4 * u + 3] = w.w;
         }
       }
-      const char* s = base + (uint32_t)(L::kScale + t * (D / 32) +
-                                        (D == 256 ? 2 * quad
-                                                  : (D == 64 ? quad / 2 : quad)));
+      const char* s = base + at_ks + (L::kScale + 8 * a * (D / 32));
       ks[a] = D == 256 ? *(const uint16_t*)s : *(const uint8_t*)s;
     }
-    vs = *(const float*)(base + (uint32_t)(L::kVScale + lane % 32 * 4));
+    vs = *(const float*)(base + at_vs + L::kVScale);
   }
   __device__ __forceinline__ void load_v(const char* base) {
-    using L = KvLayout<D>;
-    const int lane = lane_id();
 #pragma unroll
     for (int g = 0; g < D / 64; ++g) {
-      const uint4 w = *(const uint4*)(
-          base + (uint32_t)(L::kValue + (g * 64 + lane) * 16));
+      const uint4 w =
+          *(const uint4*)(base + at_v + (L::kValue + g * 64 * 16));
       v[4 * g] = w.x;
       v[4 * g + 1] = w.y;
       v[4 * g + 2] = w.z;
@@ -186,13 +191,18 @@ struct Block<D, 32> {
   uint32_t ks;
   uint32_t v[2][D / 32];  // by step of 16 tokens, then 16 channels
   float vs;
+  uint32_t at_k, at_ks, at_v, at_vs;
 
+  using L = KvLayout<D>;
+  __device__ __forceinline__ Block() {
+    const int lane = lane_id(), t = lane % 32, h = lane / 32;
+    at_k = t * (D / 2) + h * (D / 4);
+    at_ks = t * (D / 32) + h * (D / 64);
+    at_v = (h * 16 + lane % 16) * 16 + lane / 16 % 2 * 8;
+    at_vs = t * 4;
+  }
   __device__ __forceinline__ void load_k(const char* base) {
-    using L = KvLayout<D>;
-    const int lane = lane_id();
-    const int t = lane % 32, h = lane / 32;
-    const uint4* p =
-        (const uint4*)(base + (uint32_t)(t * (D / 2) + h * (D / 4)));
+    const uint4* p = (const uint4*)(base + at_k);
 #pragma unroll
     for (int u = 0; u < D / 64; ++u) {
       const uint4 w = p[u];
@@ -201,23 +211,18 @@ struct Block<D, 32> {
       k[4 * u + 2] = w.z;
       k[4 * u + 3] = w.w;
     }
-    const char* s =
-        base + (uint32_t)(L::kScale + t * (D / 32) + h * (D / 64));
+    const char* s = base + at_ks + L::kScale;
     ks = D == 64 ? *(const uint8_t*)s
                  : (D == 128 ? *(const uint16_t*)s : *(const uint32_t*)s);
-    vs = *(const float*)(base + (uint32_t)(L::kVScale + t * 4));
+    vs = *(const float*)(base + at_vs + L::kVScale);
   }
   __device__ __forceinline__ void load_v(const char* base) {
-    using L = KvLayout<D>;
-    const int lane = lane_id(), h = lane / 32;
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
       for (int g = 0; g < D / 64; ++g) {
-        const uint2 w = *(const uint2*)(
-            base + (uint32_t)(L::kValue +
-                              ((g * 4 + 2 * s2 + h) * 16 + lane % 16) * 16 +
-                              lane / 16 % 2 * 8));
+        const uint2 w = *(const uint2*)(base + at_v +
+                                        (L::kValue + (g * 4 + 2 * s2) * 256));
         v[s2][2 * g] = w.x;
         v[s2][2 * g + 1] = w.y;
       }
@@ -279,6 +284,29 @@ __device__ __forceinline__ int visible(const AttendArgs& a, int64_t len,
   const int t = r / a.group;
   const int64_t v = len - nq + t + 1;
   return r < a.rows && t < nq && v > 0 ? (int)v : 0;
+}
+
+// Splits of a row, and the blocks of one that rows of up to `most` visible
+// positions need.  A row is split by its length alone, into equal parts of at
+// most `chunk` blocks.
+struct Range {
+  int splits, first, last;
+};
+
+__device__ __forceinline__ int splits_of(const AttendArgs& a, int64_t len) {
+  const int blocks = (int)((len + kKvBlock - 1) / kKvBlock);
+  return max(1, (blocks + a.chunk - 1) / a.chunk);
+}
+
+__device__ __forceinline__ Range range_of(const AttendArgs& a, int64_t len,
+                                          int most, int split) {
+  const int blocks = (int)((len + kKvBlock - 1) / kKvBlock);
+  Range r;
+  r.splits = splits_of(a, len);
+  const int per = (blocks + r.splits - 1) / r.splits;
+  r.first = split * per;
+  r.last = min((most + kKvBlock - 1) / kKvBlock, r.first + per);
+  return r;
 }
 
 __device__ __forceinline__ const uint16_t* q_row(const AttendArgs& a,
@@ -364,9 +392,9 @@ template <bool kHalf, int N>
 __device__ __forceinline__ void put_row(const AttendArgs& a, const Work& w,
                                         int d, int rows_tile, int row, int r,
                                         bool see, float mx, float lt, int c0,
-                                        const float (&x)[N]) {
-  if (a.splits == 1) {
-    if (r >= a.rows) return;
+                                        const float (&x)[N], int splits) {
+  if (r >= a.rows) return;
+  if (splits == 1) {
     const float inv = see ? 1.0f / lt : 0.0f;
     uint32_t* out = (uint32_t*)(a.out + ((w.b * a.tokens + r / a.group) *
                                              a.q_heads +
@@ -379,11 +407,15 @@ __device__ __forceinline__ void put_row(const AttendArgs& a, const Work& w,
   } else {
     float* p = a.part + ((((w.b * a.c.heads + w.h) * a.q_tiles + w.qt) *
                               a.splits + w.split) * rows_tile + row) * (d + 2);
-#pragma unroll
-    for (int c = 0; c < N; ++c) p[2 + c0 + c] = x[c];
     if (c0 == 0) {
       p[0] = see ? mx : kNegInf;
       p[1] = lt;
+    }
+    if (!see) return;
+#pragma unroll
+    for (int c = 0; c < N; c += 2) {
+      typedef float F2 __attribute__((ext_vector_type(2)));
+      *(F2*)(p + 2 + c0 + c) = F2{x[c], x[c + 1]};
     }
   }
 }
@@ -422,10 +454,9 @@ void k_kv4_attend16(AttendArgs a) {
   }
   most = __builtin_amdgcn_readfirstlane(most);
   least = __builtin_amdgcn_readfirstlane(least);
-  const int blocks = (most + kKvBlock - 1) / kKvBlock;
-  const int per = (blocks + a.splits - 1) / a.splits;
-  const int first = wk.split * per + wave;
-  const int last = min(blocks, wk.split * per + per);
+  const Range rg = range_of(a, len, most, wk.split);
+  if (rg.splits <= wk.split) return;
+  const int first = rg.first + wave, last = rg.last;
 
   float m = kNegInf, l = 0.0f;
   F4 o[kDt];
@@ -518,16 +549,17 @@ void k_kv4_attend16(AttendArgs a) {
       x[c] = __builtin_fmaf(f[w], so[w][row][c0 + c], x[c]);
   }
   const bool see = visible(a, len, nq, row0 + row) > 0 && lt != 0.0f;
-  put_row<kHalf>(a, wk, D, 16, row, row0 + row, see, mx, lt, c0, x);
+  put_row<kHalf>(a, wk, D, 16, row, row0 + row, see, mx, lt, c0, x,
+                 rg.splits);
 }
 
-// 32 NQ query rows a workgroup: verification steps and prompts.  The query rows
+// 32 query rows a workgroup: verification steps and prompts.  The query rows
 // lie in LDS in the order of the matrix instruction's operand; every wave holds
 // O of all of them.
-template <int D, bool kHalf, int NQ>
-__global__ __launch_bounds__(64 * kWaves, D * NQ >= 256 ? 2 : 3)
+template <int D, bool kHalf>
+__global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3)
 void k_kv4_attend32(AttendArgs a) {
-  constexpr int kRows = 32 * NQ;
+  constexpr int kRows = 32;
   constexpr int kStep = D / 16;
   constexpr int kDt = D / 32;
   const Work wk = work_of(a);
@@ -546,22 +578,16 @@ void k_kv4_attend32(AttendArgs a) {
   const int64_t nq = q_len_of(a, wk.b);
   const int row0 = wk.qt * kRows;
   for (int e = threadIdx.x; e < kRows * (D / 8); e += 64 * kWaves) {
-    // operand (tile, step, lane): channels (lane / 32) D / 2 + 8 step
-    const int n = e / (kStep * 64), i = e / 64 % kStep, ln = e % 64;
-    const int r = row0 + 32 * n + ln % 32;
+    // operand (step, lane): channels (lane / 32) D / 2 + 8 step
+    const int i = e / 64, ln = e % 64;
+    const int r = row0 + ln % 32;
     const bool live = visible(a, len, nq, r) > 0;
     sq[e] = load_q8(q_row(a, wk.b, wk.h, live ? r : 0) + ln / 32 * (D / 2) +
                         8 * i,
                     a.vec, live);
   }
-  int vis[NQ];
-  int most = 0, least = 0x7fffffff;
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    vis[n] = visible(a, len, nq, row0 + 32 * n + col);
-    most = max(most, vis[n]);
-    if (vis[n]) least = min(least, vis[n]);
-  }
+  const int vis = visible(a, len, nq, row0 + col);
+  int most = vis, least = vis ? vis : 0x7fffffff;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     most = max(most, __shfl_xor(most, o));
@@ -569,23 +595,17 @@ void k_kv4_attend32(AttendArgs a) {
   }
   most = __builtin_amdgcn_readfirstlane(most);
   least = __builtin_amdgcn_readfirstlane(least);
-  const int blocks = (most + kKvBlock - 1) / kKvBlock;
-  const int per = (blocks + a.splits - 1) / a.splits;
-  const int first = wk.split * per + wave;
-  const int last = min(blocks, wk.split * per + per);
+  const Range rg = range_of(a, len, most, wk.split);
+  if (rg.splits <= wk.split) return;
+  const int first = rg.first + wave, last = rg.last;
   __syncthreads();
 
-  float m[NQ], l[NQ];
-  F16 o[NQ][kDt];
+  float m = kNegInf, l = 0.0f;
+  F16 o[kDt];
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    m[n] = kNegInf;
-    l[n] = 0.0f;
+  for (int d = 0; d < kDt; ++d)
 #pragma unroll
-    for (int d = 0; d < kDt; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[n][d][r] = 0.0f;
-  }
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
 
   each_block<Block<D, 32>>(a.c, wk.b, wk.h, KvLayout<D>::kBytes, first, last,
                            [&](Block<D, 32>& kb, int blk, auto kdone,
@@ -593,147 +613,178 @@ void k_kv4_attend32(AttendArgs a) {
     share_scales(kb.vs, sc[wave]);
     const int p0 = blk * kKvBlock + 4 * h2;
     const bool edge = blk * kKvBlock + kKvBlock > least;
-    F16 s[NQ];
+    F16 s;
 #pragma unroll
-    for (int n = 0; n < NQ; ++n)
+    for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+    // The queries' operands come from LDS kAhead steps before they are used:
+    // the matrix instructions would wait for each.
+    constexpr int kAhead = 4;
+    U4 qf[kAhead];
+    F4 ls[4], rs[4];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[n][r] = 0.0f;
+    for (int i = 0; i < kAhead; ++i) qf[i] = sq[i * 64 + lane];
 #pragma unroll
     for (int i = 0; i < kStep; ++i) {
-      const U4 kf = widen<kHalf>(kb.k[i], kb.scale(i));
+      __builtin_amdgcn_sched_barrier(0);
+      s = mma32<kHalf>(widen<kHalf>(kb.k[i], kb.scale(i)), qf[i % kAhead], s);
+      if (i + kAhead < kStep) qf[i % kAhead] = sq[(i + kAhead) * 64 + lane];
+      if (i == kStep - 2) {
 #pragma unroll
-      for (int n = 0; n < NQ; ++n)
-        s[n] = mma32<kHalf>(kf, sq[(n * kStep + i) * 64 + lane], s[n]);
+        for (int g = 0; g < 4; ++g)
+          ls[g] = *(const F4*)&sc[wave][8 * g + 4 * h2];
+      }
     }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      rs[g] = *(const F4*)&sc[wave][32 + 8 * g + 4 * h2];
     kdone();
-    U4 pf[NQ][2];
+    float top = kNegInf;
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      float top = kNegInf;
+    for (int r = 0; r < 16; ++r)
+      s[r] = __builtin_fmaf(s[r], a.scale, ls[r / 4][r % 4]);
+    if (edge) {
+      asm volatile("");  // a branch: most blocks have no edge
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const F4 ls = *(const F4*)&sc[wave][8 * g + 4 * h2];
+      for (int r = 0; r < 16; ++r)
+        if (p0 + r / 4 * 8 + r % 4 >= vis) s[r] = kNegInf;
+    }
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          s[n][4 * g + r] = __builtin_fmaf(s[n][4 * g + r], a.scale, ls[r]);
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
+    if (__any(top > m + kSlack)) {
+      const float f = follow<32>(top, &m);
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < kDt; ++d) o[d] *= f;
+    }
+    const float mu = m == kNegInf ? 0.0f : m;
+    U4 pf[2];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float w[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        w[r] = __builtin_amdgcn_exp2f(s[4 * g + r] - mu);
+        l = __builtin_fmaf(w[r], rs[g][r], l);
       }
-      if (edge) {
-        asm volatile("");  // a branch: most blocks have no edge
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (p0 + r / 4 * 8 + r % 4 >= vis[n]) s[n][r] = kNegInf;
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
-      if (__any(top > m[n] + kSlack)) {
-        const float f = follow<32>(top, &m[n]);
-        l[n] *= f;
-#pragma unroll
-        for (int d = 0; d < kDt; ++d) o[n][d] *= f;
-      }
-      const float mu = m[n] == kNegInf ? 0.0f : m[n];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const F4 rs = *(const F4*)&sc[wave][32 + 8 * g + 4 * h2];
-        float w[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          w[r] = __builtin_amdgcn_exp2f(s[n][4 * g + r] - mu);
-          l[n] = __builtin_fmaf(w[r], rs[r], l[n]);
-        }
-        pf[n][g / 2][g % 2 * 2] = pack_half(w[0], w[1]);
-        pf[n][g / 2][g % 2 * 2 + 1] = pack_half(w[2], w[3]);
-      }
+      pf[g / 2][g % 2 * 2] = pack_half(w[0], w[1]);
+      pf[g / 2][g % 2 * 2 + 1] = pack_half(w[2], w[3]);
     }
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
-      for (int d = 0; d < kDt; ++d) {
-        const U4 vf = widen<true>(kb.v[s2][d], 1.0f);
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) o[n][d] = mma32<true>(vf, pf[n][s2], o[n][d]);
-      }
+      for (int d = 0; d < kDt; ++d)
+        o[d] = mma32<true>(widen<true>(kb.v[s2][d], 1.0f), pf[s2], o[d]);
     vdone();
   });
 
-  // Join the waves in LDS, 32 rows and 64 channels at a time: 8 threads a row.
+  // Join the waves in LDS, 64 channels at a time: 8 threads a row.
   float(*so)[32][64 + 4] = (float(*)[32][64 + 4])pool;
+  l += __shfl_xor(l, 32);
+  const int row = threadIdx.x / 8, c0 = threadIdx.x % 8 * 8;
+  const bool queried = visible(a, len, nq, row0 + row) > 0;
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    l[n] += __shfl_xor(l[n], 32);
+  for (int g = 0; g < D / 64; ++g) {
+    __syncthreads();
 #pragma unroll
-    for (int g = 0; g < D / 64; ++g) {
-      __syncthreads();
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          // result rows 8 r + 4 h2 ..: channel tile 2 (r / 2) + t of the 64
-          *(F4*)&so[wave][col][(2 * (r / 2) + t) * 16 + r % 2 * 8 + 4 * h2] =
-              F4{o[n][2 * g + t][4 * r], o[n][2 * g + t][4 * r + 1],
-                 o[n][2 * g + t][4 * r + 2], o[n][2 * g + t][4 * r + 3]};
-      if (h2 == 0) {
-        sm[wave][col] = m[n];
-        sl[wave][col] = l[n];
-      }
-      __syncthreads();
-      const int row = threadIdx.x / 8, c0 = threadIdx.x % 8 * 8;
-      float mx = kNegInf;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, sm[w][row]);
-      float f[kWaves], lt = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        f[w] = sm[w][row] == kNegInf
-                   ? 0.0f
-                   : __builtin_amdgcn_exp2f(sm[w][row] - mx);
-        lt = __builtin_fmaf(f[w], sl[w][row], lt);
-      }
-      float x[8];
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        x[c] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w)
-          x[c] = __builtin_fmaf(f[w], so[w][row][c0 + c], x[c]);
-      }
-      const int r = row0 + 32 * n + row;
-      const bool see = visible(a, len, nq, r) > 0 && lt != 0.0f;
-      put_row<kHalf>(a, wk, D, kRows, 32 * n + row, r, see, mx, lt, 64 * g + c0,
-                     x);
+      for (int r = 0; r < 4; ++r)
+        // result rows 8 r + 4 h2 ..: channel tile 2 (r / 2) + t of the 64
+        *(F4*)&so[wave][col][(2 * (r / 2) + t) * 16 + r % 2 * 8 + 4 * h2] =
+            F4{o[2 * g + t][4 * r], o[2 * g + t][4 * r + 1],
+               o[2 * g + t][4 * r + 2], o[2 * g + t][4 * r + 3]};
+    if (h2 == 0) {
+      sm[wave][col] = m;
+      sl[wave][col] = l;
     }
+    __syncthreads();
+    float mx = kNegInf;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, sm[w][row]);
+    float f[kWaves], lt = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      f[w] = sm[w][row] == kNegInf ? 0.0f
+                                   : __builtin_amdgcn_exp2f(sm[w][row] - mx);
+      lt = __builtin_fmaf(f[w], sl[w][row], lt);
+    }
+    float x[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      x[c] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w)
+        x[c] = __builtin_fmaf(f[w], so[w][row][c0 + c], x[c]);
+    }
+    put_row<kHalf>(a, wk, D, kRows, row, row0 + row, queried && lt != 0.0f, mx,
+                   lt, 64 * g + c0, x, rg.splits);
   }
 }
 
-// Joins the splits of one query row and head: one workgroup of D threads.
+// Joins the splits of query rows: a wave per row and KV head.  A lane holds a
+// split's M and l, then D / 64 channels.
+constexpr int kMaxSplits = 64;
+
 template <int D, bool kHalf>
-__global__ __launch_bounds__(D) void k_kv4_join(AttendArgs a, int rows_tile) {
+__global__ __launch_bounds__(256) void k_kv4_join(AttendArgs a,
+                                                  int rows_tile) {
+  constexpr int C = D / 64;
   const int64_t b = blockIdx.z;
   const int h = blockIdx.y;
-  const int r = blockIdx.x;
-  const int c = threadIdx.x;
+  const int r = blockIdx.x * 4 + (int)(threadIdx.x / kWave);
+  const int lane = lane_id();
+  const int splits = splits_of(a, kv_len_of(a, b));
+  if (splits == 1 || r >= a.rows) return;
   const float* p =
       a.part + (((b * a.c.heads + h) * a.q_tiles + r / rows_tile) * a.splits *
                     rows_tile + r % rows_tile) * (D + 2);
   const int64_t next = (int64_t)rows_tile * (D + 2);
-  float mx = kNegInf;
-  for (int s = 0; s < a.splits; ++s) mx = fmaxf(mx, p[s * next]);
-  float lt = 0.0f, x = 0.0f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float m = p[s * next];
-    if (m == kNegInf) continue;
-    const float f = __builtin_amdgcn_exp2f(m - mx);
-    lt = __builtin_fmaf(f, p[s * next + 1], lt);
-    x = __builtin_fmaf(f, p[s * next + 2 + c], x);
+  float m = kNegInf, l = 0.0f;
+  if (lane < splits) {
+    m = p[lane * next];
+    l = p[lane * next + 1];
+  }
+  float mx = m;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+  const float f = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - mx);
+  float lt = f == 0.0f ? 0.0f : f * l;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) lt += __shfl_xor(lt, o);
+  float x[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) x[c] = 0.0f;
+  // parts of factor 0 were not written
+  uint64_t todo = ballot(f != 0.0f);
+  while (todo) {
+    float w[4], v[4][C];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int s = todo ? __builtin_ctzll(todo) : 0;
+      w[u] = todo ? __shfl(f, s) : 0.0f;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        v[u][c] = todo ? p[s * next + 2 + lane * C + c] : 0.0f;
+      todo &= todo - 1;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int c = 0; c < C; ++c) x[c] = __builtin_fmaf(w[u], v[u][c], x[c]);
   }
   const int t = r / a.group;
-  a.out[((b * a.tokens + t) * a.q_heads + h * a.group + r % a.group) * D + c] =
-      (uint16_t)from_float16b<kHalf>(lt == 0.0f ? 0.0f : x / lt);
+  uint16_t* out = a.out + ((b * a.tokens + t) * a.q_heads + h * a.group +
+                           r % a.group) * D + lane * C;
+  const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+    out[c] = (uint16_t)from_float16b<kHalf>(lt == 0.0f ? 0.0f : x[c] * inv);
 }
 
 struct Plan {
   int rows_tile;  // query rows of a workgroup
-  int q_tiles, splits;
+  int q_tiles, splits, chunk;
   size_t bytes;
 };
 
@@ -744,10 +795,14 @@ Plan plan_for(const sfx_kv4* c, int64_t batch, int64_t tokens,
   p.rows_tile = rows <= 16 ? 16 : 32;
   p.q_tiles = (int)((rows + p.rows_tile - 1) / p.rows_tile);
   const int64_t wgs = batch * c->heads * p.q_tiles;
-  const int64_t blocks = c->table_width * c->page_size / kKvBlock;
-  int64_t s = wgs > 0 ? 1024 / wgs : 1;
-  s = std::min<int64_t>(s, (blocks + 15) / 16);
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(s, 128));
+  const int64_t blocks =
+      std::max<int64_t>(1, c->table_width * c->page_size / kKvBlock);
+  const int64_t want = 1536;
+  const int64_t chunk = std::max<int64_t>(
+      {int64_t(16), (wgs * blocks + want - 1) / want,
+       (blocks + kMaxSplits - 1) / kMaxSplits});
+  p.chunk = (int)std::min(chunk, blocks);
+  p.splits = (int)((blocks + p.chunk - 1) / p.chunk);
   p.bytes = p.splits == 1 ? 0
                           : (size_t)wgs * p.splits * p.rows_tile *
                                 (c->head_dim + 2) * 4;
@@ -763,17 +818,13 @@ int launch(AttendArgs& a, int rows_tile, hipStream_t stream) {
   const dim3 block(64 * kWaves);
   if (rows_tile == 16)
     hipLaunchKernelGGL((k_kv4_attend16<D, kHalf>), grid, block, 0, stream, a);
-  else if (rows_tile == 32)
-    hipLaunchKernelGGL((k_kv4_attend32<D, kHalf, 1>), grid, block, 0, stream,
-                       a);
   else
-    hipLaunchKernelGGL((k_kv4_attend32<D, kHalf, D == 256 ? 1 : 2>), grid,
-                       block, 0, stream, a);
+    hipLaunchKernelGGL((k_kv4_attend32<D, kHalf>), grid, block, 0, stream, a);
   if (a.splits > 1)
     hipLaunchKernelGGL((k_kv4_join<D, kHalf>),
-                       dim3((unsigned)a.rows, (unsigned)a.c.heads,
+                       dim3((unsigned)(a.rows + 3) / 4, (unsigned)a.c.heads,
                             (unsigned)a.batch),
-                       dim3(D), 0, stream, a, rows_tile);
+                       dim3(256), 0, stream, a, rows_tile);
   return (int)hipGetLastError();
 }
 
@@ -821,6 +872,7 @@ extern "C" int sfx_kv4_attend(const sfx_kv4* cache, const sfx_heads* q,
   a.rows = (int)(tokens * a.group);
   a.q_tiles = p.q_tiles;
   a.splits = p.splits;
+  a.chunk = p.chunk;
   a.vec = (((uintptr_t)q->data & 15) |
            ((q->stride_b | q->stride_t | q->stride_h) & 7)) == 0;
   a.kv_len = kv_len;
