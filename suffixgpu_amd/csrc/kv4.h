@@ -33,13 +33,10 @@ struct KvLayout {
   static constexpr int kValue = kScale + kKvBlock * (D / 32);
   static constexpr int kVScale = kValue + kKvBlock * (D / 2);
   static constexpr int kBytes = kVScale + kKvBlock * 4;
-  // Word of channel c and token t, and the bit its four bits start at.
+  // Word of channel c and token t.
   __host__ __device__ static constexpr int word(int t, int c) {
     return ((c / 64 * 4 + 2 * (t / 16) + t / 4 % 2) * 16 + c % 16) * 4 +
            c / 16 % 4;
-  }
-  __host__ __device__ static constexpr int shift(int t) {
-    return 4 * (4 * (t / 8 % 2) + t % 4);
   }
 };
 
@@ -103,15 +100,6 @@ template <bool kHalf>
 __device__ __forceinline__ uint32_t from_float16b(float x) {
   if (kHalf) return __builtin_bit_cast(uint16_t, (_Float16)x);
   return __builtin_bit_cast(uint16_t, (__bf16)x);
-}
-
-// e2m1 by its four bits.
-__device__ __forceinline__ float e2m1_value(uint32_t code) {
-  const float m = code & 1 ? 1.5f : 1.0f;  // exponents 1..3: m * 2^(e - 1)
-  const int e = (code >> 1) & 3;
-  const float mag = e == 0 ? (code & 1 ? 0.5f : 0.0f)
-                           : m * (float)(1 << (e - 1));
-  return code & 8 ? -mag : mag;
 }
 
 }  // namespace sfx

@@ -16,27 +16,64 @@ struct AppendArgs {
   int start64, count64, vec;
 };
 
-// Code of the e2m1 magnitude nearest to mag / (4 quarter): the midpoints
-// between the eight are 1, 3, 5, 7, 10, 14 and 20 quarters, ties go to the even
-// code.  Callers pass quarters of at most 19 significant bits or powers of two,
-// so every comparison is exact (11 bits of an input, 5 of the factor).
-__device__ __forceinline__ uint32_t e2m1_code(float mag, float quarter) {
-  uint32_t c = mag > quarter;
-  c += mag >= 3.0f * quarter;
-  c += mag > 5.0f * quarter;
-  c += mag >= 7.0f * quarter;
-  c += mag > 10.0f * quarter;
-  c += mag >= 14.0f * quarter;
-  c += mag > 20.0f * quarter;
-  return c;
+typedef uint16_t S2 __attribute__((ext_vector_type(2)));
+typedef __bf16 B2 __attribute__((ext_vector_type(2)));
+typedef _Float16 H2 __attribute__((ext_vector_type(2)));
+typedef float F2 __attribute__((ext_vector_type(2)));
+
+constexpr uint32_t kInf = 0x7f800000u;
+
+// Rows are eight four-bit values of one token (channels in order); afterwards
+// eight of one channel, or back: two exchanges of half words and bytes, one of
+// four bits.
+__device__ __forceinline__ void transpose8(uint32_t (&a)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = a[i], y = a[i + 4];
+    a[i] = __builtin_amdgcn_perm(y, x, 0x05040100u);
+    a[i + 4] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (i & 2) continue;
+    const uint32_t x = a[i], y = a[i + 2];
+    a[i] = __builtin_amdgcn_perm(y, x, 0x06020400u);
+    a[i + 2] = __builtin_amdgcn_perm(y, x, 0x07030501u);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const uint32_t x = a[i], y = a[i + 1];
+    a[i] = (x & 0x0f0f0f0fu) | (y << 4 & 0xf0f0f0f0u);
+    a[i + 1] = (x >> 4 & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u);
+  }
+}
+
+// Token j of the octet that word row `quad` of a block holds.
+__device__ __forceinline__ int token_of(int quad, int j) {
+  return 16 * (quad / 2) + 8 * (j / 4) + 4 * (quad % 2) + j % 4;
+}
+
+// Task `e` of a block's values: eight tokens of row `quad`, channels c ..
+// c + 7.  Four neighbours are channels 16 apart, whose words are neighbours.
+__device__ __forceinline__ void task_of(int e, int* quad, int* c) {
+  *c = e / 32 * 64 + e % 4 * 16 + e / 4 % 2 * 8;
+  *quad = e / 8 % 4;
 }
 
 constexpr int kAppendThreads = 256;
 
 // One workgroup per block of 32 positions, KV head and row: eight threads a
-// token, D/8 channels each.  Keys are written from registers; the codes of the
-// values cross LDS to become words of eight tokens.  Words whose eight tokens
-// are not all new keep the others' bits.
+// token, D/8 channels each.  Keys go from registers to memory; the values'
+// four bits cross LDS, where a thread turns eight tokens by eight channels.
+// Words whose eight tokens are not all new keep the others' bits.
+//
+// The instruction that rounds to 4 bits rounds to the nearest, ties to the even
+// code, after a division by a power of two: the keys' rule.  For values, whose
+// unit is s = top / 6, it is given z = |v| (6 / top), first rounded to 18 bits
+// of mantissa: a v that lies exactly between two codes has 24 |v| = c top, c in
+// {1, 3, 5, 7, 10, 14, 20}, and any other is at least 1 / (24 2^11) of itself
+// away from that (11 significant bits), many times what the product and that
+// rounding are off; so z is a tie where v is one and on v's side elsewhere.
 template <int D, bool kHalf>
 __global__ __launch_bounds__(kAppendThreads) void k_kv4_append(AppendArgs a) {
   using L = KvLayout<D>;
@@ -54,13 +91,13 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv4_append(AppendArgs a) {
   char* base = kv_block<D>(a.c, b, h, blk);
   if (!base) return;  // the whole workgroup: no barrier is missed
 
-  __shared__ uint32_t vcode[kKvBlock][D / 4 + 1];  // a byte per channel
+  __shared__ uint32_t vcode[kKvBlock][D / 8 + 1];  // eight channels a word
   const int t = threadIdx.x / 8;
   const int sub = threadIdx.x % 8;
   const int64_t i = p0 + t - s0;  // token of the call
   const bool live = i >= 0 && i < n;
-  float x[C];
-  auto load = [&](const sfx_heads& src) {
+  uint32_t kx[C / 2], vx[C / 2];  // two channels a word
+  auto load = [&](const sfx_heads& src, uint32_t (&x)[C / 2]) {
     const uint16_t* p = (const uint16_t*)src.data +
                         (live ? b * src.stride_b + i * src.stride_t +
                                     h * src.stride_h + sub * C
@@ -69,41 +106,38 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv4_append(AppendArgs a) {
 #pragma unroll
       for (int u = 0; u < C / 8; ++u) {
         const uint4 w = live ? ((const uint4*)p)[u] : uint4{0, 0, 0, 0};
-        const uint32_t q[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          x[8 * u + 2 * j] = to_float16b<kHalf>(q[j] & 0xffff);
-          x[8 * u + 2 * j + 1] = to_float16b<kHalf>(q[j] >> 16);
-        }
+        x[4 * u] = w.x;
+        x[4 * u + 1] = w.y;
+        x[4 * u + 2] = w.z;
+        x[4 * u + 3] = w.w;
       }
     } else {
 #pragma unroll
-      for (int u = 0; u < C; ++u)
-        x[u] = live ? to_float16b<kHalf>(p[u]) : 0.0f;
+      for (int u = 0; u < C / 2; ++u)
+        x[u] = live ? (uint32_t)p[2 * u] | (uint32_t)p[2 * u + 1] << 16 : 0u;
     }
   };
-  // Largest magnitude, and whether all are finite, as one ordered integer:
-  // the bits of |x| order infinities and NaN past every finite value.
-  auto amax_bits = [&]() {
-    uint32_t m = 0;
+  load(a.k, kx);
+  load(a.v, vx);
+  // Largest magnitude as a float's bits, infinities and NaN past every finite
+  // one: the order of the 16 bits without the sign.
+  auto amax = [&](const uint32_t (&x)[C / 2], int lanes) {
+    S2 m = {0, 0};
 #pragma unroll
-    for (int u = 0; u < C; ++u) {
-      const uint32_t w = __float_as_uint(x[u]) & 0x7fffffffu;
-      m = m > w ? m : w;
+    for (int u = 0; u < C / 2; ++u)
+      m = __builtin_elementwise_max(
+          m, __builtin_bit_cast(S2, x[u] & 0x7fff7fffu));
+    uint32_t w = m.x > m.y ? m.x : m.y;
+    for (int o = 1; o < lanes; o <<= 1) {
+      const uint32_t q = __shfl_xor(w, o);
+      w = w > q ? w : q;
     }
-    return m;
+    return __float_as_uint(to_float16b<kHalf>(w));
   };
-  constexpr uint32_t kInf = 0x7f800000u;
 
   // Keys: 32 channels = kPer threads share a scale.
-  load(a.k);
-  uint32_t m = amax_bits();
   constexpr int kPer = 32 / C > 1 ? 32 / C : 1;
-#pragma unroll
-  for (int o = 1; o < kPer; o <<= 1) {
-    const uint32_t w = __shfl_xor(m, o);
-    m = m > w ? m : w;
-  }
+  uint32_t m = amax(kx, kPer);
   {
     // amax = f 2^e0 with f in [1, 2): amax / 2^(e0 - 2) is in [4, 8), and one
     // step coarser past 7.
@@ -111,18 +145,31 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv4_append(AppendArgs a) {
     int e = ex - 127 - 2 + ((m & 0x7fffffu) > 0x600000u);
     if (ex == 0) e = -126;
     e = e < -126 ? -126 : (e > (kHalf ? 13 : 125) ? (kHalf ? 13 : 125) : e);
-    const uint32_t sb = m >= kInf ? 255u : (uint32_t)(e + 127);
-    const float unit = 0.25f * __uint_as_float((uint32_t)(e + 127) << 23);
+    const float unit = __uint_as_float((uint32_t)(e + 127) << 23);
     uint32_t w[C / 8];
 #pragma unroll
     for (int u = 0; u < C / 8; ++u) {
       uint32_t q = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float y = x[8 * u + j];
-        q |= (e2m1_code(fabsf(y), unit) |
-              (__float_as_uint(y) >> 31) << 3)
-             << (4 * j);
+      if (kHalf) {
+        const uint32_t* x = kx + 4 * u;
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(
+            q, __builtin_bit_cast(H2, x[0]), unit, 0);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(
+            q, __builtin_bit_cast(H2, x[1]), unit, 1);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(
+            q, __builtin_bit_cast(H2, x[2]), unit, 2);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(
+            q, __builtin_bit_cast(H2, x[3]), unit, 3);
+      } else {
+        const uint32_t* x = kx + 4 * u;
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(
+            q, __builtin_bit_cast(B2, x[0]), unit, 0);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(
+            q, __builtin_bit_cast(B2, x[1]), unit, 1);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(
+            q, __builtin_bit_cast(B2, x[2]), unit, 2);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(
+            q, __builtin_bit_cast(B2, x[3]), unit, 3);
       }
       w[u] = q;
     }
@@ -132,42 +179,38 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv4_append(AppendArgs a) {
       for (int u = 0; u < C / 8; ++u) o[u] = w[u];
       if (sub % kPer == 0)
         ((uint8_t*)(base + L::kScale))[t * (D / 32) + sub * C / 32] =
-            (uint8_t)sb;
+            (uint8_t)(m >= kInf ? 255 : e + 127);
     }
   }
 
   // Values: one scale for the D channels.
-  load(a.v);
-  m = amax_bits();
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
-    const uint32_t w = __shfl_xor(m, o);
-    m = m > w ? m : w;
-  }
+  m = amax(vx, 8);
   {
     constexpr float kTiny = 6.0f * 0x1p-100f;
     float top = __uint_as_float(m);
-    if (m < kInf && top < kTiny) top = kTiny;
+    if (top < kTiny) top = kTiny;
+    const bool odd = m >= kInf;  // the scale says NaN, the codes are finite
     if (live && sub == 0)
       ((float*)(base + L::kVScale))[t] =
-          m >= kInf ? __uint_as_float(0x7fc00000u) : top / 6.0f;
-    if (m >= kInf) top = 1.0f;  // the scale says NaN, the codes are finite
-    // 24 |v| against multiples of the largest; both 2^-16 times where that
-    // could overflow.
-    const float pre = top >= 0x1p100f ? 0x1p-16f : 1.0f;
-    top *= pre;
-    const float mul = 24.0f * pre;
+          odd ? __uint_as_float(0x7fc00000u) : top / 6.0f;
+    const float inv = odd ? 0.0f : 6.0f / top;
+    auto z = [&](uint32_t bits) {
+      const uint32_t q = __float_as_uint(to_float16b<kHalf>(bits) * inv);
+      return __uint_as_float((q + 16u) & ~31u);
+    };
 #pragma unroll
-    for (int u = 0; u < C / 4; ++u) {
+    for (int u = 0; u < C / 8; ++u) {
+      const uint32_t* x = vx + 4 * u;
       uint32_t q = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float y = x[4 * u + j];
-        q |= (e2m1_code(mul * fabsf(y), top) |
-              (__float_as_uint(y) >> 31) << 3)
-             << (8 * j);
-      }
-      vcode[t][sub * (C / 4) + u] = q;
+      q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, z(x[0] & 0xffffu),
+                                                   z(x[0] >> 16), 1.0f, 0);
+      q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, z(x[1] & 0xffffu),
+                                                   z(x[1] >> 16), 1.0f, 1);
+      q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, z(x[2] & 0xffffu),
+                                                   z(x[2] >> 16), 1.0f, 2);
+      q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, z(x[3] & 0xffffu),
+                                                   z(x[3] >> 16), 1.0f, 3);
+      vcode[t][sub * (C / 8) + u] = q;
     }
   }
   __syncthreads();
@@ -176,22 +219,25 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv4_append(AppendArgs a) {
   const int lo = lo64 > 0 ? (int)lo64 : 0;
   const int hi = hi64 < kKvBlock ? (int)hi64 : kKvBlock;
   uint32_t* words = (uint32_t*)(base + L::kValue);
-  for (int w = threadIdx.x; w < D * 4; w += kAppendThreads) {
-    // word w: channel and token octet (word() of the layout, read backwards)
-    const int c = w / 256 * 64 + w % 4 * 16 + w / 4 % 16;
-    const int quad = w / 64 % 4;
-    uint32_t val = 0, mask = 0;
+  for (int e = threadIdx.x; e < D / 2; e += kAppendThreads) {
+    int quad, c;
+    task_of(e, &quad, &c);
+    uint32_t w[8], mask = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int tk = 16 * (quad / 2) + 8 * (j / 4) + 4 * (quad % 2) + j % 4;
-      if (tk >= lo && tk < hi) {
-        mask |= 15u << (4 * j);
-        val |= (vcode[tk][c / 4] >> (8 * (c % 4)) & 15u) << (4 * j);
-      }
+      const int tk = token_of(quad, j);
+      w[j] = vcode[tk][c / 8];
+      if (tk >= lo && tk < hi) mask |= 15u << (4 * j);
     }
     if (mask == 0) continue;
-    if (mask != 0xffffffffu) val |= words[w] & ~mask;
-    words[w] = val;
+    transpose8(w);
+    uint32_t* o = words + L::word(token_of(quad, 0), c);
+    if (mask != 0xffffffffu) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = (w[j] & mask) | (o[4 * j] & ~mask);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[4 * j] = w[j];
   }
 }
 
@@ -205,50 +251,100 @@ struct ReadArgs {
   uint16_t* v;
 };
 
-// Eight threads a token and KV head, D/8 channels each.
+// One workgroup per block of 32 positions, KV head and row, the same threads
+// and tasks as the append's.
 template <int D, bool kHalf>
 __global__ __launch_bounds__(256) void k_kv4_read(ReadArgs a) {
   using L = KvLayout<D>;
   constexpr int C = D / 8;
   const int64_t b = blockIdx.z;
   const int h = blockIdx.y;
-  const int64_t i = (int64_t)blockIdx.x * 32 + threadIdx.x / 8;
-  if (i >= a.tokens) return;
-  const int sub = threadIdx.x % 8;
   int64_t n = a.count ? load_count(a.count, a.count64, b) : a.tokens;
+  n = n < 0 ? 0 : (n < a.tokens ? n : a.tokens);
   const int64_t s0 = load_count(a.start, a.start64, b);
-  const int64_t pos = s0 + i;
+  // Rows of the result that this workgroup writes: positions of its block,
+  // where a row begins inside it and all of the first block is before it.
+  const int64_t off = s0 >= 0 ? s0 % kKvBlock : 0;
+  const int64_t i0 = (int64_t)blockIdx.x * kKvBlock - off;
   const char* base = nullptr;
-  if (i < n && s0 >= 0 && pos < a.c.positions)
-    base = kv_block<D>(a.c, b, h, pos / kKvBlock);
-  uint32_t ko[C / 2], vo[C / 2];
+  if (s0 >= 0 && i0 < n)
+    base = kv_block<D>(a.c, b, h, s0 / kKvBlock + blockIdx.x);
+  // results are [batch, tokens, heads, D]
+  auto row = [&](int64_t i) {
+    return ((b * a.tokens + i) * a.c.heads + h) * D;
+  };
+  {
+    const int t = threadIdx.x / 8;
+    const int sub = threadIdx.x % 8;
+    const int64_t i = i0 + t;
+    if (i >= 0 && i < a.tokens) {
+      const bool there = base && i < n;
+      const uint32_t* kw =
+          (const uint32_t*)(base + t * (D / 2) + sub * (C / 2));
+      uint32_t sb = 0;
+      if (there)
+        sb = ((const uint8_t*)(base + L::kScale))[t * (D / 32) + sub * C / 32];
+      const float sc = __uint_as_float(sb << 23);
+      uint4* o = (uint4*)(a.k + row(i) + sub * C);
 #pragma unroll
-  for (int u = 0; u < C / 2; ++u) ko[u] = vo[u] = 0;
-  if (base) {
-    const int t = (int)(pos % kKvBlock);
-    const uint32_t* kw = (const uint32_t*)(base + t * (D / 2) + sub * (C / 2));
-    const uint32_t sb =
-        ((const uint8_t*)(base + L::kScale))[t * (D / 32) + sub * C / 32];
-    const float ks = sb == 255 ? __uint_as_float(0x7fc00000u)
-                               : __uint_as_float(sb << 23);
-    const float vs = ((const float*)(base + L::kVScale))[t];
-    const uint32_t* vw = (const uint32_t*)(base + L::kValue);
-#pragma unroll
-    for (int u = 0; u < C; ++u) {
-      const float kf = e2m1_value(kw[u / 8] >> (4 * (u % 8)) & 15u) * ks;
-      ko[u / 2] |= from_float16b<kHalf>(kf) << (16 * (u % 2));
-      const float vf =
-          e2m1_value(vw[L::word(t, sub * C + u)] >> L::shift(t) & 15u) * vs;
-      vo[u / 2] |= from_float16b<kHalf>(vf) << (16 * (u % 2));
+      for (int u = 0; u < C / 8; ++u) {
+        uint4 r = {0, 0, 0, 0};
+        if (there) {
+          const uint32_t w = kw[u];
+          if (kHalf) {
+            r.x = __builtin_bit_cast(
+                uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 0));
+            r.y = __builtin_bit_cast(
+                uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 1));
+            r.z = __builtin_bit_cast(
+                uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 2));
+            r.w = __builtin_bit_cast(
+                uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 3));
+          } else {
+            r.x = __builtin_bit_cast(
+                uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0));
+            r.y = __builtin_bit_cast(
+                uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1));
+            r.z = __builtin_bit_cast(
+                uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2));
+            r.w = __builtin_bit_cast(
+                uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3));
+          }
+        }
+        o[u] = r;
+      }
     }
   }
-  const int64_t o = (((b * a.tokens + i) * a.c.heads + h) * D + sub * C) / 2;
+  for (int e = threadIdx.x; e < D / 2; e += 256) {
+    int quad, c;
+    task_of(e, &quad, &c);
+    uint32_t w[8];
+    if (base) {
+      const uint32_t* p = (const uint32_t*)(base + L::kValue) +
+                          L::word(token_of(quad, 0), c);
 #pragma unroll
-  for (int u = 0; u < C / 2; u += 4) {
-    *(uint4*)((uint32_t*)a.k + o + u) =
-        uint4{ko[u], ko[u + 1], ko[u + 2], ko[u + 3]};
-    *(uint4*)((uint32_t*)a.v + o + u) =
-        uint4{vo[u], vo[u + 1], vo[u + 2], vo[u + 3]};
+      for (int j = 0; j < 8; ++j) w[j] = p[4 * j];
+      transpose8(w);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int tk = token_of(quad, j);
+      const int64_t i = i0 + tk;
+      if (i < 0 || i >= a.tokens) continue;
+      uint4 r = {0, 0, 0, 0};
+      if (base && i < n) {
+        const float vs = ((const float*)(base + L::kVScale))[tk];
+        auto two = [&](F2 x) {
+          return from_float16b<kHalf>(x.x * vs) |
+                 from_float16b<kHalf>(x.y * vs) << 16;
+        };
+        r.x = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[j], 1.0f, 0));
+        r.y = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[j], 1.0f, 1));
+        r.z = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[j], 1.0f, 2));
+        r.w = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[j], 1.0f, 3));
+      }
+      *(uint4*)(a.v + row(i) + c) = r;
+    }
   }
 }
 
@@ -356,8 +452,8 @@ extern "C" int sfx_kv4_read(const sfx_kv4* cache, int64_t batch,
   l.a.count64 = count_is64;
   l.a.k = (uint16_t*)k_out;
   l.a.v = (uint16_t*)v_out;
-  l.grid = dim3((unsigned)((tokens + 31) / 32), (unsigned)cache->heads,
-                (unsigned)batch);
+  l.grid = dim3((unsigned)((tokens + kKvBlock - 2) / kKvBlock + 1),
+                (unsigned)cache->heads, (unsigned)batch);
   l.stream = stream;
   return by_shape(cache, l);
 }

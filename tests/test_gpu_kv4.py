@@ -115,6 +115,37 @@ def test_append_rounds_ties_and_extremes(gpu, dtype):
             <= np.abs(ev) * (rel + 2.0 ** -22) + tiny).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_append_values_at_the_midpoints(gpu, dtype):
+    """Values on, just below and just above every midpoint between two codes,
+    for many largest magnitudes."""
+    d, n = 128, 400
+    bits = torch.int16
+    g = torch.Generator().manual_seed(3)
+    top = (torch.rand(n, generator=g) * 3 + 0.5).to(dtype)
+    top[:64] = (torch.arange(64) * 3).to(dtype)      # exact ties
+    top[0] = 1.0
+    x = torch.zeros(n, d, dtype=dtype)
+    for i, c in enumerate((1, 3, 5, 7, 10, 14, 20)):
+        m = (top.double() * c / 24).to(dtype)
+        for j, step in enumerate((-2, -1, 0, 1, 2)):
+            y = (m.view(bits) + step).view(dtype)
+            x[:, 16 * i + 2 * j] = y
+            x[:, 16 * i + 2 * j + 1] = -y
+    x[:, 127] = top
+    assert (x.abs().amax(dim=1) == top).all()
+    x = x[None, :, None].to(gpu)
+    c, table = make(gpu, 1, n, 1, d, 64, dtype, 8)
+    c.append(x, x, table, ints([0], gpu))
+    gk, gv = c.read(table, ints([0], gpu), n)
+    np.testing.assert_array_equal(np64(gk),
+                                  target.quantize_k(np64(x), dtype == HF))
+    ev, _ = target.quantize_v(np64(x))
+    rel, tiny = target.ulp16(dtype == HF)
+    assert (np.abs(np64(gv) - ev)
+            <= np.abs(ev) * (rel + 2.0 ** -22) + tiny).all()
+
+
 def test_append_infinities_and_nan(gpu):
     """They make their group of a key, or their token's values, NaN, and the
     queries that see them; no other group, token or row."""
