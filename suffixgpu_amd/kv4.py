@@ -14,7 +14,7 @@ from __future__ import annotations
 import torch
 
 from suffixgpu_amd import _lib
-from suffixgpu_amd._lib import (SuffixGPUError, check, count_arg, lib, ptr,
+from suffixgpu_amd._lib import (SuffixGPUError, check, count_arg, lib,
                                 require_gpu, stream_of)
 
 BLOCK = 32  # tokens
@@ -72,41 +72,55 @@ class KV4Cache:
         elif pages.data_ptr() % 16:
             raise ValueError("pages must be 16-byte aligned")
         self.pages = pages
+        # what every call's C view begins with, and workspace bytes by shape
+        self._geometry = (pages.data_ptr(), self.num_pages, self.num_kv_heads,
+                          self.head_dim, self.page_size,
+                          _lib.DTYPE_CODES[dtype])
+        self._sizes: dict[tuple, int] = {}
 
     # ------------------------------------------------------------------
     def _view(self, page_table: torch.Tensor, rows: int) -> _lib.SfxKv4:
-        if (page_table.dim() != 2 or page_table.dtype != torch.int32
-                or page_table.shape[0] != rows
-                or page_table.device != self.device
-                or (page_table.shape[1] > 1 and page_table.stride(1) != 1)):
-            raise ValueError(f"page_table must be an int32 [{rows}, W] tensor "
-                             f"on {self.device} with contiguous rows")
-        return _lib.SfxKv4(self.pages.data_ptr(), self.num_pages,
-                           self.num_kv_heads, self.head_dim, self.page_size,
-                           _lib.DTYPE_CODES[self.dtype],
-                           page_table.data_ptr(), page_table.shape[1],
-                           page_table.stride(0))
+        if (page_table.dim() != 2 or page_table.dtype is not torch.int32
+                or page_table.device != self.device):
+            self._refuse_table(page_table, rows)
+        n, width = page_table.shape
+        s0, s1 = page_table.stride()
+        if n != rows or (s1 != 1 and width > 1):
+            self._refuse_table(page_table, rows)
+        return _lib.SfxKv4(*self._geometry, page_table.data_ptr(), width, s0)
+
+    def _refuse_table(self, page_table, rows):
+        require_gpu(page_table)
+        raise ValueError(f"page_table must be an int32 [{rows}, W] tensor on "
+                         f"{self.device} with contiguous rows")
 
     def _heads(self, name: str, x: torch.Tensor, heads: int | None = None):
-        if (x.dim() != 4 or x.shape[3] != self.head_dim
-                or x.dtype != self.dtype or x.device != self.device
-                or x.stride(3) != 1
-                or (heads is not None and x.shape[2] != heads)):
-            raise ValueError(
-                f"{name} must be a {self.dtype} [B, T, heads, "
-                f"{self.head_dim}] tensor on {self.device}, contiguous along "
-                "the last dimension"
-                + (f", with {heads} heads" if heads is not None else ""))
-        return _lib.SfxHeads(x.data_ptr(), x.stride(0), x.stride(1),
-                             x.stride(2))
+        """The C view of x [B, T, heads, head_dim], and B, T, heads."""
+        if x.dim() == 4 and x.dtype is self.dtype and x.device == self.device:
+            b, t, h, d = x.shape
+            sb, st, sh, sd = x.stride()
+            if (d == self.head_dim and sd == 1
+                    and (heads is None or h == heads)):
+                return _lib.SfxHeads(x.data_ptr(), sb, st, sh), b, t, h
+        require_gpu(x)
+        raise ValueError(
+            f"{name} must be a {self.dtype} [B, T, heads, {self.head_dim}] "
+            f"tensor on {self.device}, contiguous along the last dimension"
+            + (f", with {heads} heads" if heads is not None else ""))
 
-    def _counts(self, name: str, t: torch.Tensor | None, rows: int):
+    def _counts(self, name: str, t: torch.Tensor | None, rows: int,
+                optional: bool = False):
+        """(tensor to keep, address, is64) of a vector of counts."""
+        if t is None and optional:
+            return None, None, 0
         if t is None:
-            return None, 0
+            raise ValueError(f"{name} is needed")
         if t.dim() != 1 or t.shape[0] != rows or t.device != self.device:
+            require_gpu(t)
             raise ValueError(f"{name} must hold {rows} integers on "
                              f"{self.device}")
-        return count_arg(t)
+        t, is64 = count_arg(t)
+        return t, t.data_ptr(), is64
 
     def append(self, k: torch.Tensor, v: torch.Tensor,
                page_table: torch.Tensor, start: torch.Tensor,
@@ -117,21 +131,17 @@ class KV4Cache:
         A page that one row of a call writes must not be written by another
         row of it.  Infinities and NaN make their 32 channels of a key, or
         their token's values, NaN."""
-        require_gpu(k, v, page_table, start, count)
-        kh = self._heads("k", k, self.num_kv_heads)
-        vh = self._heads("v", v, self.num_kv_heads)
-        if k.shape != v.shape:
+        kh, b, t, _ = self._heads("k", k, self.num_kv_heads)
+        vh, vb, vt, _ = self._heads("v", v, self.num_kv_heads)
+        if b != vb or t != vt:
             raise ValueError("k and v differ in shape")
-        b, t = k.shape[:2]
         view = self._view(page_table, b)
-        st, st64 = self._counts("start", start, b)
-        if st is None:
-            raise ValueError("start is needed")
-        ct, ct64 = self._counts("count", count, b)
+        keep = (self._counts("start", start, b),
+                self._counts("count", count, b, optional=True))
         if b == 0 or t == 0:
             return
-        check(lib().sfx_kv4_append(view, kh, vh, b, t, st.data_ptr(), st64,
-                                   ptr(ct), ct64, stream_of(self.device)),
+        check(lib().sfx_kv4_append(view, kh, vh, b, t, *keep[0][1:],
+                                   *keep[1][1:], stream_of(self.device)),
               "KV4Cache.append")
 
     def read(self, page_table: torch.Tensor, start: torch.Tensor,
@@ -139,20 +149,17 @@ class KV4Cache:
         """The keys and values [B, tokens, num_kv_heads, head_dim] that the
         cache holds at positions ``start[b] + i``, i < ``count[b]``; zeros
         elsewhere."""
-        require_gpu(page_table, start, count)
         b = page_table.shape[0]
         view = self._view(page_table, b)
-        st, st64 = self._counts("start", start, b)
-        if st is None:
-            raise ValueError("start is needed")
-        ct, ct64 = self._counts("count", count, b)
+        keep = (self._counts("start", start, b),
+                self._counts("count", count, b, optional=True))
         shape = (b, int(tokens), self.num_kv_heads, self.head_dim)
         k = torch.empty(shape, dtype=self.dtype, device=self.device)
         v = torch.empty(shape, dtype=self.dtype, device=self.device)
-        if k.numel() == 0:
+        if b == 0 or tokens == 0:
             return k, v
-        check(lib().sfx_kv4_read(view, b, int(tokens), st.data_ptr(), st64,
-                                 ptr(ct), ct64, k.data_ptr(), v.data_ptr(),
+        check(lib().sfx_kv4_read(view, b, int(tokens), *keep[0][1:],
+                                 *keep[1][1:], k.data_ptr(), v.data_ptr(),
                                  stream_of(self.device)), "KV4Cache.read")
         return k, v
 
@@ -170,28 +177,29 @@ class KV4Cache:
         head_dim] in the cache's type: zeros for a query that sees nothing and
         for tokens from q_len on.  T = 1 is a decode step, T = k + 1 a
         verification step, a long T a chunk of a prompt."""
-        require_gpu(q, page_table, kv_len, q_len)
-        qh = self._heads("q", q)
-        b, t, heads = q.shape[:3]
+        qh, b, t, heads = self._heads("q", q)
         if heads < 1 or heads % self.num_kv_heads:
             raise ValueError(f"{heads} query heads do not share "
                              f"{self.num_kv_heads} KV heads evenly")
         view = self._view(page_table, b)
-        ln, ln64 = self._counts("kv_len", kv_len, b)
-        if ln is None:
-            raise ValueError("kv_len is needed")
-        ql, ql64 = self._counts("q_len", q_len, b)
+        keep = (self._counts("kv_len", kv_len, b),
+                self._counts("q_len", q_len, b, optional=True))
         if scale is None:
             scale = self.head_dim ** -0.5
-        out = torch.empty(q.shape, dtype=self.dtype, device=self.device)
-        if out.numel() == 0:
+        out = torch.empty(b, t, heads, self.head_dim, dtype=self.dtype,
+                          device=self.device)
+        if b == 0 or t == 0:
             return out
         L = lib()
-        nbytes = L.sfx_kv4_attend_workspace_size(view, b, t, heads)
+        key = (b, t, heads, view.table_width)
+        nbytes = self._sizes.get(key)
+        if nbytes is None:
+            nbytes = self._sizes[key] = L.sfx_kv4_attend_workspace_size(
+                view, b, t, heads)
         ws = (torch.empty(nbytes, dtype=torch.uint8, device=self.device)
               if nbytes else None)
-        check(L.sfx_kv4_attend(view, qh, b, t, heads, ln.data_ptr(), ln64,
-                               ptr(ql), ql64, float(scale), out.data_ptr(),
-                               ptr(ws), nbytes, stream_of(self.device)),
-              "KV4Cache.attend")
+        check(L.sfx_kv4_attend(view, qh, b, t, heads, *keep[0][1:],
+                               *keep[1][1:], scale, out.data_ptr(),
+                               None if ws is None else ws.data_ptr(), nbytes,
+                               stream_of(self.device)), "KV4Cache.attend")
         return out

@@ -12,36 +12,63 @@ from __future__ import annotations
 import torch
 
 from suffixgpu_amd import _lib
-from suffixgpu_amd._lib import check, lib, ptr, require_gpu, stream_of
+from suffixgpu_amd._lib import check, lib, require_gpu, stream_of
 
 
-# (device, stream) -> (counters, scratch).  The counters are zero between calls
-# (every call leaves them so), the scratch is anything; two calls that share
-# them are ordered by their stream.  Calls recorded into a HIP graph share a
-# pair of their own per device (replays must not overlap each other): eager
-# calls see to its size, so that a capture after a first eager call of that size
-# records no fill.  Outgrown pairs of graphs are kept, a graph may hold them.
-_workspaces: dict[tuple, tuple[torch.Tensor, torch.Tensor]] = {}
-_outgrown: list[tuple[torch.Tensor, torch.Tensor]] = []
+# Counters and scratch, as (counters, scratch, counters' address, bytes, scratch's
+# address, bytes), by device and stream.  The
+# counters are zero between calls (every call leaves them so), the scratch is
+# anything; two calls that share them are ordered by their stream.  Calls
+# recorded into a HIP graph have a pair of their own for each stream recorded
+# (replays of graphs recorded on one stream must not overlap): a spare one that
+# eager calls keep ready, so that a capture after a first eager call of that
+# size records no fill.  Outgrown pairs of graphs are kept, a graph may hold
+# them.
+_workspaces: dict[tuple, tuple] = {}
+_outgrown: list[tuple] = []
 
 
-def _workspace(dev: torch.device, stream: int, nc: int, ns: int):
-    capturing = torch.cuda.is_current_stream_capturing()
-    for key in (((dev, "graph"),) if capturing
-                else ((dev, "graph"), (dev, stream))):
+def _new_workspace(dev: torch.device, nc: int, ns: int) -> tuple:
+    c = torch.zeros(max(nc, 1 << 16), dtype=torch.uint8, device=dev)
+    s = torch.empty(max(ns, 1 << 18), dtype=torch.uint8, device=dev)
+    return c, s, c.data_ptr(), c.numel(), s.data_ptr(), s.numel()
+
+
+def _workspace(dev: torch.device, stream: int, nc: int, ns: int) -> tuple:
+    """The pair for `stream`, with at least nc and ns bytes."""
+    spare = _workspaces.get((dev, "spare"))
+    if torch.cuda.is_current_stream_capturing():
+        key = (dev, stream, "graph")
         ws = _workspaces.get(key)
-        if ws is None or ws[0].numel() < nc or ws[1].numel() < ns:
+        if ws is None or ws[3] < nc or ws[5] < ns:
             if ws is not None:
-                if key[1] == "graph":
-                    _outgrown.append(ws)
-                nc2 = max(nc, 2 * ws[0].numel())
-                ns2 = max(ns, 2 * ws[1].numel())
+                _outgrown.append(ws)
+            if spare is not None and spare[3] >= nc and spare[5] >= ns:
+                ws = _workspaces.pop((dev, "spare"))
             else:
-                nc2, ns2 = max(nc, 1 << 16), max(ns, 1 << 18)
-            ws = (torch.zeros(nc2, dtype=torch.uint8, device=dev),
-                  torch.empty(ns2, dtype=torch.uint8, device=dev))
+                ws = _new_workspace(dev, nc, ns)
             _workspaces[key] = ws
+        return ws
+    if spare is None or spare[3] < nc or spare[5] < ns:
+        _workspaces[dev, "spare"] = _new_workspace(dev, 2 * nc, 2 * ns)
+    ws = _workspaces.get((dev, stream))
+    if ws is None or ws[3] < nc or ws[5] < ns:
+        ws = _workspaces[dev, stream] = _new_workspace(dev, 2 * nc, 2 * ns)
     return ws
+
+
+# Workspace bytes by (batch, drafts, vocabulary).
+_sizes: dict[tuple, tuple[int, int]] = {}
+
+
+def _need(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype,
+          dev: torch.device) -> int:
+    if (t.dtype is not dtype or t.device != dev or t.shape != shape
+            or not t.is_contiguous()):
+        require_gpu(t)
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape "
+                         f"{list(shape)} on {dev}")
+    return t.data_ptr()
 
 
 def verify_draft(logits: torch.Tensor, draft: torch.Tensor,
@@ -75,54 +102,47 @@ def verify_draft(logits: torch.Tensor, draft: torch.Tensor,
     count [B] int32).  No host synchronisation; two launches on the current
     stream.
     """
-    require_gpu(logits, draft, num_valid, uniform, noise, temperature,
-                draft_probs)
-    if logits.dim() != 3 or logits.shape[1] < 1 or logits.shape[2] < 1:
+    require_gpu(logits)
+    if logits.dim() != 3:
+        raise ValueError("logits must be [B, K + 1, V]")
+    b, k1, v = logits.shape
+    if k1 < 1 or v < 1:
         raise ValueError("logits must be [B, K + 1, V]")
     code = _lib.DTYPE_CODES.get(logits.dtype)
     if code is None:
         raise ValueError("logits must be bfloat16, float16 or float32")
-    if logits.stride(2) != 1 and logits.shape[2] > 1:
+    sb, sj, sv = logits.stride()
+    if sv != 1 and v > 1:
         raise ValueError("logits must be contiguous along the vocabulary")
-    b, k1, v = logits.shape
     dev = logits.device
-    dense = [("draft", draft, (b, k1 - 1), torch.int32),
-             ("num_valid", num_valid, (b,), torch.int32)]
+    k = k1 - 1
+    dp = _need("draft", draft, (b, k), torch.int32, dev)
+    np_ = _need("num_valid", num_valid, (b,), torch.int32, dev)
+    up = ep = tp = qp = None
     if not greedy:
         if uniform is None or noise is None:
             raise ValueError("uniform and noise are needed unless greedy")
-        dense += [("uniform", uniform, (b, k1 - 1), torch.float32),
-                  ("noise", noise, (b, v), torch.float32)]
+        up = _need("uniform", uniform, (b, k), torch.float32, dev)
+        ep = _need("noise", noise, (b, v), torch.float32, dev)
         if temperature is not None:
-            dense.append(("temperature", temperature, (b,), torch.float32))
+            tp = _need("temperature", temperature, (b,), torch.float32, dev)
         if draft_probs is not None:
-            dense.append(("draft_probs", draft_probs, (b, k1 - 1, v),
-                          torch.float32))
-    for name, t, shape, dt in dense:
-        if t.dtype != dt or t.device != dev or t.shape != shape:
-            raise ValueError(f"{name} must be a {dt} tensor of shape "
-                             f"{list(shape)} on {dev}")
-        if not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
+            qp = _need("draft_probs", draft_probs, (b, k, v), torch.float32,
+                       dev)
     sampled = torch.empty(b, k1, dtype=torch.int32, device=dev)
     count = torch.empty(b, dtype=torch.int32, device=dev)
     if b == 0:
         return sampled, count
     L = lib()
+    size = _sizes.get((b, k, v))
+    if size is None:
+        size = _sizes[b, k, v] = (L.sfx_verify_counter_bytes(b, k, v),
+                                  L.sfx_verify_workspace_size(b, k, v))
     stream = stream_of(dev)
-    counters, scratch = _workspace(dev, stream,
-                                   L.sfx_verify_counter_bytes(b, k1 - 1, v),
-                                   L.sfx_verify_workspace_size(b, k1 - 1, v))
-    args = _lib.SfxVerify(
-        logits.data_ptr(), code, int(greedy), b, k1 - 1, v,
-        logits.stride(0), logits.stride(1), draft.data_ptr(),
-        num_valid.data_ptr(),
-        None if greedy else uniform.data_ptr(),
-        None if greedy else noise.data_ptr(),
-        None if greedy else ptr(temperature),
-        None if greedy else ptr(draft_probs),
-        sampled.data_ptr(), count.data_ptr())
-    check(L.sfx_verify_draft(args, counters.data_ptr(), counters.numel(),
-                             scratch.data_ptr(), scratch.numel(), stream),
-          "verify_draft")
+    ws = _workspace(dev, stream, *size)
+    check(L.sfx_verify_draft(
+        _lib.SfxVerify(logits.data_ptr(), code, int(greedy), b, k, v, sb, sj,
+                       dp, np_, up, ep, tp, qp, sampled.data_ptr(),
+                       count.data_ptr()),
+        *ws[2:], stream), "verify_draft")
     return sampled, count
