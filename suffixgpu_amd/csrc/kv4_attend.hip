@@ -420,24 +420,38 @@ __device__ __forceinline__ void put_row(const AttendArgs& a, const Work& w,
   }
 }
 
-// Up to 16 query rows a workgroup: single tokens, and small groups of drafts.
-template <int D, bool kHalf>
-__global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 4)
-void k_kv4_attend16(AttendArgs a) {
+// LDS of a workgroup: the waves' sums where they are joined (or, before, the
+// queries), and what goes with them.
+template <int kBytes>
+struct Lds {
+  __align__(16) char pool[kBytes];
+  float m[kWaves][32], l[kWaves][32];
+  float scales[kWaves][64];
+};
+
+template <int D>
+constexpr int kLds16 = kWaves * 16 * (D + 4) * 4;
+template <int D>
+constexpr int kLds32 = kWaves * 32 * (64 + 4) * 4 > 32 * D * 2
+                           ? kWaves * 32 * (64 + 4) * 4
+                           : 32 * D * 2;
+
+// 16 query rows from row0 on; rows 16 .. kTileRows of the workgroup's tile are
+// no queries.
+template <int D, bool kHalf, int kTileRows, class S>
+__device__ __forceinline__ void attend16(const AttendArgs& a, const Work& wk,
+                                         int64_t len, int64_t nq, int row0,
+                                         S& lds) {
   constexpr int kStep = D / 32;   // matrix instructions a score tile
   constexpr int kDt = D / 16;     // channel tiles
-  const Work wk = work_of(a);
-  if (!wk.any) return;
   const int lane = lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int col = lane % 16, quad = lane / 16;
-  __shared__ float so[kWaves][16][D + 4];
-  __shared__ float sm[kWaves][16], sl[kWaves][16];
-  __shared__ float sc[kWaves][64];
-
-  const int64_t len = kv_len_of(a, wk.b);
-  const int64_t nq = q_len_of(a, wk.b);
-  const int row0 = wk.qt * 16;
+  static_assert(sizeof(lds.pool) >= kLds16<D>, "LDS");
+  auto so = (float(*)[16][D + 4])lds.pool;
+  auto& sm = lds.m;
+  auto& sl = lds.l;
+  auto& sc = lds.scales;
   const int vis = visible(a, len, nq, row0 + col);
   U4 qf[kStep];
   {
@@ -455,7 +469,6 @@ void k_kv4_attend16(AttendArgs a) {
   most = __builtin_amdgcn_readfirstlane(most);
   least = __builtin_amdgcn_readfirstlane(least);
   const Range rg = range_of(a, len, most, wk.split);
-  if (rg.splits <= wk.split) return;
   const int first = rg.first + wave, last = rg.last;
 
   float m = kNegInf, l = 0.0f;
@@ -549,34 +562,30 @@ void k_kv4_attend16(AttendArgs a) {
       x[c] = __builtin_fmaf(f[w], so[w][row][c0 + c], x[c]);
   }
   const bool see = visible(a, len, nq, row0 + row) > 0 && lt != 0.0f;
-  put_row<kHalf>(a, wk, D, 16, row, row0 + row, see, mx, lt, c0, x,
+  put_row<kHalf>(a, wk, D, kTileRows, row, row0 + row, see, mx, lt, c0, x,
                  rg.splits);
+  if (kTileRows > 16)
+    put_row<kHalf>(a, wk, D, kTileRows, row + 16, row0 + row + 16, false, mx,
+                   lt, c0, x, rg.splits);
 }
 
-// 32 query rows a workgroup: verification steps and prompts.  The query rows
-// lie in LDS in the order of the matrix instruction's operand; every wave holds
-// O of all of them.
-template <int D, bool kHalf>
-__global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3)
-void k_kv4_attend32(AttendArgs a) {
+// 32 query rows from row0 on.  They lie in LDS in the order of the matrix
+// instruction's operand; every wave holds O of all of them.
+template <int D, bool kHalf, class S>
+__device__ __forceinline__ void attend32(const AttendArgs& a, const Work& wk,
+                                         int64_t len, int64_t nq, int row0,
+                                         S& lds) {
   constexpr int kRows = 32;
   constexpr int kStep = D / 16;
   constexpr int kDt = D / 32;
-  const Work wk = work_of(a);
-  if (!wk.any) return;
   const int lane = lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int col = lane % 32, h2 = lane / 32;
-  constexpr int kJoin = kWaves * 32 * (64 + 4) * 4;
-  constexpr int kQ = kRows * D * 2;
-  __shared__ __align__(16) char pool[kJoin > kQ ? kJoin : kQ];
-  __shared__ float sm[kWaves][32], sl[kWaves][32];
-  __shared__ float sc[kWaves][64];
-  U4* sq = (U4*)pool;
-
-  const int64_t len = kv_len_of(a, wk.b);
-  const int64_t nq = q_len_of(a, wk.b);
-  const int row0 = wk.qt * kRows;
+  static_assert(sizeof(lds.pool) >= kLds32<D>, "LDS");
+  U4* sq = (U4*)lds.pool;
+  auto& sm = lds.m;
+  auto& sl = lds.l;
+  auto& sc = lds.scales;
   for (int e = threadIdx.x; e < kRows * (D / 8); e += 64 * kWaves) {
     // operand (step, lane): channels (lane / 32) D / 2 + 8 step
     const int i = e / 64, ln = e % 64;
@@ -596,7 +605,6 @@ void k_kv4_attend32(AttendArgs a) {
   most = __builtin_amdgcn_readfirstlane(most);
   least = __builtin_amdgcn_readfirstlane(least);
   const Range rg = range_of(a, len, most, wk.split);
-  if (rg.splits <= wk.split) return;
   const int first = rg.first + wave, last = rg.last;
   __syncthreads();
 
@@ -679,7 +687,7 @@ void k_kv4_attend32(AttendArgs a) {
   });
 
   // Join the waves in LDS, 64 channels at a time: 8 threads a row.
-  float(*so)[32][64 + 4] = (float(*)[32][64 + 4])pool;
+  auto so = (float(*)[32][64 + 4])lds.pool;
   l += __shfl_xor(l, 32);
   const int row = threadIdx.x / 8, c0 = threadIdx.x % 8 * 8;
   const bool queried = visible(a, len, nq, row0 + row) > 0;
@@ -720,6 +728,38 @@ void k_kv4_attend32(AttendArgs a) {
     put_row<kHalf>(a, wk, D, kRows, row, row0 + row, queried && lt != 0.0f, mx,
                    lt, 64 * g + c0, x, rg.splits);
   }
+}
+
+// Up to 16 query rows a workgroup: single tokens, and small groups of drafts.
+template <int D, bool kHalf>
+__global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 4)
+void k_kv4_attend16(AttendArgs a) {
+  __shared__ Lds<kLds16<D>> lds;
+  const Work wk = work_of(a);
+  if (!wk.any) return;
+  const int64_t len = kv_len_of(a, wk.b);
+  if (splits_of(a, len) <= wk.split) return;
+  attend16<D, kHalf, 16>(a, wk, len, q_len_of(a, wk.b), wk.qt * 16, lds);
+}
+
+// 32 query rows a workgroup: verification steps and prompts.  A tile of at most
+// 16 queries (of 17 tokens with four heads to a KV head, the last four rows)
+// takes the narrower instruction, which leaves half as many columns idle; its
+// sums do not fit this kernel's LDS for heads of 256.
+template <int D, bool kHalf>
+__global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3)
+void k_kv4_attend32(AttendArgs a) {
+  __shared__ Lds<kLds32<D>> lds;
+  const Work wk = work_of(a);
+  if (!wk.any) return;
+  const int64_t len = kv_len_of(a, wk.b);
+  if (splits_of(a, len) <= wk.split) return;
+  const int64_t nq = q_len_of(a, wk.b);
+  const int row0 = wk.qt * 32;
+  if (D <= 128 && nq * a.group - row0 <= 16)
+    attend16<D <= 128 ? D : 128, kHalf, 32>(a, wk, len, nq, row0, lds);
+  else
+    attend32<D, kHalf>(a, wk, len, nq, row0, lds);
 }
 
 // Joins the splits of query rows: a wave per row and KV head.  A lane holds a
