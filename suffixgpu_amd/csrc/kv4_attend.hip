@@ -11,7 +11,11 @@
 //   O = sum 2^(y_t - M) v_t (v_t as the 4 bits stand),  l = sum 2^(y_t - M) / s_t
 // so the weights stay within 16-bit range whatever the scales are, and O / l is
 // the result.  M only follows the maximum when that has grown by more than
-// kSlack, so most blocks rescale nothing and no maximum crosses lanes.
+// kSlack, so most blocks rescale nothing and no maximum crosses lanes (with a
+// slack of 0 64 x 17 tokens over up to 8,192 take 162 us instead of 146, a
+// prompt's 2,048 507 instead of 472; with single tokens it is the same).  The
+// largest weight is then between 1 and 2^8, and float16 rounds what is below
+// 2^-14 to steps of 2^-24.
 // Weights are rounded to float16 (11 bits, the finer of the 16-bit types, also
 // where the cache is bfloat16): the products accumulate in 32 bits, l is summed
 // from the unrounded weights.
@@ -789,7 +793,8 @@ __global__ __launch_bounds__(256) void k_kv4_join(AttendArgs a,
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
   const float f = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - mx);
-  float lt = f == 0.0f ? 0.0f : f * l;
+  // a split of nothing but NaN has no M, and an l that says so
+  float lt = f == 0.0f && l == l ? 0.0f : f * l;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) lt += __shfl_xor(lt, o);
   float x[C];
@@ -828,6 +833,23 @@ struct Plan {
   size_t bytes;
 };
 
+// Query rows by 16 where a KV head has no more than that, else by 32.  Measured
+// over up to 8,192 tokens, 64 rows, 8 KV heads of 128, four query heads each: 1
+// token (4 rows) 93 us by 16 and 100 by 32, 4 tokens (16) 98 and 107, 5 tokens
+// (20) 138 and 99, 17 tokens (68) 156 and 146; a prompt's 2,048 tokens after
+// 14,336 others 562 and 472.
+//
+// Splits: so many that with every row full the launch has about `want`
+// workgroups.  More even out rows of different lengths, fewer have less to join.
+// By 16, with 1,024 / 1,536 / 3,072: the 64 x 1 above 92 / 95 / 97 us, 200 rows
+// of up to 4,096 tokens and two KV heads 32 / 37 / 43.  By 32: 64 x 17 146 / 149
+// / 155, 16 x 17 over up to 32,768 164 / 149 / 147.  Heads of 256, of which fewer
+// workgroups fit a CU, with 512 / 1,024 / 1,536: 4 x 9 over up to 131,072 183 /
+// 205 / 207, 30 x 9 over up to 8,192 108 / 98 / 111.
+// At least kLeast blocks each: one token over 2,050 10.2 us, with 8 10.7, with 4
+// 13.2.
+constexpr int64_t kLeast = 16;
+
 Plan plan_for(const sfx_kv4* c, int64_t batch, int64_t tokens,
               int64_t q_heads) {
   Plan p;
@@ -837,10 +859,11 @@ Plan plan_for(const sfx_kv4* c, int64_t batch, int64_t tokens,
   const int64_t wgs = batch * c->heads * p.q_tiles;
   const int64_t blocks =
       std::max<int64_t>(1, c->table_width * c->page_size / kKvBlock);
-  const int64_t want = 1536;
-  const int64_t chunk = std::max<int64_t>(
-      {int64_t(16), (wgs * blocks + want - 1) / want,
-       (blocks + kMaxSplits - 1) / kMaxSplits});
+  const int64_t want =
+      p.rows_tile == 16 || c->head_dim == 256 ? 1024 : 1536;
+  const int64_t chunk =
+      std::max<int64_t>({kLeast, (wgs * blocks + want - 1) / want,
+                         (blocks + kMaxSplits - 1) / kMaxSplits});
   p.chunk = (int)std::min(chunk, blocks);
   p.splits = (int)((blocks + p.chunk - 1) / p.chunk);
   p.bytes = p.splits == 1 ? 0

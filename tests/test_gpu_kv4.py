@@ -266,6 +266,30 @@ def test_attend_long_row_is_split_and_joined(gpu, t):
     check_attend(out, q, kq, vq, vs, lens, [t] * 2, BF)
 
 
+@pytest.mark.parametrize("dtype,d", [(BF, 64), (BF, 128), (HF, 128), (HF, 256)])
+@pytest.mark.parametrize("t", [1, 17])
+def test_attend_splits_of_ragged_rows(gpu, dtype, d, t):
+    """Rows of many splits beside rows of one, in tiles of both heights and a
+    last tile of a few queries."""
+    lens = [4100, 700, t, 2600]
+    c, table, kq, vq, vs = filled(gpu, 4, lens, 2, d, 64, dtype, 55)
+    q = data(gpu, 4, t, 8, d, dtype, 56)
+    out = c.attend(q, table, ints(lens, gpu))
+    check_attend(out, q, kq, vq, vs, lens, [t] * 4, dtype)
+
+
+@pytest.mark.parametrize("n", [40, 3000])
+@pytest.mark.parametrize("t", [2, 20])
+def test_attend_nan_queries_say_so(gpu, n, t):
+    """A query that holds a NaN gives NaN, in one split or many, and no other
+    query does."""
+    c, table, *_ = filled(gpu, 1, [n], 1, 128, 64, BF, 57)
+    q = data(gpu, 1, t, 2, 128, BF, 58)
+    q[0, t - 1, 1, 5] = float("nan")
+    bad = torch.isnan(c.attend(q, table, ints([n], gpu)))
+    assert bad[0, t - 1, 1].all() and int(bad.sum()) == 128
+
+
 def test_attend_scales_far_apart(gpu):
     """Values whose scales differ by 2^40 and more, tokens of zero values, a
     large softmax scale: weights stay in range."""
