@@ -16,44 +16,28 @@ from suffixgpu_amd._lib import check, lib, require_gpu, stream_of
 
 
 # Counters and scratch, as (counters, scratch, counters' address, bytes, scratch's
-# address, bytes), by device and stream.  The
-# counters are zero between calls (every call leaves them so), the scratch is
-# anything; two calls that share them are ordered by their stream.  Calls
-# recorded into a HIP graph have a pair of their own for each stream recorded
-# (replays of graphs recorded on one stream must not overlap): a spare one that
-# eager calls keep ready, so that a capture after a first eager call of that
-# size records no fill.  Outgrown pairs of graphs are kept, a graph may hold
-# them.
+# address, bytes), by device and stream.  The counters are zero between calls
+# (every call leaves them so), the scratch is anything; two calls that share them
+# are ordered by their stream.  A call recorded into a HIP graph has a pair out of
+# the graph's own memory, cleared by a node of the graph: graphs recorded on one
+# stream may be replayed on others, at the same time and in any order.
 _workspaces: dict[tuple, tuple] = {}
-_outgrown: list[tuple] = []
 
 
 def _new_workspace(dev: torch.device, nc: int, ns: int) -> tuple:
-    c = torch.zeros(max(nc, 1 << 16), dtype=torch.uint8, device=dev)
-    s = torch.empty(max(ns, 1 << 18), dtype=torch.uint8, device=dev)
-    return c, s, c.data_ptr(), c.numel(), s.data_ptr(), s.numel()
+    c = torch.zeros(nc, dtype=torch.uint8, device=dev)
+    s = torch.empty(ns, dtype=torch.uint8, device=dev)
+    return c, s, c.data_ptr(), nc, s.data_ptr(), ns
 
 
 def _workspace(dev: torch.device, stream: int, nc: int, ns: int) -> tuple:
     """The pair for `stream`, with at least nc and ns bytes."""
-    spare = _workspaces.get((dev, "spare"))
     if torch.cuda.is_current_stream_capturing():
-        key = (dev, stream, "graph")
-        ws = _workspaces.get(key)
-        if ws is None or ws[3] < nc or ws[5] < ns:
-            if ws is not None:
-                _outgrown.append(ws)
-            if spare is not None and spare[3] >= nc and spare[5] >= ns:
-                ws = _workspaces.pop((dev, "spare"))
-            else:
-                ws = _new_workspace(dev, nc, ns)
-            _workspaces[key] = ws
-        return ws
-    if spare is None or spare[3] < nc or spare[5] < ns:
-        _workspaces[dev, "spare"] = _new_workspace(dev, 2 * nc, 2 * ns)
+        return _new_workspace(dev, nc, ns)
     ws = _workspaces.get((dev, stream))
     if ws is None or ws[3] < nc or ws[5] < ns:
-        ws = _workspaces[dev, stream] = _new_workspace(dev, 2 * nc, 2 * ns)
+        ws = _workspaces[dev, stream] = _new_workspace(
+            dev, max(2 * nc, 1 << 16), max(2 * ns, 1 << 18))
     return ws
 
 
@@ -100,7 +84,7 @@ def verify_draft(logits: torch.Tensor, draft: torch.Tensor,
 
     Returns (sampled [B, K + 1] int32: kept drafts, the drawn token, then -1;
     count [B] int32).  No host synchronisation; two launches on the current
-    stream.
+    stream, and a fill before them where they are recorded into a HIP graph.
     """
     require_gpu(logits)
     if logits.dim() != 3:

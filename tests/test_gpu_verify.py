@@ -232,6 +232,36 @@ def test_verify_under_graph(gpu):
         assert torch.equal(got[0], eager[0]) and torch.equal(got[1], eager[1])
 
 
+def test_verify_graphs_of_one_stream_replayed_on_two(gpu):
+    """Two graphs recorded by the same stream share nothing: replayed at the
+    same time, before and after other calls, each gives its own result, also
+    where no call of that size came before the recording."""
+    from suffixgpu_amd import verify_draft
+    cases = [inputs(gpu, 24, 7, 60013, torch.bfloat16, s) for s in (41, 42)]
+    record, graphs, outs = torch.cuda.Stream(), [], []
+    for s in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=record):
+            outs.append(verify_draft(**s))
+        graphs.append(g)
+    want = [verify_draft(**s) for s in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(10):
+        for pair in outs:
+            for t in pair:
+                t.fill_(-7)
+        for g, st in zip(graphs, streams):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                g.replay()
+        for st in streams:
+            torch.cuda.current_stream().wait_stream(st)
+        again = verify_draft(**cases[0])
+        torch.cuda.synchronize()
+        for got, exp in zip(outs + [again], want + want[:1]):
+            assert torch.equal(got[0], exp[0]) and torch.equal(got[1], exp[1])
+
+
 def test_verify_refusals(gpu):
     from suffixgpu_amd import verify_draft
     from suffixgpu_amd._lib import SuffixGPUError
