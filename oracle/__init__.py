@@ -25,8 +25,11 @@ itself):
   traces vs golden vectors.
 * ``drafter``        -- update_state / propose_with_update KATs; end-to-end
   golden vectors (local-only and local+global).
+* ``target``         -- the operators on the target model's side of a step, which
+  have no counterpart in the reference: definitions in 64 bits, checked by
+  closed forms (tests/test_target_ops.py).
 
-No function is left "parity unpinned" except the weighted vote's fp32 sum
+No function of the reference's is left "parity unpinned" except the weighted vote's fp32 sum
 order (weights are an expand_chain option the drafter never uses): float
 sums of weights are compared within the reference's own rtol=1e-4.
 """

@@ -66,6 +66,9 @@ constexpr int kAppendThreads = 256;
 // token, D/8 channels each.  Keys go from registers to memory; the values'
 // four bits cross LDS, where a thread turns eight tokens by eight channels.
 // Words whose eight tokens are not all new keep the others' bits.
+// 4 x 4,099 float16 tokens, 8 heads of 128: 20 us for 67 MB read and 18 MB
+// written, 4.2 TB/s of the 4.9 that a large copy moves, so the memory bounds it;
+// 64 x 17 tokens take 5.4 us and one token 4.0, hardly more than a launch.
 //
 // The instruction that rounds to 4 bits rounds to the nearest, ties to the even
 // code, after a division by a power of two: the keys' rule.  For values, whose
@@ -252,7 +255,7 @@ struct ReadArgs {
 };
 
 // One workgroup per block of 32 positions, KV head and row, the same threads
-// and tasks as the append's.
+// and tasks as the append's.  4 x 4,099 tokens as there: 18 us, 4.7 TB/s.
 template <int D, bool kHalf>
 __global__ __launch_bounds__(256) void k_kv4_read(ReadArgs a) {
   using L = KvLayout<D>;

@@ -735,6 +735,9 @@ __device__ __forceinline__ void attend32(const AttendArgs& a, const Work& wk,
 }
 
 // Up to 16 query rows a workgroup: single tokens, and small groups of drafts.
+// The memory bounds it: 64 single tokens over up to 8,192, 32 query heads on 8 KV
+// heads of 128, take 83 us for 422 MB, 5.1 TB/s (a large copy moves 4.9).  Four
+// waves a SIMD, 128 registers; and 36 KB of LDS.
 template <int D, bool kHalf>
 __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 4)
 void k_kv4_attend16(AttendArgs a) {
@@ -746,10 +749,20 @@ void k_kv4_attend16(AttendArgs a) {
   attend16<D, kHalf, 16>(a, wk, len, q_len_of(a, wk.b), wk.qt * 16, lds);
 }
 
-// 32 query rows a workgroup: verification steps and prompts.  A tile of at most
-// 16 queries (of 17 tokens with four heads to a KV head, the last four rows)
-// takes the narrower instruction, which leaves half as many columns idle; its
-// sums do not fit this kernel's LDS for heads of 256.
+// 32 query rows a workgroup: verification steps and prompts.  Up to some tens of
+// rows the memory bounds it as above (4 x 9 tokens, 16 query heads on 8 KV heads
+// of 256, over up to 131,072: 198 us for 1.07 GB, 5.4 TB/s), past that the vector
+// instructions: conversions from 4 bits, exponentials and the sums beside them
+// issue in 78% of a prompt's cycles, matrix instructions in 48% (2,048 tokens
+// after 14,336 others: 552 us, 930 TFLOP/s of the 1,210 that a large matrix
+// product reaches).  64 x 17 tokens over up to 8,192 lie between: 136 us for 440
+// MB, as three tiles convert each block of a full row anew.  Three waves a SIMD;
+// four spill (64 x 17 199 us then).
+//
+// A tile of at most 16 queries (of 17 tokens with four heads to a KV head, the
+// last four rows) takes the narrower instruction, which leaves half as many
+// columns idle (64 x 17 145 us, without 157; a prompt 552 and 566); its sums do
+// not fit this kernel's LDS for heads of 256.
 template <int D, bool kHalf>
 __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3)
 void k_kv4_attend32(AttendArgs a) {
