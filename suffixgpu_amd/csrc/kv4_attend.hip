@@ -250,7 +250,12 @@ __device__ __forceinline__ U4 load_q8(const uint16_t* p, bool vec, bool live) {
 // What a workgroup works on: rows [row0, row0 + rows of a group) of KV head h
 // of batch row b, one split of the row's blocks.  Workgroups go round the eight
 // XCDs in turn: those of the same blocks and other query rows follow each other
-// on one XCD, whose L2 then holds the blocks.
+// on one XCD, whose L2 then holds the blocks.  Splits that only long rows have
+// come last, and each split goes through the rows from another one on, so that
+// what leaves at once, and rows of one length, spread over XCDs and CUs: with a
+// row's splits, or its query rows, beside each other in the same order every
+// time, 64 x 12 tokens over up to 8,192 took 165 us instead of 144, 64 x 16 181
+// instead of 157, 100 rows of four KV heads over up to 6,000 64 instead of 56.
 struct Work {
   int64_t b;
   int h, qt, split;
@@ -261,13 +266,15 @@ __device__ __forceinline__ Work work_of(const AttendArgs& a) {
   Work w;
   const int id = (int)blockIdx.x;
   const int k = id >> 3;
-  w.qt = k % a.q_tiles;
-  const int64_t item = (int64_t)(k / a.q_tiles) * 8 + (id & 7);
-  w.split = (int)(item % a.splits);
-  const int64_t bh = item / a.splits;
+  const int group = k / a.q_tiles;
+  w.qt = (k + group) % a.q_tiles;
+  const int64_t item = (int64_t)group * 8 + (id & 7);
+  const int64_t rows = a.batch * a.c.heads;
+  w.split = (int)(item / rows);
+  const int64_t bh = (item + w.split * (rows * 3 / 8)) % rows;
   w.h = (int)(bh % a.c.heads);
   w.b = bh / a.c.heads;
-  w.any = w.b < a.batch;
+  w.any = w.split < a.splits;
   return w;
 }
 
@@ -847,18 +854,19 @@ struct Plan {
 };
 
 // Query rows by 16 where a KV head has no more than that, else by 32.  Measured
-// over up to 8,192 tokens, 64 rows, 8 KV heads of 128, four query heads each: 1
-// token (4 rows) 93 us by 16 and 100 by 32, 4 tokens (16) 98 and 107, 5 tokens
-// (20) 138 and 99, 17 tokens (68) 156 and 146; a prompt's 2,048 tokens after
-// 14,336 others 562 and 472.
+// over up to 8,192 tokens, 64 rows, 8 KV heads of 128, four query heads each:
+// single tokens (4 rows a head) and 4 tokens (16) the same either way, 92 and 97
+// us, by the smaller kernel; 5 tokens (20) 107 us by 16 and 100 by 32, 17 tokens
+// (68) 160 and 149; a prompt's 2,048 tokens after 14,336 others 682 and 570.
 //
 // Splits: so many that with every row full the launch has about `want`
 // workgroups.  More even out rows of different lengths, fewer have less to join.
-// By 16, with 1,024 / 1,536 / 3,072: the 64 x 1 above 92 / 95 / 97 us, 200 rows
-// of up to 4,096 tokens and two KV heads 32 / 37 / 43.  By 32: 64 x 17 146 / 149
-// / 155, 16 x 17 over up to 32,768 164 / 149 / 147.  Heads of 256, of which fewer
-// workgroups fit a CU, with 512 / 1,024 / 1,536: 4 x 9 over up to 131,072 183 /
-// 205 / 207, 30 x 9 over up to 8,192 108 / 98 / 111.
+// By 16, of which four workgroups fit a CU, with 512 / 1,024 / 1,536 / 2,048: the
+// 64 x 1 above 91 / 93 / 101 / 94 us, 100 rows of up to 6,000 tokens and four KV
+// heads 62 / 56 / 60 / 58.  By 32, of which three fit: 64 x 17 159 / 157 / 149 /
+// 150, 16 x 17 over up to 32,768 221 / 167 / 170 / 166.  Heads of 256, two: 4 x 9
+// over up to 131,072 198 / 203 / 205 / 215, 30 x 9 over up to 8,192 97 / 101 / 109
+// / 113.
 // At least kLeast blocks each: one token over 2,050 10.2 us, with 8 10.7, with 4
 // 13.2.
 constexpr int64_t kLeast = 16;
