@@ -761,7 +761,7 @@ void k_kv4_attend16(AttendArgs a) {
 // of 256, over up to 131,072: 198 us for 1.07 GB, 5.4 TB/s), past that the vector
 // instructions: conversions from 4 bits, exponentials and the sums beside them
 // issue in 78% of a prompt's cycles, matrix instructions in 48% (2,048 tokens
-// after 14,336 others: 552 us, 930 TFLOP/s of the 1,210 that a large matrix
+// after 14,336 others: 560 us, 920 TFLOP/s of the 1,210 that a large matrix
 // product reaches).  64 x 17 tokens over up to 8,192 lie between: 136 us for 440
 // MB, as three tiles convert each block of a full row anew.  Three waves a SIMD;
 // four spill (64 x 17 199 us then).

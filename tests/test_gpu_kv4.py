@@ -278,6 +278,17 @@ def test_attend_splits_of_ragged_rows(gpu, dtype, d, t):
     check_attend(out, q, kq, vq, vs, lens, [t] * 4, dtype)
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.1, 1e-30, 1e-38, 3.0])
+@pytest.mark.parametrize("d,t", [(128, 2), (128, 20), (256, 20)])
+def test_attend_any_scale(gpu, d, t, scale):
+    """Scales of zero (a mean), below it, next to it and large ones."""
+    n = 70
+    c, table, kq, vq, vs = filled(gpu, 1, [n], 1, d, 64, BF, 59)
+    q = data(gpu, 1, t, 2, d, BF, 60)
+    out = c.attend(q, table, ints([n], gpu), scale=scale)
+    check_attend(out, q, kq, vq, vs, [n], [t], BF, scale)
+
+
 @pytest.mark.parametrize("n", [40, 3000])
 @pytest.mark.parametrize("t", [2, 20])
 def test_attend_nan_queries_say_so(gpu, n, t):
