@@ -573,7 +573,8 @@ int sfx_kv4_read(const sfx_kv4* cache, int64_t batch, int64_t tokens,
 /* Attention of the newest tokens over the cache.  Row b holds kv_len[b]
  * tokens, the last q_len[b] of which (q_len == NULL: `tokens`) are q's tokens
  * 0 .. q_len[b] - 1; query i sees the positions up to its own,
- * kv_len - q_len + i.  out [batch, tokens, q_heads, head_dim], contiguous, in
+ * kv_len - q_len + i, that the table holds, whether or not kv_len itself lies
+ * past the table or q_len past `tokens`.  out [batch, tokens, q_heads, head_dim], contiguous, in
  * the cache's type: softmax(scale q k) v over what it sees, zeros for a query
  * that sees nothing and for tokens from q_len on.  Query head g uses KV head
  * g / (q_heads / heads).  workspace: sfx_kv4_attend_workspace_size bytes,

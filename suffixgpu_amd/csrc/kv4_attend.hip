@@ -278,23 +278,32 @@ __device__ __forceinline__ Work work_of(const AttendArgs& a) {
   return w;
 }
 
+// Lengths as given, also past the table and past the queries: where a query
+// stands is their difference.
 __device__ __forceinline__ int64_t kv_len_of(const AttendArgs& a, int64_t b) {
   const int64_t n = load_count(a.kv_len, a.kv64, b);
-  return n < 0 ? 0 : (n > a.c.positions ? a.c.positions : n);
+  return n < 0 ? 0 : n;
 }
 
 __device__ __forceinline__ int64_t q_len_of(const AttendArgs& a, int64_t b) {
   if (!a.q_len) return a.tokens;
   const int64_t n = load_count(a.q_len, a.q64, b);
-  return n < 0 ? 0 : (n > a.tokens ? a.tokens : n);
+  return n < 0 ? 0 : n;
 }
 
-// Positions that row r sees; 0: none.
+// Positions of the table that row r sees; 0: none.
 __device__ __forceinline__ int visible(const AttendArgs& a, int64_t len,
                                        int64_t nq, int r) {
   const int t = r / a.group;
-  const int64_t v = len - nq + t + 1;
-  return r < a.rows && t < nq && v > 0 ? (int)v : 0;
+  if (r >= a.rows || t >= nq) return 0;
+  const int64_t v = len - nq + t + 1;  // at most len
+  return v > a.c.positions ? (int)a.c.positions : (v > 0 ? (int)v : 0);
+}
+
+// Blocks of the table that a row holds.
+__device__ __forceinline__ int blocks_of(const AttendArgs& a, int64_t len) {
+  if (len > a.c.positions) len = a.c.positions;
+  return (int)((len + kKvBlock - 1) / kKvBlock);
 }
 
 // Splits of a row, and the blocks of one that rows of up to `most` visible
@@ -305,13 +314,13 @@ struct Range {
 };
 
 __device__ __forceinline__ int splits_of(const AttendArgs& a, int64_t len) {
-  const int blocks = (int)((len + kKvBlock - 1) / kKvBlock);
+  const int blocks = blocks_of(a, len);
   return max(1, (blocks + a.chunk - 1) / a.chunk);
 }
 
 __device__ __forceinline__ Range range_of(const AttendArgs& a, int64_t len,
                                           int most, int split) {
-  const int blocks = (int)((len + kKvBlock - 1) / kKvBlock);
+  const int blocks = blocks_of(a, len);
   Range r;
   r.splits = splits_of(a, len);
   const int per = (blocks + r.splits - 1) / r.splits;
@@ -780,7 +789,8 @@ void k_kv4_attend32(AttendArgs a) {
   if (splits_of(a, len) <= wk.split) return;
   const int64_t nq = q_len_of(a, wk.b);
   const int row0 = wk.qt * 32;
-  if (D <= 128 && nq * a.group - row0 <= 16)
+  const int64_t queries = nq < a.tokens ? nq : a.tokens;
+  if (D <= 128 && queries * a.group - row0 <= 16)
     attend16<D <= 128 ? D : 128, kHalf, 32>(a, wk, len, nq, row0, lds);
   else
     attend32<D, kHalf>(a, wk, len, nq, row0, lds);

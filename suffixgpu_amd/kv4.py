@@ -171,12 +171,14 @@ class KV4Cache:
 
         Row b holds ``kv_len[b]`` tokens (as appended, the new ones included);
         its last ``q_len[b]`` (T without it) are q's tokens 0 .. q_len - 1, and
-        query i sees the positions up to its own, kv_len - q_len + i.  q_heads
-        is a multiple of num_kv_heads, consecutive query heads sharing a KV
-        head.  ``scale`` defaults to head_dim ** -0.5.  Returns [B, T, q_heads,
-        head_dim] in the cache's type: zeros for a query that sees nothing and
-        for tokens from q_len on.  T = 1 is a decode step, T = k + 1 a
-        verification step, a long T a chunk of a prompt."""
+        query i sees the positions up to its own, kv_len - q_len + i.  Both
+        count tokens past the table's end, which no query sees (``append``
+        drops them), and q_len may be more than T.  q_heads is a multiple of
+        num_kv_heads, consecutive query heads sharing a KV head.  ``scale``
+        defaults to head_dim ** -0.5.  Returns [B, T, q_heads, head_dim] in the
+        cache's type: zeros for a query that sees nothing and for tokens from
+        q_len on.  T = 1 is a decode step, T = k + 1 a verification step, a
+        long T a chunk of a prompt."""
         qh, b, t, heads = self._heads("q", q)
         if heads < 1 or heads % self.num_kv_heads:
             raise ValueError(f"{heads} query heads do not share "

@@ -442,3 +442,32 @@ def test_cache_refusals(gpu):
     c.append(k[:0], k[:0], table[:0], n[:0])
     empty = torch.empty(2, 0, dtype=torch.int32, device=gpu)
     assert not c.attend(q, empty, n).any()
+
+
+# ------------------------------------------------ lengths past the ends
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 256)])
+@pytest.mark.parametrize("t,positions", [(1, 64), (10, 64), (17, 3008)])
+def test_attend_rows_past_their_table(gpu, dtype, d, t, positions):
+    """Tokens past the table hold nothing, but count: the queries of a row
+    whose drafts run past its last page stand where kv_len and q_len say."""
+    over = [0, 1, 6, 9, t + 3]
+    b, page = len(over), 32
+    c, table, kq, vq, vs = filled(gpu, b, [positions] * b, 2, d, page, dtype,
+                                  200)
+    lens = [positions + x for x in over]
+    q = data(gpu, b, t, 8, d, dtype, 201)
+    out = c.attend(q, table, ints(lens, gpu))
+    check_attend(out, q, kq, vq, vs, lens, [t] * b, dtype)
+    far = [1 << 40] * b                     # every query past the table
+    out = c.attend(q, table, ints(far, gpu, torch.int64))
+    check_attend(out, q, kq, vq, vs, [positions + t] * b, [t] * b, dtype)
+
+
+@pytest.mark.parametrize("t", [1, 4, 20])
+def test_attend_more_new_tokens_than_queries(gpu, t):
+    """q_len past T: the queries given are the first of the new tokens."""
+    lens, qn = [70, 70, 64, 5], [t + 1, t + 30, 1 << 20, t + 2]
+    c, table, kq, vq, vs = filled(gpu, 4, lens, 2, 128, 32, BF, 210)
+    q = data(gpu, 4, t, 4, 128, BF, 211)
+    out = c.attend(q, table, ints(lens, gpu), ints(qn, gpu, torch.int64))
+    check_attend(out, q, kq, vq, vs, lens, qn, BF)
