@@ -427,9 +427,11 @@ __device__ __forceinline__ void put_row(const AttendArgs& a, const Work& w,
   } else {
     float* p = a.part + ((((w.b * a.c.heads + w.h) * a.q_tiles + w.qt) *
                               a.splits + w.split) * rows_tile + row) * (d + 2);
+    // Rows that are no queries may have met a NaN that none of theirs sees: the
+    // join takes an l of NaN for a query's.
     if (c0 == 0) {
       p[0] = see ? mx : kNegInf;
-      p[1] = lt;
+      p[1] = see ? lt : 0.0f;
     }
     if (!see) return;
 #pragma unroll
@@ -823,7 +825,7 @@ __global__ __launch_bounds__(256) void k_kv4_join(AttendArgs a,
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
   const float f = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - mx);
-  // a split of nothing but NaN has no M, and an l that says so
+  // a query's split of nothing but NaN has no M, and an l that says so
   float lt = f == 0.0f && l == l ? 0.0f : f * l;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) lt += __shfl_xor(lt, o);

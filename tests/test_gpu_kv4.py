@@ -471,3 +471,31 @@ def test_attend_more_new_tokens_than_queries(gpu, t):
     q = data(gpu, 4, t, 4, 128, BF, 211)
     out = c.attend(q, table, ints(lens, gpu), ints(qn, gpu, torch.int64))
     check_attend(out, q, kq, vq, vs, lens, qn, BF)
+
+
+# ------------------------------------- NaN and the rows that are no queries
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("n", [60, 3000])
+@pytest.mark.parametrize("t,qn", [(2, 1), (8, 5), (20, 5), (20, 12), (20, 17)])
+def test_attend_nan_stays_out_of_padding(gpu, d, n, t, qn):
+    """A NaN query, an infinite key early in the row and a NaN value there make
+    the queries that see them NaN, and leave zeros from q_len on, in one split or
+    many and in tiles of both heights."""
+    def run(k=None, v=None, q=None):
+        c, table = make(gpu, 1, n, 1, d, 64, BF, 220)
+        kk, vv = data(gpu, 1, n, 1, d, BF, 221), data(gpu, 1, n, 1, d, BF, 222)
+        qq = data(gpu, 1, t, 2, d, BF, 223)
+        for x, at in ((kk, k), (vv, v), (qq, q)):
+            if at is not None:
+                x[at] = float("inf") if x is kk else float("nan")
+        c.append(kk, vv, table, ints([0], gpu))
+        out = c.attend(qq, table, ints([n], gpu), ints([qn], gpu))
+        assert not np64(out)[0, qn:].any()      # a NaN counts as not zero
+        return torch.isnan(out[0, :qn]).all(dim=-1)
+
+    assert not run().any()
+    assert run(k=(0, 3, 0, 40)).all()
+    assert run(v=(0, 3, 0, 40)).all()
+    for r in range(qn):
+        bad = run(q=(0, r, 1, 5))
+        assert bad[r, 1] and int(bad.sum()) == 1
