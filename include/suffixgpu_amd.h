@@ -607,7 +607,8 @@ int sfx_kv4_attend(const sfx_kv4* cache, const sfx_heads* q, int64_t batch,
  * row's temperature as 0.  counters: sfx_verify_counter_bytes bytes,
  * zero-filled once; every call leaves them zero, whatever its sizes.
  * workspace: sfx_verify_workspace_size bytes of any content.  Both 16-byte
- * aligned; calls that share either must not overlap. */
+ * aligned; calls that share either must not overlap, nor may one host thread's
+ * two launches have another's between them on the stream. */
 typedef struct sfx_verify {
     const void* logits;
     int32_t dtype;             /* SFX_BF16, SFX_F16 or SFX_F32            */

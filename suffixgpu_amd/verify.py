@@ -9,6 +9,8 @@ the engine's (its tests mimic one, suffix_gpu tests/test_verification.py).
 
 from __future__ import annotations
 
+import threading
+
 import torch
 
 from suffixgpu_amd import _lib
@@ -17,11 +19,13 @@ from suffixgpu_amd._lib import check, lib, require_gpu, stream_of
 
 # Counters and scratch, as (counters, scratch, counters' address, bytes, scratch's
 # address, bytes), by device and stream.  The counters are zero between calls
-# (every call leaves them so), the scratch is anything; two calls that share them
-# are ordered by their stream.  A call recorded into a HIP graph has a pair out of
+# (every call leaves them so), the scratch is anything.  Calls that share them are
+# ordered by their stream, each call's two launches side by side: the C call lets
+# other threads run, so it is made with `_enqueue` held.  A call recorded into a HIP graph has a pair out of
 # the graph's own memory, cleared by a node of the graph: graphs recorded on one
 # stream may be replayed on others, at the same time and in any order.
 _workspaces: dict[tuple, tuple] = {}
+_enqueue = threading.Lock()
 
 
 def _new_workspace(dev: torch.device, nc: int, ns: int) -> tuple:
@@ -123,10 +127,11 @@ def verify_draft(logits: torch.Tensor, draft: torch.Tensor,
         size = _sizes[b, k, v] = (L.sfx_verify_counter_bytes(b, k, v),
                                   L.sfx_verify_workspace_size(b, k, v))
     stream = stream_of(dev)
-    ws = _workspace(dev, stream, *size)
-    check(L.sfx_verify_draft(
-        _lib.SfxVerify(logits.data_ptr(), code, int(greedy), b, k, v, sb, sj,
-                       dp, np_, up, ep, tp, qp, sampled.data_ptr(),
-                       count.data_ptr()),
-        *ws[2:], stream), "verify_draft")
+    args = _lib.SfxVerify(logits.data_ptr(), code, int(greedy), b, k, v, sb,
+                          sj, dp, np_, up, ep, tp, qp, sampled.data_ptr(),
+                          count.data_ptr())
+    with _enqueue:
+        ws = _workspace(dev, stream, *size)
+        rc = L.sfx_verify_draft(args, *ws[2:], stream)
+    check(rc, "verify_draft")
     return sampled, count

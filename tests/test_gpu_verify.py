@@ -286,3 +286,30 @@ def test_verify_refusals(gpu):
     none = verify_draft(s["logits"][:0], s["draft"][:0], s["num_valid"][:0],
                         greedy=True)
     assert none[0].shape == (0, 4) and none[1].shape == (0,)
+
+
+def test_verify_from_threads_of_one_stream(gpu):
+    """Threads that share the default stream each get their own results, of
+    sizes that differ."""
+    import threading
+
+    from suffixgpu_amd import verify_draft
+    cases = [inputs(gpu, 24, 7, 40013, torch.bfloat16, 51),
+             inputs(gpu, 40, 3, 9001, torch.float32, 52)]
+    want = [verify_draft(**s) for s in cases]
+    torch.cuda.synchronize()
+    got = [[] for _ in cases]
+
+    def work(i):
+        got[i] = [verify_draft(**cases[i]) for _ in range(40)]
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i, exp in enumerate(want):
+        assert len(got[i]) == 40
+        for a in got[i]:
+            assert torch.equal(a[0], exp[0]) and torch.equal(a[1], exp[1])

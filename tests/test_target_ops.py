@@ -4,6 +4,9 @@ and of their Python forms, and the oracle's own ground."""
 from __future__ import annotations
 
 import ctypes
+import importlib
+import threading
+import time
 
 import numpy as np
 import pytest
@@ -12,6 +15,9 @@ import torch
 from oracle import target
 from suffixgpu_amd import KV4Cache, _lib, verify_draft
 from suffixgpu_amd.kv4 import block_bytes
+
+# the module; the package's name of it is the function
+verify = importlib.import_module("suffixgpu_amd.verify")
 
 
 def cache(**kw):
@@ -175,3 +181,58 @@ def test_oracle_attention_by_hand():
     q = np.zeros((1, 2, 1, 32))
     out, _ = target.attend(q, k, v, np.ones((1, 2, 1, 1)), [2], [2])
     assert out[0, :, 0, 0].tolist() == [1.0, 2.0]
+
+
+class _FakeLib:
+    """sfx_verify_draft that takes a while, as two launches do, and says whether
+    another call came in between."""
+
+    def __init__(self):
+        self.inside = self.most = 0
+        self.lock = threading.Lock()
+
+    def sfx_verify_counter_bytes(self, *_):
+        return 64
+
+    def sfx_verify_workspace_size(self, *_):
+        return 64
+
+    def sfx_verify_draft(self, *_):
+        with self.lock:
+            self.inside += 1
+            self.most = max(self.most, self.inside)
+        time.sleep(0.02)
+        with self.lock:
+            self.inside -= 1
+        return 0
+
+
+def test_verify_calls_of_two_threads_do_not_interleave(monkeypatch):
+    """A call's two launches hand their counters over, which calls on one stream
+    share: no other thread's launch comes between them."""
+    fake = _FakeLib()
+    monkeypatch.setattr(verify, "lib", lambda: fake)
+    monkeypatch.setattr(verify, "require_gpu", lambda *_: None)
+    monkeypatch.setattr(verify, "stream_of", lambda _: 0)
+    monkeypatch.setattr(verify, "_workspaces", {})
+    monkeypatch.setattr(verify, "_sizes", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing",
+                        lambda: False)
+    x = torch.zeros(1, 2, 8)
+    draft, num = (torch.zeros(1, 1, dtype=torch.int32),
+                  torch.zeros(1, dtype=torch.int32))
+    errors = []
+
+    def work():
+        try:
+            for _ in range(3):
+                verify_draft(x, draft, num, greedy=True)
+        except Exception as e:          # a thread's own exception is lost
+            errors.append(e)
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors and fake.most == 1
