@@ -56,7 +56,8 @@ struct KvView {
 template <int D>
 __device__ __forceinline__ char* kv_block(const KvView& c, int64_t b, int h,
                                           int64_t blk) {
-  if (blk < 0 || blk * kKvBlock >= c.positions) return nullptr;
+  // in blocks: a start next to 2^63 is past the table too
+  if ((uint64_t)blk >= (uint64_t)c.positions / kKvBlock) return nullptr;
   const int64_t page = c.table[b * c.table_stride + (blk >> c.page_shift)];
   if (page < 0 || page >= c.num_pages) return nullptr;
   const int64_t in = blk & ((int64_t(1) << c.page_shift) - 1);

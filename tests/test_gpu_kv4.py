@@ -499,3 +499,20 @@ def test_attend_nan_stays_out_of_padding(gpu, d, n, t, qn):
     for r in range(qn):
         bad = run(q=(0, r, 1, 5))
         assert bad[r, 1] and int(bad.sum()) == 1
+
+
+def test_positions_at_the_end_of_64_bits(gpu):
+    """Starts and lengths next to 2^63 lie past the table like any other:
+    nothing is read or written there."""
+    d, heads, t = 64, 2, 70
+    c, table, kq, vq, vs = filled(gpu, 2, [64, 64], heads, d, 32, BF, 260)
+    before = c.pages.clone()
+    far = ints([(1 << 63) - 1, (1 << 63) - 33], gpu, torch.int64)
+    gk, gv = c.read(table, far, t)
+    assert not np64(gk).any() and not np64(gv).any()
+    k = data(gpu, 2, t, heads, d, BF, 261)
+    c.append(k, k, table, far)
+    assert torch.equal(before, c.pages)
+    q = data(gpu, 2, 3, heads, d, BF, 262)
+    check_attend(c.attend(q, table, far), q, kq, vq, vs, [67, 67], [3, 3], BF)
+    assert not np64(c.attend(q, table, ints([64, 64], gpu), far)).any()
