@@ -133,5 +133,7 @@ def verify_draft(logits: torch.Tensor, draft: torch.Tensor,
     with _enqueue:
         ws = _workspace(dev, stream, *size)
         rc = L.sfx_verify_draft(args, *ws[2:], stream)
+        if rc:      # its counters may be anything
+            _workspaces.pop((dev, stream), None)
     check(rc, "verify_draft")
     return sampled, count

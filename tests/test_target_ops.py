@@ -236,3 +236,32 @@ def test_verify_calls_of_two_threads_do_not_interleave(monkeypatch):
     for t in threads:
         t.join()
     assert not errors and fake.most == 1
+
+
+def test_verify_counters_of_a_failed_call_are_not_used_again(monkeypatch):
+    """A call that fails between its launches leaves its counters anyhow: the next
+    one gets others, which are zero."""
+    seen = []
+
+    class Fake(_FakeLib):
+        def sfx_verify_draft(self, _, counters, nbytes, *__):
+            words = (ctypes.c_uint8 * nbytes).from_address(counters)
+            seen.append(bytes(words) == bytes(nbytes))
+            words[0] = 1
+            return 1 if len(seen) == 1 else 0
+
+    fake = Fake()
+    monkeypatch.setattr(verify, "lib", lambda: fake)
+    monkeypatch.setattr(verify, "require_gpu", lambda *_: None)
+    monkeypatch.setattr(verify, "stream_of", lambda _: 0)
+    monkeypatch.setattr(verify, "_workspaces", {})
+    monkeypatch.setattr(verify, "_sizes", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing",
+                        lambda: False)
+    x = torch.zeros(1, 2, 8)
+    draft, num = (torch.zeros(1, 1, dtype=torch.int32),
+                  torch.zeros(1, dtype=torch.int32))
+    with pytest.raises(_lib.SuffixGPUError):
+        verify_draft(x, draft, num, greedy=True)
+    verify_draft(x, draft, num, greedy=True)
+    assert seen == [True, True]
