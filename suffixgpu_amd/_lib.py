@@ -306,6 +306,13 @@ def stream_of(device: torch.device) -> int:
     return _raw_stream(device.index)
 
 
+def elsewhere(device: torch.device) -> bool:
+    """Whether another device is current: launches on a default stream go to
+    the current one."""
+    return (device.index is not None
+            and torch.cuda.current_device() != device.index)
+
+
 def make_params(k: int, max_pattern_len: int, max_occurrences: int,
                 min_match_len: int, thresholds, caps,
                 max_spec_factor: float | None, max_spec_offset: float,

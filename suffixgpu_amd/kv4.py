@@ -14,8 +14,8 @@ from __future__ import annotations
 import torch
 
 from suffixgpu_amd import _lib
-from suffixgpu_amd._lib import (SuffixGPUError, check, count_arg, lib,
-                                require_gpu, stream_of)
+from suffixgpu_amd._lib import (SuffixGPUError, check, count_arg, elsewhere,
+                                lib, require_gpu, stream_of)
 
 BLOCK = 32  # tokens
 
@@ -131,6 +131,9 @@ class KV4Cache:
         A page that one row of a call writes must not be written by another
         row of it.  Infinities and NaN make their 32 channels of a key, or
         their token's values, NaN."""
+        if elsewhere(self.device):
+            with torch.cuda.device(self.device):
+                return self.append(k, v, page_table, start, count)
         kh, b, t, _ = self._heads("k", k, self.num_kv_heads)
         vh, vb, vt, _ = self._heads("v", v, self.num_kv_heads)
         if b != vb or t != vt:
@@ -149,6 +152,9 @@ class KV4Cache:
         """The keys and values [B, tokens, num_kv_heads, head_dim] that the
         cache holds at positions ``start[b] + i``, i < ``count[b]``; zeros
         elsewhere."""
+        if elsewhere(self.device):
+            with torch.cuda.device(self.device):
+                return self.read(page_table, start, tokens, count)
         b = page_table.shape[0]
         view = self._view(page_table, b)
         keep = (self._counts("start", start, b),
@@ -179,6 +185,9 @@ class KV4Cache:
         cache's type: zeros for a query that sees nothing and for tokens from
         q_len on.  T = 1 is a decode step, T = k + 1 a verification step, a
         long T a chunk of a prompt."""
+        if elsewhere(self.device):
+            with torch.cuda.device(self.device):
+                return self.attend(q, page_table, kv_len, q_len, scale)
         qh, b, t, heads = self._heads("q", q)
         if heads < 1 or heads % self.num_kv_heads:
             raise ValueError(f"{heads} query heads do not share "

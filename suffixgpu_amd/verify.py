@@ -14,7 +14,8 @@ import threading
 import torch
 
 from suffixgpu_amd import _lib
-from suffixgpu_amd._lib import check, lib, require_gpu, stream_of
+from suffixgpu_amd._lib import (check, elsewhere, lib, require_gpu,
+                                stream_of)
 
 
 # Counters and scratch, as (counters, scratch, counters' address, bytes, scratch's
@@ -91,6 +92,11 @@ def verify_draft(logits: torch.Tensor, draft: torch.Tensor,
     stream, and a fill before them where they are recorded into a HIP graph.
     """
     require_gpu(logits)
+    dev = logits.device
+    if elsewhere(dev):
+        with torch.cuda.device(dev):
+            return verify_draft(logits, draft, num_valid, uniform, noise,
+                                temperature, draft_probs, greedy)
     if logits.dim() != 3:
         raise ValueError("logits must be [B, K + 1, V]")
     b, k1, v = logits.shape
@@ -102,7 +108,6 @@ def verify_draft(logits: torch.Tensor, draft: torch.Tensor,
     sb, sj, sv = logits.stride()
     if sv != 1 and v > 1:
         raise ValueError("logits must be contiguous along the vocabulary")
-    dev = logits.device
     k = k1 - 1
     dp = _need("draft", draft, (b, k), torch.int32, dev)
     np_ = _need("num_valid", num_valid, (b,), torch.int32, dev)

@@ -58,3 +58,26 @@ def keys_by_definition(corpus: torch.Tensor, sa: torch.Tensor,
         if bool(bad.any()):
             r = r0 + int(bad.nonzero()[0, 0])
             raise AssertionError(f"key row {r} differs from its definition")
+
+
+@pytest.fixture
+def elsewhere(gpu, monkeypatch):
+    """As if another device than the tensors' were current; the devices that
+    calls then make current."""
+    import torch
+    now, entered = [gpu.index + 1], []
+    real = torch.cuda.device
+
+    class Device(real):
+        def __enter__(self):
+            now.append(self.idx)
+            entered.append(self.idx)
+            return super().__enter__()
+
+        def __exit__(self, *e):
+            now.pop()
+            return super().__exit__(*e)
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[-1])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    return entered

@@ -516,3 +516,16 @@ def test_positions_at_the_end_of_64_bits(gpu):
     q = data(gpu, 2, 3, heads, d, BF, 262)
     check_attend(c.attend(q, table, far), q, kq, vq, vs, [67, 67], [3, 3], BF)
     assert not np64(c.attend(q, table, ints([64, 64], gpu), far)).any()
+
+
+def test_cache_calls_make_their_device_current(gpu, elsewhere):
+    """Launches go to the current device, whichever the tensors' is."""
+    lens = [70, 33]
+    c, table, kq, vq, vs = filled(gpu, 2, lens, 2, 64, 32, BF, 270)
+    assert elsewhere == [0]
+    q = data(gpu, 2, 3, 4, 64, BF, 271)
+    out = c.attend(q, table, ints(lens, gpu))
+    check_attend(out, q, kq, vq, vs, lens, [3, 3], BF)
+    gk, _ = c.read(table, ints([0, 0], gpu), 33)
+    np.testing.assert_array_equal(np64(gk), kq[:, :33])
+    assert elsewhere == [0, 0, 0]

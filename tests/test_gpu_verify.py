@@ -313,3 +313,9 @@ def test_verify_from_threads_of_one_stream(gpu):
         assert len(got[i]) == 40
         for a in got[i]:
             assert torch.equal(a[0], exp[0]) and torch.equal(a[1], exp[1])
+
+
+def test_verify_makes_its_device_current(gpu, elsewhere):
+    """Launches go to the current device, whichever the tensors' is."""
+    check(inputs(gpu, 6, 4, 3000, torch.bfloat16, 61))
+    assert elsewhere == [0]
