@@ -71,12 +71,17 @@ class KV4Cache:
                              f"tensor on {self.device}")
         elif pages.data_ptr() % 16:
             raise ValueError("pages must be 16-byte aligned")
-        self.pages = pages
+        self._pages = pages
         # what every call's C view begins with, and workspace bytes by shape
         self._geometry = (pages.data_ptr(), self.num_pages, self.num_kv_heads,
                           self.head_dim, self.page_size,
                           _lib.DTYPE_CODES[dtype])
         self._sizes: dict[tuple, int] = {}
+
+    @property
+    def pages(self) -> torch.Tensor:
+        """The pool, for as long as the cache lives."""
+        return self._pages
 
     # ------------------------------------------------------------------
     def _view(self, page_table: torch.Tensor, rows: int) -> _lib.SfxKv4:

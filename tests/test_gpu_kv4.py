@@ -529,3 +529,10 @@ def test_cache_calls_make_their_device_current(gpu, elsewhere):
     gk, _ = c.read(table, ints([0, 0], gpu), 33)
     np.testing.assert_array_equal(np64(gk), kq[:, :33])
     assert elsewhere == [0, 0, 0]
+
+
+def test_cache_keeps_its_pool(gpu):
+    """Calls hold the pool's address, so the pool cannot be exchanged."""
+    c, _ = make(gpu, 1, 32, 1, 64, 32, BF, 280)
+    with pytest.raises(AttributeError):
+        c.pages = torch.zeros_like(c.pages)
