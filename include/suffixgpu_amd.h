@@ -521,7 +521,7 @@ int sfx_ingest_swapped(void* state, hipStream_t stream);
  *   D/64 x 64 x 16   values: the 32-bit word [c / 64][2 s + h][c % 16]
  *                    [c / 16 % 4] holds in its j-th 4 bits channel c of
  *                    token 16 s + 8 (j / 4) + 4 h + j % 4 of the block
- *   32 x 4 bytes     value scales (float), one per token
+ *   32 x 4 bytes     value scales (float), one per token, not negative
  * Four bits are a sign and one of 0, .5, 1, 1.5, 2, 3, 4, 6.  A byte of 255
  * as a key scale makes its 32 channels NaN.
  * table: [rows, table_width] page ids with a row stride (elements); position

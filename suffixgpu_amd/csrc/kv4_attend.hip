@@ -16,11 +16,19 @@
 // prompt's 2,048 507 instead of 472; with single tokens it is the same).  The
 // largest weight is then between 1 and 2^8, and float16 rounds what is below
 // 2^-14 to steps of 2^-24.
+// A term of l is 2^(x_t - M), and where s_t is far below the scale that M comes
+// from, 2^(y_t - M) vanishes before 1 / s_t can bring it back: a token of zeros
+// beside one of large values would not count.  So from its first block on with a
+// scale outside [2^-20, 2^60], zero and NaN included, a wave takes l's
+// exponentials for themselves, relative to a maximum of x_t (ml), at the price of
+// a second exponential per score.  As long as all scales lie within, what
+// vanishes is less than 2^-106 a token, and the largest term at least 2^-60.
 // Weights are rounded to float16 (11 bits, the finer of the 16-bit types, also
 // where the cache is bfloat16): the products accumulate in 32 bits, l is summed
 // from the unrounded weights.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kv4.h"
 #include "launch.h"
@@ -40,6 +48,7 @@ typedef uint32_t U4 __attribute__((ext_vector_type(4)));
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kSlack = 8.0f;
 constexpr int kWaves = 4;
+constexpr int kPart = 4;  // floats before the channels of a split's part
 
 struct AttendArgs {
   KvView c;
@@ -58,7 +67,8 @@ struct AttendArgs {
   int kv64, q64;
   float scale;     // times log2(e)
   uint16_t* out;
-  float* part;     // [batch, heads, q_tiles, splits, rows of a group, D + 2]
+  float* part;     // [batch, heads, q_tiles, splits, rows of a group,
+                   //  kPart + D]: M, l, what l is relative to, and O
 };
 
 // Eight 4-bit values of a word as 16-bit ones, times `scale` (a power of two,
@@ -352,18 +362,27 @@ __device__ __forceinline__ void share_scales(float vs, float* lds) {
   asm volatile("" ::: "memory");
 }
 
+// Whether any of a block's tokens that a row of the wave may see (those before
+// `most`) has a scale outside [2^-20, 2^60], NaN and zero included.
+__device__ __forceinline__ bool scales_apart(float vs, int blk, int most) {
+  constexpr uint32_t kLo = (127 - 20) << 23, kHi = (127 + 60) << 23;
+  return __any(__float_as_uint(vs) - kLo > kHi - kLo &&
+               lane_id() % 32 < most - blk * kKvBlock);
+}
+
 // Goes through blocks first, first + kWaves, ... below last of row b and KV head
 // h, by one wave for which all of these are the same: body(block, index, kdone,
 // vdone) calls kdone() when it has used the keys and vdone() when it has used
 // the values, which load the next block's into the same registers.  A second
 // set for the loads under way would cost a wave in three; issued this early
 // they are as well hidden.  A block's page id is read (as a scalar) one block
-// ahead of that.  Blocks without a page are left out.
-template <class B, class F>
-__device__ __forceinline__ void each_block(const KvView& c, int64_t b, int h,
-                                           int bytes, int first, int last,
-                                           F body) {
-  if (first >= last || c.num_pages == 0) return;
+// ahead of that.  Blocks without a page are left out.  Ends before a block that
+// stop(block, index) says to stop at; returns where it ended.
+template <class B, class P, class F>
+__device__ __forceinline__ int each_block(const KvView& c, int64_t b, int h,
+                                          int bytes, int first, int last,
+                                          P stop, F body) {
+  if (first >= last || c.num_pages == 0) return last;
   typedef const __attribute__((address_space(4))) int32_t* Ids;
   const Ids ids = (Ids)(uintptr_t)(c.table + b * c.table_stride);
   const int in_page = (1 << c.page_shift) - 1;
@@ -379,10 +398,12 @@ __device__ __forceinline__ void each_block(const KvView& c, int64_t b, int h,
   int32_t id = page(first), id1 = page(first + kWaves);
   x.load_k(at(id, first));
   x.load_v(at(id, first));
-  for (int blk = first; blk < last; blk += kWaves) {
+  int blk = first;
+  for (; blk < last; blk += kWaves) {
     const char* next = at(id1, blk + kWaves);
     const int32_t id2 = page(blk + 2 * kWaves);
     if (good(id)) {
+      if (stop(x, blk)) break;
       body(x, blk, [&]() { x.load_k(next); }, [&]() { x.load_v(next); });
     } else {
       x.load_k(next);
@@ -391,6 +412,31 @@ __device__ __forceinline__ void each_block(const KvView& c, int64_t b, int h,
     id = id1;
     id1 = id2;
   }
+  return blk;
+}
+
+// Goes through a wave's blocks in one loop with l relative to M and, from the
+// first block on whose scales are apart, in another with l for itself:
+// body(apart, ...) as above, apart a constant; switched() between them.  (One
+// loop with a flag takes ten registers more, and a workgroup of a CU with them.)
+template <class B, class G, class F>
+__device__ __forceinline__ bool both_loops(const KvView& c, int64_t b, int h,
+                                           int bytes, int first, int last,
+                                           int most, G switched, F body) {
+  const int at = each_block<B>(
+      c, b, h, bytes, first, last,
+      [&](const B& x, int blk) { return scales_apart(x.vs, blk, most); },
+      [&](B& x, int blk, auto kdone, auto vdone) {
+        body(std::false_type(), x, blk, kdone, vdone);
+      });
+  if (at >= last) return false;
+  switched();
+  each_block<B>(
+      c, b, h, bytes, at, last, [](const B&, int) { return false; },
+      [&](B& x, int blk, auto kdone, auto vdone) {
+        body(std::true_type(), x, blk, kdone, vdone);
+      });
+  return true;
 }
 
 // Follows the maximum of a row's scores when it has grown by more than kSlack:
@@ -406,38 +452,90 @@ __device__ __forceinline__ float follow(float top, float* m) {
   return f;
 }
 
+// Adds a lane's N weights of a block to l = sum 2^(x - ml): x(j, less) is the
+// j-th score in base 2 less `less`, -inf where the row does not see it.
+template <int kLanes, int N, class F>
+__device__ __forceinline__ void sum_apart(F x, float* ml, float* l) {
+  float top = kNegInf;
+#pragma unroll
+  for (int j = 0; j < N; ++j) top = fmaxf(top, x(j, 0.0f));
+  if (__any(top > *ml + kSlack)) *l *= follow<kLanes>(top, ml);
+  const float less = *ml == kNegInf ? 0.0f : *ml;
+#pragma unroll
+  for (int j = 0; j < N; ++j) *l += __builtin_amdgcn_exp2f(x(j, less));
+}
+
+// M, l and what l is relative to.
+struct Sums {
+  float m, l, ml;
+};
+
+// What a result's channels are O times: 2^(M - ml) / l, by halves of the power,
+// which may be larger than a float where the result is not.
+struct Factor {
+  float inv, half;
+  __device__ __forceinline__ Factor(const Sums& s) {
+    half = __builtin_amdgcn_exp2f(0.5f * (s.m - s.ml));
+    inv = half / s.l;
+  }
+  __device__ __forceinline__ float operator()(float o) const {
+    return o * inv * half;
+  }
+};
+
+// Joins the waves' sums of a row; f: the factors of their O.
+template <class S>
+__device__ __forceinline__ Sums join_waves(const S& lds, int row,
+                                           float (&f)[kWaves]) {
+  Sums r = {kNegInf, 0.0f, kNegInf};
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    r.m = fmaxf(r.m, lds.m[w][row]);
+    r.ml = fmaxf(r.ml, lds.ml[w][row]);
+  }
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const float m = lds.m[w][row], ml = lds.ml[w][row];
+    f[w] = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - r.m);
+    const float fl = ml == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ml - r.ml);
+    r.l = __builtin_fmaf(fl, lds.l[w][row], r.l);
+  }
+  return r;
+}
+
 // Writes a row's joined channels c0 .. c0 + N of the workgroup's waves: to the
-// result, or to this split's part.  x: the sum, lt: l, mx: M.
+// result, or to this split's part.  x: the sum O.
 template <bool kHalf, int N>
 __device__ __forceinline__ void put_row(const AttendArgs& a, const Work& w,
                                         int d, int rows_tile, int row, int r,
-                                        bool see, float mx, float lt, int c0,
+                                        bool see, const Sums& sums, int c0,
                                         const float (&x)[N], int splits) {
   if (r >= a.rows) return;
   if (splits == 1) {
-    const float inv = see ? 1.0f / lt : 0.0f;
+    const Factor by(sums);
     uint32_t* out = (uint32_t*)(a.out + ((w.b * a.tokens + r / a.group) *
                                              a.q_heads +
                                          w.h * a.group + r % a.group) * d + c0);
 #pragma unroll
     for (int c = 0; c < N; c += 2)
-      out[c / 2] = see ? from_float16b<kHalf>(x[c] * inv) |
-                             from_float16b<kHalf>(x[c + 1] * inv) << 16
+      out[c / 2] = see ? from_float16b<kHalf>(by(x[c])) |
+                             from_float16b<kHalf>(by(x[c + 1])) << 16
                        : 0u;
   } else {
     float* p = a.part + ((((w.b * a.c.heads + w.h) * a.q_tiles + w.qt) *
-                              a.splits + w.split) * rows_tile + row) * (d + 2);
+                              a.splits + w.split) * rows_tile + row) * (d + kPart);
     // Rows that are no queries may have met a NaN that none of theirs sees: the
     // join takes an l of NaN for a query's.
     if (c0 == 0) {
-      p[0] = see ? mx : kNegInf;
-      p[1] = see ? lt : 0.0f;
+      p[0] = see ? sums.m : kNegInf;
+      p[1] = see ? sums.l : 0.0f;
+      p[2] = see ? sums.ml : kNegInf;
     }
     if (!see) return;
 #pragma unroll
     for (int c = 0; c < N; c += 2) {
       typedef float F2 __attribute__((ext_vector_type(2)));
-      *(F2*)(p + 2 + c0 + c) = F2{x[c], x[c + 1]};
+      *(F2*)(p + kPart + c0 + c) = F2{x[c], x[c + 1]};
     }
   }
 }
@@ -447,7 +545,7 @@ __device__ __forceinline__ void put_row(const AttendArgs& a, const Work& w,
 template <int kBytes>
 struct Lds {
   __align__(16) char pool[kBytes];
-  float m[kWaves][32], l[kWaves][32];
+  float m[kWaves][32], l[kWaves][32], ml[kWaves][32];
   float scales[kWaves][64];
 };
 
@@ -493,14 +591,16 @@ __device__ __forceinline__ void attend16(const AttendArgs& a, const Work& wk,
   const Range rg = range_of(a, len, most, wk.split);
   const int first = rg.first + wave, last = rg.last;
 
-  float m = kNegInf, l = 0.0f;
+  float m = kNegInf, l = 0.0f, ml = kNegInf;
   F4 o[kDt];
 #pragma unroll
   for (int d = 0; d < kDt; ++d) o[d] = F4{0, 0, 0, 0};
 
-  each_block<Block<D, 16>>(a.c, wk.b, wk.h, KvLayout<D>::kBytes, first, last,
-                           [&](Block<D, 16>& kb, int blk, auto kdone,
-                               auto vdone) {
+  const bool apart = both_loops<Block<D, 16>>(
+      a.c, wk.b, wk.h, KvLayout<D>::kBytes, first, last, most,
+      [&]() { ml = m; },
+      [&](auto apart, Block<D, 16>& kb, int blk, auto kdone, auto vdone) {
+    constexpr bool kApart = decltype(apart)::value;
     share_scales(kb.vs, sc[wave]);
     const int p0 = blk * kKvBlock + 16 * (quad / 2) + 4 * (quad % 2);
     const bool edge = blk * kKvBlock + kKvBlock > least;
@@ -511,6 +611,14 @@ __device__ __forceinline__ void attend16(const AttendArgs& a, const Work& wk,
       for (int i = 0; i < kStep; ++i)
         s[t] = mma16<kHalf>(widen<kHalf>(kb.k[t][i], kb.scale(t, i)), qf[i],
                             s[t]);
+    if constexpr (kApart) {
+      auto x = [&](int j, float less) {
+        return p0 + 8 * (j / 4) + j % 4 < vis
+                   ? __builtin_fmaf(s[j / 4][j % 4], a.scale, -less)
+                   : kNegInf;
+      };
+      sum_apart<16, 8>(x, &ml, &l);
+    }
     kdone();
     F4 ls[2], rs[2];
 #pragma unroll
@@ -535,7 +643,7 @@ __device__ __forceinline__ void attend16(const AttendArgs& a, const Work& wk,
     for (int j = 0; j < 8; ++j) top = fmaxf(top, y[j]);
     if (__any(top > m + kSlack)) {
       const float f = follow<16>(top, &m);
-      l *= f;
+      if (!kApart) l *= f;
 #pragma unroll
       for (int d = 0; d < kDt; ++d) o[d] *= f;
     }
@@ -544,7 +652,8 @@ __device__ __forceinline__ void attend16(const AttendArgs& a, const Work& wk,
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       w[j] = __builtin_amdgcn_exp2f(y[j] - mu);
-      l = __builtin_fmaf(w[j], rs[j / 4][j % 4], l);
+      // (times zero a weight of NaN still makes l NaN)
+      l = __builtin_fmaf(w[j], kApart ? 0.0f : rs[j / 4][j % 4], l);
     }
     const U4 pf = {pack_half(w[0], w[1]), pack_half(w[2], w[3]),
                    pack_half(w[4], w[5]), pack_half(w[6], w[7])};
@@ -555,6 +664,7 @@ __device__ __forceinline__ void attend16(const AttendArgs& a, const Work& wk,
   });
 
   // Join the waves in LDS; 16 threads a row, D / 16 channels each.
+  if (!apart) ml = m;
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
 #pragma unroll
@@ -562,19 +672,12 @@ __device__ __forceinline__ void attend16(const AttendArgs& a, const Work& wk,
   if (quad == 0) {
     sm[wave][col] = m;
     sl[wave][col] = l;
+    lds.ml[wave][col] = ml;
   }
   __syncthreads();
   const int row = threadIdx.x / 16, c0 = threadIdx.x % 16 * (D / 16);
-  float mx = kNegInf;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, sm[w][row]);
-  float f[kWaves], lt = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    f[w] = sm[w][row] == kNegInf ? 0.0f
-                                 : __builtin_amdgcn_exp2f(sm[w][row] - mx);
-    lt = __builtin_fmaf(f[w], sl[w][row], lt);
-  }
+  float f[kWaves];
+  const Sums sums = join_waves(lds, row, f);
   float x[D / 16];
 #pragma unroll
   for (int c = 0; c < D / 16; ++c) {
@@ -583,12 +686,12 @@ __device__ __forceinline__ void attend16(const AttendArgs& a, const Work& wk,
     for (int w = 0; w < kWaves; ++w)
       x[c] = __builtin_fmaf(f[w], so[w][row][c0 + c], x[c]);
   }
-  const bool see = visible(a, len, nq, row0 + row) > 0 && lt != 0.0f;
-  put_row<kHalf>(a, wk, D, kTileRows, row, row0 + row, see, mx, lt, c0, x,
+  const bool see = visible(a, len, nq, row0 + row) > 0 && sums.l != 0.0f;
+  put_row<kHalf>(a, wk, D, kTileRows, row, row0 + row, see, sums, c0, x,
                  rg.splits);
   if (kTileRows > 16)
-    put_row<kHalf>(a, wk, D, kTileRows, row + 16, row0 + row + 16, false, mx,
-                   lt, c0, x, rg.splits);
+    put_row<kHalf>(a, wk, D, kTileRows, row + 16, row0 + row + 16, false, sums,
+                   c0, x, rg.splits);
 }
 
 // 32 query rows from row0 on.  They lie in LDS in the order of the matrix
@@ -630,16 +733,18 @@ __device__ __forceinline__ void attend32(const AttendArgs& a, const Work& wk,
   const int first = rg.first + wave, last = rg.last;
   __syncthreads();
 
-  float m = kNegInf, l = 0.0f;
+  float m = kNegInf, l = 0.0f, ml = kNegInf;
   F16 o[kDt];
 #pragma unroll
   for (int d = 0; d < kDt; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
 
-  each_block<Block<D, 32>>(a.c, wk.b, wk.h, KvLayout<D>::kBytes, first, last,
-                           [&](Block<D, 32>& kb, int blk, auto kdone,
-                               auto vdone) {
+  const bool apart = both_loops<Block<D, 32>>(
+      a.c, wk.b, wk.h, KvLayout<D>::kBytes, first, last, most,
+      [&]() { ml = m; },
+      [&](auto apart, Block<D, 32>& kb, int blk, auto kdone, auto vdone) {
+    constexpr bool kApart = decltype(apart)::value;
     share_scales(kb.vs, sc[wave]);
     const int p0 = blk * kKvBlock + 4 * h2;
     const bool edge = blk * kKvBlock + kKvBlock > least;
@@ -668,6 +773,14 @@ __device__ __forceinline__ void attend32(const AttendArgs& a, const Work& wk,
 #pragma unroll
     for (int g = 0; g < 4; ++g)
       rs[g] = *(const F4*)&sc[wave][32 + 8 * g + 4 * h2];
+    if constexpr (kApart) {
+      auto x = [&](int r, float less) {
+        return p0 + r / 4 * 8 + r % 4 < vis
+                   ? __builtin_fmaf(s[r], a.scale, -less)
+                   : kNegInf;
+      };
+      sum_apart<32, 16>(x, &ml, &l);
+    }
     kdone();
     float top = kNegInf;
 #pragma unroll
@@ -683,7 +796,7 @@ __device__ __forceinline__ void attend32(const AttendArgs& a, const Work& wk,
     for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
     if (__any(top > m + kSlack)) {
       const float f = follow<32>(top, &m);
-      l *= f;
+      if (!kApart) l *= f;
 #pragma unroll
       for (int d = 0; d < kDt; ++d) o[d] *= f;
     }
@@ -695,7 +808,7 @@ __device__ __forceinline__ void attend32(const AttendArgs& a, const Work& wk,
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         w[r] = __builtin_amdgcn_exp2f(s[4 * g + r] - mu);
-        l = __builtin_fmaf(w[r], rs[g][r], l);
+        l = __builtin_fmaf(w[r], kApart ? 0.0f : rs[g][r], l);
       }
       pf[g / 2][g % 2 * 2] = pack_half(w[0], w[1]);
       pf[g / 2][g % 2 * 2 + 1] = pack_half(w[2], w[3]);
@@ -710,6 +823,7 @@ __device__ __forceinline__ void attend32(const AttendArgs& a, const Work& wk,
 
   // Join the waves in LDS, 64 channels at a time: 8 threads a row.
   auto so = (float(*)[32][64 + 4])lds.pool;
+  if (!apart) ml = m;
   l += __shfl_xor(l, 32);
   const int row = threadIdx.x / 8, c0 = threadIdx.x % 8 * 8;
   const bool queried = visible(a, len, nq, row0 + row) > 0;
@@ -727,18 +841,11 @@ __device__ __forceinline__ void attend32(const AttendArgs& a, const Work& wk,
     if (h2 == 0) {
       sm[wave][col] = m;
       sl[wave][col] = l;
+      lds.ml[wave][col] = ml;
     }
     __syncthreads();
-    float mx = kNegInf;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, sm[w][row]);
-    float f[kWaves], lt = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      f[w] = sm[w][row] == kNegInf ? 0.0f
-                                   : __builtin_amdgcn_exp2f(sm[w][row] - mx);
-      lt = __builtin_fmaf(f[w], sl[w][row], lt);
-    }
+    float f[kWaves];
+    const Sums sums = join_waves(lds, row, f);
     float x[8];
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
@@ -747,8 +854,8 @@ __device__ __forceinline__ void attend32(const AttendArgs& a, const Work& wk,
       for (int w = 0; w < kWaves; ++w)
         x[c] = __builtin_fmaf(f[w], so[w][row][c0 + c], x[c]);
     }
-    put_row<kHalf>(a, wk, D, kRows, row, row0 + row, queried && lt != 0.0f, mx,
-                   lt, 64 * g + c0, x, rg.splits);
+    put_row<kHalf>(a, wk, D, kRows, row, row0 + row,
+                   queried && sums.l != 0.0f, sums, 64 * g + c0, x, rg.splits);
   }
 }
 
@@ -814,21 +921,25 @@ __global__ __launch_bounds__(256) void k_kv4_join(AttendArgs a,
   if (splits == 1 || r >= a.rows) return;
   const float* p =
       a.part + (((b * a.c.heads + h) * a.q_tiles + r / rows_tile) * a.splits *
-                    rows_tile + r % rows_tile) * (D + 2);
-  const int64_t next = (int64_t)rows_tile * (D + 2);
-  float m = kNegInf, l = 0.0f;
-  if (lane < splits) {
-    m = p[lane * next];
-    l = p[lane * next + 1];
+                    rows_tile + r % rows_tile) * (D + kPart);
+  const int64_t next = (int64_t)rows_tile * (D + kPart);
+  Sums part = {kNegInf, 0.0f, kNegInf};
+  if (lane < splits)
+    part = {p[lane * next], p[lane * next + 1], p[lane * next + 2]};
+  Sums sums = part;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    sums.m = fmaxf(sums.m, __shfl_xor(sums.m, o));
+    sums.ml = fmaxf(sums.ml, __shfl_xor(sums.ml, o));
   }
-  float mx = m;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-  const float f = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - mx);
+  const float f =
+      part.m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(part.m - sums.m);
   // a query's split of nothing but NaN has no M, and an l that says so
-  float lt = f == 0.0f && l == l ? 0.0f : f * l;
+  sums.l = part.l * (part.ml == kNegInf
+                         ? 0.0f
+                         : __builtin_amdgcn_exp2f(part.ml - sums.ml));
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) lt += __shfl_xor(lt, o);
+  for (int o = 32; o > 0; o >>= 1) sums.l += __shfl_xor(sums.l, o);
   float x[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) x[c] = 0.0f;
@@ -842,7 +953,7 @@ __global__ __launch_bounds__(256) void k_kv4_join(AttendArgs a,
       w[u] = todo ? __shfl(f, s) : 0.0f;
 #pragma unroll
       for (int c = 0; c < C; ++c)
-        v[u][c] = todo ? p[s * next + 2 + lane * C + c] : 0.0f;
+        v[u][c] = todo ? p[s * next + kPart + lane * C + c] : 0.0f;
       todo &= todo - 1;
     }
 #pragma unroll
@@ -853,10 +964,10 @@ __global__ __launch_bounds__(256) void k_kv4_join(AttendArgs a,
   const int t = r / a.group;
   uint16_t* out = a.out + ((b * a.tokens + t) * a.q_heads + h * a.group +
                            r % a.group) * D + lane * C;
-  const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+  const Factor by(sums);
 #pragma unroll
   for (int c = 0; c < C; ++c)
-    out[c] = (uint16_t)from_float16b<kHalf>(lt == 0.0f ? 0.0f : x[c] * inv);
+    out[c] = (uint16_t)from_float16b<kHalf>(sums.l == 0.0f ? 0.0f : by(x[c]));
 }
 
 struct Plan {
@@ -901,7 +1012,7 @@ Plan plan_for(const sfx_kv4* c, int64_t batch, int64_t tokens,
   p.splits = (int)((blocks + p.chunk - 1) / p.chunk);
   p.bytes = p.splits == 1 ? 0
                           : (size_t)wgs * p.splits * p.rows_tile *
-                                (c->head_dim + 2) * 4;
+                                (c->head_dim + kPart) * 4;
   return p;
 }
 

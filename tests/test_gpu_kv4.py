@@ -536,3 +536,75 @@ def test_cache_keeps_its_pool(gpu):
     c, _ = make(gpu, 1, 32, 1, 64, 32, BF, 280)
     with pytest.raises(AttributeError):
         c.pages = torch.zeros_like(c.pages)
+
+
+# ---------------------------------------------- value scales of any size
+@pytest.mark.parametrize("big", [1.0, 1e20, 3e38])
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("t", [1, 20])
+@pytest.mark.parametrize("n,at", [(2, 1), (2, 0), (70, 40), (70, 69),
+                                  (300, 200), (3000, 0), (3000, 2999)])
+def test_attend_counts_tokens_of_small_values(gpu, n, at, t, d, big):
+    """Tokens of equal scores, one of which holds values of `big`, the others
+    zeros or values at the least scale: each counts once, whether it shares the
+    block, the wave or the split."""
+    c, table = make(gpu, 1, n, 1, d, 64, BF, 230)
+    k = data(gpu, 1, n, 1, d, BF, 231)
+    v = torch.zeros(1, n, 1, d, dtype=BF, device=gpu)
+    v[0, ::2] = 2.0 ** -100
+    v[0, at] = big
+    c.append(k, v, table, ints([0], gpu))
+    q = torch.zeros(1, t, 2, d, dtype=BF, device=gpu)
+    out = np64(c.attend(q, table, ints([n], gpu)))[0]
+    see = np.maximum(np.arange(n - t + 1, n + 1), 0)
+    top = float(torch.tensor(big).to(BF))
+    want = np.where(see > at, top / np.maximum(see, 1), 0.0)[:, None, None]
+    # the value's and the result's rounding, approximations of 1 / s and of
+    # exponentials (2^-17); the small values beside it
+    tol = want * (2.0 ** -8 + 2.0 ** -15) + 2.0 ** -99
+    assert (np.abs(out - want) <= tol).all(), (out[:, 0, 0], want[:, 0, 0])
+
+
+@pytest.mark.parametrize("t", [1, 20])
+@pytest.mark.parametrize("n", [64, 3000])
+def test_attend_values_of_every_exponent(gpu, t, n):
+    """Values from the least scale to the type's largest side by side, under
+    scores that favour one or the other."""
+    d = 128
+    c, table = make(gpu, 1, n, 1, d, 64, BF, 240)
+    k = data(gpu, 1, n, 1, d, BF, 241)
+    g = torch.Generator().manual_seed(242)
+    e = torch.randint(-104, 122, (1, n, 1, 1), generator=g)
+    v = torch.randn(1, n, 1, d, generator=g).clamp(-4, 4)
+    v = torch.ldexp(v, e).to(BF).to(gpu)
+    c.append(k, v, table, ints([0], gpu))
+    q = data(gpu, 1, t, 2, d, BF, 243)
+    kq = target.quantize_k(np64(k), False)
+    vq, vs = target.quantize_v(np64(v))
+    for scale in (0.002, 0.05, 1.0):
+        out = c.attend(q, table, ints([n], gpu), scale=scale)
+        check_attend(out, q, kq, vq, vs, [n], [t], BF, scale)
+
+
+@pytest.mark.parametrize("t", [1, 20])
+@pytest.mark.parametrize("d,heads", [(64, 1), (128, 2), (256, 1)])
+def test_attend_value_scales_of_zero_count(gpu, t, d, heads):
+    """Blocks that were never written (zeros throughout) hold keys and values of
+    zero: their tokens count in the sum of weights as any other."""
+    n, lo = 200, 77
+    c, table = make(gpu, 1, n, heads, d, 32, BF, 250)
+    c.pages.zero_()
+    k = data(gpu, 1, n - lo, heads, d, BF, 251)
+    v = data(gpu, 1, n - lo, heads, d, BF, 252)
+    c.append(k, v, table, ints([lo], gpu))
+    q = data(gpu, 1, t, 2 * heads, d, BF, 253)
+    kq = np.zeros((1, n, heads, d))
+    vq, vs = np.zeros((1, n, heads, d)), np.ones((1, n, heads, 1))
+    kq[:, lo:] = target.quantize_k(np64(k), False)
+    vq[:, lo:], vs[:, lo:] = target.quantize_v(np64(v))
+    for scale in (0.01, 0.1):
+        out = c.attend(q, table, ints([n], gpu), scale=scale)
+        check_attend(out, q, kq, vq, vs, [n], [t], BF, scale)
+    # a row of nothing else has a mean of zeros
+    c.pages.zero_()
+    assert not np64(c.attend(q, table, ints([n], gpu))).any()
