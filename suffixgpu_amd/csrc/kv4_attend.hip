@@ -18,17 +18,19 @@
 // 2^-14 to steps of 2^-24.
 // A term of l is 2^(x_t - M), and where s_t is far below the scale that M comes
 // from, 2^(y_t - M) vanishes before 1 / s_t can bring it back: a token of zeros
-// beside one of large values would not count.  So from its first block on with a
-// scale outside [2^-20, 2^60], zero and NaN included, a wave takes l's
-// exponentials for themselves, relative to a maximum of x_t (ml), at the price of
-// a second exponential per score.  As long as all scales lie within, what
-// vanishes is less than 2^-106 a token, and the largest term at least 2^-60.
+// beside one of large values would not count.  As long as all scales lie within
+// [2^-20, 2^60], what vanishes is less than 2^-106 a token, and the largest term at
+// least 2^-60.  A wave that has met another scale, zero and NaN included, goes
+// through its keys once more, for l alone, relative to the maximum of x_t (ml).
+// O is what it is.  (The other ways to take an l of its own cost where no scale
+// needs it: with a branch between a block's loads and products, into a loop that
+// takes both sums, 200 tokens over up to 4,096 each, 16 query heads on two KV heads
+// of 128, took 49 us instead of 46.)
 // Weights are rounded to float16 (11 bits, the finer of the 16-bit types, also
 // where the cache is bfloat16): the products accumulate in 32 bits, l is summed
 // from the unrounded weights.
 
 #include <algorithm>
-#include <type_traits>
 
 #include "kv4.h"
 #include "launch.h"
@@ -349,7 +351,7 @@ __device__ __forceinline__ const uint16_t* q_row(const AttendArgs& a,
 // Scale of a block's values in base 2, and one over it, of the tokens that a
 // lane's scores belong to: each lane works out one token's, and they cross in
 // the wave's own 64 floats of LDS, in order as its accesses are.
-// 1 / s is finite whatever the scale: a row that does not see a token (of a
+// 1 / s is at most what sums of it leave finite, whatever the scale: a row that does not see a token (of a
 // NaN, or past the end, where a block holds anything) multiplies it by zero,
 // and one that sees a NaN has it from the logarithm.
 __device__ __forceinline__ void share_scales(float vs, float* lds) {
@@ -357,7 +359,7 @@ __device__ __forceinline__ void share_scales(float vs, float* lds) {
   const float x =
       lane_id() < 32
           ? __builtin_amdgcn_logf(vs)
-          : fminf(fmaxf(__builtin_amdgcn_rcpf(vs), 0.0f), 0x1p101f);
+          : fminf(fmaxf(__builtin_amdgcn_rcpf(vs), 0.0f), 0x1p21f);
   lds[lane_id() / 32 * 32 + t] = x;
   asm volatile("" ::: "memory");
 }
@@ -376,13 +378,12 @@ __device__ __forceinline__ bool scales_apart(float vs, int blk, int most) {
 // the values, which load the next block's into the same registers.  A second
 // set for the loads under way would cost a wave in three; issued this early
 // they are as well hidden.  A block's page id is read (as a scalar) one block
-// ahead of that.  Blocks without a page are left out.  Ends before a block that
-// stop(block, index) says to stop at; returns where it ended.
-template <class B, class P, class F>
-__device__ __forceinline__ int each_block(const KvView& c, int64_t b, int h,
-                                          int bytes, int first, int last,
-                                          P stop, F body) {
-  if (first >= last || c.num_pages == 0) return last;
+// ahead of that.  Blocks without a page are left out.
+template <class B, class F>
+__device__ __forceinline__ void each_block(const KvView& c, int64_t b, int h,
+                                           int bytes, int first, int last,
+                                           F body) {
+  if (first >= last || c.num_pages == 0) return;
   typedef const __attribute__((address_space(4))) int32_t* Ids;
   const Ids ids = (Ids)(uintptr_t)(c.table + b * c.table_stride);
   const int in_page = (1 << c.page_shift) - 1;
@@ -398,12 +399,10 @@ __device__ __forceinline__ int each_block(const KvView& c, int64_t b, int h,
   int32_t id = page(first), id1 = page(first + kWaves);
   x.load_k(at(id, first));
   x.load_v(at(id, first));
-  int blk = first;
-  for (; blk < last; blk += kWaves) {
+  for (int blk = first; blk < last; blk += kWaves) {
     const char* next = at(id1, blk + kWaves);
     const int32_t id2 = page(blk + 2 * kWaves);
     if (good(id)) {
-      if (stop(x, blk)) break;
       body(x, blk, [&]() { x.load_k(next); }, [&]() { x.load_v(next); });
     } else {
       x.load_k(next);
@@ -412,31 +411,6 @@ __device__ __forceinline__ int each_block(const KvView& c, int64_t b, int h,
     id = id1;
     id1 = id2;
   }
-  return blk;
-}
-
-// Goes through a wave's blocks in one loop with l relative to M and, from the
-// first block on whose scales are apart, in another with l for itself:
-// body(apart, ...) as above, apart a constant; switched() between them.  (One
-// loop with a flag takes ten registers more, and a workgroup of a CU with them.)
-template <class B, class G, class F>
-__device__ __forceinline__ bool both_loops(const KvView& c, int64_t b, int h,
-                                           int bytes, int first, int last,
-                                           int most, G switched, F body) {
-  const int at = each_block<B>(
-      c, b, h, bytes, first, last,
-      [&](const B& x, int blk) { return scales_apart(x.vs, blk, most); },
-      [&](B& x, int blk, auto kdone, auto vdone) {
-        body(std::false_type(), x, blk, kdone, vdone);
-      });
-  if (at >= last) return false;
-  switched();
-  each_block<B>(
-      c, b, h, bytes, at, last, [](const B&, int) { return false; },
-      [&](B& x, int blk, auto kdone, auto vdone) {
-        body(std::true_type(), x, blk, kdone, vdone);
-      });
-  return true;
 }
 
 // Follows the maximum of a row's scores when it has grown by more than kSlack:
@@ -591,16 +565,16 @@ __device__ __forceinline__ void attend16(const AttendArgs& a, const Work& wk,
   const Range rg = range_of(a, len, most, wk.split);
   const int first = rg.first + wave, last = rg.last;
 
-  float m = kNegInf, l = 0.0f, ml = kNegInf;
+  float m = kNegInf, l = 0.0f;
+  bool apart = false;
   F4 o[kDt];
 #pragma unroll
   for (int d = 0; d < kDt; ++d) o[d] = F4{0, 0, 0, 0};
 
-  const bool apart = both_loops<Block<D, 16>>(
-      a.c, wk.b, wk.h, KvLayout<D>::kBytes, first, last, most,
-      [&]() { ml = m; },
-      [&](auto apart, Block<D, 16>& kb, int blk, auto kdone, auto vdone) {
-    constexpr bool kApart = decltype(apart)::value;
+  each_block<Block<D, 16>>(a.c, wk.b, wk.h, KvLayout<D>::kBytes, first, last,
+                           [&](Block<D, 16>& kb, int blk, auto kdone,
+                               auto vdone) {
+    apart |= scales_apart(kb.vs, blk, most);
     share_scales(kb.vs, sc[wave]);
     const int p0 = blk * kKvBlock + 16 * (quad / 2) + 4 * (quad % 2);
     const bool edge = blk * kKvBlock + kKvBlock > least;
@@ -611,14 +585,6 @@ __device__ __forceinline__ void attend16(const AttendArgs& a, const Work& wk,
       for (int i = 0; i < kStep; ++i)
         s[t] = mma16<kHalf>(widen<kHalf>(kb.k[t][i], kb.scale(t, i)), qf[i],
                             s[t]);
-    if constexpr (kApart) {
-      auto x = [&](int j, float less) {
-        return p0 + 8 * (j / 4) + j % 4 < vis
-                   ? __builtin_fmaf(s[j / 4][j % 4], a.scale, -less)
-                   : kNegInf;
-      };
-      sum_apart<16, 8>(x, &ml, &l);
-    }
     kdone();
     F4 ls[2], rs[2];
 #pragma unroll
@@ -643,7 +609,7 @@ __device__ __forceinline__ void attend16(const AttendArgs& a, const Work& wk,
     for (int j = 0; j < 8; ++j) top = fmaxf(top, y[j]);
     if (__any(top > m + kSlack)) {
       const float f = follow<16>(top, &m);
-      if (!kApart) l *= f;
+      l *= f;
 #pragma unroll
       for (int d = 0; d < kDt; ++d) o[d] *= f;
     }
@@ -652,8 +618,7 @@ __device__ __forceinline__ void attend16(const AttendArgs& a, const Work& wk,
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       w[j] = __builtin_amdgcn_exp2f(y[j] - mu);
-      // (times zero a weight of NaN still makes l NaN)
-      l = __builtin_fmaf(w[j], kApart ? 0.0f : rs[j / 4][j % 4], l);
+      l = __builtin_fmaf(w[j], rs[j / 4][j % 4], l);
     }
     const U4 pf = {pack_half(w[0], w[1]), pack_half(w[2], w[3]),
                    pack_half(w[4], w[5]), pack_half(w[6], w[7])};
@@ -663,8 +628,32 @@ __device__ __forceinline__ void attend16(const AttendArgs& a, const Work& wk,
     vdone();
   });
 
+  float ml = m;
+  if (apart) {
+    const float before = l;
+    l = 0.0f;
+    ml = kNegInf;
+    each_block<Block<D, 16>>(a.c, wk.b, wk.h, KvLayout<D>::kBytes, first, last,
+                             [&](Block<D, 16>& kb, int blk, auto kdone, auto) {
+      const int p0 = blk * kKvBlock + 16 * (quad / 2) + 4 * (quad % 2);
+      F4 s[2] = {F4{0, 0, 0, 0}, F4{0, 0, 0, 0}};
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < kStep; ++i)
+          s[t] = mma16<kHalf>(widen<kHalf>(kb.k[t][i], kb.scale(t, i)), qf[i],
+                              s[t]);
+      kdone();
+      sum_apart<16, 8>([&](int j, float less) {
+        return p0 + 8 * (j / 4) + j % 4 < vis
+                   ? __builtin_fmaf(s[j / 4][j % 4], a.scale, -less)
+                   : kNegInf;
+      }, &ml, &l);
+    });
+    if (before != before) l = before;  // a value's NaN
+  }
+
   // Join the waves in LDS; 16 threads a row, D / 16 channels each.
-  if (!apart) ml = m;
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
 #pragma unroll
@@ -733,18 +722,18 @@ __device__ __forceinline__ void attend32(const AttendArgs& a, const Work& wk,
   const int first = rg.first + wave, last = rg.last;
   __syncthreads();
 
-  float m = kNegInf, l = 0.0f, ml = kNegInf;
+  float m = kNegInf, l = 0.0f;
+  bool apart = false;
   F16 o[kDt];
 #pragma unroll
   for (int d = 0; d < kDt; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
 
-  const bool apart = both_loops<Block<D, 32>>(
-      a.c, wk.b, wk.h, KvLayout<D>::kBytes, first, last, most,
-      [&]() { ml = m; },
-      [&](auto apart, Block<D, 32>& kb, int blk, auto kdone, auto vdone) {
-    constexpr bool kApart = decltype(apart)::value;
+  each_block<Block<D, 32>>(a.c, wk.b, wk.h, KvLayout<D>::kBytes, first, last,
+                           [&](Block<D, 32>& kb, int blk, auto kdone,
+                               auto vdone) {
+    apart |= scales_apart(kb.vs, blk, most);
     share_scales(kb.vs, sc[wave]);
     const int p0 = blk * kKvBlock + 4 * h2;
     const bool edge = blk * kKvBlock + kKvBlock > least;
@@ -773,14 +762,6 @@ __device__ __forceinline__ void attend32(const AttendArgs& a, const Work& wk,
 #pragma unroll
     for (int g = 0; g < 4; ++g)
       rs[g] = *(const F4*)&sc[wave][32 + 8 * g + 4 * h2];
-    if constexpr (kApart) {
-      auto x = [&](int r, float less) {
-        return p0 + r / 4 * 8 + r % 4 < vis
-                   ? __builtin_fmaf(s[r], a.scale, -less)
-                   : kNegInf;
-      };
-      sum_apart<32, 16>(x, &ml, &l);
-    }
     kdone();
     float top = kNegInf;
 #pragma unroll
@@ -796,7 +777,7 @@ __device__ __forceinline__ void attend32(const AttendArgs& a, const Work& wk,
     for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
     if (__any(top > m + kSlack)) {
       const float f = follow<32>(top, &m);
-      if (!kApart) l *= f;
+      l *= f;
 #pragma unroll
       for (int d = 0; d < kDt; ++d) o[d] *= f;
     }
@@ -808,7 +789,7 @@ __device__ __forceinline__ void attend32(const AttendArgs& a, const Work& wk,
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         w[r] = __builtin_amdgcn_exp2f(s[4 * g + r] - mu);
-        l = __builtin_fmaf(w[r], kApart ? 0.0f : rs[g][r], l);
+        l = __builtin_fmaf(w[r], rs[g][r], l);
       }
       pf[g / 2][g % 2 * 2] = pack_half(w[0], w[1]);
       pf[g / 2][g % 2 * 2 + 1] = pack_half(w[2], w[3]);
@@ -821,12 +802,40 @@ __device__ __forceinline__ void attend32(const AttendArgs& a, const Work& wk,
     vdone();
   });
 
+  float ml = m;
+  if (apart) {
+    const float before = l;
+    l = 0.0f;
+    ml = kNegInf;
+    each_block<Block<D, 32>>(a.c, wk.b, wk.h, KvLayout<D>::kBytes, first, last,
+                             [&](Block<D, 32>& kb, int blk, auto kdone, auto) {
+      const int p0 = blk * kKvBlock + 4 * h2;
+      F16 s;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
+        s = mma32<kHalf>(widen<kHalf>(kb.k[i], kb.scale(i)), sq[i * 64 + lane],
+                         s);
+      }
+      kdone();
+      sum_apart<32, 16>([&](int r, float less) {
+        return p0 + r / 4 * 8 + r % 4 < vis
+                   ? __builtin_fmaf(s[r], a.scale, -less)
+                   : kNegInf;
+      }, &ml, &l);
+    });
+    if (before != before) l = before;  // a value's NaN
+  }
+
   // Join the waves in LDS, 64 channels at a time: 8 threads a row.
   auto so = (float(*)[32][64 + 4])lds.pool;
-  if (!apart) ml = m;
   l += __shfl_xor(l, 32);
   const int row = threadIdx.x / 8, c0 = threadIdx.x % 8 * 8;
   const bool queried = visible(a, len, nq, row0 + row) > 0;
+  float f[kWaves];
+  Sums sums;
 #pragma unroll
   for (int g = 0; g < D / 64; ++g) {
     __syncthreads();
@@ -838,14 +847,13 @@ __device__ __forceinline__ void attend32(const AttendArgs& a, const Work& wk,
         *(F4*)&so[wave][col][(2 * (r / 2) + t) * 16 + r % 2 * 8 + 4 * h2] =
             F4{o[2 * g + t][4 * r], o[2 * g + t][4 * r + 1],
                o[2 * g + t][4 * r + 2], o[2 * g + t][4 * r + 3]};
-    if (h2 == 0) {
+    if (g == 0 && h2 == 0) {
       sm[wave][col] = m;
       sl[wave][col] = l;
       lds.ml[wave][col] = ml;
     }
     __syncthreads();
-    float f[kWaves];
-    const Sums sums = join_waves(lds, row, f);
+    if (g == 0) sums = join_waves(lds, row, f);
     float x[8];
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
