@@ -7,15 +7,16 @@
 // exponentials are at once the operand of the second product (kv4.h).
 //
 // With s_t the scale of token t's values, x_t its score in base 2 and
-// y_t = x_t + log2 s_t, a wave keeps M >= about max y_t and sums
+// y_t = x_t + log2 s_t, a wave keeps an M near max y_t and sums
 //   O = sum 2^(y_t - M) v_t (v_t as the 4 bits stand),  l = sum 2^(y_t - M) / s_t
 // so the weights stay within 16-bit range whatever the scales are, and O / l is
-// the result.  M only follows the maximum when that has grown by more than
-// kSlack, so most blocks rescale nothing and no maximum crosses lanes (with a
-// slack of 0 64 x 17 tokens over up to 8,192 take 162 us instead of 146, a
-// prompt's 2,048 507 instead of 472; with single tokens it is the same).  The
-// largest weight is then between 1 and 2^8, and float16 rounds what is below
-// 2^-14 to steps of 2^-24.
+// the result.  M is the maximum less kLift and only follows it when that has
+// grown by more than 8, so most blocks rescale nothing and no maximum crosses
+// lanes (followed at once, 64 x 17 tokens over up to 8,192 take 168 us instead of
+// 156, a prompt's 2,048 after 14,336 others 644 instead of 604; with single tokens
+// it is the same).  The largest weight is then between 2^7 and 2^15 of float16's 2^16, and
+// what is rounded to steps of 2^-24 is below 2^-21 of it: however many tokens
+// weigh little beside a heavy one, O has what l counts.
 // A term of l is 2^(x_t - M), and where s_t is far below the scale that M comes
 // from, 2^(y_t - M) vanishes before 1 / s_t can bring it back: a token of zeros
 // beside one of large values would not count.  As long as all scales lie within
@@ -48,7 +49,8 @@ typedef __bf16 B8 __attribute__((ext_vector_type(8)));
 typedef uint32_t U4 __attribute__((ext_vector_type(4)));
 
 constexpr float kNegInf = -__builtin_inff();
-constexpr float kSlack = 8.0f;
+constexpr float kLift = 7.0f;   // the largest weight is at least 2^kLift
+constexpr float kSlack = 15.0f;  // and at most 2^kSlack
 constexpr int kWaves = 4;
 constexpr int kPart = 4;  // floats before the channels of a split's part
 
@@ -413,14 +415,14 @@ __device__ __forceinline__ void each_block(const KvView& c, int64_t b, int h,
   }
 }
 
-// Follows the maximum of a row's scores when it has grown by more than kSlack:
-// then O and l shrink by the factor returned, else it is 1.  kLanes: distance
-// of the lanes that share a row.
+// Follows the maximum of a row's scores: *m becomes at least that less kLift, O
+// and l shrink by the factor returned.  kLanes: distance of the lanes that share
+// a row.
 template <int kLanes>
 __device__ __forceinline__ float follow(float top, float* m) {
   if (kLanes == 16) top = fmaxf(top, __shfl_xor(top, 16));
   top = fmaxf(top, __shfl_xor(top, 32));
-  const float mn = fmaxf(*m, top);
+  const float mn = fmaxf(*m, top - kLift);
   const float f = mn == *m ? 1.0f : __builtin_amdgcn_exp2f(*m - mn);
   *m = mn;
   return f;

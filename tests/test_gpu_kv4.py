@@ -608,3 +608,31 @@ def test_attend_value_scales_of_zero_count(gpu, t, d, heads):
     # a row of nothing else has a mean of zeros
     c.pages.zero_()
     assert not np64(c.attend(q, table, ints([n], gpu))).any()
+
+
+@pytest.mark.parametrize("t", [1, 17])
+def test_attend_many_light_tokens_beside_a_heavy_one(gpu, t):
+    """2^18 tokens in one split, one in each wave's share 2^25.1 times as heavy
+    as every other: the others are 2^-9 of the sum, and count in the result as
+    they do in the sum of weights."""
+    from suffixgpu_amd import KV4Cache
+    n, d, page, b = 1 << 18, 64, 1 << 16, 1600
+    heavy = [0, 32, 64, 96]
+    c = KV4Cache(n // page, 1, d, page_size=page, dtype=HF, device=gpu)
+    table = torch.arange(n // page, dtype=torch.int32, device=gpu)[None]
+    k = torch.zeros(1, n, 1, d, dtype=HF, device=gpu)
+    v = torch.full((1, n, 1, d), -1.0, dtype=HF, device=gpu)
+    k[0, heavy, 0, 0], v[0, heavy] = 6.0, 1.0
+    c.append(k, v, table, ints([0], gpu))
+    q = torch.zeros(b, t, 1, d, dtype=HF, device=gpu)
+    q[..., 0] = 1.0
+    out = c.attend(q, table.expand(b, -1), ints([n], gpu).expand(b),
+                   scale=25.1 * np.log(2.0) / 6.0)
+    light = np.arange(n - t + 1, n + 1) - len(heavy)
+    light = light * 2.0 ** -25.1
+    want = ((len(heavy) - light) / (len(heavy) + light))[None, :, None, None]
+    # the sum of weights of a lane that begins with a heavy one may lose its
+    # light ones (2^15 at most, 2^-10 of it); 2^12 products summed in 32 bits; the
+    # result's rounding
+    tol = 2.0 ** -10 + 2.0 ** -11 + 2.0 ** -12
+    assert (np.abs(np64(out) - want) <= tol).all(), np64(out)[0, :, 0, 0]
