@@ -321,8 +321,10 @@ __device__ __forceinline__ int blocks_of(const AttendArgs& a, int64_t len) {
 }
 
 // Splits of a row, and the blocks of one that rows of up to `most` visible
-// positions need.  A row is split by its length alone, into equal parts of at
-// most `chunk` blocks.
+// positions need.  A row is split into equal parts of at most `chunk` blocks,
+// which is one number for the call: from its rows, tiles and table width
+// (plan_for).  So the order of a row's sums, and its last bits, follow the call's
+// shape, but not what the other rows hold.
 struct Range {
   int splits, first, last;
 };
@@ -1000,6 +1002,9 @@ struct Plan {
 // 150, 16 x 17 over up to 32,768 221 / 167 / 170 / 166.  Heads of 256, two: 4 x 9
 // over up to 131,072 198 / 203 / 205 / 215, 30 x 9 over up to 8,192 97 / 101 / 109
 // / 113.
+// Both of these are for tables about as wide as the rows.  What the rows hold is
+// known on the device alone, so the plan takes every row as full: in a table many
+// times wider than the rows, they have fewer splits than these figures stand for.
 // At least kLeast blocks each: one token over 2,050 10.2 us, with 8 10.7, with 4
 // 13.2.
 constexpr int64_t kLeast = 16;

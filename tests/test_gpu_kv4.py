@@ -636,3 +636,26 @@ def test_attend_many_light_tokens_beside_a_heavy_one(gpu, t):
     # result's rounding
     tol = 2.0 ** -10 + 2.0 ** -11 + 2.0 ** -12
     assert (np.abs(np64(out) - want) <= tol).all(), np64(out)[0, :, 0, 0]
+
+
+@pytest.mark.parametrize("t", [1, 3, 20])
+def test_attend_rows_alone_together_and_in_wider_tables(gpu, t):
+    """How a row is split follows the call's shape; what it gives does not, up to
+    the order of its sums: rows by themselves, among many others, and in tables
+    far wider than the rows."""
+    lens = [900, 77, 2500]
+    c, table, kq, vq, vs = filled(gpu, 3, lens, 2, 128, 64, BF, 290)
+    q = data(gpu, 3, t, 8, 128, BF, 291)
+    wide = torch.full((3, 20 * table.shape[1]), -1, dtype=torch.int32,
+                      device=gpu)
+    wide[:, :table.shape[1]] = table
+    for tab in (table, wide):
+        for i in range(3):
+            out = c.attend(q[i:i + 1], tab[i:i + 1], ints(lens[i:i + 1], gpu))
+            check_attend(out, q[i:i + 1], kq[i:i + 1], vq[i:i + 1],
+                         vs[i:i + 1], lens[i:i + 1], [t], BF)
+        many = torch.arange(120, device=gpu) % 3
+        out = c.attend(q[many], tab[many], ints(lens, gpu)[many])
+        check_attend(out[:3], q, kq, vq, vs, lens, [t] * 3, BF)
+        for i in range(3, 120, 3):
+            assert torch.equal(out[i:i + 3], out[:3])
