@@ -593,11 +593,12 @@ int sfx_kv4_attend(const sfx_kv4* cache, const sfx_heads* q, int64_t batch,
  * token after j drafted ones.  p_j = softmax(logits / temperature); a NaN
  * counts as -inf, equal +inf share.  Temperature 0 (or below, or NaN): p_j is
  * one at the first of the largest logits.  temperature == NULL: 1.
- * Draft j < min(num_valid[b], K) (and before the first id outside
- * [0, vocab)) is accepted iff uniform[b][j] q(draft) < p_j(draft), q =
- * draft_probs[b][j] or, with draft_probs == NULL, one at the draft.  At the
- * first draft not accepted a token is drawn from max(p_j - q, 0) (from p_j
- * where that is empty), after num_valid accepted ones from p_j: the one with
+ * A row's drafts are the first min(num_valid[b], K), fewer where one of them is
+ * outside [0, vocab): they end before it.  Draft j is accepted iff
+ * uniform[b][j] q(draft) < p_j(draft), q = draft_probs[b][j] or, with
+ * draft_probs == NULL, one at the draft.  At the first draft not accepted a
+ * token is drawn from max(p_j - q, 0) (from p_j where that is empty), when all
+ * are accepted from p_j after them: the one with
  * the largest probability / noise[b][token], the lowest on ties; noise is
  * exponentially distributed, every value > 0.  A position without any logit
  * above -inf accepts and draws nothing.
@@ -605,7 +606,8 @@ int sfx_kv4_attend(const sfx_kv4* cache, const sfx_heads* q, int64_t batch,
  * them; count [batch] their number.  uniform [batch, K] and noise
  * [batch, vocab] may be NULL only with all_greedy != 0, which takes every
  * row's temperature as 0.  counters: sfx_verify_counter_bytes bytes,
- * zero-filled once; every call leaves them zero, whatever its sizes.
+ * zero-filled once; every call that returns 0 leaves them zero, whatever
+ * its sizes.
  * workspace: sfx_verify_workspace_size bytes of any content.  Both 16-byte
  * aligned; calls that share either must not overlap, nor may one host thread's
  * two launches have another's between them on the stream. */

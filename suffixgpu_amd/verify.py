@@ -70,7 +70,7 @@ def verify_draft(logits: torch.Tensor, draft: torch.Tensor,
     """Verify ``draft`` [B, K] (int32, ``num_valid`` [B] of each row) against
     ``logits`` [B, K + 1, V] (bfloat16, float16 or float32; any strides but a
     contiguous vocabulary), position j holding the target's logits after j
-    drafts.
+    drafts.  An id outside the vocabulary ends a row's drafts as num_valid does.
 
     With p = softmax(logits / temperature), draft j stays iff
     ``uniform[b, j] * q < p[draft]``; q is ``draft_probs[b, j, draft]``
