@@ -19,14 +19,11 @@
 // weigh little beside a heavy one, O has what l counts.
 // A term of l is 2^(x_t - M), and where s_t is far below the scale that M comes
 // from, 2^(y_t - M) vanishes before 1 / s_t can bring it back: a token of zeros
-// beside one of large values would not count.  As long as all scales lie within
-// [2^-20, 2^60], what vanishes is less than 2^-106 a token, and the largest term at
-// least 2^-60.  A wave that has met another scale, zero and NaN included, goes
-// through its keys once more, for l alone, relative to the maximum of x_t (ml).
-// O is what it is.  (The other ways to take an l of its own cost where no scale
-// needs it: with a branch between a block's loads and products, into a loop that
-// takes both sums, 200 tokens over up to 4,096 each, 16 query heads on two KV heads
-// of 128, took 49 us instead of 46.)
+// beside one of large values would not count.  What vanishes is less than
+// 2^-126 / s_t a token.  A wave one of whose l is not 2^28 times the largest of
+// that (or so small that it is not a normal number) goes through its keys once
+// more, for l alone, relative to the maximum of x_t (ml); O is what it is.
+// Values of zero beside others of up to 2^7 do not come to that.
 // Weights are rounded to float16 (11 bits, the finer of the 16-bit types, also
 // where the cache is bfloat16): the products accumulate in 32 bits, l is summed
 // from the unrounded weights.
@@ -352,28 +349,52 @@ __device__ __forceinline__ const uint16_t* q_row(const AttendArgs& a,
          (int64_t)(h * a.group + r % a.group) * a.q.stride_h;
 }
 
-// Scale of a block's values in base 2, and one over it, of the tokens that a
-// lane's scores belong to: each lane works out one token's, and they cross in
-// the wave's own 64 floats of LDS, in order as its accesses are.
-// 1 / s is at most what sums of it leave finite, whatever the scale: a row that does not see a token (of a
-// NaN, or past the end, where a block holds anything) multiplies it by zero,
-// and one that sees a NaN has it from the logarithm.
-__device__ __forceinline__ void share_scales(float vs, float* lds) {
+// Scale of a block's values in base 2, and kUnit over it (l is summed that much
+// smaller, so that no sum overflows), of the tokens that a lane's scores belong
+// to: each lane works out one token's, and they cross in the wave's own 64 floats
+// of LDS, in order as its accesses are.
+// kUnit / s is finite whatever the scale: a row that does not see a token (of a
+// NaN, or past the end, where a block holds anything) multiplies it by zero, and
+// one that sees a NaN has it from the logarithm.
+// *most: the largest kUnit / s of the block's first `held` tokens.
+constexpr float kUnit = 0x1p-24f;
+constexpr float kUnitLog2 = -24.0f;
+
+__device__ __forceinline__ void share_scales(float vs, int held, float* lds,
+                                             float* most) {
   const int t = lane_id() % 32;
-  const float x =
-      lane_id() < 32
-          ? __builtin_amdgcn_logf(vs)
-          : fminf(fmaxf(__builtin_amdgcn_rcpf(vs), 0.0f), 0x1p21f);
+  const float inv = __builtin_amdgcn_rcpf(vs) * kUnit;
+  if (t < held) *most = fmaxf(*most, inv);
+  const float x = lane_id() < 32 ? __builtin_amdgcn_logf(vs)
+                                 : fminf(fmaxf(inv, 0.0f), 0x1p77f);
   lds[lane_id() / 32 * 32 + t] = x;
   asm volatile("" ::: "memory");
 }
 
-// Whether any of a block's tokens that a row of the wave may see (those before
-// `most`) has a scale outside [2^-20, 2^60], NaN and zero included.
-__device__ __forceinline__ bool scales_apart(float vs, int blk, int most) {
-  constexpr uint32_t kLo = (127 - 20) << 23, kHi = (127 + 60) << 23;
-  return __any(__float_as_uint(vs) - kLo > kHi - kLo &&
-               lane_id() % 32 < most - blk * kKvBlock);
+// Largest of a wave's values.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ float max_step(float v) {
+  const int x = __builtin_bit_cast(int, v);
+  return fmaxf(v, __builtin_bit_cast(
+                      float, __builtin_amdgcn_update_dpp(x, x, kCtrl, kRows,
+                                                         0xf, false)));
+}
+__device__ __forceinline__ float wave_most(float v) {
+  v = max_step<0x111, 0xf>(v);
+  v = max_step<0x112, 0xf>(v);
+  v = max_step<0x114, 0xf>(v);
+  v = max_step<0x118, 0xf>(v);
+  v = max_step<0x142, 0xa>(v);
+  v = max_step<0x143, 0xc>(v);
+  return __builtin_bit_cast(
+      float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
+// Whether terms that vanished could be missing in the sum l of a row that sees
+// a token of the wave; inv: the wave's share of `most` above.
+__device__ __forceinline__ bool short_of(float l, bool sees, float inv) {
+  const float least = fmaxf(wave_most(inv) * 0x1p-98f, 0x1p-110f);
+  return __any(sees && l < least);
 }
 
 // Goes through blocks first, first + kWaves, ... below last of row b and KV head
@@ -418,14 +439,14 @@ __device__ __forceinline__ void each_block(const KvView& c, int64_t b, int h,
 }
 
 // Follows the maximum of a row's scores: *m becomes at least that less kLift, O
-// and l shrink by the factor returned.  kLanes: distance of the lanes that share
-// a row.
+// and l shrink by the square of the factor returned, l in two steps, as it may
+// be far from one.  kLanes: distance of the lanes that share a row.
 template <int kLanes>
 __device__ __forceinline__ float follow(float top, float* m) {
   if (kLanes == 16) top = fmaxf(top, __shfl_xor(top, 16));
   top = fmaxf(top, __shfl_xor(top, 32));
   const float mn = fmaxf(*m, top - kLift);
-  const float f = mn == *m ? 1.0f : __builtin_amdgcn_exp2f(*m - mn);
+  const float f = mn == *m ? 1.0f : __builtin_amdgcn_exp2f(0.5f * (*m - mn));
   *m = mn;
   return f;
 }
@@ -437,7 +458,10 @@ __device__ __forceinline__ void sum_apart(F x, float* ml, float* l) {
   float top = kNegInf;
 #pragma unroll
   for (int j = 0; j < N; ++j) top = fmaxf(top, x(j, 0.0f));
-  if (__any(top > *ml + kSlack)) *l *= follow<kLanes>(top, ml);
+  if (__any(top > *ml + kSlack)) {
+    const float f = follow<kLanes>(top, ml);
+    *l = *l * f * f;
+  }
   const float less = *ml == kNegInf ? 0.0f : *ml;
 #pragma unroll
   for (int j = 0; j < N; ++j) *l += __builtin_amdgcn_exp2f(x(j, less));
@@ -569,8 +593,7 @@ __device__ __forceinline__ void attend16(const AttendArgs& a, const Work& wk,
   const Range rg = range_of(a, len, most, wk.split);
   const int first = rg.first + wave, last = rg.last;
 
-  float m = kNegInf, l = 0.0f;
-  bool apart = false;
+  float m = kNegInf, l = 0.0f, inv = 0.0f;
   F4 o[kDt];
 #pragma unroll
   for (int d = 0; d < kDt; ++d) o[d] = F4{0, 0, 0, 0};
@@ -578,8 +601,7 @@ __device__ __forceinline__ void attend16(const AttendArgs& a, const Work& wk,
   each_block<Block<D, 16>>(a.c, wk.b, wk.h, KvLayout<D>::kBytes, first, last,
                            [&](Block<D, 16>& kb, int blk, auto kdone,
                                auto vdone) {
-    apart |= scales_apart(kb.vs, blk, most);
-    share_scales(kb.vs, sc[wave]);
+    share_scales(kb.vs, most - blk * kKvBlock, sc[wave], &inv);
     const int p0 = blk * kKvBlock + 16 * (quad / 2) + 4 * (quad % 2);
     const bool edge = blk * kKvBlock + kKvBlock > least;
     F4 s[2] = {F4{0, 0, 0, 0}, F4{0, 0, 0, 0}};
@@ -613,9 +635,9 @@ __device__ __forceinline__ void attend16(const AttendArgs& a, const Work& wk,
     for (int j = 0; j < 8; ++j) top = fmaxf(top, y[j]);
     if (__any(top > m + kSlack)) {
       const float f = follow<16>(top, &m);
-      l *= f;
+      l = l * f * f;
 #pragma unroll
-      for (int d = 0; d < kDt; ++d) o[d] *= f;
+      for (int d = 0; d < kDt; ++d) o[d] *= f * f;
     }
     const float mu = m == kNegInf ? 0.0f : m;
     float w[8];
@@ -632,10 +654,15 @@ __device__ __forceinline__ void attend16(const AttendArgs& a, const Work& wk,
     vdone();
   });
 
-  float ml = m;
-  if (apart) {
-    const float before = l;
-    l = 0.0f;
+  // The lanes of a row have their own sums until here.
+  auto row_sum = [](float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+  };
+  l = row_sum(l);
+  float ml = m - kUnitLog2;
+  if (short_of(l, vis > first * kKvBlock, inv)) {
+    float lx = 0.0f;
     ml = kNegInf;
     each_block<Block<D, 16>>(a.c, wk.b, wk.h, KvLayout<D>::kBytes, first, last,
                              [&](Block<D, 16>& kb, int blk, auto kdone, auto) {
@@ -652,14 +679,13 @@ __device__ __forceinline__ void attend16(const AttendArgs& a, const Work& wk,
         return p0 + 8 * (j / 4) + j % 4 < vis
                    ? __builtin_fmaf(s[j / 4][j % 4], a.scale, -less)
                    : kNegInf;
-      }, &ml, &l);
+      }, &ml, &lx);
     });
-    if (before != before) l = before;  // a value's NaN
+    lx = row_sum(lx);
+    l = l == l ? lx : l;  // a value's NaN stays
   }
 
   // Join the waves in LDS; 16 threads a row, D / 16 channels each.
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
 #pragma unroll
   for (int d = 0; d < kDt; ++d) *(F4*)&so[wave][col][d * 16 + quad * 4] = o[d];
   if (quad == 0) {
@@ -726,8 +752,7 @@ __device__ __forceinline__ void attend32(const AttendArgs& a, const Work& wk,
   const int first = rg.first + wave, last = rg.last;
   __syncthreads();
 
-  float m = kNegInf, l = 0.0f;
-  bool apart = false;
+  float m = kNegInf, l = 0.0f, inv = 0.0f;
   F16 o[kDt];
 #pragma unroll
   for (int d = 0; d < kDt; ++d)
@@ -737,8 +762,7 @@ __device__ __forceinline__ void attend32(const AttendArgs& a, const Work& wk,
   each_block<Block<D, 32>>(a.c, wk.b, wk.h, KvLayout<D>::kBytes, first, last,
                            [&](Block<D, 32>& kb, int blk, auto kdone,
                                auto vdone) {
-    apart |= scales_apart(kb.vs, blk, most);
-    share_scales(kb.vs, sc[wave]);
+    share_scales(kb.vs, most - blk * kKvBlock, sc[wave], &inv);
     const int p0 = blk * kKvBlock + 4 * h2;
     const bool edge = blk * kKvBlock + kKvBlock > least;
     F16 s;
@@ -781,9 +805,9 @@ __device__ __forceinline__ void attend32(const AttendArgs& a, const Work& wk,
     for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
     if (__any(top > m + kSlack)) {
       const float f = follow<32>(top, &m);
-      l *= f;
+      l = l * f * f;
 #pragma unroll
-      for (int d = 0; d < kDt; ++d) o[d] *= f;
+      for (int d = 0; d < kDt; ++d) o[d] *= f * f;
     }
     const float mu = m == kNegInf ? 0.0f : m;
     U4 pf[2];
@@ -806,10 +830,14 @@ __device__ __forceinline__ void attend32(const AttendArgs& a, const Work& wk,
     vdone();
   });
 
-  float ml = m;
-  if (apart) {
-    const float before = l;
-    l = 0.0f;
+  // The lanes of a row have their own sums until here.
+  auto row_sum = [](float x) {
+    return x + __shfl_xor(x, 32);
+  };
+  l = row_sum(l);
+  float ml = m - kUnitLog2;
+  if (short_of(l, vis > first * kKvBlock, inv)) {
+    float lx = 0.0f;
     ml = kNegInf;
     each_block<Block<D, 32>>(a.c, wk.b, wk.h, KvLayout<D>::kBytes, first, last,
                              [&](Block<D, 32>& kb, int blk, auto kdone, auto) {
@@ -828,14 +856,14 @@ __device__ __forceinline__ void attend32(const AttendArgs& a, const Work& wk,
         return p0 + r / 4 * 8 + r % 4 < vis
                    ? __builtin_fmaf(s[r], a.scale, -less)
                    : kNegInf;
-      }, &ml, &l);
+      }, &ml, &lx);
     });
-    if (before != before) l = before;  // a value's NaN
+    lx = row_sum(lx);
+    l = l == l ? lx : l;  // a value's NaN stays
   }
 
   // Join the waves in LDS, 64 channels at a time: 8 threads a row.
   auto so = (float(*)[32][64 + 4])lds.pool;
-  l += __shfl_xor(l, 32);
   const int row = threadIdx.x / 8, c0 = threadIdx.x % 8 * 8;
   const bool queried = visible(a, len, nq, row0 + row) > 0;
   float f[kWaves];
