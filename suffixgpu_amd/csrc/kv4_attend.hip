@@ -14,9 +14,9 @@
 // grown by more than 8, so most blocks rescale nothing and no maximum crosses
 // lanes (followed at once, 64 x 17 tokens over up to 8,192 take 168 us instead of
 // 156, a prompt's 2,048 after 14,336 others 644 instead of 604; with single tokens
-// it is the same).  The largest weight is then between 2^7 and 2^15 of float16's 2^16, and
-// what is rounded to steps of 2^-24 is below 2^-21 of it: however many tokens
-// weigh little beside a heavy one, O has what l counts.
+// it is the same).  The largest weight is then between 2^7 and 2^15, of float16's
+// 2^16, and what is rounded to steps of 2^-24 is below 2^-21 of it: however many
+// tokens weigh little beside a heavy one, O has what l counts.
 // A term of l is 2^(x_t - M), and where s_t is far below the scale that M comes
 // from, 2^(y_t - M) vanishes before 1 / s_t can bring it back: a token of zeros
 // beside one of large values would not count.  What vanishes is less than
