@@ -901,7 +901,7 @@ __device__ __forceinline__ void attend32(const AttendArgs& a, const Work& wk,
 
 // Up to 16 query rows a workgroup: single tokens, and small groups of drafts.
 // The memory bounds it: 64 single tokens over up to 8,192, 32 query heads on 8 KV
-// heads of 128, take 83 us for 422 MB, 5.1 TB/s (a large copy moves 4.9).  Four
+// heads of 128, take 87 us for 422 MB, 4.9 TB/s (as a large copy moves).  Four
 // waves a SIMD, 128 registers; and 36 KB of LDS.
 template <int D, bool kHalf>
 __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 4)
@@ -916,11 +916,11 @@ void k_kv4_attend16(AttendArgs a) {
 
 // 32 query rows a workgroup: verification steps and prompts.  Up to some tens of
 // rows the memory bounds it as above (4 x 9 tokens, 16 query heads on 8 KV heads
-// of 256, over up to 131,072: 198 us for 1.07 GB, 5.4 TB/s), past that the vector
+// of 256, over up to 131,072: 211 us for 1.07 GB, 5.1 TB/s), past that the vector
 // instructions: conversions from 4 bits, exponentials and the sums beside them
-// issue in 78% of a prompt's cycles, matrix instructions in 48% (2,048 tokens
-// after 14,336 others: 560 us, 920 TFLOP/s of the 1,210 that a large matrix
-// product reaches).  64 x 17 tokens over up to 8,192 lie between: 136 us for 440
+// issue in 80% of a prompt's cycles, matrix instructions in 48% (2,048 tokens
+// after 14,336 others: 582 us, 886 TFLOP/s of the 1,210 that a large matrix
+// product reaches).  64 x 17 tokens over up to 8,192 lie between: 148 us for 440
 // MB, as three tiles convert each block of a full row anew.  Three waves a SIMD;
 // four spill (64 x 17 199 us then).
 //
