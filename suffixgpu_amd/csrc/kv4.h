@@ -51,18 +51,24 @@ struct KvView {
   int page_shift;      // log2(page_size / 32)
 };
 
-// Address of block `blk` (32 positions) of row b and KV head h, or NULL where
-// the table holds no page.
+// Place in the pool of block `blk` (32 positions) of row b and KV head h, or -1
+// where the table holds no page.
+__device__ __forceinline__ int64_t kv_place(const KvView& c, int64_t b, int h,
+                                            int64_t blk) {
+  // in blocks: a start next to 2^63 is past the table too
+  if ((uint64_t)blk >= (uint64_t)c.positions / kKvBlock) return -1;
+  const int64_t page = c.table[b * c.table_stride + (blk >> c.page_shift)];
+  if (page < 0 || page >= c.num_pages) return -1;
+  const int64_t in = blk & ((int64_t(1) << c.page_shift) - 1);
+  return ((page * c.heads + h) << c.page_shift) + in;
+}
+
+// Its address, or NULL.
 template <int D>
 __device__ __forceinline__ char* kv_block(const KvView& c, int64_t b, int h,
                                           int64_t blk) {
-  // in blocks: a start next to 2^63 is past the table too
-  if ((uint64_t)blk >= (uint64_t)c.positions / kKvBlock) return nullptr;
-  const int64_t page = c.table[b * c.table_stride + (blk >> c.page_shift)];
-  if (page < 0 || page >= c.num_pages) return nullptr;
-  const int64_t in = blk & ((int64_t(1) << c.page_shift) - 1);
-  return c.pages + ((((page * c.heads + h) << c.page_shift) + in)) *
-                       (int64_t)KvLayout<D>::kBytes;
+  const int64_t at = kv_place(c, b, h, blk);
+  return at < 0 ? nullptr : c.pages + at * (int64_t)KvLayout<D>::kBytes;
 }
 
 inline bool kv_view(const sfx_kv4* c, KvView* v) {
