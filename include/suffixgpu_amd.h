@@ -32,7 +32,7 @@ extern "C" {
 
 #define SFX_EINVAL (-1)
 #define SFX_MAX_CANDIDATES 32
-#define SFX_ABI_VERSION 16
+#define SFX_ABI_VERSION 17
 
 /* Drafter configuration shared by the local and global paths.
  * Mirrors the constructor arguments of SuffixGPUDrafter
@@ -632,6 +632,141 @@ size_t sfx_verify_counter_bytes(int64_t batch, int64_t k, int64_t vocab);
 int sfx_verify_draft(const sfx_verify* args, void* counters,
                      size_t counter_bytes, void* workspace,
                      size_t workspace_bytes, hipStream_t stream);
+
+/* ---- log probabilities ------------------------------------------------- */
+
+/* Log probabilities of given tokens.  logits [batch, positions, vocab] with
+ * element strides of row and position; p = softmax(logits / temperature[b]) as
+ * sfx_verify_draft has it: a NaN counts as -inf, equal +inf share, temperature
+ * 0 (or below, or NaN) is one at the first of the largest logits, NULL is 1.
+ * logprob [batch, positions]: log p(token); entropy: -sum p log p, natural
+ * logarithms.  top_tokens, top_logprobs [batch, positions, top]: the tokens of
+ * the `top` (0 .. SFX_LOGPROBS_TOP) largest logits, the lowest first on ties,
+ * and their log p; -1 and -inf where fewer logits are above -inf.
+ * A position whose token lies outside [0, vocab) is not read: 0, 0, -1, -inf.
+ * Without any logit above -inf: -inf, 0, -1, -inf.
+ * workspace: sfx_logprobs_workspace_size bytes, 16-byte aligned, of any
+ * content; calls that may overlap have their own. */
+#define SFX_LOGPROBS_TOP 32
+typedef struct sfx_logprobs {
+    const void* logits;
+    int32_t dtype;             /* SFX_BF16, SFX_F16 or SFX_F32            */
+    int64_t batch, positions, vocab;
+    int64_t stride_b, stride_j;
+    const int32_t* tokens;     /* [batch, positions]                      */
+    const float* temperature;  /* [batch] or NULL                         */
+    int64_t top;
+    float* logprob;            /* [batch, positions]                      */
+    float* entropy;            /* [batch, positions]                      */
+    int32_t* top_tokens;       /* [batch, positions, top]                 */
+    float* top_logprobs;
+} sfx_logprobs;
+
+size_t sfx_logprobs_workspace_size(int64_t batch, int64_t positions,
+                                   int64_t vocab, int64_t top);
+int sfx_token_logprobs(const sfx_logprobs* args, void* workspace,
+                       size_t workspace_bytes, hipStream_t stream);
+
+/* ---- page tables --------------------------------------------------------- */
+
+/* A pool of pages and the tables of the rows that hold them.  The caller sets
+ * it up once: free_pages a stack of the free page ids, its *num_free lowest
+ * entries used; held[r] pages of row r, which are table[r][0 .. held[r]), -1
+ * behind them.  From then on the calls below change it; those on one pool must
+ * not overlap. */
+typedef struct sfx_pages {
+    int32_t* free_pages;  /* [num_pages]                                  */
+    int32_t* num_free;    /* [1]                                          */
+    int32_t* held;        /* [rows]                                       */
+    int32_t* table;       /* [rows, table_width], contiguous              */
+    int64_t num_pages;
+    int64_t rows;         /* up to SFX_PAGES_ROWS                         */
+    int64_t table_width;
+    int64_t page_size;    /* a power of two, up to 65536                  */
+    int32_t* plan;        /* [3 rows + 4], of any content                 */
+} sfx_pages;
+
+#define SFX_PAGES_ROWS 4096
+
+/* Rows 0 .. n - 1 hold ceil(lengths[r] / page_size) pages afterwards, at most
+ * table_width; a negative length leaves its row as it is.  Rows that grow take
+ * from the top of the stack, the first row first, while there are any of those
+ * that were free when the call began; rows that shrink give back their last
+ * pages, which are free from the next call on (the first row's first on top).
+ * So lengths put back as they were put the pages back as well.  room [n]: the
+ * tokens that each row's pages hold. */
+int sfx_pages_resize(const sfx_pages* pool, const void* lengths,
+                     int32_t lengths_is64, int64_t n, int32_t* room,
+                     hipStream_t stream);
+
+/* slots [n, tokens]: where position start[r] + i of row r lies, page id *
+ * page_size + position % page_size, for i < count[r] (all without it); -1 where
+ * the row holds no page, and from count on. */
+int sfx_pages_slots(const sfx_pages* pool, const void* start,
+                    int32_t start_is64, const void* count, int32_t count_is64,
+                    int64_t n, int64_t tokens, int64_t* slots,
+                    hipStream_t stream);
+
+/* ---- attention over selected blocks -------------------------------------- */
+
+/* Bounds of the cache's keys, a block of 32 tokens and a KV head at a time, in
+ * the order of the cache's blocks: range [num_pages, heads, page_size / 32,
+ * 2 D] holds the least (D channels) and the largest (D channels) key of the
+ * block in units of 2^unit, rounded outwards; unit is the exponent of the
+ * largest magnitude's power of two, less 6, between -100 and 100 (larger keys
+ * count as 127 units); 127: the block holds a NaN.
+ * sfx_kv4_bounds_update sets them for the blocks that hold positions start[b]
+ * .. start[b] + min(count[b], tokens) - 1, of the tokens up to those; it
+ * follows every append. */
+typedef struct sfx_kv4_bounds {
+    int8_t* range;  /* 16-byte aligned */
+    int8_t* unit;
+} sfx_kv4_bounds;
+
+int sfx_kv4_bounds_update(const sfx_kv4* cache, const sfx_kv4_bounds* bounds,
+                          int64_t batch, int64_t tokens, const void* start,
+                          int32_t start_is64, const void* count,
+                          int32_t count_is64, hipStream_t stream);
+
+/* Which blocks a query token attends to, per KV head.  Queries stand where
+ * sfx_kv4_attend has them.  Of the blocks up to its own, a query takes the
+ * first `first`, the last `recent` (its own among them), then those with the
+ * largest
+ *   2^unit sum_c (P_c largest_c - N_c least_c),
+ * the lowest on ties, `blocks` in all; blocks that the table does not hold are
+ * no candidates, a block with a NaN comes before all but the first and the
+ * recent ones.  P and N: with 2^x the power of two at or below the largest
+ * magnitude of the KV head's query channels, these times 2^(14 - x) rounded to
+ * whole numbers (to the even one; infinities and NaN are 0), sums over its
+ * query heads of the positive and of the negated negative ones, both divided by
+ * the same power of two, 1 or more, that leaves 7 bits, halves up, at most 127.
+ * selected [batch, tokens, heads, blocks]: positions / 32, ascending, -1 behind
+ * them and for what is no query.  1 <= recent, first + recent <= blocks.
+ * workspace: sfx_kv4_select_workspace_size bytes, 16-byte aligned, of any
+ * content; calls that may overlap have their own. */
+size_t sfx_kv4_select_workspace_size(const sfx_kv4* cache, int64_t batch,
+                                     int64_t tokens);
+int sfx_kv4_select(const sfx_kv4* cache, const sfx_kv4_bounds* bounds,
+                   const sfx_heads* q, int64_t batch, int64_t tokens,
+                   int64_t q_heads, const void* kv_len, int32_t kv_len_is64,
+                   const void* q_len, int32_t q_len_is64, int64_t blocks,
+                   int64_t first, int64_t recent, int32_t* selected,
+                   void* workspace, size_t workspace_bytes,
+                   hipStream_t stream);
+
+/* sfx_kv4_attend over the positions of the blocks selected [batch, tokens,
+ * heads, blocks] that each query sees.  In any order; an entry that names no
+ * block of the table counts as none, a block named twice counts twice. */
+size_t sfx_kv4_attend_blocks_workspace_size(const sfx_kv4* cache,
+                                            int64_t batch, int64_t tokens,
+                                            int64_t q_heads, int64_t blocks);
+int sfx_kv4_attend_blocks(const sfx_kv4* cache, const sfx_heads* q,
+                          int64_t batch, int64_t tokens, int64_t q_heads,
+                          const int32_t* selected, int64_t blocks,
+                          const void* kv_len, int32_t kv_len_is64,
+                          const void* q_len, int32_t q_len_is64, float scale,
+                          void* out, void* workspace, size_t workspace_bytes,
+                          hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,6 +1,7 @@
 """The operators on the target model's side of a step, by their definitions, in
-numpy and 64 bits: verification of drafts, the rounding of keys and values to
-4 bits, and attention over what they then stand for."""
+numpy and 64 bits: verification of drafts, log probabilities, page tables, the
+rounding of keys and values to 4 bits, and attention over what they then stand for,
+all of it or selected blocks."""
 
 from __future__ import annotations
 
@@ -112,6 +113,26 @@ def quantize_v(v):
     return np.where(finite, y, np.nan), top / 6
 
 
+def _attend_row(q, k, v, vscale, scale):
+    """One query head's (result, bound) over the tokens of k, v and vscale."""
+    kk, vv = k.astype(np.float64), v.astype(np.float64)
+    qq = q.astype(np.float64)
+    x = kk @ qq * scale
+    with np.errstate(invalid="ignore", over="ignore"):
+        w = np.exp(x - x.max())
+        w /= w.sum()
+    # products are exact, sums of d + 1 terms are not, the score in base 2 and
+    # log2 of the scale are rounded
+    ls = np.abs(np.log2(vscale)) + 1
+    ex = ((q.shape[-1] + 4) * 2.0 ** -24 * (np.abs(kk) @ np.abs(qq))
+          * abs(scale) + (np.abs(x) * 2 + ls) * 2.0 ** -22).max()
+    mass = w @ np.abs(vv)
+    # float16 weights: 2^-11 relative (and as much again for approximations),
+    # 2^-25 of the largest below its range
+    return w @ vv, (mass * (2.0 ** -11 + 2.0 ** -14 + 3 * ex)
+                    + 2.0 ** -25 * 6 * len(x) * vscale.max())
+
+
 def attend(q, k, v, vscale, kv_len, q_len, scale=None):
     """q [B, T, Hq, D], k and v [B, L, H, D] as they stand in the cache, vscale
     [B, L, H, 1].  Returns (out, bound): how far a result computed with
@@ -129,25 +150,9 @@ def attend(q, k, v, vscale, kv_len, q_len, scale=None):
             if see <= 0:
                 continue
             for a in range(hq):
-                kk = k[i, :see, a // g].astype(np.float64)
-                vv = v[i, :see, a // g].astype(np.float64)
-                qq = q[i, j, a].astype(np.float64)
-                x = kk @ qq * scale
-                with np.errstate(invalid="ignore", over="ignore"):
-                    w = np.exp(x - x.max())
-                    w /= w.sum()
-                out[i, j, a] = w @ vv
-                # products are exact, sums of d + 1 terms are not, the score
-                # in base 2 and log2 of the scale are rounded
-                ls = np.abs(np.log2(vscale[i, :see, a // g, 0])) + 1
-                ex = ((d + 4) * 2.0 ** -24 * (np.abs(kk) @ np.abs(qq))
-                      * abs(scale) + (np.abs(x) * 2 + ls) * 2.0 ** -22).max()
-                mass = w @ np.abs(vv)
-                # float16 weights: 2^-11 relative (and as much again for
-                # approximations), 2^-25 of the largest below its range
-                bound[i, j, a] = (mass * (2.0 ** -11 + 2.0 ** -14 + 3 * ex)
-                                  + 2.0 ** -25 * 6 * see
-                                  * vscale[i, :see, a // g].max())
+                out[i, j, a], bound[i, j, a] = _attend_row(
+                    q[i, j, a], k[i, :see, a // g], v[i, :see, a // g],
+                    vscale[i, :see, a // g, 0], scale)
     return out, bound
 
 
@@ -156,3 +161,179 @@ def ulp16(half: bool):
     return (2.0 ** -11, 2.0 ** -25) if half else (2.0 ** -8, 2.0 ** -134)
 
 
+BLOCK = 32
+
+
+def attend_blocks(q, selected, k, v, vscale, kv_len, q_len, scale=None):
+    """As attend, over the positions of selected [B, T, H, N] blocks; those that
+    name no block of k's length count as none."""
+    b, t, hq, d = q.shape
+    n, h = k.shape[1:3]
+    g = hq // h
+    scale = d ** -0.5 if scale is None else scale
+    out = np.zeros(q.shape)
+    bound = np.zeros(q.shape)
+    for i in range(b):
+        for j in range(min(int(q_len[i]), t)):
+            see = min(int(kv_len[i]) - int(q_len[i]) + j + 1, n)
+            for a in range(hq):
+                at = [p for x in selected[i, j, a // g].tolist() if x >= 0
+                      for p in range(BLOCK * x, min(BLOCK * x + BLOCK, see))]
+                if at:
+                    out[i, j, a], bound[i, j, a] = _attend_row(
+                        q[i, j, a], k[i, at, a // g], v[i, at, a // g],
+                        vscale[i, at, a // g, 0], scale)
+    return out, bound
+
+
+def key_bounds(k):
+    """[n <= 32, D] keys of a block -> (least, largest, unit) in whole units;
+    unit 127 and zeros where there is a NaN."""
+    d = k.shape[-1]
+    if np.isnan(k).any():
+        return np.zeros(d, int), np.zeros(d, int), 127
+    top = np.abs(k).max()
+    unit = -100
+    if top > 0:
+        unit = int(np.clip(np.frexp(top)[1] - 7, -100, 100))
+    lo = np.floor(np.ldexp(k.min(axis=0), -unit))
+    hi = np.ceil(np.ldexp(k.max(axis=0), -unit))
+    return (np.clip(lo, -127, 127).astype(int),
+            np.clip(hi, -127, 127).astype(int), unit)
+
+
+def pack_query(q):
+    """[G, D] query heads -> (P, N), whole numbers of 7 bits."""
+    x = np.where(np.isfinite(q), q, 0.0).astype(np.float64)
+    top = np.abs(x).max()
+    if top == 0:
+        z = np.zeros(q.shape[-1], int)
+        return z, z
+    z = np.rint(np.ldexp(x, 15 - int(np.frexp(top)[1]))).astype(np.int64)
+    p, n = np.maximum(z, 0).sum(axis=0), np.maximum(-z, 0).sum(axis=0)
+    shift = max(0, int(max(p.max(), n.max())).bit_length() - 7)
+    return tuple(np.minimum((x + ((1 << shift) >> 1)) >> shift, 127)
+                 for x in (p, n))
+
+
+def select_blocks(q, bounds, kv_len, q_len, positions, blocks, first, recent):
+    """q [B, T, Hq, D]; bounds[i][j][a]: key_bounds of row i's block j and KV head
+    a, None where the table holds no page.  Python integers decide."""
+    b, t, hq, _ = q.shape
+    h = len(bounds[0][0]) if bounds and bounds[0] else 1
+    g = hq // h
+    out = np.full((b, t, h, blocks), -1, dtype=np.int32)
+    for i in range(b):
+        for j in range(min(int(q_len[i]), t)):
+            see = min(int(kv_len[i]) - int(q_len[i]) + j + 1, positions)
+            last = -(-see // BLOCK) - 1
+            for a in range(h):
+                p, n = pack_query(q[i, j, a * g:(a + 1) * g])
+                ranked = []
+                for x in range(last + 1):
+                    if bounds[i][x][a] is None:
+                        continue
+                    lo, hi, unit = bounds[i][x][a]
+                    if x < first or x > last - recent:
+                        key = (2, 0)
+                    elif unit == 127:
+                        key = (1, 0)
+                    else:   # in units of 2^-100
+                        key = (0, int(p @ hi - n @ lo) << (unit + 100))
+                    ranked.append((key, -x))
+                ranked.sort(reverse=True)
+                got = sorted(-x for _, x in ranked[:blocks])
+                out[i, j, a, :len(got)] = got
+    return out
+
+
+def logprobs(logits, tokens, temperature=None, top=0):
+    """(logprob, entropy, top tokens, top logprobs, and how far the first, the
+    second and the last may be off computed in 32 bits)."""
+    b, n, v = logits.shape
+    lp, h = np.zeros((b, n)), np.zeros((b, n))
+    ids = np.full((b, n, top), -1, dtype=np.int32)
+    alt = np.full((b, n, top), -np.inf)
+    tol = np.zeros((b, n)), np.zeros((b, n)), np.zeros((b, n, top))
+    for i in range(b):
+        t = 1.0 if temperature is None else float(temperature[i])
+        for j in range(n):
+            d = int(tokens[i, j])
+            if not 0 <= d < v:
+                continue
+            x = logits[i, j].astype(np.float64)
+            x = np.where(np.isnan(x), -np.inf, x)
+            lp[i, j] = -np.inf
+            order = np.argsort(-x, kind="stable")
+            if x[order[0]] == -np.inf:
+                continue
+            if t > 0:
+                with np.errstate(invalid="ignore", over="ignore"):
+                    z = np.where(x == x[order[0]], 0.0, (x - x[order[0]]) / t)
+            else:
+                z = np.full(v, -np.inf)
+                z[order[0]] = 0.0
+            e = np.exp(z)
+            rest = np.delete(e, order[0]).sum()
+            log = np.log1p(rest)
+            with np.errstate(invalid="ignore"):
+                ze = np.where(e > 0, -z * e, 0.0)
+                zze = np.where(e > 0, z * z * e, 0.0)
+            lp[i, j] = z[d] - log
+            h[i, j] = log + ze.sum() / (1 + rest)
+            best = order[:top][x[order[:top]] > -np.inf]
+            ids[i, j, :len(best)] = best
+            alt[i, j, :len(best)] = z[best] - log
+            if not t > 0:
+                continue
+            # the exponent is rounded four times, its power once more; a sum has
+            # at most 64 additions behind one another; log1p and the result are
+            # off by 2^-23 each
+            u = 2.0 ** -24
+            off = (u * (4 * ze.sum() + 4 * rest + 64 * rest) / (1 + rest)
+                   + 4 * u * log)
+            with np.errstate(invalid="ignore"):
+                def of(y):
+                    return np.where(y > -np.inf, off + 6 * u * np.abs(y), 0.0)
+                tol[0][i, j] = of(z[d])
+                tol[2][i, j, :len(best)] = of(z[best])
+            tol[1][i, j] = (off + u * (4 * zze.sum() + 72 * ze.sum())
+                            / (1 + rest) * (1 + rest / (1 + rest))
+                            + off * ze.sum() / (1 + rest) + 4 * u * h[i, j])
+    return lp, h, ids, alt, tol
+
+
+class Pages:
+    """A pool of pages by lists: free (its end on top), and each row's."""
+
+    def __init__(self, num_pages, rows, width, page_size):
+        self.free = list(range(num_pages - 1, -1, -1))
+        self.rows = [[] for _ in range(rows)]
+        self.width, self.page_size = width, page_size
+
+    def resize(self, lengths):
+        back = []
+        for row, n in zip(self.rows, lengths):
+            if n < 0:
+                continue
+            want = min(-(-int(n) // self.page_size), self.width)
+            while len(row) < want and self.free:
+                row.append(self.free.pop())
+            back += row[want:]
+            del row[want:]
+        self.free += reversed(back)
+        return [len(r) * self.page_size for r in self.rows[:len(lengths)]]
+
+    def table(self):
+        return np.array([r + [-1] * (self.width - len(r)) for r in self.rows],
+                        dtype=np.int32)
+
+    def slots(self, start, tokens, count=None):
+        out = np.full((len(start), tokens), -1, dtype=np.int64)
+        for r, s in enumerate(start):
+            for i in range(tokens if count is None else min(tokens, count[r])):
+                p = int(s) + i
+                if 0 <= int(s) and p // self.page_size < len(self.rows[r]):
+                    out[r, i] = (self.rows[r][p // self.page_size]
+                                 * self.page_size + p % self.page_size)
+        return out

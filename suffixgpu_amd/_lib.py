@@ -18,7 +18,7 @@ import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libsuffixgpu_amd.so"
 MAX_CANDIDATES = 32
-ABI_VERSION = 16
+ABI_VERSION = 17
 
 c_i32 = ctypes.c_int32
 c_i64 = ctypes.c_int64
@@ -94,7 +94,32 @@ class SfxVerify(ctypes.Structure):
     ]
 
 
+class SfxKv4Bounds(ctypes.Structure):
+    _fields_ = [("range", c_p), ("unit", c_p)]
+
+
+class SfxLogprobs(ctypes.Structure):
+    _fields_ = [
+        ("logits", c_p), ("dtype", c_i32), ("batch", c_i64),
+        ("positions", c_i64), ("vocab", c_i64),
+        ("stride_b", c_i64), ("stride_j", c_i64),
+        ("tokens", c_p), ("temperature", c_p), ("top", c_i64),
+        ("logprob", c_p), ("entropy", c_p), ("top_tokens", c_p),
+        ("top_logprobs", c_p),
+    ]
+
+
+class SfxPages(ctypes.Structure):
+    _fields_ = [
+        ("free_pages", c_p), ("num_free", c_p), ("held", c_p), ("table", c_p),
+        ("num_pages", c_i64), ("rows", c_i64), ("table_width", c_i64),
+        ("page_size", c_i64), ("plan", c_p),
+    ]
+
+
 APPEND_MAX_DOCS = 64
+LOGPROBS_TOP = 32
+PAGES_ROWS = 4096
 # element types of the target-side operators
 DTYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
@@ -193,6 +218,32 @@ SIGNATURES = {
     "sfx_verify_draft": (c_i32, [ctypes.POINTER(SfxVerify), c_p,
                                  ctypes.c_size_t, c_p, ctypes.c_size_t,
                                  c_p]),
+    "sfx_logprobs_workspace_size": (ctypes.c_size_t,
+                                    [c_i64, c_i64, c_i64, c_i64]),
+    "sfx_token_logprobs": (c_i32, [ctypes.POINTER(SfxLogprobs), c_p,
+                                   ctypes.c_size_t, c_p]),
+    "sfx_pages_resize": (c_i32, [ctypes.POINTER(SfxPages), c_p, c_i32, c_i64,
+                                 c_p, c_p]),
+    "sfx_pages_slots": (c_i32, [ctypes.POINTER(SfxPages), c_p, c_i32, c_p,
+                                c_i32, c_i64, c_i64, c_p, c_p]),
+    "sfx_kv4_bounds_update": (c_i32, [ctypes.POINTER(SfxKv4),
+                                      ctypes.POINTER(SfxKv4Bounds), c_i64,
+                                      c_i64, c_p, c_i32, c_p, c_i32, c_p]),
+    "sfx_kv4_select_workspace_size": (ctypes.c_size_t,
+                                      [ctypes.POINTER(SfxKv4), c_i64, c_i64]),
+    "sfx_kv4_select": (c_i32, [ctypes.POINTER(SfxKv4),
+                               ctypes.POINTER(SfxKv4Bounds),
+                               ctypes.POINTER(SfxHeads), c_i64, c_i64, c_i64,
+                               c_p, c_i32, c_p, c_i32, c_i64, c_i64, c_i64,
+                               c_p, c_p, ctypes.c_size_t, c_p]),
+    "sfx_kv4_attend_blocks_workspace_size": (ctypes.c_size_t,
+                                             [ctypes.POINTER(SfxKv4), c_i64,
+                                              c_i64, c_i64, c_i64]),
+    "sfx_kv4_attend_blocks": (c_i32, [ctypes.POINTER(SfxKv4),
+                                      ctypes.POINTER(SfxHeads), c_i64, c_i64,
+                                      c_i64, c_p, c_i64, c_p, c_i32, c_p,
+                                      c_i32, ctypes.c_float, c_p, c_p,
+                                      ctypes.c_size_t, c_p]),
 }
 
 _lib = None

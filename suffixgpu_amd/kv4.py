@@ -6,7 +6,10 @@ as e2m1 with a power-of-two scale per 32 channels, values as e2m1 with a float32
 scale per token.  ``append`` writes the newest tokens'
 keys and values, drafts among them; ``attend`` is the attention of those tokens'
 queries, each over everything up to itself; a rejected draft's entries are
-simply overwritten by the next ``append``.  No counterpart in the reference.
+simply overwritten by the next ``append``.  For long rows a cache may hold the
+bounds of its keys, block by block: ``select_blocks`` chooses by them which
+blocks of 32 tokens a query can have its largest scores in, and ``attend_blocks``
+attends to those alone.  No counterpart in the reference.
 """
 
 from __future__ import annotations
@@ -34,14 +37,20 @@ class KV4Cache:
     the pool (its layout is in include/suffixgpu_amd.h); an existing one may be
     passed.  Which pages a request holds is the caller's: every call takes
     ``page_table`` [B, W] int32, position p of row b lying in page
-    ``page_table[b, p // page_size]``.  Page ids outside [0, num_pages) hold
-    nothing: nothing is written there and no query sees them.
+    ``page_table[b, p // page_size]`` (``PagePool`` makes such tables).  Page ids
+    outside [0, num_pages) hold nothing: nothing is written there and no query
+    sees them.
+
+    ``bounds=True`` holds the bounds of the keys too (2 head_dim + 1 bytes for 32
+    tokens of a KV head, 6% more), which ``append`` then keeps: what
+    ``select_blocks`` needs.  A pool that was filled before has them from
+    ``update_bounds``.
     """
 
     def __init__(self, num_pages: int, num_kv_heads: int, head_dim: int,
                  page_size: int = 64, dtype: torch.dtype = torch.bfloat16,
                  device: torch.device | str = "cuda",
-                 pages: torch.Tensor | None = None):
+                 pages: torch.Tensor | None = None, bounds: bool = False):
         if head_dim not in (64, 128, 256):
             raise ValueError("head_dim must be 64, 128 or 256")
         if not 32 <= page_size <= 65536 or page_size & (page_size - 1):
@@ -77,6 +86,15 @@ class KV4Cache:
                           self.head_dim, self.page_size,
                           _lib.DTYPE_CODES[dtype])
         self._sizes: dict[tuple, int] = {}
+        # ranges and units of the keys (include/suffixgpu_amd.h), their C view
+        self._range = self._unit = self._bounds = None
+        if bounds:
+            self._range = torch.zeros(shape[:3] + (2 * self.head_dim,),
+                                      dtype=torch.int8, device=self.device)
+            self._unit = torch.zeros(shape[:3], dtype=torch.int8,
+                                     device=self.device)
+            self._bounds = _lib.SfxKv4Bounds(self._range.data_ptr(),
+                                             self._unit.data_ptr())
 
     @property
     def pages(self) -> torch.Tensor:
@@ -131,7 +149,8 @@ class KV4Cache:
                page_table: torch.Tensor, start: torch.Tensor,
                count: torch.Tensor | None = None) -> None:
         """Write tokens i < ``count[b]`` (all without it) of ``k`` and ``v``
-        [B, T, num_kv_heads, head_dim] at positions ``start[b] + i``.
+        [B, T, num_kv_heads, head_dim] at positions ``start[b] + i``, and the
+        bounds of the blocks that these lie in, where the cache holds them.
 
         A page that one row of a call writes must not be written by another
         row of it.  Infinities and NaN make their 32 channels of a key, or
@@ -148,9 +167,13 @@ class KV4Cache:
                 self._counts("count", count, b, optional=True))
         if b == 0 or t == 0:
             return
-        check(lib().sfx_kv4_append(view, kh, vh, b, t, *keep[0][1:],
-                                   *keep[1][1:], stream_of(self.device)),
-              "KV4Cache.append")
+        L, stream = lib(), stream_of(self.device)
+        check(L.sfx_kv4_append(view, kh, vh, b, t, *keep[0][1:],
+                               *keep[1][1:], stream), "KV4Cache.append")
+        if self._bounds is not None:
+            check(L.sfx_kv4_bounds_update(view, self._bounds, b, t,
+                                          *keep[0][1:], *keep[1][1:], stream),
+                  "KV4Cache.append")
 
     def read(self, page_table: torch.Tensor, start: torch.Tensor,
              tokens: int, count: torch.Tensor | None = None):
@@ -218,4 +241,144 @@ class KV4Cache:
                                *keep[1][1:], scale, out.data_ptr(),
                                None if ws is None else ws.data_ptr(), nbytes,
                                stream_of(self.device)), "KV4Cache.attend")
+        return out
+
+    # ------------------------------------------------ over selected blocks
+    def _need_bounds(self):
+        if self._bounds is None:
+            raise ValueError("the cache holds no bounds: make it with "
+                             "bounds=True")
+
+    def update_bounds(self, page_table: torch.Tensor, start: torch.Tensor,
+                      tokens: int, count: torch.Tensor | None = None) -> None:
+        """Set the bounds of the blocks that hold positions ``start[b] + i``,
+        i < ``min(tokens, count[b])`` (tokens without it), from what they hold
+        up to the last of these.  ``append`` does it by itself; this is for pages
+        that something else has written."""
+        self._need_bounds()
+        if elsewhere(self.device):
+            with torch.cuda.device(self.device):
+                return self.update_bounds(page_table, start, tokens, count)
+        b = page_table.shape[0]
+        view = self._view(page_table, b)
+        keep = (self._counts("start", start, b),
+                self._counts("count", count, b, optional=True))
+        check(lib().sfx_kv4_bounds_update(view, self._bounds, b, int(tokens),
+                                          *keep[0][1:], *keep[1][1:],
+                                          stream_of(self.device)),
+              "KV4Cache.update_bounds")
+
+    def bounds(self, page_table: torch.Tensor):
+        """(least, largest) key [B, blocks, num_kv_heads, head_dim] float32 of
+        each block of the rows, as ``select_blocks`` knows them: at most and at
+        least what ``read`` gives.  Blocks without a page: zeros; with a NaN: NaN."""
+        self._need_bounds()
+        view = self._view(page_table, page_table.shape[0])
+        b, w = page_table.shape
+        ids = page_table.long()
+        held = (ids >= 0) & (ids < self.num_pages)
+        if view.num_pages == 0 or w == 0:
+            z = torch.zeros(b, w * (self.page_size // BLOCK),
+                            self.num_kv_heads, self.head_dim,
+                            device=self.device)
+            return z, z.clone()
+        ids = torch.where(held, ids, 0)
+        unit = self._unit[ids].float()
+        unit = torch.where(unit == 127, float("nan"), torch.exp2(unit))
+        x = self._range[ids].float() * unit[..., None]
+        x = torch.where(held[:, :, None, None, None], x, 0.0)
+        # [B, W, heads, blocks, 2 D] -> [B, W * blocks, heads, 2 D]
+        x = x.transpose(2, 3).reshape(b, -1, self.num_kv_heads,
+                                      2 * self.head_dim)
+        return x[..., :self.head_dim], x[..., self.head_dim:]
+
+    def select_blocks(self, q: torch.Tensor, page_table: torch.Tensor,
+                      kv_len: torch.Tensor, q_len: torch.Tensor | None = None,
+                      blocks: int = 64, first: int = 1,
+                      recent: int = 2) -> torch.Tensor:
+        """The ``blocks`` blocks of 32 tokens that each of the newest tokens'
+        queries ``q`` (as ``attend`` takes them) attends to, per KV head: of those
+        up to the query's own the ``first`` first ones, the ``recent`` last ones,
+        its own among them, and those in which the sum of the KV head's query
+        heads' scores can be the largest, the lowest on ties.
+
+        Returns [B, T, num_kv_heads, blocks] int32: block i of a row holds its
+        positions 32 i to 32 i + 31; ascending, -1 behind them (and for tokens
+        that are no queries).  Whole numbers decide, so the result is the same
+        on any call; their rule is in include/suffixgpu_amd.h."""
+        self._need_bounds()
+        if elsewhere(self.device):
+            with torch.cuda.device(self.device):
+                return self.select_blocks(q, page_table, kv_len, q_len, blocks,
+                                          first, recent)
+        qh, b, t, heads = self._heads("q", q)
+        if heads < 1 or heads % self.num_kv_heads:
+            raise ValueError(f"{heads} query heads do not share "
+                             f"{self.num_kv_heads} KV heads evenly")
+        if first < 0 or recent < 1 or not first + recent <= blocks <= 32768:
+            raise ValueError("first >= 0, recent >= 1 and first + recent <= "
+                             "blocks <= 32768")
+        view = self._view(page_table, b)
+        keep = (self._counts("kv_len", kv_len, b),
+                self._counts("q_len", q_len, b, optional=True))
+        out = torch.empty(b, t, self.num_kv_heads, blocks, dtype=torch.int32,
+                          device=self.device)
+        if b == 0 or t == 0:
+            return out
+        L = lib()
+        nbytes = L.sfx_kv4_select_workspace_size(view, b, t)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        check(L.sfx_kv4_select(view, self._bounds, qh, b, t, heads,
+                               *keep[0][1:], *keep[1][1:], blocks, first,
+                               recent, out.data_ptr(), ws.data_ptr(), nbytes,
+                               stream_of(self.device)),
+              "KV4Cache.select_blocks")
+        return out
+
+    def attend_blocks(self, q: torch.Tensor, selected: torch.Tensor,
+                      page_table: torch.Tensor, kv_len: torch.Tensor,
+                      q_len: torch.Tensor | None = None,
+                      scale: float | None = None) -> torch.Tensor:
+        """``attend`` over the positions of the ``selected`` blocks [B, T,
+        num_kv_heads, N] int32 (as ``select_blocks`` gives them, or another
+        layer's) that each query sees.  Entries may stand in any order; one that
+        names no block of the table counts as none, a block that is named twice
+        counts twice.  Zeros for a query that sees nothing."""
+        if elsewhere(self.device):
+            with torch.cuda.device(self.device):
+                return self.attend_blocks(q, selected, page_table, kv_len,
+                                          q_len, scale)
+        qh, b, t, heads = self._heads("q", q)
+        if heads < 1 or heads % self.num_kv_heads:
+            raise ValueError(f"{heads} query heads do not share "
+                             f"{self.num_kv_heads} KV heads evenly")
+        if (selected.dim() != 4 or selected.dtype is not torch.int32
+                or selected.device != self.device
+                or selected.shape[:3] != (b, t, self.num_kv_heads)
+                or not 1 <= selected.shape[3] <= 32768
+                or not selected.is_contiguous()):
+            require_gpu(selected)
+            raise ValueError(f"selected must be a contiguous int32 [{b}, {t}, "
+                             f"{self.num_kv_heads}, N] tensor on {self.device}"
+                             ", 1 <= N <= 32768")
+        n = selected.shape[3]
+        view = self._view(page_table, b)
+        keep = (self._counts("kv_len", kv_len, b),
+                self._counts("q_len", q_len, b, optional=True))
+        if scale is None:
+            scale = self.head_dim ** -0.5
+        out = torch.empty(b, t, heads, self.head_dim, dtype=self.dtype,
+                          device=self.device)
+        if b == 0 or t == 0:
+            return out
+        L = lib()
+        nbytes = L.sfx_kv4_attend_blocks_workspace_size(view, b, t, heads, n)
+        ws = (torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+              if nbytes else None)
+        check(L.sfx_kv4_attend_blocks(view, qh, b, t, heads,
+                                      selected.data_ptr(), n, *keep[0][1:],
+                                      *keep[1][1:], scale, out.data_ptr(),
+                                      None if ws is None else ws.data_ptr(),
+                                      nbytes, stream_of(self.device)),
+              "KV4Cache.attend_blocks")
         return out
