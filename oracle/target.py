@@ -166,7 +166,7 @@ BLOCK = 32
 
 def attend_blocks(q, selected, k, v, vscale, kv_len, q_len, scale=None):
     """As attend, over the positions of selected [B, T, H, N] blocks; those that
-    name no block of k's length count as none."""
+    name no block of k's length count as none, those named twice as one."""
     b, t, hq, d = q.shape
     n, h = k.shape[1:3]
     g = hq // h
@@ -177,7 +177,8 @@ def attend_blocks(q, selected, k, v, vscale, kv_len, q_len, scale=None):
         for j in range(min(int(q_len[i]), t)):
             see = min(int(kv_len[i]) - int(q_len[i]) + j + 1, n)
             for a in range(hq):
-                at = [p for x in selected[i, j, a // g].tolist() if x >= 0
+                at = [p for x in sorted(set(selected[i, j, a // g].tolist()))
+                      if x >= 0
                       for p in range(BLOCK * x, min(BLOCK * x + BLOCK, see))]
                 if at:
                     out[i, j, a], bound[i, j, a] = _attend_row(

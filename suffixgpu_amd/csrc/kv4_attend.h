@@ -556,7 +556,10 @@ constexpr int kLds32 = kWaves * 32 * (64 + 4) * 4 > 32 * D * 2
                            ? kWaves * 32 * (64 + 4) * 4
                            : 32 * D * 2;
 
-// Blocks first, first + kWaves, ... of a split that a wave of attend16 takes.
+// Which blocks a wave of attend16 takes: each(a, wk, bytes, vis, body) calls
+// body(block, index, v, whole, kdone, vdone) with the positions v that the lane's
+// row sees if it takes the block (vis, or 0), whole where every row does.  Here
+// blocks first, first + kWaves, ... of a split, by all rows.
 struct SplitBlocks {
   int splits, first, last;
   __device__ __forceinline__ SplitBlocks(const AttendArgs& a, const Work& wk,
@@ -572,8 +575,11 @@ struct SplitBlocks {
   }
   template <class B, class F>
   __device__ __forceinline__ void each(const AttendArgs& a, const Work& wk,
-                                       int bytes, F body) const {
-    each_block<B>(a.c, wk.b, wk.h, bytes, first, last, body);
+                                       int bytes, int vis, F body) const {
+    each_block<B>(a.c, wk.b, wk.h, bytes, first, last,
+                  [&](B& x, int blk, auto kdone, auto vdone) {
+                    body(x, blk, vis, true, kdone, vdone);
+                  });
   }
 };
 
@@ -609,7 +615,7 @@ __device__ __forceinline__ void attend16(const A& a, const Work& wk,
   }
   most = __builtin_amdgcn_readfirstlane(most);
   least = __builtin_amdgcn_readfirstlane(least);
-  const Blocks blocks(a, wk, len, most, wave);
+  Blocks blocks(a, wk, len, most, wave);
 
   float m = kNegInf, l = 0.0f, inv = 0.0f;
   F4 o[kDt];
@@ -617,11 +623,11 @@ __device__ __forceinline__ void attend16(const A& a, const Work& wk,
   for (int d = 0; d < kDt; ++d) o[d] = F4{0, 0, 0, 0};
 
   blocks.template each<Block<D, 16>>(
-      a, wk, KvLayout<D>::kBytes,
-      [&](Block<D, 16>& kb, int blk, auto kdone, auto vdone) {
+      a, wk, KvLayout<D>::kBytes, vis,
+      [&](Block<D, 16>& kb, int blk, int v, bool whole, auto kdone, auto vdone) {
     share_scales(kb.vs, most - blk * kKvBlock, sc[wave], &inv);
     const int p0 = blk * kKvBlock + 16 * (quad / 2) + 4 * (quad % 2);
-    const bool edge = blk * kKvBlock + kKvBlock > least;
+    const bool edge = blk * kKvBlock + kKvBlock > least || !whole;
     F4 s[2] = {F4{0, 0, 0, 0}, F4{0, 0, 0, 0}};
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -647,7 +653,7 @@ __device__ __forceinline__ void attend16(const A& a, const Work& wk,
       asm volatile("");  // a branch: most blocks have no edge
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (p0 + 8 * (j / 4) + j % 4 >= vis) y[j] = kNegInf;
+        if (p0 + 8 * (j / 4) + j % 4 >= v) y[j] = kNegInf;
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = fmaxf(top, y[j]);
@@ -683,8 +689,8 @@ __device__ __forceinline__ void attend16(const A& a, const Work& wk,
     float lx = 0.0f;
     ml = kNegInf;
     blocks.template each<Block<D, 16>>(
-        a, wk, KvLayout<D>::kBytes,
-        [&](Block<D, 16>& kb, int blk, auto kdone, auto) {
+        a, wk, KvLayout<D>::kBytes, vis,
+        [&](Block<D, 16>& kb, int blk, int v, bool, auto kdone, auto) {
       const int p0 = blk * kKvBlock + 16 * (quad / 2) + 4 * (quad % 2);
       F4 s[2] = {F4{0, 0, 0, 0}, F4{0, 0, 0, 0}};
 #pragma unroll
@@ -695,7 +701,7 @@ __device__ __forceinline__ void attend16(const A& a, const Work& wk,
                               s[t]);
       kdone();
       sum_apart<16, 8>([&](int j, float less) {
-        return p0 + 8 * (j / 4) + j % 4 < vis
+        return p0 + 8 * (j / 4) + j % 4 < v
                    ? __builtin_fmaf(s[j / 4][j % 4], a.scale, -less)
                    : kNegInf;
       }, &ml, &lx);

@@ -1,7 +1,8 @@
 // Attention over selected blocks of the 4-bit cache.  The mathematics is in
-// kv4_attend.h: a workgroup takes a query token's heads of one KV head (16 rows of
-// the matrix instruction, of which the group's are queries) over its list of
-// blocks, or over a part of the list.
+// kv4_attend.h: a workgroup takes the query heads of one KV head of as many tokens
+// as give 16 rows, over the blocks that any of these tokens selected (or a part of
+// them); a row passes over the blocks of the others.  Neighbouring tokens select
+// much the same blocks, each of which is then loaded and converted once.
 
 #include <algorithm>
 
@@ -15,83 +16,255 @@ namespace {
 struct ListArgs : AttendArgs {
   const int32_t* selected;  // [batch, tokens, heads, width]
   int width;
-  int per;    // entries of a split
-  int tiles;  // of 16 query heads
+  int span;   // query tokens of a tile
+  int tiles;  // of 16 query heads, of a token with more than that
+  // with a span of more than one: the blocks of each tile [batch, heads, tiles of
+  // the query, span * width] and their number
+  int2* entry;
+  int32_t* entries;
 };
 
-// Entries wave, wave + kWaves, ... of a split.
-struct ListBlocks {
-  int splits, first, last, limit;
-  const int32_t* list;
-  __device__ __forceinline__ ListBlocks(const ListArgs& a, const Work& wk,
-                                        int64_t, int most, int wave) {
+// The first query row of tile qt, and the row behind its last.
+__device__ __forceinline__ int first_row(const ListArgs& a, int qt) {
+  return a.tiles > 1 ? qt / a.tiles * a.group + qt % a.tiles * 16
+                     : qt * a.span * a.group;
+}
+__device__ __forceinline__ int end_row(const ListArgs& a, int qt) {
+  const int t = a.tiles > 1 ? qt / a.tiles + 1 : (qt + 1) * a.span;
+  return (int)min((int64_t)t, a.tokens) * a.group;
+}
+
+// The blocks that any token of a tile has in its list, in order, with the tokens
+// that take them (a bit each), by a workgroup: a window of the row's blocks at a
+// time, of which each token has a bit for each, so that a block named twice is
+// one.  4,096 tiles of four tokens with 64 blocks each of 512: 12 us.
+constexpr int kUnionThreads = 256;
+constexpr int kWindow = 2048;  // blocks
+
+__global__ __launch_bounds__(kUnionThreads) void k_kv4_union(ListArgs a) {
+  constexpr int kWords = kWindow / 32;
+  constexpr int kUnionWaves = kUnionThreads / kWave;
+  static_assert(kWindow == 8 * kUnionThreads, "a thread has eight blocks");
+  __shared__ uint32_t bits[16][kWords];
+  __shared__ int sums[kUnionWaves];
+  const int tid = threadIdx.x, lane = lane_id(), wave = tid / kWave;
+  const int64_t tile = blockIdx.x;  // [batch, heads, q_tiles]
+  const int qt = (int)(tile % a.q_tiles);
+  const int h = (int)(tile / a.q_tiles % a.c.heads);
+  const int64_t b = tile / a.q_tiles / a.c.heads;
+  const int64_t len = kv_len_of(a, b), nq = q_len_of(a, b);
+  const int t0 = qt * a.span;
+  const int32_t* lists =
+      a.selected + ((b * a.tokens + t0) * a.c.heads + h) * a.width;
+  const int64_t next = (int64_t)a.c.heads * a.width;
+  int2* out = a.entry + tile * a.span * a.width;
+  // a later token sees no less
+  int limit = 0;
+  for (int k = 0; k < a.span; ++k)
+    limit = max(limit, (visible(a, len, nq, (t0 + k) * a.group) + kKvBlock - 1) /
+                           kKvBlock);
+  int count = 0;
+  for (int w0 = 0; w0 < limit; w0 += kWindow) {
+    for (int i = tid; i < a.span * kWords; i += kUnionThreads)
+      bits[i / kWords][i % kWords] = 0;
+    __syncthreads();
+    for (int k = wave; k < a.span; k += kUnionWaves) {
+      // none where the token is none
+      const int sees = visible(a, len, nq, (t0 + k) * a.group);
+      const int n = min((sees + kKvBlock - 1) / kKvBlock - w0, kWindow);
+      if (n <= 0) continue;
+      for (int e = lane; e < a.width; e += kWave) {
+        const int64_t r = (int64_t)lists[k * next + e] - w0;
+        if (r >= 0 && r < n) atomicOr(&bits[k][r / 32], 1u << (r % 32));
+      }
+    }
+    __syncthreads();
+    const int word = tid / 4, at = tid % 4 * 8;
+    uint32_t any = 0;
+    for (int k = 0; k < a.span; ++k) any |= bits[k][word] >> at;
+    any &= 255u;
+    const uint32_t n = (uint32_t)__builtin_popcount(any);
+    const uint32_t to = wave_incl_scan(n);
+    if (lane == kWave - 1) sums[wave] = (int)to;
+    __syncthreads();
+    int pos = count + (int)(to - n);
+#pragma unroll
+    for (int w = 0; w < kUnionWaves; ++w) {
+      if (w < wave) pos += sums[w];
+      count += sums[w];
+    }
+    while (any) {
+      const int bit = at + __builtin_ctz(any);
+      any &= any - 1;
+      int m = 0;
+      for (int k = 0; k < a.span; ++k) m |= (bits[k][word] >> bit & 1) << k;
+      out[pos++] = int2{w0 + word * 32 + bit, m};
+    }
+    __syncthreads();
+  }
+  if (tid == 0) a.entries[tile] = count;
+}
+
+typedef const __attribute__((address_space(4))) int32_t* Scalars;
+
+// threadIdx.x for what is worked out again in a loop rather than kept in a
+// register, of which the attention has none to spare.
+__device__ __forceinline__ int fresh_thread() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
+// As each_block, over entries first, first + step, ... below last: block(e) is
+// the block of entry e, negative where there is none, takes(e) the tokens that
+// take it.  A block's page id is read a block ahead of its loads.
+template <class B, class Block_, class Takes, class F>
+__device__ __forceinline__ void each_entry(const KvView& c, int64_t b, int h,
+                                           int bytes, int first, int step,
+                                           int last, Block_ block, Takes takes,
+                                           F body) {
+  if (first >= last || c.num_pages == 0) return;
+  const Scalars ids = (Scalars)(uintptr_t)(c.table + b * c.table_stride);
+  const int in_page = (1 << c.page_shift) - 1;
+  auto page = [&](int blk) { return blk < 0 ? -1 : ids[blk >> c.page_shift]; };
+  auto good = [&](int32_t id) { return id >= 0 && id < c.num_pages; };
+  // past the last block, and without a page: memory that is there
+  auto at = [&](int32_t id, int blk) {
+    return good(id) ? c.pages + ((((int64_t)id * c.heads + h) << c.page_shift) +
+                                 (blk & in_page)) * bytes
+                    : c.pages;
+  };
+  B x;
+  int blk = block(first), blk1 = block(min(first + step, last - 1));
+  int32_t id = page(blk), id1 = page(blk1);
+  x.load_k(at(id, blk));
+  x.load_v(at(id, blk));
+  for (int e = first; e < last; e += step) {
+    const char* next = at(id1, blk1);
+    const int blk2 = block(min(e + 2 * step, last - 1));
+    const int32_t id2 = page(blk2);
+    if (good(id)) {
+      body(x, blk, takes(e), [&]() { x.load_k(next); },
+           [&]() { x.load_v(next); });
+    } else {
+      x.load_k(next);
+      x.load_v(next);
+    }
+    blk = blk1;
+    blk1 = blk2;
+    id = id1;
+    id1 = id2;
+  }
+}
+
+// The list of a single token.  It ascends, as select_blocks gives it, or each of
+// its entries is looked for among those before it.
+struct OneList {
+  int splits, first, step, last, limit;
+  bool ascends;
+  Scalars list;
+  __device__ __forceinline__ OneList(const ListArgs& a, const Work& wk, int64_t,
+                                     int most, int wave) {
     splits = a.splits;
-    first = wk.split * a.per + wave;
-    last = min(wk.split * a.per + a.per, a.width);
+    first = wk.split * kWaves + wave;
+    step = splits * kWaves;
+    last = a.width;
     limit = (most + kKvBlock - 1) / kKvBlock;
-    list = a.selected +
-           ((wk.b * a.tokens + wk.qt / a.tiles) * a.c.heads + wk.h) * a.width;
+    const int32_t* p =
+        a.selected +
+        ((wk.b * a.tokens + wk.qt / a.tiles) * a.c.heads + wk.h) * a.width;
+    bool bad = false;
+    for (int e = lane_id(); e < last; e += kWave) {
+      const int x = p[e], y = e ? p[e - 1] : -1;
+      bad |= x >= 0 && x < limit && e > 0 && (y < 0 || y >= x);
+    }
+    ascends = !__any(bad);
+    list = (Scalars)(uintptr_t)p;
   }
   __device__ __forceinline__ bool seen(int vis) const {
     return vis > 0 && first < last;
   }
-  // As each_block, with 64 entries at a time in the wave's lanes: their places in
-  // the pool are looked up at once, entries without a block left out.
   template <class B, class F>
   __device__ __forceinline__ void each(const ListArgs& a, const Work& wk,
-                                       int bytes, F body) const {
-    for (int e0 = first; e0 < last; e0 += kWaves * kWave) {
-      const int e = e0 + lane_id() * kWaves;
-      const int blk = e < last ? list[e] : -1;
-      int64_t at64 = -1;
-      if (blk >= 0 && blk < limit) at64 = kv_place(a.c, wk.b, wk.h, blk);
-      uint64_t todo = ballot(at64 >= 0);
-      if (!todo) continue;
-      // in 32 bits: a pool of 2^32 blocks would be 9 TB
-      const uint32_t at = (uint32_t)at64;
-      auto place = [&](int i) {
-        return a.c.pages +
-               (uint64_t)(uint32_t)__builtin_amdgcn_readlane(at, i) * bytes;
-      };
-      B x;
-      int i = __builtin_ctzll(todo);
-      x.load_k(place(i));
-      x.load_v(place(i));
-      while (true) {
-        todo &= todo - 1;
-        // (after the last one: itself again)
-        const int j = todo ? __builtin_ctzll(todo) : i;
-        const char* next = place(j);
-        body(x, __builtin_amdgcn_readlane(blk, i), [&]() { x.load_k(next); },
-             [&]() { x.load_v(next); });
-        if (!todo) break;
-        i = j;
+                                       int bytes, int vis, F body) const {
+    auto block = [&](int e) {
+      const int x = list[e];
+      if (x < 0 || x >= limit) return -1;
+      if (!ascends) {
+        const int32_t* p = (const int32_t*)(uintptr_t)list;
+        bool twice = false;
+        for (int i = fresh_thread() % kWave; i < e; i += kWave)
+          twice |= p[i] == x;
+        if (__any(twice)) return -1;
       }
-    }
+      return x;
+    };
+    each_entry<B>(a.c, wk.b, wk.h, bytes, first, step, last, block,
+                  [](int) { return 1; },
+                  [&](B& x, int blk, int, auto kdone, auto vdone) {
+                    body(x, blk, vis, true, kdone, vdone);
+                  });
   }
 };
 
-template <int D, bool kHalf>
+// The blocks of a tile of several tokens, from k_kv4_union.
+struct TileList {
+  int splits, first, step, last, full;
+  int inv;   // 2^16 over the group, upwards
+  Scalars entry;
+  bool saw = false;
+  __device__ __forceinline__ TileList(const ListArgs& a, const Work& wk,
+                                      int64_t, int, int wave) {
+    splits = a.splits;
+    first = wk.split * kWaves + wave;
+    step = splits * kWaves;
+    const int64_t tile = (wk.b * a.c.heads + wk.h) * a.q_tiles + wk.qt;
+    last = ((Scalars)(uintptr_t)a.entries)[tile];
+    entry = (Scalars)(uintptr_t)(a.entry + tile * a.span * a.width);
+    full = (1 << a.span) - 1;
+    inv = 65535 / a.group + 1;
+  }
+  __device__ __forceinline__ bool seen(int) const { return saw; }
+  template <class B, class F>
+  __device__ __forceinline__ void each(const ListArgs& a, const Work& wk,
+                                       int bytes, int vis, F body) {
+    each_entry<B>(a.c, wk.b, wk.h, bytes, first, step, last,
+                  [&](int e) { return entry[2 * e]; },
+                  [&](int e) { return entry[2 * e + 1]; },
+                  [&](B& x, int blk, int takes, auto kdone, auto vdone) {
+                    // the lane's row's token
+                    const int t = __mul24(fresh_thread() % 16, inv) >> 16;
+                    const int v = takes >> t & 1 ? vis : 0;
+                    saw |= v > 0;
+                    body(x, blk, v, takes == full, kdone, vdone);
+                  });
+  }
+};
+
+template <int D, bool kHalf, class List>
 __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 4)
 void k_kv4_attend_blocks(ListArgs a) {
   __shared__ Lds<kLds16<D>> lds;
   const Work wk = work_of(a);
   if (!wk.any) return;
   const int64_t len = kv_len_of(a, wk.b), nq = q_len_of(a, wk.b);
-  const int t = wk.qt / a.tiles;
-  const int row0 = t * a.group + wk.qt % a.tiles * 16, end = (t + 1) * a.group;
-  if (visible(a, len, nq, row0) == 0) {
-    // no query: what is split is the join's
+  const int row0 = first_row(a, wk.qt), end = end_row(a, wk.qt);
+  // the last token sees the most
+  if (visible(a, len, nq, std::min<int64_t>(end, nq * a.group) - 1) == 0 ||
+      nq * a.group <= row0) {
+    // no queries: what is split is the join's
     if (a.splits == 1) {
-      uint4* out = (uint4*)(a.out + ((wk.b * a.tokens + t) * a.q_heads +
-                                     wk.h * a.group + row0 - t * a.group) * D);
-      const int n = min(16, end - row0) * (D / 8);
-      for (int i = threadIdx.x; i < n; i += 64 * kWaves)
-        out[i] = uint4{0, 0, 0, 0};
+      const int n = min(16, end - row0);
+      for (int i = threadIdx.x; i < n * (D / 8); i += 64 * kWaves) {
+        const int r = row0 + i / (D / 8);
+        ((uint4*)(a.out + ((wk.b * a.tokens + r / a.group) * a.q_heads +
+                           wk.h * a.group + r % a.group) * D))[i % (D / 8)] =
+            uint4{0, 0, 0, 0};
+      }
     }
     return;
   }
-  attend16<D, kHalf, 16, ListBlocks>(a, wk, len, nq, row0, end, lds);
+  attend16<D, kHalf, 16, List>(a, wk, len, nq, row0, end, lds);
 }
 
 template <int D, bool kHalf>
@@ -105,33 +278,37 @@ __global__ __launch_bounds__(256) void k_kv4_join_blocks(ListArgs a) {
       a.out[((b * a.tokens + t) * a.q_heads + h * a.group + g) * D + c] = 0;
     return;
   }
-  join_splits<D, kHalf>(a, b, h, r, t * a.tiles + g / 16, g % 16, 16, a.splits);
+  const int tile = a.tiles > 1 ? t * a.tiles + g / 16 : t / a.span;
+  join_splits<D, kHalf>(a, b, h, r, tile, r - first_row(a, tile), 16, a.splits);
 }
 
 struct Plan {
-  int tiles, per, splits;
+  int span, tiles, splits;
   int64_t q_tiles;
-  size_t bytes;
+  size_t part, entry, bytes;  // of the splits' parts, of the tiles' entries, all
 };
 
-// A list is split where there are too few of them for the chip.
+size_t round_up(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// Lists are split where there are too few of them for the chip.
 constexpr int64_t kWant = 1024;  // workgroups
 constexpr int64_t kLeast = 16;   // entries of one
 
 Plan plan_for(const sfx_kv4* c, int64_t batch, int64_t tokens, int64_t q_heads,
               int64_t width) {
   Plan p;
-  p.tiles = (int)((q_heads / c->heads + 15) / 16);
-  p.q_tiles = tokens * p.tiles;
+  const int64_t group = q_heads / c->heads;
+  p.tiles = (int)((group + 15) / 16);
+  p.span = (int)std::min<int64_t>(std::max<int64_t>(1, 16 / group), tokens);
+  p.q_tiles = p.tiles > 1 ? tokens * p.tiles : (tokens + p.span - 1) / p.span;
   const int64_t wgs = batch * c->heads * p.q_tiles;
-  const int64_t per =
-      std::max<int64_t>({kLeast, (wgs * width + kWant - 1) / kWant,
-                         (width + kMaxSplits - 1) / kMaxSplits});
-  p.per = (int)std::min(per, width);
-  p.splits = (int)((width + p.per - 1) / p.per);
-  p.bytes = p.splits == 1 ? 0
-                          : (size_t)wgs * p.splits * 16 *
-                                (c->head_dim + kPart) * 4;
+  p.splits = (int)std::max<int64_t>(
+      1, std::min<int64_t>({kWant / wgs, p.span * width / kLeast, kMaxSplits}));
+  p.part = p.splits == 1 ? 0
+                         : round_up((size_t)wgs * p.splits * 16 *
+                                    (c->head_dim + kPart) * 4);
+  p.entry = p.span == 1 ? 0 : round_up((size_t)wgs * p.span * width * 8);
+  p.bytes = p.part + p.entry + (p.span == 1 ? 0 : (size_t)wgs * 4);
   return p;
 }
 
@@ -149,9 +326,17 @@ int launch(const ListArgs& a, hipStream_t stream) {
   const int64_t items = (a.batch * a.c.heads * a.splits + 7) / 8 * 8;
   if (items * a.q_tiles >= (int64_t(1) << 32) / (64 * kWaves))
     return SFX_EINVAL;  // more threads than a grid takes
-  hipLaunchKernelGGL((k_kv4_attend_blocks<D, kHalf>),
-                     dim3((unsigned)(items * a.q_tiles)), dim3(64 * kWaves), 0,
-                     stream, a);
+  const dim3 grid((unsigned)(items * a.q_tiles)), block(64 * kWaves);
+  if (a.span == 1) {
+    hipLaunchKernelGGL((k_kv4_attend_blocks<D, kHalf, OneList>), grid, block, 0,
+                       stream, a);
+  } else {
+    hipLaunchKernelGGL(k_kv4_union,
+                       dim3((unsigned)(a.batch * a.c.heads * a.q_tiles)),
+                       dim3(kUnionThreads), 0, stream, a);
+    hipLaunchKernelGGL((k_kv4_attend_blocks<D, kHalf, TileList>), grid, block,
+                       0, stream, a);
+  }
   if (a.splits > 1)
     hipLaunchKernelGGL((k_kv4_join_blocks<D, kHalf>),
                        dim3((unsigned)(a.rows + 3) / 4, (unsigned)a.c.heads,
@@ -199,7 +384,7 @@ extern "C" int sfx_kv4_attend_blocks(
   a.rows = (int)(tokens * a.group);
   a.q_tiles = (int)p.q_tiles;
   a.splits = p.splits;
-  a.per = p.per;
+  a.span = p.span;
   a.tiles = p.tiles;
   a.chunk = 1;
   a.vec = (((uintptr_t)q->data & 15) |
@@ -211,6 +396,8 @@ extern "C" int sfx_kv4_attend_blocks(
   a.scale = scale * 1.44269504088896340736f;
   a.out = (uint16_t*)out;
   a.part = (float*)workspace;
+  a.entry = (int2*)((char*)workspace + p.part);
+  a.entries = (int32_t*)((char*)workspace + p.part + p.entry);
   a.batch = batch;
   a.selected = selected;
   a.width = (int)blocks;

@@ -343,7 +343,7 @@ class KV4Cache:
         num_kv_heads, N] int32 (as ``select_blocks`` gives them, or another
         layer's) that each query sees.  Entries may stand in any order; one that
         names no block of the table counts as none, a block that is named twice
-        counts twice.  Zeros for a query that sees nothing."""
+        as one.  Zeros for a query that sees nothing."""
         if elsewhere(self.device):
             with torch.cuda.device(self.device):
                 return self.attend_blocks(q, selected, page_table, kv_len,
