@@ -128,7 +128,8 @@ struct SelectArgs : AttendArgs {
   const int8_t* range;
   const int8_t* unit;
   int want, sinks, recent;  // blocks: in all, first, last
-  int tiles;     // of 16 query tokens
+  int span;      // query tokens of a tile
+  int tiles;
   int chunks;    // of kScoreChunk blocks
   int64_t pitch; // of a query's keys
   uint32_t* keys;     // [batch, tokens, heads, pitch]
@@ -149,37 +150,67 @@ template <int D, bool kHalf>
 __device__ __forceinline__ void pack_query(const SelectArgs& a, int64_t b,
                                            int h, int64_t t, int8_t* out) {
   constexpr int C = D / kWave;  // channels of a lane
+  constexpr int kHold = 8;      // query heads kept; of more all are read twice
   const int lane = lane_id();
   const uint16_t* q = (const uint16_t*)a.q.data + b * a.q.stride_b +
                       t * a.q.stride_t + (int64_t)h * a.group * a.q.stride_h +
                       lane * C;
-  auto bits = [&](int g, int c) {
-    const uint32_t x = q[g * a.q.stride_h + c];
-    return (x & 0x7fffu) >= (kHalf ? 0x7c00u : 0x7f80u) ? 0u : x;
+  struct Head {
+    uint16_t x[C];
   };
-  int top = 0;
-  for (int g = 0; g < a.group; ++g)
+  auto read = [&](int g) {
+    Head r;
+    const uint16_t* p = q + (int64_t)g * a.q.stride_h;
+    if (C == 1) {
+      r.x[0] = p[0];
+    } else if (a.vec) {
+      typedef uint32_t W __attribute__((ext_vector_type(C > 1 ? C / 2 : 1)));
+      const W w = *(const W*)p;
+      __builtin_memcpy(r.x, &w, 2 * C);
+    } else {
 #pragma unroll
-    for (int c = 0; c < C; ++c) top = max(top, (int)(bits(g, c) & 0x7fffu));
-  top = wave_max_i32(top);
+      for (int c = 0; c < C; ++c) r.x[c] = p[c];
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if ((r.x[c] & 0x7fffu) >= (kHalf ? 0x7c00u : 0x7f80u)) r.x[c] = 0;
+    return r;
+  };
+  Head held[kHold] = {};
+#pragma unroll
+  for (int g = 0; g < kHold; ++g)
+    if (g < a.group) held[g] = read(g);
+  uint32_t top = 0;
+  auto most_of = [&](const Head& x) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) top = max(top, x.x[c] & 0x7fffu);
+  };
+#pragma unroll
+  for (int g = 0; g < kHold; ++g) most_of(held[g]);
+  for (int g = kHold; g < a.group; ++g) most_of(read(g));
+  top = wave_all_max(top);
   // 2^e is the power of two above the largest
-  const int e =
-      __builtin_amdgcn_frexp_expf(to_float16b<kHalf>((uint32_t)top));
+  const int e = __builtin_amdgcn_frexp_expf(to_float16b<kHalf>(top));
   uint32_t p[C], n[C];
-  uint32_t most = 0;
 #pragma unroll
   for (int c = 0; c < C; ++c) p[c] = n[c] = 0;
-  for (int g = 0; g < a.group; ++g)
+  auto add = [&](const Head& x) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int z = (int)rintf(
-          __builtin_amdgcn_ldexpf(to_float16b<kHalf>(bits(g, c)), 15 - e));
+          __builtin_amdgcn_ldexpf(to_float16b<kHalf>(x.x[c]), 15 - e));
       p[c] += (uint32_t)max(z, 0);
       n[c] += (uint32_t)max(-z, 0);
     }
+  };
+#pragma unroll
+  for (int g = 0; g < kHold; ++g)
+    if (g < a.group) add(held[g]);
+  for (int g = kHold; g < a.group; ++g) add(read(g));
+  uint32_t most = 0;
 #pragma unroll
   for (int c = 0; c < C; ++c) most = max(most, max(p[c], n[c]));
-  most = (uint32_t)wave_max_i32((int)most);
+  most = wave_all_max(most);
   const int shift = most ? max(0, 32 - __builtin_clz(most) - 7) : 0;
   const uint32_t half = shift ? 1u << (shift - 1) : 0u;
 #pragma unroll
@@ -222,7 +253,7 @@ __global__ __launch_bounds__(kScoreThreads) void k_kv4_scores(SelectArgs a) {
   const int64_t b = bh / a.c.heads;
   const int h = (int)(bh % a.c.heads);
   const int64_t len = kv_len_of(a, b), nq = q_len_of(a, b);
-  const int64_t t0 = (int64_t)tile * 16;
+  const int64_t t0 = (int64_t)tile * 16;  // (the span)
   const int64_t last = std::min(std::min(nq, a.tokens), t0 + 16) - 1;
   const int64_t blk0 = chunk * kScoreChunk;
   if (last < t0 || blk0 * kKvBlock >= token_sees(a, len, nq, last)) return;
@@ -268,73 +299,182 @@ __global__ __launch_bounds__(kScoreThreads) void k_kv4_scores(SelectArgs a) {
   }
 }
 
-// The key of block j of a query whose last block is `last`, first and recent
-// blocks above all others.
-__device__ __forceinline__ uint32_t ranked(const SelectArgs& a, uint32_t key,
-                                           int j, int last) {
-  if (j > last || key == 0) return 0;
-  return j < a.sinks || j > last - a.recent ? 0xffffffffu : key;
+// Whether a query whose last block is `last` takes block j whatever its score.
+__device__ __forceinline__ bool always(const SelectArgs& a, int j, int last) {
+  return j < a.sinks || j > last - a.recent;
 }
 
-// A wave per query token and KV head, whose keys it keeps: the threshold bit by
-// bit, then the blocks past it, and those at it while there is room.
-constexpr int kPickRegs = 16;
-
-__global__ __launch_bounds__(256) void k_kv4_pick(SelectArgs a) {
-  const int64_t list = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
-  if (list >= a.batch * a.tokens * a.c.heads) return;
+// The blocks of a query with the keys key[0 .. last] in LDS, by a wave that keeps
+// kRegs of them in each lane: the least key that is taken, bit by bit, below the
+// bits that all have and until as many as are wanted lie past it; then the blocks
+// past it, and those at it while there is room.
+template <int kRegs>
+__device__ __forceinline__ void pick_blocks(int sinks, int recent, int all,
+                                            int last, const uint32_t* key,
+                                            int32_t* out) {
   const int lane = lane_id();
-  const int64_t b = list / (a.tokens * a.c.heads);
-  const int64_t t = list / a.c.heads % a.tokens;
-  const int sees = token_sees(a, kv_len_of(a, b), q_len_of(a, b), t);
-  const int last = __builtin_amdgcn_readfirstlane((sees + kKvBlock - 1) /
-                                                  kKvBlock) - 1;
-  const uint32_t* keys = a.keys + list * a.pitch;
-  int32_t* out = a.selected + list * a.want;
-  const int regs = last / kWave + 1;
-  uint32_t k[kPickRegs];
+  uint32_t k[kRegs];
+  uint32_t sure = 0;  // a bit for each register
+  uint32_t hi = 0, lo = 0;
+  int want = all;
 #pragma unroll
-  for (int i = 0; i < kPickRegs; ++i) {
+  for (int i = 0; i < kRegs; ++i) {
     const int j = i * kWave + lane;
-    k[i] = 0;
-    if (i < regs && j <= last) k[i] = ranked(a, keys[j], j, last);
+    k[i] = j <= last ? key[j] : 0;
+    const bool is = k[i] && (j < sinks || j > last - recent);
+    want -= popc(ballot(is));
+    if (is) {
+      sure |= 1u << i;
+      k[i] = 0;
+    }
+    hi = max(hi, k[i]);
+    lo = max(lo, 0u - k[i]);  // (none is the least)
   }
   auto at_least = [&](uint32_t x) {
     int n = 0;
 #pragma unroll
-    for (int i = 0; i < kPickRegs; ++i)
-      if (i < regs) n += popc(ballot(k[i] >= x));
+    for (int i = 0; i < kRegs; ++i) n += popc(ballot(k[i] >= x));
     return n;
   };
-  uint32_t line = 1;
-  if (at_least(1) > a.want) {
-    line = 0;
-    for (int bit = 31; bit >= 0; --bit) {
+  // line: keys past it are taken, and `room` of those at it
+  uint32_t line = 0;
+  int room = 0;
+  if (want <= 0) {
+    line = 0xffffffffu;
+  } else if (at_least(1) > want) {
+    hi = wave_all_max(hi);
+    lo = 0u - wave_all_max(lo);
+    int bit = 31 - __builtin_clz((hi ^ lo) | 1u);
+    line = hi >> bit >> 1 << bit << 1;
+    for (; bit >= 0; --bit) {
       const uint32_t x = line | 1u << bit;
-      if (at_least(x) >= a.want) line = x;
+      const int n = at_least(x);
+      if (n >= want) line = x;
+      if (n == want) break;
     }
+    if (bit >= 0)
+      --line;  // those past it now are the wanted ones
+    else
+      room = want - at_least(line + 1);
   }
-  int above = 0;
+  int n = 0;
 #pragma unroll
-  for (int i = 0; i < kPickRegs; ++i)
-    if (i < regs) above += popc(ballot(k[i] > line));
-  int room = a.want - above, n = 0;  // room: for those at the line
-#pragma unroll
-  for (int i = 0; i < kPickRegs; ++i) {
-    if (i >= regs) continue;
-    const uint64_t eq = ballot(k[i] == line && line > 0);
-    const bool in = k[i] > line || (k[i] == line && rank_lt(eq) < room);
+  for (int i = 0; i < kRegs; ++i) {
+    bool in = k[i] > line || (sure >> i & 1);
+    if (room > 0) {
+      const uint64_t eq = ballot(k[i] == line);
+      in = in || (k[i] == line && rank_lt(eq) < room);
+      room -= popc(eq);
+    }
     const uint64_t m = ballot(in);
     if (in) out[n + rank_lt(m)] = i * kWave + lane;
     n += popc(m);
-    room -= popc(eq);
-    if (room < 0) room = 0;
   }
-  for (int i = n + lane; i < a.want; i += kWave) out[i] = -1;
+  for (int i = n + lane; i < all; i += kWave) out[i] = -1;
 }
 
-// The same by a workgroup, for tables of more blocks than a wave keeps: the keys
-// stay in memory, and four passes narrow the threshold down by 8 bits each.
+// Scores and choice at once, where a workgroup holds the keys of its tokens: rows
+// of up to 1,024 blocks.
+constexpr int kSelectThreads = 512;
+constexpr int kSelectTokens = 32;
+
+template <int D, bool kHalf>
+__global__ __launch_bounds__(kSelectThreads) void k_kv4_select(SelectArgs a) {
+  constexpr int kStep = 2 * D / 64;  // matrix instructions a tile
+  constexpr int kPitch = 2 * D + 16;
+  constexpr int kSelectWaves = kSelectThreads / kWave;
+  extern __shared__ __align__(16) char lds[];
+  const int id = (int)blockIdx.x;
+  // tiles of one row and KV head follow each other on one XCD
+  const int k = id >> 3;
+  const int tile = k % a.tiles;
+  const int64_t bh = (int64_t)(k / a.tiles) * 8 + (id & 7);
+  if (bh >= a.batch * a.c.heads) return;
+  const int64_t b = bh / a.c.heads;
+  const int h = (int)(bh % a.c.heads);
+  const int64_t len = kv_len_of(a, b), nq = q_len_of(a, b);
+  const int64_t t0 = (int64_t)tile * a.span;
+  const int tokens = (int)std::min<int64_t>(a.span, a.tokens - t0);
+  const int queries = (int)std::max<int64_t>(
+      0, std::min<int64_t>(tokens, nq - t0));
+  auto sq = (int8_t(*)[kPitch])lds;
+  // (rows 4 banks apart)
+  const int pitch = (int)a.pitch + 4;
+  uint32_t* keys = (uint32_t*)(lds + (a.span + 15) / 16 * 16 * kPitch);
+  const int blocks =
+      queries ? (token_sees(a, len, nq, t0 + queries - 1) + kKvBlock - 1) /
+                    kKvBlock
+              : 0;
+  const int lane = lane_id();
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int i16 = lane % 16, quad = lane / 16;
+
+  // bounds of 16 blocks; the next ones are on their way while these are used
+  I4 r[kStep];
+  int unit;
+  auto load = [&](int blk0) {
+    const int64_t at = blk0 < blocks ? kv_place(a.c, b, h, blk0 + i16) : -1;
+    unit = at < 0 ? kNoPage : a.unit[at];
+    const I4* p = (const I4*)(a.range + (at < 0 ? 0 : at) * (2 * D)) + quad;
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) r[i] = at < 0 ? I4{0, 0, 0, 0} : p[4 * i];
+  };
+  load(wave * 16);
+  const int rows = (tokens + 15) / 16 * 16;
+  for (int i = wave; i < rows; i += kSelectWaves) {
+    if (i < queries) {
+      pack_query<D, kHalf>(a, b, h, t0 + i, sq[i]);
+    } else {
+      for (int c = lane; c < D / 2; c += kWave) ((uint32_t*)sq[i])[c] = 0;
+    }
+  }
+  __syncthreads();
+  for (int blk0 = wave * 16; blk0 < blocks; blk0 += kSelectWaves * 16) {
+    I4 now[kStep];
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) now[i] = r[i];
+    const int u = unit;
+    load(blk0 + kSelectWaves * 16);
+    int us[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) us[e] = __shfl(u, quad * 4 + e);
+    for (int q0 = 0; q0 < queries; q0 += 16) {
+      I4 s = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < kStep; ++i)
+        s = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+            now[i], *(const I4*)&sq[q0 + i16][i * 64 + quad * 16], s, 0, 0, 0);
+      if (q0 + i16 < queries)
+        *(uint4*)(keys + (q0 + i16) * pitch + blk0 + quad * 4) =
+            uint4{score_key(s[0], us[0]), score_key(s[1], us[1]),
+                  score_key(s[2], us[2]), score_key(s[3], us[3])};
+    }
+  }
+  __syncthreads();
+  for (int i = wave; i < tokens; i += kSelectWaves) {
+    const int last = __builtin_amdgcn_readfirstlane(
+        (token_sees(a, len, nq, t0 + i) + kKvBlock - 1) / kKvBlock - 1);
+    const uint32_t* own = keys + i * pitch;
+    int32_t* out =
+        a.selected + ((b * a.tokens + t0 + i) * a.c.heads + h) * a.want;
+    if (last < 4 * kWave)
+      pick_blocks<4>(a.sinks, a.recent, a.want, last, own, out);
+    else if (last < 8 * kWave)
+      pick_blocks<8>(a.sinks, a.recent, a.want, last, own, out);
+    else
+      pick_blocks<16>(a.sinks, a.recent, a.want, last, own, out);
+  }
+}
+
+// The key of block j for what follows: first and recent blocks above all others.
+__device__ __forceinline__ uint32_t ranked(const SelectArgs& a, uint32_t key,
+                                           int j, int last) {
+  if (j > last || key == 0) return 0;
+  return always(a, j, last) ? 0xffffffffu : key;
+}
+
+// The choice by a workgroup, for tables of more blocks than a wave keeps: the keys
+// are in memory, and four passes narrow the threshold down by 8 bits each.
 constexpr int kWideThreads = 1024;
 
 __global__ __launch_bounds__(kWideThreads) void k_kv4_pick_wide(SelectArgs a) {
@@ -436,21 +576,48 @@ bool select_ok(const sfx_kv4* c, int64_t batch, int64_t tokens) {
          batch * tokens <= ((int64_t(1) << 22) - 1) / c->heads;
 }
 
+bool held_in_lds(const sfx_kv4* c) {
+  return pitch_of(c) <= 16 * kWave;
+}
+
 template <int D, bool kHalf>
-int launch(const SelectArgs& a, hipStream_t stream) {
+int launch_held(SelectArgs a, hipStream_t stream) {
+  // As many tokens as a workgroup's 64 KB hold keys of; past kSelectTokens in
+  // tiles of 16.
+  const int64_t row = 4 * (a.pitch + 4), packed = 2 * D + 16;
+  const int64_t room = 65536 - kSelectTokens * packed;
+  a.span = (int)std::min<int64_t>(a.tokens <= kSelectTokens ? a.tokens : 16,
+                                  room / row);
+  a.tiles = (int)((a.tokens + a.span - 1) / a.span);
+  const size_t lds = (a.span + 15) / 16 * 16 * packed + a.span * row;
+  const int64_t items = (a.batch * a.c.heads + 7) / 8 * 8;
+  if (items * a.tiles >= (int64_t(1) << 32) / kSelectThreads)
+    return SFX_EINVAL;
+  hipLaunchKernelGGL((k_kv4_select<D, kHalf>),
+                     dim3((unsigned)(items * a.tiles)), dim3(kSelectThreads),
+                     lds, stream, a);
+  return (int)hipGetLastError();
+}
+
+template <int D, bool kHalf>
+int launch_wide(SelectArgs a, hipStream_t stream) {
+  a.span = 16;
+  a.tiles = (int)((a.tokens + 15) / 16);
   const int64_t lists = a.batch * a.tokens * a.c.heads;
   const int64_t items = (a.batch * a.c.heads * a.chunks + 7) / 8 * 8;
   if (items * a.tiles >= (int64_t(1) << 32) / kScoreThreads) return SFX_EINVAL;
   hipLaunchKernelGGL((k_kv4_scores<D, kHalf>),
                      dim3((unsigned)(items * a.tiles)), dim3(kScoreThreads), 0,
                      stream, a);
-  if (a.c.positions / kKvBlock <= kPickRegs * kWave)
-    hipLaunchKernelGGL(k_kv4_pick, dim3((unsigned)((lists + 3) / 4)), dim3(256),
-                       0, stream, a);
-  else
-    hipLaunchKernelGGL(k_kv4_pick_wide, dim3((unsigned)lists),
-                       dim3(kWideThreads), 0, stream, a);
+  hipLaunchKernelGGL(k_kv4_pick_wide, dim3((unsigned)lists),
+                     dim3(kWideThreads), 0, stream, a);
   return (int)hipGetLastError();
+}
+
+template <int D, bool kHalf>
+int launch(const SelectArgs& a, const sfx_kv4* cache, hipStream_t stream) {
+  return held_in_lds(cache) ? launch_held<D, kHalf>(a, stream)
+                            : launch_wide<D, kHalf>(a, stream);
 }
 
 constexpr int64_t kMaxTokens = int64_t(1) << 28;  // the grid's limit
@@ -503,7 +670,7 @@ extern "C" int sfx_kv4_bounds_update(const sfx_kv4* cache,
 extern "C" size_t sfx_kv4_select_workspace_size(const sfx_kv4* cache,
                                                 int64_t batch,
                                                 int64_t tokens) {
-  if (!select_ok(cache, batch, tokens)) return 0;
+  if (!select_ok(cache, batch, tokens) || held_in_lds(cache)) return 0;
   return (size_t)(batch * tokens * cache->heads) * (size_t)pitch_of(cache) * 4;
 }
 
@@ -536,12 +703,13 @@ extern "C" int sfx_kv4_select(const sfx_kv4* cache,
   a.kv64 = kv_len_is64;
   a.q_len = q_len;
   a.q64 = q_len_is64;
+  a.vec = (((uintptr_t)q->data & 15) |
+           ((q->stride_b | q->stride_t | q->stride_h) & 7)) == 0;
   a.range = bounds->range;
   a.unit = bounds->unit;
   a.want = (int)blocks;
   a.sinks = (int)first;
   a.recent = (int)recent;
-  a.tiles = (int)((tokens + 15) / 16);
   a.pitch = pitch_of(cache);
   a.chunks = (int)((a.pitch + kScoreChunk - 1) / kScoreChunk);
   a.keys = (uint32_t*)workspace;
@@ -549,12 +717,12 @@ extern "C" int sfx_kv4_select(const sfx_kv4* cache,
   const bool half = cache->dtype == SFX_F16;
   switch (cache->head_dim) {
     case 64:
-      return half ? launch<64, true>(a, stream) : launch<64, false>(a, stream);
+      return half ? launch<64, true>(a, cache, stream) : launch<64, false>(a, cache, stream);
     case 128:
-      return half ? launch<128, true>(a, stream)
-                  : launch<128, false>(a, stream);
+      return half ? launch<128, true>(a, cache, stream)
+                  : launch<128, false>(a, cache, stream);
     default:
-      return half ? launch<256, true>(a, stream)
-                  : launch<256, false>(a, stream);
+      return half ? launch<256, true>(a, cache, stream)
+                  : launch<256, false>(a, cache, stream);
   }
 }

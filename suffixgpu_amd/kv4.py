@@ -327,10 +327,12 @@ class KV4Cache:
             return out
         L = lib()
         nbytes = L.sfx_kv4_select_workspace_size(view, b, t)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        ws = (torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+              if nbytes else None)
         check(L.sfx_kv4_select(view, self._bounds, qh, b, t, heads,
                                *keep[0][1:], *keep[1][1:], blocks, first,
-                               recent, out.data_ptr(), ws.data_ptr(), nbytes,
+                               recent, out.data_ptr(),
+                               None if ws is None else ws.data_ptr(), nbytes,
                                stream_of(self.device)),
               "KV4Cache.select_blocks")
         return out
