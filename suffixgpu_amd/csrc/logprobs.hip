@@ -7,11 +7,10 @@
 //   log p_i = z_i - log(1 + R),   H = log(1 + R) - sum z e^z / (1 + R).
 //
 // The first launch takes 8,192 logits a workgroup, which stay in registers: their
-// largest, R and sum z e^z, and their n largest in order.  Of the maxima of
-// pieces of 16 vectors (contiguous, so that the lowest index wins ties) the n
-// largest hold the n largest logits: all that reach the least of those n maxima
-// and lie in those pieces are ranked, a few more than n.  The second launch joins
-// a position's parts.  Positions without a token leave at once.
+// largest, R and sum z e^z, and their n largest in order.  A number that n of the
+// maxima of its pieces reach, and few more, is one that the n largest logits reach,
+// and few others: those are ranked.  The second launch joins a position's parts.
+// Positions without a token leave at once.
 
 #include <algorithm>
 
@@ -86,14 +85,63 @@ __device__ __forceinline__ void join(Part& p, const Part& q, float c) {
   p.at = a.top == b.top ? min(a.at, b.at) : a.at;
 }
 
-constexpr int kCap = 256;  // candidates that are ranked
+// Order of floats as unsigned numbers.
+__device__ __forceinline__ uint32_t order_of(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return u >> 31 ? ~u : u | 0x80000000u;
+}
+
+// Place of the lane's entry among those of lanes 0 .. count - 1.
+__device__ __forceinline__ int place_of(const Entry& m, int count) {
+  int r = 0;
+#pragma unroll 4
+  for (int i = 0; i < count; ++i) {
+    const float y = __builtin_bit_cast(
+        float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, m.x), i));
+    r += before(y, __builtin_amdgcn_readlane(m.at, i), m.x, m.at);
+  }
+  return r;
+}
+
+// A number that n of a wave's R values a lane reach (there are as many), and few
+// more: by halves, until no more than n + kFew do.
+constexpr int kFew = 6;
+
+template <int R>
+__device__ __forceinline__ float reached_by(const float (&x)[R], int n) {
+  uint32_t k[R], hi = 0, lo = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    k[i] = order_of(x[i]);
+    hi = max(hi, k[i]);
+    lo = max(lo, ~k[i]);
+  }
+  hi = wave_all_max(hi);
+  lo = ~wave_all_max(lo);
+  int bit = 31 - __builtin_clz((hi ^ lo) | 1u);
+  uint32_t line = lo >> bit >> 1 << bit << 1;
+  for (; bit >= 0; --bit) {
+    const uint32_t y = line | 1u << bit;
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) count += popc(ballot(k[i] >= y));
+    if (count >= n) {
+      line = y;
+      if (count <= n + kFew) break;
+    }
+  }
+  // (below -inf where all are taken; the line may lie between two floats)
+  line = max(line, order_of(kNegInf));
+  return __uint_as_float(line >> 31 ? line & 0x7fffffffu : ~line);
+}
 
 template <int DT, bool kTop>
 __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
   using S = Share<DT>;
   constexpr int E = S::E, U = S::U;
   constexpr int kSegs = U * kThreads / 16;  // pieces of 16 vectors
-  static_assert(kSegs >= SFX_LOGPROBS_TOP && kCap >= SFX_LOGPROBS_TOP, "");
+  constexpr int kRegs = kSegs / kWave;      // their maxima a lane
+  static_assert(kSegs % kWave == 0 && kSegs >= SFX_LOGPROBS_TOP, "");
   const int chunk = blockIdx.x % a.chunks;
   const int64_t pos = blockIdx.x / a.chunks;
   const int64_t b = pos / a.v.positions, j = pos % a.v.positions;
@@ -102,10 +150,8 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
   const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id();
   __shared__ Part lds[kWaves];
   __shared__ float seg[kTop ? kSegs : 1];
-  __shared__ uint32_t chosen[kTop ? (kSegs + 31) / 32 : 1];
-  __shared__ Entry cand[kTop ? kCap : 1];
-  __shared__ int n_cand;
-  __shared__ float least;
+  __shared__ Entry cand[kTop ? kWaves : 1][kWave];
+  __shared__ int counts[kWaves];
   const float t = temperature_of(a.v, b);
   const bool greedy = !(t > 0.0f);
   const float c = greedy ? 0.0f : scale_of(t);
@@ -134,7 +180,6 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
       m = fmaxf(m, dpp<0x140, 0xf>(m, m));   // row mirrored
       if (lane % 16 == 0) seg[u * (kThreads / 16) + tid / 16] = m;
     }
-    if (tid == 0) n_cand = 0;
   }
   Part p = {top, 0.0f, 0.0f, 0x7fffffff};
   if (greedy) {
@@ -156,15 +201,15 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
       zsum = __builtin_fmaf(z, e, zsum);
     };
     auto add_special = [&](float x) {
-      const bool is = x == top;
-      equal += is;
-      const float z =
-          is ? kFloor : fmaxf(__builtin_fmaf(x, 0.5f, half) * c, kFloor);
+      equal += popc(ballot(x == top));
+      const float z = x == top
+                          ? kFloor
+                          : fmaxf(__builtin_fmaf(x, 0.5f, half) * c, kFloor);
       const float e = __builtin_amdgcn_exp2f(z);
       sum += e;
       zsum = __builtin_fmaf(z, e, zsum);
     };
-    add_special(s.single);
+    if (ballot(s.extra >= 0)) add_special(s.single);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       // one vector in U holds the wave's largest
@@ -176,7 +221,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
         for (int e = 0; e < E; ++e) add(s.get(u, e));
       }
     }
-    p.rest = wave_sum(sum) + (wave_sum((float)equal) - 1.0f);
+    p.rest = wave_sum(sum) + ((float)equal - 1.0f);
     p.zsum = wave_sum(zsum);
   }
   if (lane == 0) lds[wave] = p;
@@ -188,49 +233,55 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
   }
   if (!kTop) return;
 
-  // The n pieces with the largest maxima, the lowest on ties.
+  // What reaches the n largest pieces' maxima, at least n of them.
   const int n = (int)a.v.top;
-  if (tid < kSegs) {
-    const float m = seg[tid];
-    int rank = 0;
-    for (int i = 0; i < kSegs; ++i) rank += before(seg[i], i, m, tid);
-    const bool in = rank < n && m > kNegInf;
-    const uint64_t w = ballot(in);
-    if (lane == 0) {
-      chosen[2 * wave] = (uint32_t)w;
-      chosen[2 * wave + 1] = (uint32_t)(w >> 32);
-    }
-    if (rank == n - 1) least = m;
-  }
-  __syncthreads();
-  const float floor = least;
-  auto offer = [&](float x, int i) {
-    if (x >= floor && x > kNegInf) {
-      const int k = atomicAdd(&n_cand, 1);
-      if (k < kCap) cand[k] = Entry{x, i};
-    }
+  float segs[kRegs];
+#pragma unroll
+  for (int i = 0; i < kRegs; ++i) segs[i] = seg[i * kWave + lane];
+  const float line = reached_by(segs, n);
+  int count = 0;
+  auto offer = [&](float x, int i, bool in) {
+    const bool is = in && x >= line && x > kNegInf;
+    const uint64_t m = ballot(is);
+    const int k = count + rank_lt(m);
+    if (is && k < kWave) cand[wave][k] = Entry{x, i};
+    count += popc(m);
   };
+  if (ballot(s.extra >= 0)) offer(s.single, s.extra, s.extra >= 0);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int sg = u * (kThreads / 16) + tid / 16;
-    if ((chosen[sg / 32] >> (sg % 32) & 1) && vtop[u] >= floor) {
+    if (ballot(vtop[u] >= line)) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) offer(s.get(u, e), s.index(u * E + e));
+      for (int e = 0; e < E; ++e) {
+        const float x = s.get(u, e);
+        if (ballot(x >= line)) offer(x, s.index(u * E + e), true);
+      }
     }
   }
-  if (s.extra >= 0) offer(s.single, s.extra);
+  if (lane == 0) counts[wave] = count;
   __syncthreads();
   Entry* out = a.entry + (pos * a.chunks + chunk) * n;
-  const int count = n_cand;
-  if (count <= kCap) {
-    if (tid < n && tid >= count) out[tid] = Entry{kNegInf, -1};
-    if (tid < count) {
-      const Entry m = cand[tid];
-      int rank = 0;
-      for (int i = 0; i < count; ++i)
-        rank += before(cand[i].x, cand[i].at, m.x, m.at);
-      if (rank < n) out[rank] = m;
-    }
+  int all = 0;
+  bool fits = true;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    fits = fits && counts[w] <= kWave;
+    all += counts[w];
+  }
+  if (fits && all <= kWave) {
+    if (wave > 0) return;
+    int w = 0, i = lane;
+#pragma unroll
+    for (int v = 0; v + 1 < kWaves; ++v)
+      if (w == v && i >= counts[v]) {
+        i -= counts[v];
+        ++w;
+      }
+    Entry m = {kNegInf, 0x7fffffff};
+    if (lane < all) m = cand[w][i];
+    const int r = place_of(m, all);
+    if (lane < all && r < n) out[r] = m;
+    if (lane >= all && lane < n) out[lane] = Entry{kNegInf, -1};
     return;
   }
   // Many equal logits: one after the other, the best of what comes after the
@@ -248,112 +299,138 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
       if (before(q.x, q.at, best.x, best.at)) best = q;
     }
     __syncthreads();
-    if (lane == 0) cand[wave] = best;
+    if (lane == 0) cand[wave][0] = best;
     __syncthreads();
-    best = cand[0];
+    best = cand[0][0];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w)
-      if (before(cand[w].x, cand[w].at, best.x, best.at)) best = cand[w];
+      if (before(cand[w][0].x, cand[w][0].at, best.x, best.at))
+        best = cand[w][0];
     if (tid == 0) out[k] = best;
     last = best;
   }
 }
 
-// A position's parts; a workgroup each.
-constexpr int kJoin = 1024;  // candidates at a time
+// A position's parts, by a wave.
+//
+// Its n largest logits are among the entries of the parts' lists.  They reach what
+// n of the lanes' largest entries reach, and few others do.
+constexpr int kHeld = 8;  // entries a lane keeps; of more all are read again
 
 template <int DT, bool kTop>
 __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogArgs a) {
   using T = typename Elem<DT>::T;
-  const int64_t pos = blockIdx.x;
+  const int wave = threadIdx.x / kWave, lane = lane_id();
+  const int64_t pos = (int64_t)blockIdx.x * kWaves + wave;
+  if (pos >= a.v.batch * a.v.positions) return;  // (no barriers below)
   const int64_t b = pos / a.v.positions, j = pos % a.v.positions;
-  const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id();
   const int n = (int)a.v.top;
   const int32_t tok = a.v.tokens[pos];
   const bool given = tok >= 0 && tok < a.v.vocab;
-  __shared__ Part lds[kWaves];
-  __shared__ Entry cand[kTop ? kJoin : 1];
   if (!given) {
-    if (tid == 0) {
+    if (lane == 0) {
       a.v.logprob[pos] = 0.0f;
       a.v.entropy[pos] = 0.0f;
     }
-    if (kTop && tid < n) {
-      a.v.top_tokens[pos * n + tid] = -1;
-      a.v.top_logprobs[pos * n + tid] = kNegInf;
+    if (kTop && lane < n) {
+      a.v.top_tokens[pos * n + lane] = -1;
+      a.v.top_logprobs[pos * n + lane] = kNegInf;
     }
     return;
   }
+  const int lists = a.chunks;
+  const int all = lists * n;
+  const Entry* in = a.entry + pos * all;
+  auto entry = [&](int i) {
+    return kTop && i < all ? in[i] : Entry{kNegInf, -1};
+  };
+  Entry held[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) held[i] = entry(i * kWave + lane);
+  const T* row = (const T*)a.v.logits + b * a.v.stride_b + j * a.v.stride_j;
+  const float x = Elem<DT>::get(row[tok]);
   const float t = temperature_of(a.v, b);
   const bool greedy = !(t > 0.0f);
   const float c = greedy ? 0.0f : scale_of(t);
   Part p = {kNegInf, 0.0f, 0.0f, 0x7fffffff};
-  for (int i = tid; i < a.chunks; i += kThreads)
-    join(p, a.part[pos * a.chunks + i], c);
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const Part q = {__shfl_xor(p.top, o), __shfl_xor(p.rest, o),
-                    __shfl_xor(p.zsum, o), __shfl_xor(p.at, o)};
-    join(p, q, c);
+  for (int i = lane; i < lists; i += kWave) {
+    const Part part = a.part[pos * lists + i];
+    if (i == lane)
+      p = part;
+    else
+      join(p, part, c);
   }
-  if (lane == 0) lds[wave] = p;
-  __syncthreads();
-  p = lds[0];
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) join(p, lds[w], c);
-  const float log_sum = greedy ? 0.0f : log1pf(p.rest);
-  auto log_p = [&](float x, int i) {
-    if (!(x > kNegInf)) return kNegInf;
+  // One lane's largest is the position's: R is without it.
+  const float top = wave_max(p.top);
+  p.at = wave_min(p.top == top ? p.at : 0x7fffffff);
+  const int owner = __builtin_ctzll(ballot(p.top == top));
+  const float d = fmaxf(half_below(p.top, top) * c, kFloor);
+  const float f = p.top == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(d);
+  const float rest =
+      wave_sum(lane == owner ? p.rest : (1.0f + p.rest) * f);
+  const float zsum = wave_sum((p.zsum + d * (1.0f + p.rest)) * f);
+  const float log_sum = greedy ? 0.0f : log1pf(rest);
+  auto log_p = [&](float y, int i) {
+    if (!(y > kNegInf)) return kNegInf;
     if (greedy) return i == p.at ? 0.0f : kNegInf;
-    return 2.0f * (half_below(x, p.top) / t) - log_sum;
+    return 2.0f * (half_below(y, top) / t) - log_sum;
   };
-  if (tid == 0) {
-    const T* row =
-        (const T*)a.v.logits + b * a.v.stride_b + j * a.v.stride_j;
-    a.v.logprob[pos] = log_p(Elem<DT>::get(row[tok]), tok);
-    const bool some = p.top > kNegInf && !greedy;
-    a.v.entropy[pos] =
-        some ? log_sum - p.zsum * kLn2 / (1.0f + p.rest) : 0.0f;
+  if (lane == 0) {
+    a.v.logprob[pos] = log_p(x, tok);
+    const bool some = top > kNegInf && !greedy;
+    a.v.entropy[pos] = some ? log_sum - zsum * kLn2 / (1.0f + rest) : 0.0f;
   }
   if (!kTop) return;
-  // The best of the parts' lists, kJoin candidates at a time behind the best of
-  // those before.
-  const Entry* in = a.entry + pos * a.chunks * n;
-  const int all = a.chunks * n;
-  int kept = 0;
-  for (int i0 = 0; i0 < all;) {
-    const int take = min(kJoin - kept, all - i0);
-    for (int i = tid; i < take; i += kThreads) cand[kept + i] = in[i0 + i];
-    __syncthreads();
-    i0 += take;
-    const int count = kept + take;
-    Entry mine[kJoin / kThreads];
-    int rank[kJoin / kThreads];
+
+  float most[1] = {held[0].x};
 #pragma unroll
-    for (int k = 0; k < kJoin / kThreads; ++k) {
-      const int i = k * kThreads + tid;
-      rank[k] = n;
-      if (i < count) {
-        mine[k] = cand[i];
-        rank[k] = 0;
-        for (int q = 0; q < count; ++q)
-          rank[k] += before(cand[q].x, cand[q].at, mine[k].x, mine[k].at);
+  for (int i = 1; i < kHeld; ++i) most[0] = fmaxf(most[0], held[i].x);
+  for (int i = kHeld * kWave + lane; i < all; i += kWave)
+    most[0] = fmaxf(most[0], in[i].x);
+  const float line = reached_by(most, n);
+  __shared__ Entry kept[kWaves][kWave];
+  int count = 0;
+  auto keep = [&](const Entry& y) {
+    const bool is = y.at >= 0 && y.x >= line;
+    const uint64_t m = ballot(is);
+    const int at = count + rank_lt(m);
+    if (is && at < kWave) kept[wave][at] = y;
+    count += popc(m);
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (i * kWave < all) keep(held[i]);
+  for (int i0 = kHeld * kWave; i0 < all; i0 += kWave) keep(entry(i0 + lane));
+  wave_lds_sync();
+  Entry best = {kNegInf, -1};  // lane k: the k-th
+  if (count <= kWave) {
+    Entry mine = {kNegInf, 0x7fffffff};
+    if (lane < count) mine = kept[wave][lane];
+    const int r = place_of(mine, count);
+    wave_lds_sync();
+    if (lane < count && r < n) kept[wave][r] = mine;
+    wave_lds_sync();
+    if (lane < min(n, count)) best = kept[wave][lane];
+  } else {
+    // Many equal ones: one after the other, the first behind the last.
+    Entry last = {__builtin_inff(), -1};
+    for (int k = 0; k < n; ++k) {
+      Entry y = {kNegInf, 0x7fffffff};
+      for (int i = lane; i < all; i += kWave) {
+        const Entry e = in[i];
+        if (e.at >= 0 && before(last.x, last.at, e.x, e.at) &&
+            before(e.x, e.at, y.x, y.at))
+          y = e;
       }
+      last.x = wave_max(y.x);
+      last.at = wave_min(y.x == last.x ? y.at : 0x7fffffff);
+      if (lane == k) best = last;
     }
-    __syncthreads();
-    if (tid < n) cand[tid] = Entry{kNegInf, -1};
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kJoin / kThreads; ++k)
-      if (rank[k] < n && mine[k].at >= 0) cand[rank[k]] = mine[k];
-    __syncthreads();
-    kept = min(n, count);
   }
-  if (tid < n) {
-    const Entry e = cand[tid];
-    const bool there = e.at >= 0;
-    a.v.top_tokens[pos * n + tid] = e.at;
-    a.v.top_logprobs[pos * n + tid] = there ? log_p(e.x, e.at) : kNegInf;
+  if (lane < n) {
+    a.v.top_tokens[pos * n + lane] = best.at;
+    a.v.top_logprobs[pos * n + lane] =
+        best.at >= 0 ? log_p(best.x, best.at) : kNegInf;
   }
 }
 
@@ -386,7 +463,8 @@ int launch_as(const LogArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL((k_logprobs_scan<DT, kTop>),
                      dim3((unsigned)(rows * a.chunks)), dim3(kThreads), 0,
                      stream, a);
-  hipLaunchKernelGGL((k_logprobs_join<DT, kTop>), dim3((unsigned)rows),
+  hipLaunchKernelGGL((k_logprobs_join<DT, kTop>),
+                     dim3((unsigned)((rows + kWaves - 1) / kWaves)),
                      dim3(kThreads), 0, stream, a);
   return (int)hipGetLastError();
 }
