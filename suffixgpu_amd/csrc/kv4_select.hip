@@ -130,7 +130,8 @@ struct SelectArgs : AttendArgs {
   int want, sinks, recent;  // blocks: in all, first, last
   int span;      // query tokens of a tile
   int tiles;
-  int chunks;    // of kScoreChunk blocks
+  int piece;     // blocks of a workgroup of k_kv4_scores
+  int pieces;
   int64_t pitch; // of a query's keys
   uint32_t* keys;     // [batch, tokens, heads, pitch]
   int32_t* selected;  // [batch, tokens, heads, want]
@@ -231,77 +232,93 @@ __device__ __forceinline__ uint32_t score_key(int32_t dot, int unit) {
   return x >> 31 ? ~x : x | 0x80000000u;
 }
 
-constexpr int kScoreThreads = 256;
-constexpr int kScoreTiles = 2;  // of 16 blocks, per wave
-constexpr int kScoreChunk = kScoreThreads / kWave * kScoreTiles * 16;
+// Scores of blocks [blk0, end) of row b and KV head h for its query tokens t0 ..
+// t0 + queries - 1 (packed into sq here, with zeros up to `rows`, a multiple of
+// 16), by a workgroup: put(query, block, keys) of four blocks each.  A wave takes
+// 16 blocks at a time; the next ones are on their way while these are used.
+constexpr int kSelectThreads = 512;
 
-// Scores of 128 blocks for up to 16 query tokens of a row and KV head.
-template <int D, bool kHalf>
-__global__ __launch_bounds__(kScoreThreads) void k_kv4_scores(SelectArgs a) {
-  constexpr int kStep = 2 * D / 64;  // matrix instructions a tile
-  constexpr int kPitch = 2 * D + 16;
-  __shared__ __align__(16) int8_t sq[16][kPitch];
-  const int id = (int)blockIdx.x;
-  // tiles of one piece of the cache follow each other on one XCD
-  const int k = id >> 3;
-  const int tile = k % a.tiles;
-  const int64_t item = (int64_t)(k / a.tiles) * 8 + (id & 7);
-  const int64_t rows = a.batch * a.c.heads;
-  const int64_t bh = item % rows;
-  const int64_t chunk = item / rows;
-  if (chunk >= a.chunks) return;
-  const int64_t b = bh / a.c.heads;
-  const int h = (int)(bh % a.c.heads);
-  const int64_t len = kv_len_of(a, b), nq = q_len_of(a, b);
-  const int64_t t0 = (int64_t)tile * 16;  // (the span)
-  const int64_t last = std::min(std::min(nq, a.tokens), t0 + 16) - 1;
-  const int64_t blk0 = chunk * kScoreChunk;
-  if (last < t0 || blk0 * kKvBlock >= token_sees(a, len, nq, last)) return;
-  const int lane = lane_id(), wave = threadIdx.x / kWave;
+template <int D, bool kHalf, class Put>
+__device__ __forceinline__ void score_blocks(
+    const SelectArgs& a, int64_t b, int h, int64_t t0, int queries, int rows,
+    int blk0, int end, int8_t (*sq)[2 * D + 16], Put put) {
+  constexpr int kStep = 2 * D / 64;  // matrix instructions of 16 blocks
+  constexpr int kSelectWaves = kSelectThreads / kWave;
+  const int lane = lane_id();
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int i16 = lane % 16, quad = lane / 16;
-
-  // the bounds of the wave's blocks
-  I4 r[kScoreTiles][kStep];
-  int unit[kScoreTiles];
-#pragma unroll
-  for (int t = 0; t < kScoreTiles; ++t) {
-    const int64_t blk = blk0 + (wave * kScoreTiles + t) * 16 + i16;
-    const int64_t at = kv_place(a.c, b, h, blk);
-    unit[t] = at < 0 ? kNoPage : a.unit[at];
+  I4 r[kStep];
+  int unit;
+  auto load = [&](int blk) {
+    const int64_t at = blk < end ? kv_place(a.c, b, h, blk + i16) : -1;
+    unit = at < 0 ? kNoPage : a.unit[at];
     const I4* p = (const I4*)(a.range + (at < 0 ? 0 : at) * (2 * D)) + quad;
 #pragma unroll
-    for (int i = 0; i < kStep; ++i) r[t][i] = at < 0 ? I4{0, 0, 0, 0} : p[4 * i];
-  }
-  for (int i = wave; i < 16; i += kScoreThreads / kWave) {
-    if (t0 + i <= last) {
+    for (int i = 0; i < kStep; ++i) r[i] = at < 0 ? I4{0, 0, 0, 0} : p[4 * i];
+  };
+  load(blk0 + wave * 16);
+  for (int i = wave; i < rows; i += kSelectWaves) {
+    if (i < queries) {
       pack_query<D, kHalf>(a, b, h, t0 + i, sq[i]);
     } else {
-      for (int c = lane; c < 2 * D; c += kWave) sq[i][c] = 0;
+      for (int c = lane; c < D / 2; c += kWave) ((uint32_t*)sq[i])[c] = 0;
     }
   }
   __syncthreads();
-  const int64_t t = t0 + i16;
-  uint32_t* out = a.keys + ((b * a.tokens + t) * a.c.heads + h) * a.pitch;
+  for (int blk = blk0 + wave * 16; blk < end; blk += kSelectWaves * 16) {
+    I4 now[kStep];
 #pragma unroll
-  for (int w = 0; w < kScoreTiles; ++w) {
-    I4 s = {0, 0, 0, 0};
+    for (int i = 0; i < kStep; ++i) now[i] = r[i];
+    int us[4];
 #pragma unroll
-    for (int i = 0; i < kStep; ++i)
-      s = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-          r[w][i], *(const I4*)&sq[i16][i * 64 + quad * 16], s, 0, 0, 0);
-    uint32_t key[4];
+    for (int e = 0; e < 4; ++e) us[e] = __shfl(unit, quad * 4 + e);
+    load(blk + kSelectWaves * 16);
+    for (int q0 = 0; q0 < queries; q0 += 16) {
+      I4 s = {0, 0, 0, 0};
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      key[e] = score_key(s[e], __shfl(unit[w], quad * 4 + e));
-    const int64_t blk = blk0 + (wave * kScoreTiles + w) * 16 + quad * 4;
-    if (t <= last && blk < a.pitch)
-      *(uint4*)(out + blk) = uint4{key[0], key[1], key[2], key[3]};
+      for (int i = 0; i < kStep; ++i)
+        s = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+            now[i], *(const I4*)&sq[q0 + i16][i * 64 + quad * 16], s, 0, 0, 0);
+      if (q0 + i16 < queries)
+        put(q0 + i16, blk + quad * 4,
+            uint4{score_key(s[0], us[0]), score_key(s[1], us[1]),
+                  score_key(s[2], us[2]), score_key(s[3], us[3])});
+    }
   }
 }
 
-// Whether a query whose last block is `last` takes block j whatever its score.
-__device__ __forceinline__ bool always(const SelectArgs& a, int j, int last) {
-  return j < a.sinks || j > last - a.recent;
+// The scores of a piece of a row's blocks, into memory: for rows whose keys a
+// workgroup does not hold.
+constexpr int kScorePiece = 128;  // blocks: pieces are multiples of it
+
+template <int D, bool kHalf>
+__global__ __launch_bounds__(kSelectThreads) void k_kv4_scores(SelectArgs a) {
+  __shared__ __align__(16) int8_t sq[16][2 * D + 16];
+  // tiles of one piece follow each other on one XCD (32 bits hold all of these)
+  const uint32_t k = blockIdx.x / 8;
+  const int tile = (int)(k % (uint32_t)a.tiles);
+  const uint32_t item = k / (uint32_t)a.tiles * 8 + blockIdx.x % 8;
+  const uint32_t rows = (uint32_t)a.batch * (uint32_t)a.c.heads;
+  const uint32_t bh = item % rows;
+  const int piece = (int)(item / rows);
+  if (piece >= a.pieces) return;
+  const int64_t b = bh / (uint32_t)a.c.heads;
+  const int h = (int)(bh % (uint32_t)a.c.heads);
+  const int64_t len = kv_len_of(a, b), nq = q_len_of(a, b);
+  const int64_t t0 = (int64_t)tile * 16;
+  const int queries = (int)std::max<int64_t>(
+      0, std::min<int64_t>(std::min<int64_t>(a.tokens, nq) - t0, 16));
+  const int blk0 = piece * a.piece;
+  if (queries == 0) return;
+  const int end = std::min(
+      blk0 + a.piece,
+      (token_sees(a, len, nq, t0 + queries - 1) + kKvBlock - 1) / kKvBlock);
+  if (blk0 >= end) return;
+  uint32_t* keys = a.keys + ((b * a.tokens + t0) * a.c.heads + h) * a.pitch;
+  score_blocks<D, kHalf>(
+      a, b, h, t0, queries, 16, blk0, end, sq, [&](int q, int blk, uint4 key) {
+        *(uint4*)(keys + (int64_t)q * a.c.heads * a.pitch + blk) = key;
+      });
 }
 
 // The blocks of a query with the keys key[0 .. last] in LDS, by a wave that keeps
@@ -375,23 +392,21 @@ __device__ __forceinline__ void pick_blocks(int sinks, int recent, int all,
 
 // Scores and choice at once, where a workgroup holds the keys of its tokens: rows
 // of up to 1,024 blocks.
-constexpr int kSelectThreads = 512;
 constexpr int kSelectTokens = 32;
 
 template <int D, bool kHalf>
 __global__ __launch_bounds__(kSelectThreads) void k_kv4_select(SelectArgs a) {
-  constexpr int kStep = 2 * D / 64;  // matrix instructions a tile
   constexpr int kPitch = 2 * D + 16;
   constexpr int kSelectWaves = kSelectThreads / kWave;
   extern __shared__ __align__(16) char lds[];
-  const int id = (int)blockIdx.x;
-  // tiles of one row and KV head follow each other on one XCD
-  const int k = id >> 3;
-  const int tile = k % a.tiles;
-  const int64_t bh = (int64_t)(k / a.tiles) * 8 + (id & 7);
-  if (bh >= a.batch * a.c.heads) return;
-  const int64_t b = bh / a.c.heads;
-  const int h = (int)(bh % a.c.heads);
+  // tiles of one row and KV head follow each other on one XCD (32 bits hold all
+  // of these)
+  const uint32_t k = blockIdx.x / 8;
+  const int tile = (int)(k % (uint32_t)a.tiles);
+  const uint32_t bh = k / (uint32_t)a.tiles * 8 + blockIdx.x % 8;
+  if (bh >= (uint32_t)a.batch * (uint32_t)a.c.heads) return;
+  const int64_t b = bh / (uint32_t)a.c.heads;
+  const int h = (int)(bh % (uint32_t)a.c.heads);
   const int64_t len = kv_len_of(a, b), nq = q_len_of(a, b);
   const int64_t t0 = (int64_t)tile * a.span;
   const int tokens = (int)std::min<int64_t>(a.span, a.tokens - t0);
@@ -405,52 +420,12 @@ __global__ __launch_bounds__(kSelectThreads) void k_kv4_select(SelectArgs a) {
       queries ? (token_sees(a, len, nq, t0 + queries - 1) + kKvBlock - 1) /
                     kKvBlock
               : 0;
-  const int lane = lane_id();
+  score_blocks<D, kHalf>(a, b, h, t0, queries, (tokens + 15) / 16 * 16, 0,
+                         blocks, sq, [&](int q, int blk, uint4 key) {
+                           *(uint4*)(keys + q * pitch + blk) = key;
+                         });
+  __syncthreads();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int i16 = lane % 16, quad = lane / 16;
-
-  // bounds of 16 blocks; the next ones are on their way while these are used
-  I4 r[kStep];
-  int unit;
-  auto load = [&](int blk0) {
-    const int64_t at = blk0 < blocks ? kv_place(a.c, b, h, blk0 + i16) : -1;
-    unit = at < 0 ? kNoPage : a.unit[at];
-    const I4* p = (const I4*)(a.range + (at < 0 ? 0 : at) * (2 * D)) + quad;
-#pragma unroll
-    for (int i = 0; i < kStep; ++i) r[i] = at < 0 ? I4{0, 0, 0, 0} : p[4 * i];
-  };
-  load(wave * 16);
-  const int rows = (tokens + 15) / 16 * 16;
-  for (int i = wave; i < rows; i += kSelectWaves) {
-    if (i < queries) {
-      pack_query<D, kHalf>(a, b, h, t0 + i, sq[i]);
-    } else {
-      for (int c = lane; c < D / 2; c += kWave) ((uint32_t*)sq[i])[c] = 0;
-    }
-  }
-  __syncthreads();
-  for (int blk0 = wave * 16; blk0 < blocks; blk0 += kSelectWaves * 16) {
-    I4 now[kStep];
-#pragma unroll
-    for (int i = 0; i < kStep; ++i) now[i] = r[i];
-    const int u = unit;
-    load(blk0 + kSelectWaves * 16);
-    int us[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) us[e] = __shfl(u, quad * 4 + e);
-    for (int q0 = 0; q0 < queries; q0 += 16) {
-      I4 s = {0, 0, 0, 0};
-#pragma unroll
-      for (int i = 0; i < kStep; ++i)
-        s = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-            now[i], *(const I4*)&sq[q0 + i16][i * 64 + quad * 16], s, 0, 0, 0);
-      if (q0 + i16 < queries)
-        *(uint4*)(keys + (q0 + i16) * pitch + blk0 + quad * 4) =
-            uint4{score_key(s[0], us[0]), score_key(s[1], us[1]),
-                  score_key(s[2], us[2]), score_key(s[3], us[3])};
-    }
-  }
-  __syncthreads();
   for (int i = wave; i < tokens; i += kSelectWaves) {
     const int last = __builtin_amdgcn_readfirstlane(
         (token_sees(a, len, nq, t0 + i) + kKvBlock - 1) / kKvBlock - 1);
@@ -466,30 +441,173 @@ __global__ __launch_bounds__(kSelectThreads) void k_kv4_select(SelectArgs a) {
   }
 }
 
+// The choice by a workgroup of 1,024 threads, for rows whose keys are in memory.
+constexpr int kWideThreads = 1024;
+constexpr int kWideWaves = kWideThreads / kWave;
+
+struct WideList {
+  int last;
+  const uint32_t* keys;
+  int32_t* out;
+  __device__ __forceinline__ WideList(const SelectArgs& a) {
+    const uint32_t list = blockIdx.x, token = list / (uint32_t)a.c.heads;
+    const uint32_t b = token / (uint32_t)a.tokens;
+    const uint32_t t = token % (uint32_t)a.tokens;
+    const int sees = token_sees(a, kv_len_of(a, b), q_len_of(a, b), t);
+    last = (sees + kKvBlock - 1) / kKvBlock - 1;
+    keys = a.keys + list * a.pitch;
+    out = a.selected + (int64_t)list * a.want;
+  }
+};
+
+// As pick_blocks, the keys of up to 1,024 kRegs blocks in the workgroup's
+// registers; two bits of the line at a time, as each step is a barrier.
+template <int kRegs>
+__global__ __launch_bounds__(kWideThreads) void k_kv4_pick_wide(SelectArgs a) {
+  // (16 waves: a row of a wave's lanes sums up one number of each)
+  static_assert(kWideWaves == 16, "");
+  __shared__ uint32_t of_wave[3][4][kWideWaves];
+  __shared__ uint32_t at[kRegs * kWideWaves];  // past the line, and on it << 16
+  const int tid = threadIdx.x, lane = lane_id();
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const WideList l(a);
+  uint32_t k[kRegs], sure = 0, hi = 0, lo = 0;
+  uint32_t n_sure = 0, n_some = 0;
+#pragma unroll
+  for (int i = 0; i < kRegs; ++i) {
+    const int j = i * kWideThreads + tid;
+    k[i] = j <= l.last ? l.keys[j] : 0;
+  }
+#pragma unroll
+  for (int i = 0; i < kRegs; ++i) {
+    const int j = i * kWideThreads + tid;
+    const bool is = k[i] && (j < a.sinks || j > l.last - a.recent);
+    n_sure += (uint32_t)popc(ballot(is));
+    if (is) {
+      sure |= 1u << i;
+      k[i] = 0;
+    }
+    n_some += (uint32_t)popc(ballot(k[i] > 0));
+    hi = max(hi, k[i]);
+    lo = max(lo, 0u - k[i]);  // (none is the least)
+  }
+  hi = wave_all_max(hi);
+  lo = wave_all_max(lo);
+  if (lane == 0) {
+    of_wave[2][0][wave] = n_sure;
+    of_wave[2][1][wave] = n_some;
+    of_wave[2][2][wave] = hi;
+    of_wave[2][3][wave] = lo;
+  }
+  __syncthreads();
+  auto row_sums = [&](int turn) {
+    return row16_incl_scan(of_wave[turn][lane / 16][lane % 16]);
+  };
+  auto of_row = [](uint32_t x, int row) {
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, 16 * row + 15);
+  };
+  const uint32_t sums = row_sums(2);
+  const int want = a.want - (int)of_row(sums, 0);
+  const int some = (int)of_row(sums, 1);
+  hi = wave_all_max(lane < kWideWaves ? of_wave[2][2][lane] : 0);
+  lo = 0u - wave_all_max(lane < kWideWaves ? of_wave[2][3][lane] : 0);
+  int turn = 0;
+  // keys of at least x, x + step, x + 2 step
+  auto at_least = [&](uint32_t x, uint32_t step, int (&n)[3]) {
+#pragma unroll
+    for (int s = 0; s < 3; ++s) {
+      n[s] = 0;
+#pragma unroll
+      for (int i = 0; i < kRegs; ++i)
+        n[s] += popc(ballot(k[i] >= x + s * step));
+      if (lane == 0) of_wave[turn][s][wave] = (uint32_t)n[s];
+    }
+    __syncthreads();
+    const uint32_t sums = row_sums(turn);
+#pragma unroll
+    for (int s = 0; s < 3; ++s) n[s] = (int)of_row(sums, s);
+    turn ^= 1;
+  };
+  uint32_t line = 0;
+  int room = 0;
+  if (want <= 0) {
+    line = 0xffffffffu;
+  } else if (some > want) {
+    // (an even number of bits is left)
+    int bit = (31 - __builtin_clz((hi ^ lo) | 1u)) & ~1;
+    line = bit < 30 ? hi >> (bit + 2) << (bit + 2) : 0;
+    bool exact = false;
+    for (; bit >= 0 && !exact; bit -= 2) {
+      const uint32_t step = 1u << bit;
+      int n[3];
+      at_least(line + step, step, n);
+      uint32_t past = 0;
+#pragma unroll
+      for (int s = 0; s < 3; ++s) {
+        if (n[s] >= want) past = (uint32_t)(s + 1) * step;
+        exact = exact || n[s] == want;
+      }
+      line += past;
+    }
+    if (exact) {
+      --line;  // those past it now are the wanted ones
+    } else {
+      int n[3];
+      at_least(line + 1, 0, n);
+      room = want - n[0];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kRegs; ++i) {
+    const uint64_t gt = ballot(k[i] > line || (sure >> i & 1));
+    const uint64_t eq = ballot(room > 0 && k[i] == line);
+    if (lane == 0)
+      at[i * kWideWaves + wave] = (uint32_t)(popc(gt) | popc(eq) << 16);
+  }
+  __syncthreads();
+  // what comes before each 64, and in all; no sum passes 16 bits
+  uint32_t all = 0;
+  if (wave == 0) {
+    for (int i0 = 0; i0 < kRegs * kWideWaves; i0 += kWave) {
+      const uint32_t x = at[i0 + lane];
+      const uint32_t to = wave_incl_scan(x);
+      at[i0 + lane] = all + to - x;
+      all += (uint32_t)__builtin_amdgcn_readlane((int)to, kWave - 1);
+    }
+    const int n = (int)(all & 0xffffu) + min((int)(all >> 16), room);
+    for (int i = n + lane; i < a.want; i += kWave) l.out[i] = -1;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kRegs; ++i) {
+    const uint32_t before = at[i * kWideWaves + wave];
+    const bool over = k[i] > line || (sure >> i & 1);
+    const bool on = room > 0 && k[i] == line;
+    const int gt = (int)(before & 0xffffu) + rank_lt(ballot(over));
+    const int eq = (int)(before >> 16) + rank_lt(ballot(on));
+    if (over || (on && eq < room))
+      l.out[gt + min(eq, room)] = i * kWideThreads + tid;
+  }
+}
+
 // The key of block j for what follows: first and recent blocks above all others.
 __device__ __forceinline__ uint32_t ranked(const SelectArgs& a, uint32_t key,
                                            int j, int last) {
   if (j > last || key == 0) return 0;
-  return always(a, j, last) ? 0xffffffffu : key;
+  return j < a.sinks || j > last - a.recent ? 0xffffffffu : key;
 }
 
-// The choice by a workgroup, for tables of more blocks than a wave keeps: the keys
-// are in memory, and four passes narrow the threshold down by 8 bits each.
-constexpr int kWideThreads = 1024;
-
-__global__ __launch_bounds__(kWideThreads) void k_kv4_pick_wide(SelectArgs a) {
-  constexpr int kWideWaves = kWideThreads / kWave;
+// Rows of any length: the keys stay in memory, and four passes narrow the line
+// down by 8 bits each.
+__global__ __launch_bounds__(kWideThreads) void k_kv4_pick_far(SelectArgs a) {
   __shared__ int hist[256];
   __shared__ int sums[kWideWaves];
   __shared__ int found[2];
-  const int64_t list = blockIdx.x;
   const int tid = threadIdx.x, lane = lane_id(), wave = tid / kWave;
-  const int64_t b = list / (a.tokens * a.c.heads);
-  const int64_t t = list / a.c.heads % a.tokens;
-  const int sees = token_sees(a, kv_len_of(a, b), q_len_of(a, b), t);
-  const int last = (sees + kKvBlock - 1) / kKvBlock - 1;
-  const uint32_t* keys = a.keys + list * a.pitch;
-  int32_t* out = a.selected + list * a.want;
+  const WideList l(a);
+  const int last = l.last;
+  const uint32_t* keys = l.keys;
+  int32_t* out = l.out;
   uint32_t line = 0, mask = 0;
   int want = a.want;  // of the keys that agree with the line so far
   for (int shift = 24; shift >= 0; shift -= 8) {
@@ -604,13 +722,25 @@ int launch_wide(SelectArgs a, hipStream_t stream) {
   a.span = 16;
   a.tiles = (int)((a.tokens + 15) / 16);
   const int64_t lists = a.batch * a.tokens * a.c.heads;
-  const int64_t items = (a.batch * a.c.heads * a.chunks + 7) / 8 * 8;
-  if (items * a.tiles >= (int64_t(1) << 32) / kScoreThreads) return SFX_EINVAL;
+  // two workgroups a CU where the rows are few, long pieces where they are many
+  const int64_t whole = a.batch * a.c.heads * a.tiles;
+  const int64_t piece = std::min<int64_t>(whole * a.pitch / 512, 1024);
+  a.piece = (int)std::max<int64_t>(piece / kScorePiece, 1) * kScorePiece;
+  a.pieces = (int)((a.pitch + a.piece - 1) / a.piece);
+  const int64_t items = (a.batch * a.c.heads * a.pieces + 7) / 8 * 8;
+  if (items * a.tiles >= (int64_t(1) << 32) / kSelectThreads)
+    return SFX_EINVAL;
   hipLaunchKernelGGL((k_kv4_scores<D, kHalf>),
-                     dim3((unsigned)(items * a.tiles)), dim3(kScoreThreads), 0,
+                     dim3((unsigned)(items * a.tiles)), dim3(kSelectThreads), 0,
                      stream, a);
-  hipLaunchKernelGGL(k_kv4_pick_wide, dim3((unsigned)lists),
-                     dim3(kWideThreads), 0, stream, a);
+  const dim3 grid((unsigned)lists), block(kWideThreads);
+  const int64_t blocks = a.c.positions / kKvBlock;
+  if (blocks <= 4 * kWideThreads)
+    hipLaunchKernelGGL(k_kv4_pick_wide<4>, grid, block, 0, stream, a);
+  else if (blocks <= 16 * kWideThreads)
+    hipLaunchKernelGGL(k_kv4_pick_wide<16>, grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL(k_kv4_pick_far, grid, block, 0, stream, a);
   return (int)hipGetLastError();
 }
 
@@ -711,7 +841,6 @@ extern "C" int sfx_kv4_select(const sfx_kv4* cache,
   a.sinks = (int)first;
   a.recent = (int)recent;
   a.pitch = pitch_of(cache);
-  a.chunks = (int)((a.pitch + kScoreChunk - 1) / kScoreChunk);
   a.keys = (uint32_t*)workspace;
   a.selected = selected;
   const bool half = cache->dtype == SFX_F16;

@@ -187,7 +187,29 @@ def test_selection_over_a_wide_table(gpu):
         np.testing.assert_array_equal(got.cpu().numpy(), exp)
 
 
-@pytest.mark.parametrize("cap", [1024, 40000])
+@pytest.mark.parametrize("n", [140000, 530000])
+def test_selection_over_a_long_row(gpu, n):
+    """Rows whose keys a workgroup keeps in many registers, or not at all."""
+    b, d, page = 2, 64, 4096
+    lens = [n, n - 40000]
+    c, table = make(gpu, b, n, 1, d, page, BF, 45)
+    g = torch.Generator(device=gpu).manual_seed(46)
+    k = torch.randn(b, n, 1, d, generator=g, device=gpu).to(BF)
+    k[:, 5000:6000] *= 4
+    k[0, 9:70000:31] = 1.0
+    c.append(k, k, table, ints([0, 0], gpu), ints(lens, gpu))
+    kq = target.quantize_k(np64(k), False)
+    q = data(gpu, b, 1, 2, d, BF, 47)
+    kv = ints(lens, gpu)
+    bounds = bounds_of(kq, lens, page, table.shape[1])
+    for blocks, first, recent in ((70, 1, 2), (3000, 0, 1), (32768, 1, 1)):
+        got = c.select_blocks(q, table, kv, None, blocks, first, recent)
+        exp = target.select_blocks(np64(q), bounds, lens, [1] * b,
+                                   table.shape[1] * page, blocks, first, recent)
+        np.testing.assert_array_equal(got.cpu().numpy(), exp)
+
+
+@pytest.mark.parametrize("cap", [1024, 40000, 140000, 530000])
 def test_ties_go_to_the_lowest_blocks(gpu, cap):
     """Equal keys, zero queries, blocks of NaN, queries of NaN."""
     b, d, n = 4, 64, 9
