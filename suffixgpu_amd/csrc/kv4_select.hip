@@ -146,20 +146,19 @@ __device__ __forceinline__ int token_sees(const SelectArgs& a, int64_t len,
 }
 
 // P and -N of a query token and KV head, in 7 bits, by a wave: [0, D) against the
-// least keys, [D, 2 D) against the largest.
+// least keys, [D, 2 D) against the largest.  Made in two steps, so that one
+// query's heads can be on their way while another's are packed.
 template <int D, bool kHalf>
-__device__ __forceinline__ void pack_query(const SelectArgs& a, int64_t b,
-                                           int h, int64_t t, int8_t* out) {
-  constexpr int C = D / kWave;  // channels of a lane
-  constexpr int kHold = 8;      // query heads kept; of more all are read twice
-  const int lane = lane_id();
-  const uint16_t* q = (const uint16_t*)a.q.data + b * a.q.stride_b +
-                      t * a.q.stride_t + (int64_t)h * a.group * a.q.stride_h +
-                      lane * C;
+struct PackQuery {
+  static constexpr int C = D / kWave;  // channels of a lane
+  static constexpr int kHold = 8;  // query heads kept; of more all are read twice
   struct Head {
     uint16_t x[C];
   };
-  auto read = [&](int g) {
+  const uint16_t* q;
+  Head held[kHold];
+
+  __device__ __forceinline__ Head read(const SelectArgs& a, int g) const {
     Head r;
     const uint16_t* p = q + (int64_t)g * a.q.stride_h;
     if (C == 1) {
@@ -172,54 +171,76 @@ __device__ __forceinline__ void pack_query(const SelectArgs& a, int64_t b,
 #pragma unroll
       for (int c = 0; c < C; ++c) r.x[c] = p[c];
     }
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-      if ((r.x[c] & 0x7fffu) >= (kHalf ? 0x7c00u : 0x7f80u)) r.x[c] = 0;
     return r;
-  };
-  Head held[kHold] = {};
+  }
+  __device__ __forceinline__ PackQuery() {}
+  __device__ __forceinline__ PackQuery(const SelectArgs& a, int64_t b, int h,
+                                       int64_t t) {
+    q = (const uint16_t*)a.q.data + b * a.q.stride_b + t * a.q.stride_t +
+        (int64_t)h * a.group * a.q.stride_h + lane_id() * C;
 #pragma unroll
-  for (int g = 0; g < kHold; ++g)
-    if (g < a.group) held[g] = read(g);
-  uint32_t top = 0;
-  auto most_of = [&](const Head& x) {
+    for (int g = 0; g < kHold; ++g)
+      if (g < a.group) held[g] = read(a, g);
+  }
+  __device__ __forceinline__ void put(const SelectArgs& a, int8_t* out) const {
+    const int lane = lane_id();
+    constexpr uint32_t kInf = kHalf ? 0x7c00u : 0x7f80u;
+    uint32_t top = 0;
+    auto most_of = [&](const Head& x) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) top = max(top, x.x[c] & 0x7fffu);
-  };
+      for (int c = 0; c < C; ++c) {
+        const uint32_t m = x.x[c] & 0x7fffu;
+        top = max(top, m < kInf ? m : 0u);
+      }
+    };
 #pragma unroll
-  for (int g = 0; g < kHold; ++g) most_of(held[g]);
-  for (int g = kHold; g < a.group; ++g) most_of(read(g));
-  top = wave_all_max(top);
-  // 2^e is the power of two above the largest
-  const int e = __builtin_amdgcn_frexp_expf(to_float16b<kHalf>(top));
-  uint32_t p[C], n[C];
+    for (int g = 0; g < kHold; ++g)
+      if (g < a.group) most_of(held[g]);
+    for (int g = kHold; g < a.group; ++g) most_of(read(a, g));
+    top = wave_all_max(top);
+    // 2^e is the power of two above the largest
+    const int e = __builtin_amdgcn_frexp_expf(to_float16b<kHalf>(top));
+    uint32_t p[C], n[C];
 #pragma unroll
-  for (int c = 0; c < C; ++c) p[c] = n[c] = 0;
-  auto add = [&](const Head& x) {
+    for (int c = 0; c < C; ++c) p[c] = n[c] = 0;
+    auto add = [&](const Head& x) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const uint32_t u = (x.x[c] & 0x7fffu) < kInf ? x.x[c] : 0u;
+        const int z =
+            (int)rintf(__builtin_amdgcn_ldexpf(to_float16b<kHalf>(u), 15 - e));
+        p[c] += (uint32_t)max(z, 0);
+        n[c] += (uint32_t)max(-z, 0);
+      }
+    };
+#pragma unroll
+    for (int g = 0; g < kHold; ++g)
+      if (g < a.group) add(held[g]);
+    for (int g = kHold; g < a.group; ++g) add(read(a, g));
+    uint32_t most = 0;
+#pragma unroll
+    for (int c = 0; c < C; ++c) most = max(most, max(p[c], n[c]));
+    most = wave_all_max(most);
+    const int shift = most ? max(0, 32 - __builtin_clz(most) - 7) : 0;
+    const uint32_t half = shift ? 1u << (shift - 1) : 0u;
+    uint32_t lo = 0, hi = 0;  // bytes, of up to four channels
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int z = (int)rintf(
-          __builtin_amdgcn_ldexpf(to_float16b<kHalf>(x.x[c]), 15 - e));
-      p[c] += (uint32_t)max(z, 0);
-      n[c] += (uint32_t)max(-z, 0);
+      lo |= (-min((n[c] + half) >> shift, 127u) & 255u) << (8 * c);
+      hi |= min((p[c] + half) >> shift, 127u) << (8 * c);
     }
-  };
-#pragma unroll
-  for (int g = 0; g < kHold; ++g)
-    if (g < a.group) add(held[g]);
-  for (int g = kHold; g < a.group; ++g) add(read(g));
-  uint32_t most = 0;
-#pragma unroll
-  for (int c = 0; c < C; ++c) most = max(most, max(p[c], n[c]));
-  most = wave_all_max(most);
-  const int shift = most ? max(0, 32 - __builtin_clz(most) - 7) : 0;
-  const uint32_t half = shift ? 1u << (shift - 1) : 0u;
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    out[lane * C + c] = (int8_t)-(int)min((n[c] + half) >> shift, 127u);
-    out[D + lane * C + c] = (int8_t)min((p[c] + half) >> shift, 127u);
+    if (C == 1) {
+      out[lane] = (int8_t)lo;
+      out[D + lane] = (int8_t)hi;
+    } else if (C == 2) {
+      ((uint16_t*)out)[lane] = (uint16_t)lo;
+      ((uint16_t*)(out + D))[lane] = (uint16_t)hi;
+    } else {
+      ((uint32_t*)out)[lane] = lo;
+      ((uint32_t*)(out + D))[lane] = hi;
+    }
   }
-}
+};
 
 // Order of scores as whole numbers; 0 is no score's.
 __device__ __forceinline__ uint32_t score_key(int32_t dot, int unit) {
@@ -235,7 +256,8 @@ __device__ __forceinline__ uint32_t score_key(int32_t dot, int unit) {
 // Scores of blocks [blk0, end) of row b and KV head h for its query tokens t0 ..
 // t0 + queries - 1 (packed into sq here, with zeros up to `rows`, a multiple of
 // 16), by a workgroup: put(query, block, keys) of four blocks each.  A wave takes
-// 16 blocks at a time; the next ones are on their way while these are used.
+// 16 blocks at a time; the next ones, and the places of those after them, are on
+// their way while these are used.
 constexpr int kSelectThreads = 512;
 
 template <int D, bool kHalf, class Put>
@@ -247,32 +269,48 @@ __device__ __forceinline__ void score_blocks(
   const int lane = lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int i16 = lane % 16, quad = lane / 16;
+  // (in 32 bits: a pool of 2^31 blocks would be 4 TB)
+  auto place = [&](int blk) {
+    return blk < end ? (int)kv_place(a.c, b, h, blk + i16) : -1;
+  };
   I4 r[kStep];
   int unit;
-  auto load = [&](int blk) {
-    const int64_t at = blk < end ? kv_place(a.c, b, h, blk + i16) : -1;
+  auto load = [&](int at) {
     unit = at < 0 ? kNoPage : a.unit[at];
-    const I4* p = (const I4*)(a.range + (at < 0 ? 0 : at) * (2 * D)) + quad;
+    const I4* p =
+        (const I4*)(a.range + (int64_t)(at < 0 ? 0 : at) * (2 * D)) + quad;
 #pragma unroll
     for (int i = 0; i < kStep; ++i) r[i] = at < 0 ? I4{0, 0, 0, 0} : p[4 * i];
   };
-  load(blk0 + wave * 16);
-  for (int i = wave; i < rows; i += kSelectWaves) {
-    if (i < queries) {
-      pack_query<D, kHalf>(a, b, h, t0 + i, sq[i]);
-    } else {
-      for (int c = lane; c < D / 2; c += kWave) ((uint32_t*)sq[i])[c] = 0;
+  constexpr int kAll = kSelectWaves * 16;
+  load(place(blk0 + wave * 16));
+  int next = place(blk0 + wave * 16 + kAll);
+  {
+    typedef PackQuery<D, kHalf> Pack;
+    Pack now;
+    if (wave < queries) now = Pack(a, b, h, t0 + wave);
+    for (int i = wave; i < rows; i += kSelectWaves) {
+      if (i < queries) {
+        Pack then;
+        if (i + kSelectWaves < queries)
+          then = Pack(a, b, h, t0 + i + kSelectWaves);
+        now.put(a, sq[i]);
+        now = then;
+      } else {
+        for (int c = lane; c < D / 2; c += kWave) ((uint32_t*)sq[i])[c] = 0;
+      }
     }
   }
   __syncthreads();
-  for (int blk = blk0 + wave * 16; blk < end; blk += kSelectWaves * 16) {
+  for (int blk = blk0 + wave * 16; blk < end; blk += kAll) {
     I4 now[kStep];
 #pragma unroll
     for (int i = 0; i < kStep; ++i) now[i] = r[i];
     int us[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) us[e] = __shfl(unit, quad * 4 + e);
-    load(blk + kSelectWaves * 16);
+    load(next);
+    next = place(blk + 2 * kAll);
     for (int q0 = 0; q0 < queries; q0 += 16) {
       I4 s = {0, 0, 0, 0};
 #pragma unroll
@@ -322,13 +360,14 @@ __global__ __launch_bounds__(kSelectThreads) void k_kv4_scores(SelectArgs a) {
 }
 
 // The blocks of a query with the keys key[0 .. last] in LDS, by a wave that keeps
-// kRegs of them in each lane: the least key that is taken, bit by bit, below the
-// bits that all have and until as many as are wanted lie past it; then the blocks
-// past it, and those at it while there is room.
+// kRegs of them in each lane: the least key that is taken, from counts of 64 equal
+// parts of the keys' range and then bit by bit, until as many as are wanted lie past
+// it; then the blocks past it, and those at it while there is room.
+// bins: 64 words of the wave's own.
 template <int kRegs>
 __device__ __forceinline__ void pick_blocks(int sinks, int recent, int all,
                                             int last, const uint32_t* key,
-                                            int32_t* out) {
+                                            uint32_t* bins, int32_t* out) {
   const int lane = lane_id();
   uint32_t k[kRegs];
   uint32_t sure = 0;  // a bit for each register
@@ -338,41 +377,55 @@ __device__ __forceinline__ void pick_blocks(int sinks, int recent, int all,
   for (int i = 0; i < kRegs; ++i) {
     const int j = i * kWave + lane;
     k[i] = j <= last ? key[j] : 0;
-    const bool is = k[i] && (j < sinks || j > last - recent);
-    want -= popc(ballot(is));
-    if (is) {
-      sure |= 1u << i;
-      k[i] = 0;
+    if (i * kWave < sinks || (i + 1) * kWave > last - recent) {
+      const bool is = k[i] && (j < sinks || j > last - recent);
+      want -= popc(ballot(is));
+      if (is) {
+        sure |= 1u << i;
+        k[i] = 0;
+      }
     }
     hi = max(hi, k[i]);
     lo = max(lo, 0u - k[i]);  // (none is the least)
   }
-  auto at_least = [&](uint32_t x) {
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < kRegs; ++i) n += popc(ballot(k[i] >= x));
-    return n;
-  };
   // line: keys past it are taken, and `room` of those at it
-  uint32_t line = 0;
+  uint32_t line = 0xffffffffu;
   int room = 0;
-  if (want <= 0) {
-    line = 0xffffffffu;
-  } else if (at_least(1) > want) {
+  if (want > 0) {
     hi = wave_all_max(hi);
     lo = 0u - wave_all_max(lo);
-    int bit = 31 - __builtin_clz((hi ^ lo) | 1u);
-    line = hi >> bit >> 1 << bit << 1;
-    for (; bit >= 0; --bit) {
-      const uint32_t x = line | 1u << bit;
-      const int n = at_least(x);
-      if (n >= want) line = x;
-      if (n == want) break;
+    const int shift = max(0, 26 - __builtin_clz((hi - lo) | 1u));
+    bins[lane] = 0;
+    wave_lds_sync();
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i)
+      if (k[i]) atomicAdd(&bins[(k[i] - lo) >> shift], 1u);
+    wave_lds_sync();
+    const int upto = (int)wave_incl_scan(bins[kWave - 1 - lane]);
+    const uint64_t enough = ballot(upto >= want);
+    line = 0;
+    if (enough && __builtin_amdgcn_readlane(upto, kWave - 1) > want) {
+      const int f = __builtin_ctzll(enough);
+      line = lo + ((uint32_t)(kWave - 1 - f) << shift);
+      int n = __builtin_amdgcn_readlane(upto, f);
+      auto at_least = [&](uint32_t x) {
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < kRegs; ++i) c += popc(ballot(k[i] >= x));
+        return c;
+      };
+      for (int bit = shift - 1; bit >= 0 && n != want; --bit) {
+        const int c = at_least(line + (1u << bit));
+        if (c >= want) {
+          line += 1u << bit;
+          n = c;
+        }
+      }
+      if (n == want)
+        --line;  // those past it now are the wanted ones
+      else
+        room = want - at_least(line + 1);
     }
-    if (bit >= 0)
-      --line;  // those past it now are the wanted ones
-    else
-      room = want - at_least(line + 1);
   }
   int n = 0;
 #pragma unroll
@@ -399,6 +452,7 @@ __global__ __launch_bounds__(kSelectThreads) void k_kv4_select(SelectArgs a) {
   constexpr int kPitch = 2 * D + 16;
   constexpr int kSelectWaves = kSelectThreads / kWave;
   extern __shared__ __align__(16) char lds[];
+  __shared__ uint32_t bins[kSelectWaves][kWave];
   // tiles of one row and KV head follow each other on one XCD (32 bits hold all
   // of these)
   const uint32_t k = blockIdx.x / 8;
@@ -433,11 +487,11 @@ __global__ __launch_bounds__(kSelectThreads) void k_kv4_select(SelectArgs a) {
     int32_t* out =
         a.selected + ((b * a.tokens + t0 + i) * a.c.heads + h) * a.want;
     if (last < 4 * kWave)
-      pick_blocks<4>(a.sinks, a.recent, a.want, last, own, out);
+      pick_blocks<4>(a.sinks, a.recent, a.want, last, own, bins[wave], out);
     else if (last < 8 * kWave)
-      pick_blocks<8>(a.sinks, a.recent, a.want, last, own, out);
+      pick_blocks<8>(a.sinks, a.recent, a.want, last, own, bins[wave], out);
     else
-      pick_blocks<16>(a.sinks, a.recent, a.want, last, own, out);
+      pick_blocks<16>(a.sinks, a.recent, a.want, last, own, bins[wave], out);
   }
 }
 
@@ -703,7 +757,7 @@ int launch_held(SelectArgs a, hipStream_t stream) {
   // As many tokens as a workgroup's 64 KB hold keys of; past kSelectTokens in
   // tiles of 16.
   const int64_t row = 4 * (a.pitch + 4), packed = 2 * D + 16;
-  const int64_t room = 65536 - kSelectTokens * packed;
+  const int64_t room = 65536 - kSelectThreads * 4 - kSelectTokens * packed;
   a.span = (int)std::min<int64_t>(a.tokens <= kSelectTokens ? a.tokens : 16,
                                   room / row);
   a.tiles = (int)((a.tokens + a.span - 1) / a.span);
