@@ -38,26 +38,27 @@ __device__ __forceinline__ int end_row(const ListArgs& a, int qt) {
 // that take them (a bit each), by a workgroup: a window of the row's blocks at a
 // time, of which each token has a bit for each, so that a block named twice is
 // one.  4,096 tiles of four tokens with 64 blocks each of 512: 12 us.
-constexpr int kUnionThreads = 256;
-constexpr int kWindow = 2048;  // blocks
-
+// 1,024 threads for rows that a window of 256 does not span: 32 of eight tokens with
+// 96 blocks each of up to 4,096 take 7.5 us, by 256 threads 9.
+template <int kUnionThreads>
 __global__ __launch_bounds__(kUnionThreads) void k_kv4_union(ListArgs a) {
+  constexpr int kWindow = 8 * kUnionThreads;  // eight blocks a thread
   constexpr int kWords = kWindow / 32;
   constexpr int kUnionWaves = kUnionThreads / kWave;
-  static_assert(kWindow == 8 * kUnionThreads, "a thread has eight blocks");
   __shared__ uint32_t bits[16][kWords];
   __shared__ int sums[kUnionWaves];
   const int tid = threadIdx.x, lane = lane_id(), wave = tid / kWave;
-  const int64_t tile = blockIdx.x;  // [batch, heads, q_tiles]
-  const int qt = (int)(tile % a.q_tiles);
-  const int h = (int)(tile / a.q_tiles % a.c.heads);
-  const int64_t b = tile / a.q_tiles / a.c.heads;
+  const uint32_t tile = blockIdx.x;  // [batch, heads, q_tiles]
+  const int qt = (int)(tile % (uint32_t)a.q_tiles);
+  const uint32_t bh = tile / (uint32_t)a.q_tiles;
+  const int h = (int)(bh % (uint32_t)a.c.heads);
+  const int64_t b = bh / (uint32_t)a.c.heads;
   const int64_t len = kv_len_of(a, b), nq = q_len_of(a, b);
   const int t0 = qt * a.span;
   const int32_t* lists =
       a.selected + ((b * a.tokens + t0) * a.c.heads + h) * a.width;
   const int64_t next = (int64_t)a.c.heads * a.width;
-  int2* out = a.entry + tile * a.span * a.width;
+  int2* out = a.entry + (int64_t)tile * a.span * a.width;
   // a later token sees no less
   int limit = 0;
   for (int k = 0; k < a.span; ++k)
@@ -290,8 +291,12 @@ struct Plan {
 
 size_t round_up(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// Lists are split where there are too few of them for the chip.
-constexpr int64_t kWant = 1024;  // workgroups
+// Lists are split where there are too few of them for the chip.  With 256 / 512 /
+// 1,024 / 2,048 workgroups wanted: 64 x 1 tokens, 64 blocks each, 28 / 27 / 32 / 34 us;
+// 4 x 9 with 96 blocks and heads of 256 38 / 32 / 41 / 53; one token with 128 the
+// same.  At least 8 / 16 / 32 entries: the one token 12.3 / 12.5 / 14.6, 8 x 1 with 128
+// blocks 17.4 / 15.8 / 16.2.
+constexpr int64_t kWant = 512;  // workgroups
 constexpr int64_t kLeast = 16;   // entries of one
 
 Plan plan_for(const sfx_kv4* c, int64_t batch, int64_t tokens, int64_t q_heads,
@@ -324,16 +329,18 @@ bool shapes_ok(const sfx_kv4* c, int64_t batch, int64_t tokens,
 template <int D, bool kHalf>
 int launch(const ListArgs& a, hipStream_t stream) {
   const int64_t items = (a.batch * a.c.heads * a.splits + 7) / 8 * 8;
-  if (items * a.q_tiles >= (int64_t(1) << 32) / (64 * kWaves))
-    return SFX_EINVAL;  // more threads than a grid takes
+  // more threads than a grid takes, also of 1,024 a tile
+  if (items * a.q_tiles >= (int64_t(1) << 32) / 1024) return SFX_EINVAL;
   const dim3 grid((unsigned)(items * a.q_tiles)), block(64 * kWaves);
   if (a.span == 1) {
     hipLaunchKernelGGL((k_kv4_attend_blocks<D, kHalf, OneList>), grid, block, 0,
                        stream, a);
   } else {
-    hipLaunchKernelGGL(k_kv4_union,
-                       dim3((unsigned)(a.batch * a.c.heads * a.q_tiles)),
-                       dim3(kUnionThreads), 0, stream, a);
+    const dim3 tiles((unsigned)(a.batch * a.c.heads * a.q_tiles));
+    if (a.c.positions / kKvBlock <= 2048)
+      hipLaunchKernelGGL(k_kv4_union<256>, tiles, dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL(k_kv4_union<1024>, tiles, dim3(1024), 0, stream, a);
     hipLaunchKernelGGL((k_kv4_attend_blocks<D, kHalf, TileList>), grid, block,
                        0, stream, a);
   }
