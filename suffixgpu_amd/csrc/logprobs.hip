@@ -7,9 +7,9 @@
 //   log p_i = z_i - log(1 + R),   H = log(1 + R) - sum z e^z / (1 + R).
 //
 // The first launch takes 8,192 logits a workgroup, which stay in registers: their
-// largest, R and sum z e^z, and their n largest in order.  A number that n of the
-// maxima of its pieces reach, and few more, is one that the n largest logits reach,
-// and few others: those are ranked.  The second launch joins a position's parts.
+// largest, R and sum z e^z, and what reaches a number that n of the maxima of its
+// 64 parts reach, and few more: the n largest, and few others.  The second launch
+// joins a position's parts and ranks what is left of those.
 // Positions without a token leave at once.
 
 #include <algorithm>
@@ -22,7 +22,7 @@ namespace sfx {
 namespace {
 
 constexpr int kWaves = kThreads / kWave;
-constexpr float kMaxScale = 0x1.fffffep127f;
+constexpr float kMaxScale = 0x1.fffffep126f;
 constexpr float kLn2 = 0.69314718055994530942f;
 // 2^kFloor is zero in 32 bits; where z may be -inf or a NaN, z e^z shall be zero.
 constexpr float kFloor = -160.0f;
@@ -43,7 +43,7 @@ struct LogArgs {
   sfx_logprobs v;
   int chunks;
   Part* part;    // [batch * positions, chunks]
-  Entry* entry;  // [batch * positions, chunks, top]
+  Entry* entry;  // [batch * positions, chunks, top + kSpare]
 };
 
 __device__ __forceinline__ float temperature_of(const sfx_logprobs& v,
@@ -52,15 +52,23 @@ __device__ __forceinline__ float temperature_of(const sfx_logprobs& v,
   return t > 0.0f ? t : 0.0f;
 }
 
+// A value of another lane of the row of 16.
+template <int kCtrl>
+__device__ __forceinline__ float lane_of(float x) {
+  return __builtin_bit_cast(
+      float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), kCtrl, 0xf,
+                                      0xf, true));
+}
+
 // Half the difference to the largest, which is a float where the difference is
 // too large for one; 0 where infinities meet.
 __device__ __forceinline__ float half_below(float x, float top) {
   return x == top ? 0.0f : __builtin_fmaf(x, 0.5f, -0.5f * top);
 }
 
-// Base-2 scale of such a half.
+// Base-2 scale of a difference; twice that of a half is a float too.
 __device__ __forceinline__ float scale_of(float t) {
-  return fminf(2.0f * kLog2e / t, kMaxScale);
+  return fminf(kLog2e / t, kMaxScale);
 }
 
 // Whether candidate (x, i) comes before (y, j).
@@ -77,7 +85,7 @@ __device__ __forceinline__ void join(Part& p, const Part& q, float c) {
   }
   const bool swap = q.top > p.top;
   const Part a = swap ? q : p, b = swap ? p : q;
-  const float d = fmaxf(half_below(b.top, a.top) * c, kFloor);
+  const float d = fmaxf(half_below(b.top, a.top) * (2.0f * c), kFloor);
   const float f = __builtin_amdgcn_exp2f(d);
   p.top = a.top;
   p.rest = a.rest + (1.0f + b.rest) * f;
@@ -103,28 +111,19 @@ __device__ __forceinline__ int place_of(const Entry& m, int count) {
   return r;
 }
 
-// A number that n of a wave's R values a lane reach (there are as many), and few
-// more: by halves, until no more than n + kFew do.
+// A number that n of a wave's lanes reach (at most 64), and few more: by halves,
+// until no more than n + kFew do.
 constexpr int kFew = 6;
+constexpr int kSpare = 8;  // entries of a list beside the n, which are in no order
 
-template <int R>
-__device__ __forceinline__ float reached_by(const float (&x)[R], int n) {
-  uint32_t k[R], hi = 0, lo = 0;
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    k[i] = order_of(x[i]);
-    hi = max(hi, k[i]);
-    lo = max(lo, ~k[i]);
-  }
-  hi = wave_all_max(hi);
-  lo = ~wave_all_max(lo);
+__device__ __forceinline__ float reached_by(float x, int n) {
+  const uint32_t k = order_of(x);
+  const uint32_t hi = wave_all_max(k), lo = ~wave_all_max(~k);
   int bit = 31 - __builtin_clz((hi ^ lo) | 1u);
   uint32_t line = lo >> bit >> 1 << bit << 1;
   for (; bit >= 0; --bit) {
     const uint32_t y = line | 1u << bit;
-    int count = 0;
-#pragma unroll
-    for (int i = 0; i < R; ++i) count += popc(ballot(k[i] >= y));
+    const int count = popc(ballot(k >= y));
     if (count >= n) {
       line = y;
       if (count <= n + kFew) break;
@@ -139,9 +138,7 @@ template <int DT, bool kTop>
 __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
   using S = Share<DT>;
   constexpr int E = S::E, U = S::U;
-  constexpr int kSegs = U * kThreads / 16;  // pieces of 16 vectors
-  constexpr int kRegs = kSegs / kWave;      // their maxima a lane
-  static_assert(kSegs % kWave == 0 && kSegs >= SFX_LOGPROBS_TOP, "");
+  static_assert(kThreads / 4 == kWave && kWave >= SFX_LOGPROBS_TOP, "");
   const int chunk = blockIdx.x % a.chunks;
   const int64_t pos = blockIdx.x / a.chunks;
   const int64_t b = pos / a.v.positions, j = pos % a.v.positions;
@@ -149,7 +146,8 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
   if (tok < 0 || tok >= a.v.vocab) return;
   const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id();
   __shared__ Part lds[kWaves];
-  __shared__ float seg[kTop ? kSegs : 1];
+  __shared__ float group[kTop ? kWave : 1];  // maxima of four threads' logits
+  __shared__ float lds_line;
   __shared__ Entry cand[kTop ? kWaves : 1][kWave];
   __shared__ int counts[kWaves];
   const float t = temperature_of(a.v, b);
@@ -159,92 +157,118 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
                              b * a.v.stride_b + j * a.v.stride_j;
   S s(row, a.v.vocab, chunk);
   s.load(row);
-  // largest of each vector, of the thread, of the wave
-  float vtop[U], top = fmaxf(s.single, kNegInf);
+  // The logits as floats, once; the largest of each vector, of the thread, of the
+  // wave.
+  float x[U][E], vtop[U], top = fmaxf(s.single, kNegInf);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     vtop[u] = kNegInf;
 #pragma unroll
-    for (int e = 0; e < E; ++e) vtop[u] = fmaxf(vtop[u], s.get(u, e));
+    for (int e = 0; e < E; ++e) {
+      x[u][e] = s.get(u, e);
+      vtop[u] = fmaxf(vtop[u], x[u][e]);
+    }
     top = fmaxf(top, vtop[u]);
   }
   const float mine = top;
   top = wave_max(top);
   if (kTop) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float m = vtop[u];
-      m = fmaxf(m, dpp<0xb1, 0xf>(m, m));    // lane ^ 1
-      m = fmaxf(m, dpp<0x4e, 0xf>(m, m));    // lane ^ 2
-      m = fmaxf(m, dpp<0x141, 0xf>(m, m));   // half of a row mirrored
-      m = fmaxf(m, dpp<0x140, 0xf>(m, m));   // row mirrored
-      if (lane % 16 == 0) seg[u * (kThreads / 16) + tid / 16] = m;
-    }
+    float m = fmaxf(mine, lane_of<0xb1>(mine));  // lane ^ 1
+    m = fmaxf(m, lane_of<0x4e>(m));              // lane ^ 2
+    if (lane % 4 == 0) group[tid / 4] = m;
   }
   Part p = {top, 0.0f, 0.0f, 0x7fffffff};
   if (greedy) {
     if (mine == top && top > kNegInf) {
       int at = 0x7fffffff;
-      s.again([&](float x, int i) { at = x == top ? min(at, i) : at; });
+      s.again([&](float y, int i) { at = y == top ? min(at, i) : at; });
       p.at = at;
     }
     p.at = wave_min(p.at);
   } else if (top > kNegInf) {
-    s.forget();
+    // z = x c - top c in one step, with top c rounded; what that is off, the same
+    // for all, is put right in the sums.
+    if (kTop && DT != SFX_F32) {
+      // unpacked again where they are used: kept as floats they would cost the
+      // kernel that also ranks a wave in seven
+      s.forget();
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[u][e] = s.get(u, e);
+    }
+    const float tc = top * c, off = __builtin_fmaf(top, c, -tc);
     float sum = 0.0f, zsum = 0.0f;
     int equal = 0;
-    const float half = -0.5f * top;
-    auto add = [&](float x) {
-      const float z = fmaxf(__builtin_fmaf(x, 0.5f, half) * c, kFloor);
+    auto add = [&](float z) {
+      z = fmaxf(z, kFloor);
       const float e = __builtin_amdgcn_exp2f(z);
       sum += e;
       zsum = __builtin_fmaf(z, e, zsum);
     };
-    auto add_special = [&](float x) {
-      equal += popc(ballot(x == top));
-      const float z = x == top
-                          ? kFloor
-                          : fmaxf(__builtin_fmaf(x, 0.5f, half) * c, kFloor);
-      const float e = __builtin_amdgcn_exp2f(z);
-      sum += e;
-      zsum = __builtin_fmaf(z, e, zsum);
-    };
-    if (ballot(s.extra >= 0)) add_special(s.single);
+    auto take = [&](auto z_of) {
+      auto add_special = [&](float y) {
+        equal += popc(ballot(y == top));
+        add(y == top ? kFloor : z_of(y));
+      };
+      if (ballot(s.extra >= 0)) add_special(s.single);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      // one vector in U holds the wave's largest
-      if (ballot(vtop[u] == top)) {
+      for (int u = 0; u < U; ++u) {
+        // one vector in U holds the wave's largest
+        if (ballot(vtop[u] == top)) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) add_special(s.get(u, e));
-      } else {
+          for (int e = 0; e < E; ++e) add_special(x[u][e]);
+        } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) add(s.get(u, e));
+          for (int e = 0; e < E; ++e) add(z_of(x[u][e]));
+        }
       }
+    };
+    if (fabsf(tc) < 0x1p60f && c < 0x1p60f) {
+      take([&](float y) { return __builtin_fmaf(y, c, -tc); });
+      sum = wave_sum(sum);
+      zsum = wave_sum(zsum);
+      const float f = __builtin_amdgcn_exp2f(-off);
+      zsum = (zsum - off * sum) * f;
+      sum *= f;
+    } else {
+      // infinities, and what grows too large: a difference first, by halves
+      const float half = -0.5f * top, c2 = 2.0f * c;
+      s.again([&](float y, int) {
+        const bool is = y == top;
+        equal += is;
+        add(is ? kFloor : __builtin_fmaf(y, 0.5f, half) * c2);
+      });
+      sum = wave_sum(sum);
+      zsum = wave_sum(zsum);
+      equal = (int)wave_sum((float)equal);
     }
-    p.rest = wave_sum(sum) + ((float)equal - 1.0f);
-    p.zsum = wave_sum(zsum);
+    p.rest = sum + ((float)equal - 1.0f);
+    p.zsum = zsum;
   }
   if (lane == 0) lds[wave] = p;
   __syncthreads();
+  const int n = (int)a.v.top;
+  if (kTop && wave == 1) {
+    // what n groups' maxima reach, so at least n logits, and few more
+    const float y = reached_by(group[lane], n);
+    if (lane == 0) lds_line = y;
+  }
   if (tid == 0) {
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) join(p, lds[w], c);
     a.part[pos * a.chunks + chunk] = p;
   }
   if (!kTop) return;
-
-  // What reaches the n largest pieces' maxima, at least n of them.
-  const int n = (int)a.v.top;
-  float segs[kRegs];
-#pragma unroll
-  for (int i = 0; i < kRegs; ++i) segs[i] = seg[i * kWave + lane];
-  const float line = reached_by(segs, n);
+  if (DT != SFX_F32) s.forget();
+  __syncthreads();
+  const float line = lds_line;
   int count = 0;
-  auto offer = [&](float x, int i, bool in) {
-    const bool is = in && x >= line && x > kNegInf;
+  auto offer = [&](float y, int i, bool in) {
+    const bool is = in && y >= line && y > kNegInf;
     const uint64_t m = ballot(is);
     const int k = count + rank_lt(m);
-    if (is && k < kWave) cand[wave][k] = Entry{x, i};
+    if (is && k < kWave) cand[wave][k] = Entry{y, i};
     count += popc(m);
   };
   if (ballot(s.extra >= 0)) offer(s.single, s.extra, s.extra >= 0);
@@ -252,15 +276,15 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
   for (int u = 0; u < U; ++u) {
     if (ballot(vtop[u] >= line)) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float x = s.get(u, e);
-        if (ballot(x >= line)) offer(x, s.index(u * E + e), true);
-      }
+      for (int e = 0; e < E; ++e)
+        if (ballot(s.get(u, e) >= line))
+          offer(s.get(u, e), s.index(u * E + e), true);
     }
   }
   if (lane == 0) counts[wave] = count;
   __syncthreads();
-  Entry* out = a.entry + (pos * a.chunks + chunk) * n;
+  const int room = n + kSpare;
+  Entry* out = a.entry + (pos * a.chunks + chunk) * room;
   int all = 0;
   bool fits = true;
 #pragma unroll
@@ -277,13 +301,18 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
         i -= counts[v];
         ++w;
       }
-    Entry m = {kNegInf, 0x7fffffff};
+    Entry m = {kNegInf, -1};
     if (lane < all) m = cand[w][i];
+    if (all <= room) {
+      if (lane < room) out[lane] = m;
+      return;
+    }
     const int r = place_of(m, all);
     if (lane < all && r < n) out[r] = m;
-    if (lane >= all && lane < n) out[lane] = Entry{kNegInf, -1};
+    if (lane >= n && lane < room) out[lane] = Entry{kNegInf, -1};
     return;
   }
+  if (tid >= n && tid < room) out[tid] = Entry{kNegInf, -1};
   // Many equal logits: one after the other, the best of what comes after the
   // last.
   Entry last = {__builtin_inff(), -1};
@@ -339,7 +368,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogArgs a) {
     return;
   }
   const int lists = a.chunks;
-  const int all = lists * n;
+  const int all = lists * (n + kSpare);
   const Entry* in = a.entry + pos * all;
   auto entry = [&](int i) {
     return kTop && i < all ? in[i] : Entry{kNegInf, -1};
@@ -364,7 +393,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogArgs a) {
   const float top = wave_max(p.top);
   p.at = wave_min(p.top == top ? p.at : 0x7fffffff);
   const int owner = __builtin_ctzll(ballot(p.top == top));
-  const float d = fmaxf(half_below(p.top, top) * c, kFloor);
+  const float d = fmaxf(half_below(p.top, top) * (2.0f * c), kFloor);
   const float f = p.top == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(d);
   const float rest =
       wave_sum(lane == owner ? p.rest : (1.0f + p.rest) * f);
@@ -382,11 +411,11 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogArgs a) {
   }
   if (!kTop) return;
 
-  float most[1] = {held[0].x};
+  float most = held[0].x;
 #pragma unroll
-  for (int i = 1; i < kHeld; ++i) most[0] = fmaxf(most[0], held[i].x);
+  for (int i = 1; i < kHeld; ++i) most = fmaxf(most, held[i].x);
   for (int i = kHeld * kWave + lane; i < all; i += kWave)
-    most[0] = fmaxf(most[0], in[i].x);
+    most = fmaxf(most, in[i].x);
   const float line = reached_by(most, n);
   __shared__ Entry kept[kWaves][kWave];
   int count = 0;
@@ -446,7 +475,8 @@ size_t part_bytes(int64_t rows, int64_t vocab) {
 
 size_t bytes_for(int64_t rows, int64_t vocab, int64_t top) {
   return part_bytes(rows, vocab) +
-         (size_t)rows * chunks_for(vocab) * top * sizeof(Entry);
+         (top ? (size_t)rows * chunks_for(vocab) * (top + kSpare) * sizeof(Entry)
+              : 0);
 }
 
 bool sizes_ok(int64_t batch, int64_t positions, int64_t vocab, int64_t top) {
