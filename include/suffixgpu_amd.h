@@ -673,7 +673,7 @@ int sfx_token_logprobs(const sfx_logprobs* args, void* workspace,
  * it up once: free_pages a stack of the free page ids, its *num_free lowest
  * entries used; held[r] pages of row r, which are table[r][0 .. held[r]), -1
  * behind them.  From then on the calls below change it; those on one pool must
- * not overlap. */
+ * not overlap, nor may one host thread's launches have another's between them. */
 typedef struct sfx_pages {
     int32_t* free_pages;  /* [num_pages]                                  */
     int32_t* num_free;    /* [1]                                          */
@@ -742,8 +742,9 @@ int sfx_kv4_bounds_update(const sfx_kv4* cache, const sfx_kv4_bounds* bounds,
  * the same power of two, 1 or more, that leaves 7 bits, halves up, at most 127.
  * selected [batch, tokens, heads, blocks]: positions / 32, ascending, -1 behind
  * them and for what is no query.  1 <= recent, first + recent <= blocks.
- * workspace: sfx_kv4_select_workspace_size bytes, 16-byte aligned, of any
- * content; calls that may overlap have their own. */
+ * workspace: sfx_kv4_select_workspace_size bytes (none for tables of up to 1,024
+ * blocks, past that 4 for each query token, KV head and block), 16-byte aligned,
+ * of any content; calls that may overlap have their own. */
 size_t sfx_kv4_select_workspace_size(const sfx_kv4* cache, int64_t batch,
                                      int64_t tokens);
 int sfx_kv4_select(const sfx_kv4* cache, const sfx_kv4_bounds* bounds,

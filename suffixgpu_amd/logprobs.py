@@ -17,6 +17,10 @@ from suffixgpu_amd._lib import (check, elsewhere, lib, require_gpu,
                                 stream_of)
 
 
+# Workspace bytes by (batch, positions, vocabulary, alternatives).
+_sizes: dict[tuple, int] = {}
+
+
 class TokenLogprobs(NamedTuple):
     logprob: torch.Tensor       # [B, J] float32
     entropy: torch.Tensor       # [B, J] float32
@@ -69,21 +73,24 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor,
                          f"tensor on {dev}")
     if not 0 <= top <= _lib.LOGPROBS_TOP:
         raise ValueError(f"top must be in 0..{_lib.LOGPROBS_TOP}")
-    lp = torch.empty(2, b, j, dtype=torch.float32, device=dev)
+    logprob, entropy = torch.empty(2, b, j, dtype=torch.float32,
+                                   device=dev).unbind(0)
     ids = torch.empty(b, j, top, dtype=torch.int32, device=dev)
     alt = torch.empty(b, j, top, dtype=torch.float32, device=dev)
-    out = TokenLogprobs(lp[0], lp[1], ids, alt)
+    out = TokenLogprobs(logprob, entropy, ids, alt)
     if b == 0 or j == 0:
         return out
     L = lib()
-    nbytes = L.sfx_logprobs_workspace_size(b, j, v, top)
+    nbytes = _sizes.get((b, j, v, top))
+    if nbytes is None:
+        nbytes = _sizes[b, j, v, top] = L.sfx_logprobs_workspace_size(b, j, v,
+                                                                     top)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    at = lp.data_ptr()
     args = _lib.SfxLogprobs(logits.data_ptr(), code, b, j, v, sb, sj,
                             tokens.data_ptr(),
                             None if temperature is None
                             else temperature.data_ptr(),
-                            top, at, at + 4 * b * j,
+                            top, logprob.data_ptr(), entropy.data_ptr(),
                             ids.data_ptr() or None, alt.data_ptr() or None)
     check(L.sfx_token_logprobs(args, ws.data_ptr(), nbytes, stream_of(dev)),
           "token_logprobs")

@@ -8,6 +8,8 @@ whose cache is the engine's.
 
 from __future__ import annotations
 
+import threading
+
 import torch
 
 from suffixgpu_amd import _lib
@@ -52,6 +54,7 @@ class PagePool:
         self._held = torch.zeros(self.rows, **i32)
         self._table = torch.full((self.rows, self.width), -1, **i32)
         self._plan = torch.empty(3 * self.rows + 4, **i32)
+        self._enqueue = threading.Lock()
         self._view = _lib.SfxPages(
             self._stack.data_ptr() or None, self._num_free.data_ptr(),
             self._held.data_ptr(), self._table.data_ptr(), self.num_pages,
@@ -95,10 +98,12 @@ class PagePool:
         n = t.shape[0]
         room = torch.empty(n, dtype=torch.int32, device=self.device)
         if n:
-            check(lib().sfx_pages_resize(self._view, t.data_ptr(), is64, n,
-                                         room.data_ptr(),
-                                         stream_of(self.device)),
-                  "PagePool.resize")
+            # (the C call lets other threads run)
+            with self._enqueue:
+                rc = lib().sfx_pages_resize(self._view, t.data_ptr(), is64, n,
+                                            room.data_ptr(),
+                                            stream_of(self.device))
+            check(rc, "PagePool.resize")
         return room
 
     def slots(self, start: torch.Tensor, tokens: int,
