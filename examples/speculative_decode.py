@@ -3,15 +3,21 @@ model's attention over a cache held in 4 bits, and the verification of the
 drafts.
 
     python examples/speculative_decode.py [--batch 8] [--new 128] [--sample]
+                                          [--blocks 0]
 
 The target model is a stand-in of random weights (one attention layer between an
 embedding and its transpose); what matters is the loop around it, which is an
 engine's:
 
     propose_with_update   the last step's tokens enter the rows, a draft comes out
+    PagePool.resize       pages for the tokens that come, and those back that
+                          rejected drafts and finished rows held
     KV4Cache.append       keys and values of the newest token and the draft
-    KV4Cache.attend       their queries over the whole cache
+    KV4Cache.attend       their queries over the whole cache; with --blocks N
+                          .select_blocks and .attend_blocks: over N blocks of 32
+                          tokens each
     verify_draft          which drafts stay, and the token after them
+    token_logprobs        what is reported of the tokens
 
 No step reads device memory on the host.  A rejected draft's keys and values stay
 in the cache until the next append overwrites them.
@@ -27,7 +33,8 @@ import torch
 
 sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
 
-from suffixgpu_amd import KV4Cache, SuffixGPUDrafter, verify_draft  # noqa: E402
+from suffixgpu_amd import (KV4Cache, PagePool, SuffixGPUDrafter,  # noqa: E402
+                           token_logprobs, verify_draft)
 
 
 class TinyTarget:
@@ -50,9 +57,10 @@ class TinyTarget:
         half = torch.arange(width // 2, device=device)
         self.freq = 0.5 ** (half * (10.0 / half.numel()))
 
-    def forward(self, tokens, start, count, cache, table):
+    def forward(self, tokens, start, count, cache, table, blocks=0):
         """Logits [B, T, V] (float32) of tokens [B, T] at positions start + i,
-        i < count, which enter the cache."""
+        i < count, which enter the cache; attention over the whole of it, or over
+        `blocks` selected blocks."""
         b, t = tokens.shape
         x = self.embed[tokens.clamp(min=0).long()]
         pos = (start[:, None] + torch.arange(t, device=start.device))
@@ -63,15 +71,21 @@ class TinyTarget:
         k = y[:, :, self.heads:self.heads + self.kv_heads]
         v = y[:, :, self.heads + self.kv_heads:]
         cache.append(k, v, table, start, count)
-        o = cache.attend(q, table, start + count, count)
+        end = start + count
+        if blocks:
+            chosen = cache.select_blocks(q, table, end, count, blocks)
+            o = cache.attend_blocks(q, chosen, table, end, count)
+        else:
+            o = cache.attend(q, table, end, count)
         x = x + 0.25 * (o.reshape(b, t, -1) @ self.out)
         return (x @ self.lm).float()
 
 
 def decode(batch=8, prompt=48, new=128, k=8, vocab=128, temperature=0.0,
-           seed=0, device="cuda", draft=True):
+           seed=0, device="cuda", draft=True, blocks=0, report=False):
     """Decodes `batch` random prompts until every row has `new` more tokens.
-    Returns (rows [batch, prompt + new] of tokens, steps)."""
+    Returns (rows [batch, prompt + new] of tokens, steps), with `report` also the
+    new tokens' log probabilities [batch, new] under the target's logits."""
     dev = torch.device(device, torch.cuda.current_device())
     g = torch.Generator(device=dev).manual_seed(seed)
     longest = prompt + new + k + 1
@@ -79,9 +93,8 @@ def decode(batch=8, prompt=48, new=128, k=8, vocab=128, temperature=0.0,
     page = 64
     width = -(-longest // page)
     cache = KV4Cache(batch * width, model.kv_heads, model.head_dim,
-                     page_size=page, device=dev)
-    table = torch.randperm(batch * width, generator=g, device=dev).to(
-        torch.int32).view(batch, width)
+                     page_size=page, device=dev, bounds=blocks > 0)
+    pool = PagePool(batch * width, batch, width, page_size=page, device=dev)
     drafter = SuffixGPUDrafter(k=k, device=dev, max_pattern_len=16,
                                num_backoff=4)
     rows = torch.zeros(batch, longest, dtype=torch.int32, device=dev)
@@ -90,7 +103,19 @@ def decode(batch=8, prompt=48, new=128, k=8, vocab=128, temperature=0.0,
     # the prompts' keys and values, and the first token of every row
     zero = torch.zeros(batch, dtype=torch.int32, device=dev)
     counts = torch.full((batch,), prompt, dtype=torch.int32, device=dev)
-    logits = model.forward(rows[:, :prompt], zero, counts, cache, table)
+    pool.resize(counts)
+    logits = model.forward(rows[:, :prompt], zero, counts, cache, pool.table,
+                           blocks)
+    # (a column behind the rows for what is no token)
+    logprobs = torch.zeros(batch, longest + 1, device=dev)
+
+    def note(logits, sampled, start):
+        if report:
+            at = start[:, None] + torch.arange(sampled.shape[1], device=dev)
+            at = torch.where((sampled >= 0) & (at < longest), at, longest)
+            logprobs.scatter_(1, at.long(),
+                              token_logprobs(logits, sampled).logprob)
+
     temp = torch.full((batch,), float(temperature), device=dev)
 
     def verify(logits, drafts, valid):
@@ -105,6 +130,7 @@ def decode(batch=8, prompt=48, new=128, k=8, vocab=128, temperature=0.0,
 
     none = torch.empty(batch, 0, dtype=torch.int32, device=dev)
     sampled, _ = verify(logits[:, -1:], none, zero)
+    note(logits[:, -1:], sampled, counts)
     steps = 0
     # (the host looks at the counts now and then only to know when to stop)
     while True:
@@ -113,16 +139,20 @@ def decode(batch=8, prompt=48, new=128, k=8, vocab=128, temperature=0.0,
         if not draft:
             valid = torch.zeros_like(valid)
         if steps % 8 == 0 and int(counts.min()) >= prompt + new:
-            return rows[:, :prompt + new], steps
+            done = (rows[:, :prompt + new], steps)
+            return (*done, logprobs[:, prompt:prompt + new]) if report else done
         # rows that are done stay where they are
         done = counts >= prompt + new
         valid = torch.where(done, 0, valid)
         counts = counts.clamp(max=prompt + new)
         last = rows.gather(1, (counts - 1).long()[:, None])
+        # a row that is done gives its pages back; its token is written nowhere
+        pool.resize(torch.where(done, 0, counts + valid))
         logits = model.forward(torch.cat([last, drafts], 1), counts - 1,
-                               valid + 1, cache, table)
+                               valid + 1, cache, pool.table, blocks)
         sampled, _ = verify(logits, drafts, valid)
         sampled = torch.where(done[:, None], -1, sampled)
+        note(logits, sampled, counts)
         steps += 1
 
 
@@ -132,13 +162,16 @@ def main():
     ap.add_argument("--new", type=int, default=128)
     ap.add_argument("--sample", action="store_true",
                     help="temperature 0.2 instead of the likeliest token")
+    ap.add_argument("--blocks", type=int, default=0,
+                    help="attend to so many blocks of 32 tokens (all: 0)")
     a = ap.parse_args()
     t = 0.2 if a.sample else 0.0
-    rows, steps = decode(batch=a.batch, new=a.new, temperature=t)
+    rows, steps, lp = decode(batch=a.batch, new=a.new, temperature=t,
+                             blocks=a.blocks, report=True)
     plain, plain_steps = decode(batch=a.batch, new=a.new, temperature=t,
-                                draft=False)
+                                draft=False, blocks=a.blocks)
     print(f"{a.new} tokens for {a.batch} requests: {steps} steps with drafts, "
-          f"{plain_steps} without")
+          f"{plain_steps} without; {-lp.mean().item():.2f} nats a token")
     if t == 0:
         same = (rows == plain).float().mean().item()
         print(f"{100 * same:.1f}% of the tokens are the same either way")
