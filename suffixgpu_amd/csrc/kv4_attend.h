@@ -153,9 +153,11 @@ struct Block<D, 16> {
     at_k = t * (D / 2) + quad * (D / 8);
     at_ks = t * (D / 32) + (D == 256 ? 2 * quad : (D == 64 ? quad / 2 : quad));
     at_v = lane * 16;
-    at_vs = lane % 32 * 4;
+    at_vs = L::kVScale + lane % 32 * 4;
   }
+  // (the compiler would keep the places as 64 bits, and add the base to each)
   __device__ __forceinline__ void load_k(const char* base) {
+    asm volatile("" : "+v"(at_k), "+v"(at_ks), "+v"(at_vs));
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
       const char* p = base + at_k + 8 * a * (D / 2);
@@ -176,9 +178,10 @@ struct Block<D, 16> {
       const char* s = base + at_ks + (L::kScale + 8 * a * (D / 32));
       ks[a] = D == 256 ? *(const uint16_t*)s : *(const uint8_t*)s;
     }
-    vs = *(const float*)(base + at_vs + L::kVScale);
+    vs = *(const float*)(base + at_vs);
   }
   __device__ __forceinline__ void load_v(const char* base) {
+    asm volatile("" : "+v"(at_v));
 #pragma unroll
     for (int g = 0; g < D / 64; ++g) {
       const uint4 w =
@@ -556,10 +559,44 @@ constexpr int kLds32 = kWaves * 32 * (64 + 4) * 4 > 32 * D * 2
                            ? kWaves * 32 * (64 + 4) * 4
                            : 32 * D * 2;
 
-// Which blocks a wave of attend16 takes: each(a, wk, bytes, vis, body) calls
-// body(block, index, v, whole, kdone, vdone) with the positions v that the lane's
-// row sees if it takes the block (vis, or 0), whole where every row does.  Here
-// blocks first, first + kWaves, ... of a split, by all rows.
+// A wave's 16 query rows and their products with a block's keys: here as 16-bit
+// operands.  row(r): the address of the tile's row r, sees(r): whether it sees a
+// position; pool: LDS of the workgroup, free again after the constructor.
+template <int D, bool kHalf>
+struct WideQueries {
+  static constexpr int kStep = D / 32;  // matrix instructions a score tile
+  U4 q[kStep];
+  template <class Row, class Sees>
+  __device__ __forceinline__ WideQueries(Row row, Sees sees, bool vec, char*) {
+    const int lane = lane_id();
+    const bool live = sees(lane % 16);
+    const uint16_t* p = row(live ? lane % 16 : 0) + lane / 16 * (D / 4);
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) q[i] = load_q8(p + 8 * i, vec, live);
+  }
+  __device__ __forceinline__ void scores(const Block<D, 16>& kb,
+                                         F4 (&s)[2]) const {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      s[t] = F4{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < kStep; ++i)
+        s[t] = mma16<kHalf>(widen<kHalf>(kb.k[t][i], kb.scale(t, i)), q[i],
+                            s[t]);
+    }
+  }
+};
+
+// Which of a tile's rows take a block: all of them.
+struct AllRows {
+  __device__ __forceinline__ bool whole() const { return true; }
+  __device__ __forceinline__ bool lanes() const { return true; }
+};
+
+// Which blocks a wave of attend16 takes: each(a, wk, bytes, body) calls
+// body(block, index, rows, kdone, vdone); rows.whole() is whether all of the tile's
+// rows take the block, rows.lanes() whether the lane's does.  Here blocks first,
+// first + kWaves, ... of a split, by all rows.
 struct SplitBlocks {
   int splits, first, last;
   __device__ __forceinline__ SplitBlocks(const AttendArgs& a, const Work& wk,
@@ -575,21 +612,21 @@ struct SplitBlocks {
   }
   template <class B, class F>
   __device__ __forceinline__ void each(const AttendArgs& a, const Work& wk,
-                                       int bytes, int vis, F body) const {
+                                       int bytes, F body) const {
     each_block<B>(a.c, wk.b, wk.h, bytes, first, last,
                   [&](B& x, int blk, auto kdone, auto vdone) {
-                    body(x, blk, vis, true, kdone, vdone);
+                    body(x, blk, AllRows(), kdone, vdone);
                   });
   }
 };
 
 // 16 query rows from row0 on, of which those from `end` on are no queries; nor
 // are rows 16 .. kTileRows of the workgroup's tile.
-template <int D, bool kHalf, int kTileRows, class Blocks, class A, class S>
+template <int D, bool kHalf, int kTileRows, class Blocks,
+          class Queries = WideQueries<D, kHalf>, class A, class S>
 __device__ __forceinline__ void attend16(const A& a, const Work& wk,
                                          int64_t len, int64_t nq, int row0,
                                          int end, S& lds) {
-  constexpr int kStep = D / 32;   // matrix instructions a score tile
   constexpr int kDt = D / 16;     // channel tiles
   const int lane = lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -600,13 +637,12 @@ __device__ __forceinline__ void attend16(const A& a, const Work& wk,
   auto& sl = lds.l;
   auto& sc = lds.scales;
   const int vis = row0 + col < end ? visible(a, len, nq, row0 + col) : 0;
-  U4 qf[kStep];
-  {
-    const uint16_t* p =
-        q_row(a, wk.b, wk.h, vis ? row0 + col : 0) + quad * (D / 4);
-#pragma unroll
-    for (int i = 0; i < kStep; ++i) qf[i] = load_q8(p + 8 * i, a.vec, vis > 0);
-  }
+  const Queries qs(
+      [&](int r) { return q_row(a, wk.b, wk.h, row0 + r); },
+      [&](int r) {
+        return row0 + r < end && visible(a, len, nq, row0 + r) > 0;
+      },
+      a.vec, lds.pool);
   int most = vis, least = vis ? vis : 0x7fffffff;
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) {
@@ -623,18 +659,13 @@ __device__ __forceinline__ void attend16(const A& a, const Work& wk,
   for (int d = 0; d < kDt; ++d) o[d] = F4{0, 0, 0, 0};
 
   blocks.template each<Block<D, 16>>(
-      a, wk, KvLayout<D>::kBytes, vis,
-      [&](Block<D, 16>& kb, int blk, int v, bool whole, auto kdone, auto vdone) {
+      a, wk, KvLayout<D>::kBytes,
+      [&](Block<D, 16>& kb, int blk, auto rows, auto kdone, auto vdone) {
     share_scales(kb.vs, most - blk * kKvBlock, sc[wave], &inv);
     const int p0 = blk * kKvBlock + 16 * (quad / 2) + 4 * (quad % 2);
-    const bool edge = blk * kKvBlock + kKvBlock > least || !whole;
-    F4 s[2] = {F4{0, 0, 0, 0}, F4{0, 0, 0, 0}};
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < kStep; ++i)
-        s[t] = mma16<kHalf>(widen<kHalf>(kb.k[t][i], kb.scale(t, i)), qf[i],
-                            s[t]);
+    const bool edge = blk * kKvBlock + kKvBlock > least;
+    F4 s[2];
+    qs.scores(kb, s);
     kdone();
     F4 ls[2], rs[2];
 #pragma unroll
@@ -653,7 +684,13 @@ __device__ __forceinline__ void attend16(const A& a, const Work& wk,
       asm volatile("");  // a branch: most blocks have no edge
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (p0 + 8 * (j / 4) + j % 4 >= v) y[j] = kNegInf;
+        if (p0 + 8 * (j / 4) + j % 4 >= vis) y[j] = kNegInf;
+    }
+    if (!rows.whole()) {
+      asm volatile("");
+      const bool in = rows.lanes();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = in ? y[j] : kNegInf;
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = fmaxf(top, y[j]);
@@ -689,16 +726,12 @@ __device__ __forceinline__ void attend16(const A& a, const Work& wk,
     float lx = 0.0f;
     ml = kNegInf;
     blocks.template each<Block<D, 16>>(
-        a, wk, KvLayout<D>::kBytes, vis,
-        [&](Block<D, 16>& kb, int blk, int v, bool, auto kdone, auto) {
+        a, wk, KvLayout<D>::kBytes,
+        [&](Block<D, 16>& kb, int blk, auto rows, auto kdone, auto) {
+      const int v = rows.lanes() ? vis : 0;
       const int p0 = blk * kKvBlock + 16 * (quad / 2) + 4 * (quad % 2);
-      F4 s[2] = {F4{0, 0, 0, 0}, F4{0, 0, 0, 0}};
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < kStep; ++i)
-          s[t] = mma16<kHalf>(widen<kHalf>(kb.k[t][i], kb.scale(t, i)), qf[i],
-                              s[t]);
+      F4 s[2];
+      qs.scores(kb, s);
       kdone();
       sum_apart<16, 8>([&](int j, float less) {
         return p0 + 8 * (j / 4) + j % 4 < v
