@@ -758,8 +758,7 @@ int sfx_kv4_select(const sfx_kv4* cache, const sfx_kv4_bounds* bounds,
 /* sfx_kv4_attend over the positions of the blocks selected [batch, tokens,
  * heads, blocks] that each query sees.  In any order; an entry that names no
  * block of the table counts as none, a block named twice as one.  The products
- * of queries and keys, before `scale`, are sums in 32 bits; with heads of 128
- * and 256 a bfloat16 channel is taken to 2^-21 of the largest of its 32. */
+ * of queries and keys, before `scale`, are sums in 32 bits. */
 size_t sfx_kv4_attend_blocks_workspace_size(const sfx_kv4* cache,
                                             int64_t batch, int64_t tokens,
                                             int64_t q_heads, int64_t blocks);

@@ -113,9 +113,8 @@ def quantize_v(v):
     return np.where(finite, y, np.nan), top / 6
 
 
-def _attend_row(q, k, v, vscale, scale, q_step=0.0):
-    """One query head's (result, bound) over the tokens of k, v and vscale; q_step:
-    how far a channel of the query may be off, of the largest of its 32."""
+def _attend_row(q, k, v, vscale, scale):
+    """One query head's (result, bound) over the tokens of k, v and vscale."""
     kk, vv = k.astype(np.float64), v.astype(np.float64)
     qq = q.astype(np.float64)
     x = kk @ qq * scale
@@ -127,9 +126,6 @@ def _attend_row(q, k, v, vscale, scale, q_step=0.0):
     ls = np.abs(np.log2(vscale)) + 1
     ex = ((q.shape[-1] + 4) * 2.0 ** -24 * (np.abs(kk) @ np.abs(qq))
           * abs(scale) + (np.abs(x) * 2 + ls) * 2.0 ** -22).max()
-    if q_step:
-        most = np.abs(qq).reshape(-1, 32).max(axis=1).repeat(32)
-        ex += q_step * abs(scale) * (np.abs(kk) @ most).max()
     mass = w @ np.abs(vv)
     # float16 weights: 2^-11 relative (and as much again for approximations),
     # 2^-25 of the largest below its range
@@ -168,8 +164,7 @@ def ulp16(half: bool):
 BLOCK = 32
 
 
-def attend_blocks(q, selected, k, v, vscale, kv_len, q_len, scale=None,
-                  q_step=0.0):
+def attend_blocks(q, selected, k, v, vscale, kv_len, q_len, scale=None):
     """As attend, over the positions of selected [B, T, H, N] blocks; those that
     name no block of k's length count as none, those named twice as one."""
     b, t, hq, d = q.shape
@@ -188,7 +183,7 @@ def attend_blocks(q, selected, k, v, vscale, kv_len, q_len, scale=None,
                 if at:
                     out[i, j, a], bound[i, j, a] = _attend_row(
                         q[i, j, a], k[i, at, a // g], v[i, at, a // g],
-                        vscale[i, at, a // g, 0], scale, q_step)
+                        vscale[i, at, a // g, 0], scale)
     return out, bound
 
 

@@ -559,34 +559,6 @@ constexpr int kLds32 = kWaves * 32 * (64 + 4) * 4 > 32 * D * 2
                            ? kWaves * 32 * (64 + 4) * 4
                            : 32 * D * 2;
 
-// A wave's 16 query rows and their products with a block's keys: here as 16-bit
-// operands.  row(r): the address of the tile's row r, sees(r): whether it sees a
-// position; pool: LDS of the workgroup, free again after the constructor.
-template <int D, bool kHalf>
-struct WideQueries {
-  static constexpr int kStep = D / 32;  // matrix instructions a score tile
-  U4 q[kStep];
-  template <class Row, class Sees>
-  __device__ __forceinline__ WideQueries(Row row, Sees sees, bool vec, char*) {
-    const int lane = lane_id();
-    const bool live = sees(lane % 16);
-    const uint16_t* p = row(live ? lane % 16 : 0) + lane / 16 * (D / 4);
-#pragma unroll
-    for (int i = 0; i < kStep; ++i) q[i] = load_q8(p + 8 * i, vec, live);
-  }
-  __device__ __forceinline__ void scores(const Block<D, 16>& kb,
-                                         F4 (&s)[2]) const {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      s[t] = F4{0, 0, 0, 0};
-#pragma unroll
-      for (int i = 0; i < kStep; ++i)
-        s[t] = mma16<kHalf>(widen<kHalf>(kb.k[t][i], kb.scale(t, i)), q[i],
-                            s[t]);
-    }
-  }
-};
-
 // Which of a tile's rows take a block: all of them.
 struct AllRows {
   __device__ __forceinline__ bool whole() const { return true; }
@@ -622,11 +594,11 @@ struct SplitBlocks {
 
 // 16 query rows from row0 on, of which those from `end` on are no queries; nor
 // are rows 16 .. kTileRows of the workgroup's tile.
-template <int D, bool kHalf, int kTileRows, class Blocks,
-          class Queries = WideQueries<D, kHalf>, class A, class S>
+template <int D, bool kHalf, int kTileRows, class Blocks, class A, class S>
 __device__ __forceinline__ void attend16(const A& a, const Work& wk,
                                          int64_t len, int64_t nq, int row0,
                                          int end, S& lds) {
+  constexpr int kStep = D / 32;   // matrix instructions a score tile
   constexpr int kDt = D / 16;     // channel tiles
   const int lane = lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -637,12 +609,13 @@ __device__ __forceinline__ void attend16(const A& a, const Work& wk,
   auto& sl = lds.l;
   auto& sc = lds.scales;
   const int vis = row0 + col < end ? visible(a, len, nq, row0 + col) : 0;
-  const Queries qs(
-      [&](int r) { return q_row(a, wk.b, wk.h, row0 + r); },
-      [&](int r) {
-        return row0 + r < end && visible(a, len, nq, row0 + r) > 0;
-      },
-      a.vec, lds.pool);
+  U4 qf[kStep];
+  {
+    const uint16_t* p =
+        q_row(a, wk.b, wk.h, vis ? row0 + col : 0) + quad * (D / 4);
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) qf[i] = load_q8(p + 8 * i, a.vec, vis > 0);
+  }
   int most = vis, least = vis ? vis : 0x7fffffff;
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) {
@@ -664,8 +637,13 @@ __device__ __forceinline__ void attend16(const A& a, const Work& wk,
     share_scales(kb.vs, most - blk * kKvBlock, sc[wave], &inv);
     const int p0 = blk * kKvBlock + 16 * (quad / 2) + 4 * (quad % 2);
     const bool edge = blk * kKvBlock + kKvBlock > least;
-    F4 s[2];
-    qs.scores(kb, s);
+    F4 s[2] = {F4{0, 0, 0, 0}, F4{0, 0, 0, 0}};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < kStep; ++i)
+        s[t] = mma16<kHalf>(widen<kHalf>(kb.k[t][i], kb.scale(t, i)), qf[i],
+                            s[t]);
     kdone();
     F4 ls[2], rs[2];
 #pragma unroll
@@ -730,8 +708,13 @@ __device__ __forceinline__ void attend16(const A& a, const Work& wk,
         [&](Block<D, 16>& kb, int blk, auto rows, auto kdone, auto) {
       const int v = rows.lanes() ? vis : 0;
       const int p0 = blk * kKvBlock + 16 * (quad / 2) + 4 * (quad % 2);
-      F4 s[2];
-      qs.scores(kb, s);
+      F4 s[2] = {F4{0, 0, 0, 0}, F4{0, 0, 0, 0}};
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < kStep; ++i)
+          s[t] = mma16<kHalf>(widen<kHalf>(kb.k[t][i], kb.scale(t, i)), qf[i],
+                              s[t]);
       kdone();
       sum_apart<16, 8>([&](int j, float less) {
         return p0 + 8 * (j / 4) + j % 4 < v

@@ -5,7 +5,6 @@
 // much the same blocks, each of which is then loaded and converted once.
 
 #include <algorithm>
-#include <type_traits>
 
 #include "kv4_attend.h"
 #include "launch.h"
@@ -257,121 +256,6 @@ struct TileList {
   }
 };
 
-// Query rows in bfloat16 for products with the keys as the 4 bits stand: the matrix
-// instruction of 128 channels takes 4-bit values and the power of two that 32 of
-// them share, so no key is converted; a query is the sum of two 8-bit numbers
-// (e4m3) of four digits each, the second 2^-4 of the first.  32 channels have their
-// power of two, with which the largest lies in [2^7, 2^8) of the numbers' 448: what
-// falls below the second numbers' steps is less than 2^-21 of that.  The matrix units
-// take for it a fifth less than for 16 bits, the vector units, which bound these
-// kernels, 34 instructions a block less of 160: 2,048 tokens of a prompt with 64 blocks
-// of 512 each take 143 us instead of 158, 64 x 17 tokens 42 instead of 45, 1,024 of a
-// prompt with heads of 256 123 instead of 126, single tokens the same.  float16 has 11
-// digits: three numbers give nothing (77 us and 76).
-//
-// Operands (16 x 16 x 128): lane 16 p + i has channels 32 p .. 32 p + 31 of key i
-// and the power of two of the same of query row i, but of the row's numbers those of
-// channels 16 p .. 16 p + 15 and 64 + 16 p .. 64 + 16 p + 15.  With heads of 256 a
-// lane's keys are channels 64 p .. 64 p + 63, half of them a step.
-typedef int I8 __attribute__((ext_vector_type(8)));
-
-template <int D>
-struct NarrowQueries {
-  static constexpr int kStep = D / 128, kTerm = 2;
-  I8 q[kStep][kTerm];
-  int scale[kStep];  // a byte for each of the numbers
-  // A thread of the workgroup works on eight channels of a row.
-  template <class Row, class Sees>
-  __device__ __forceinline__ NarrowQueries(Row row, Sees sees, bool vec,
-                                           char* pool) {
-    int* const scales = (int*)(pool + kStep * kTerm * 2048);
-    const int r = (int)threadIdx.x / 16;
-    const bool live = sees(r);
-    const uint16_t* from = row(live ? r : 0);
-#pragma unroll
-    for (int i = 0; i < kStep; ++i) {
-      const int ch = ((int)threadIdx.x % 16 + 16 * i) * 8, n = ch / 32;
-      const int step = n % kStep, k = n / kStep * 32 + ch % 32;
-      const U4 w = load_q8(from + ch, vec, live);
-      // the largest magnitude of the 32, as bits
-      int top = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        top = max(top, (int)max(w[j] & 0x7fffu, w[j] >> 16 & 0x7fffu));
-      top = max(top, __builtin_amdgcn_mov_dpp(top, 0xb1, 0xf, 0xf, true));
-      top = max(top, __builtin_amdgcn_mov_dpp(top, 0x4e, 0xf, 0xf, true));
-      // its exponent, no lower than what the numbers' scales reach (whose NaN
-      // stands for that and for infinities)
-      int x = __builtin_amdgcn_frexp_expf(
-                  to_float16b<false>((uint32_t)max(top, 1))) - 1;
-      x = max(x, -108);
-      const int e = x + 120;
-      if (ch % 32 == 0)
-        scales[step * 64 + k / 32 * 16 + r] =
-            top >= 0x7f80 ? 0xffff : e | (e - 4) << 8;
-      float v[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        v[j] = __builtin_amdgcn_ldexpf(
-            to_float16b<false>(j % 2 ? w[j / 2] >> 16 : w[j / 2] & 0xffffu),
-            7 - x);
-      char* to = pool + step * kTerm * 2048 + k / 64 * 1024 +
-                 (k % 64 / 16 * 16 + r) * 16 + k % 16;
-#pragma unroll
-      for (int t = 0; t < kTerm; ++t) {
-        int y[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          y[j] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * j], v[4 * j + 1], 0,
-                                                 false);
-          y[j] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * j + 2], v[4 * j + 3],
-                                                 y[j], true);
-          const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(y[j], false);
-          const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(y[j], true);
-          v[4 * j] = (v[4 * j] - lo[0]) * 16.0f;
-          v[4 * j + 1] = (v[4 * j + 1] - lo[1]) * 16.0f;
-          v[4 * j + 2] = (v[4 * j + 2] - hi[0]) * 16.0f;
-          v[4 * j + 3] = (v[4 * j + 3] - hi[1]) * 16.0f;
-        }
-        *(int2*)(to + t * 2048) = int2{y[0], y[1]};
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kStep; ++i) {
-      scale[i] = scales[i * 64 + lane_id()];
-#pragma unroll
-      for (int t = 0; t < kTerm; ++t) {
-        const char* at = pool + (i * kTerm + t) * 2048 + lane_id() * 16;
-        const int4 a = *(const int4*)at, b = *(const int4*)(at + 1024);
-        q[i][t] = I8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-      }
-    }
-    __syncthreads();
-  }
-  template <int kTile, int kAt>
-  __device__ __forceinline__ F4 product(const Block<D, 16>& kb, F4 c) const {
-    constexpr int i = kAt / kTerm, t = kAt % kTerm;
-    const auto& w = kb.k[kTile];
-    const I8 k = {(int)w[4 * i], (int)w[4 * i + 1], (int)w[4 * i + 2],
-                  (int)w[4 * i + 3]};
-    // 4: the first operand's type; the scales' bytes i and t
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-        k, q[i][t], c, 4, 0, i, (int)kb.ks[kTile], t, scale[i]);
-  }
-  template <int kAt = 0>
-  __device__ __forceinline__ void scores(const Block<D, 16>& kb,
-                                         F4 (&s)[2]) const {
-    if constexpr (kAt == 0) s[0] = s[1] = F4{0, 0, 0, 0};
-    if constexpr (kAt < kStep * kTerm) {
-      // one tile after the other: a product does not wait for the last
-      s[0] = product<0, kAt>(kb, s[0]);
-      s[1] = product<1, kAt>(kb, s[1]);
-      scores<kAt + 1>(kb, s);
-    }
-  }
-};
-
 template <int D, bool kHalf, class List>
 __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 4)
 void k_kv4_attend_blocks(ListArgs a) {
@@ -395,11 +279,7 @@ void k_kv4_attend_blocks(ListArgs a) {
     }
     return;
   }
-  // (of 64 channels the instruction would be half empty)
-  using Queries =
-      std::conditional_t<kHalf || D == 64, WideQueries<D, kHalf>,
-                         NarrowQueries<D == 64 ? 128 : D>>;
-  attend16<D, kHalf, 16, List, Queries>(a, wk, len, nq, row0, end, lds);
+  attend16<D, kHalf, 16, List>(a, wk, len, nq, row0, end, lds);
 }
 
 template <int D, bool kHalf>
