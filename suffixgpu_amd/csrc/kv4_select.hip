@@ -10,6 +10,14 @@
 // units of a power of two), so it has one value whatever the order of its sums,
 // and a selection has one right answer.  The sums are below 2^22 and exact as
 // floats; times the power of two they rank the blocks.
+//
+// Scores are matrix instructions on a few bytes each; what bounds the selection is
+// the choice, vector and scalar instructions that depend on each other.  It is made
+// where the keys are: in LDS and a wave's registers for rows of up to 1,024 blocks (64
+// x 1 tokens over up to 32,768 29 us a call, with the scores in memory and a second
+// launch 54; 64 x 17 over up to 8,192 16 and 50; a prompt's 2,048 over 16,384 40 and
+// 113), in a workgroup's registers past that (one token over 131,072 5.9 + 8.7 us,
+// 4 x 9 with heads of 256 15.8 + 13), and in memory past 16,384 blocks.
 
 #include <algorithm>
 
@@ -36,7 +44,8 @@ struct BoundsArgs {
 typedef float F2 __attribute__((ext_vector_type(2)));
 
 // A wave per block of 32 positions, KV head and row: a lane has eight channels of
-// every 512 / D-th token.
+// every 512 / D-th token.  A step's new tokens: 4 to 5 us, a launch's latency; a
+// prompt's 14,336 tokens 9 MB (every block's keys once).
 template <int D>
 __global__ __launch_bounds__(kWave) void k_kv4_bounds(BoundsArgs a) {
   using L = KvLayout<D>;
@@ -363,7 +372,8 @@ __global__ __launch_bounds__(kSelectThreads) void k_kv4_scores(SelectArgs a) {
 // kRegs of them in each lane: the least key that is taken, from counts of 64 equal
 // parts of the keys' range and then bit by bit, until as many as are wanted lie past
 // it; then the blocks past it, and those at it while there is room.
-// bins: 64 words of the wave's own.
+// bins: 64 words of the wave's own.  Bit by bit from the start 64 x 17 tokens take 18.4 us,
+// 2,048 of a prompt 44, with the counts first 16.2 and 40.
 template <int kRegs>
 __device__ __forceinline__ void pick_blocks(int sinks, int recent, int all,
                                             int last, const uint32_t* key,
@@ -515,7 +525,9 @@ struct WideList {
 };
 
 // As pick_blocks, the keys of up to 1,024 kRegs blocks in the workgroup's
-// registers; two bits of the line at a time, as each step is a barrier.
+// registers; two bits of the line at a time, as each step is a barrier (a bit at a
+// time, with the scores in shorter pieces, one token over 131,072 took 20 us instead of
+// 16, 4 x 9 36 instead of 28).
 template <int kRegs>
 __global__ __launch_bounds__(kWideThreads) void k_kv4_pick_wide(SelectArgs a) {
   // (16 waves: a row of a wave's lanes sums up one number of each)

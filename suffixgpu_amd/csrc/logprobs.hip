@@ -11,6 +11,14 @@
 // 64 parts reach, and few more: the n largest, and few others.  The second launch
 // joins a position's parts and ranks what is left of those.
 // Positions without a token leave at once.
+//
+// Memory bounds it where there are no alternatives: 2,048 positions of 128,256
+// bfloat16 logits take 103 us, 5.1 TB/s.  With alternatives it is the vector
+// instructions, 17 a logit with one (116 to 128 us) and 20 with twenty: 256 positions
+// 30 us, 66 MB at 2.2 TB/s, 19 without any.  8,192 logits a workgroup are 32 a lane,
+// which is what stays in registers beside the rest with seven waves a SIMD; for eight
+// the compiler spills.  One position of 32,000 is the latency of the two launches
+// (5.2 + 4.5 us).
 
 #include <algorithm>
 
