@@ -44,9 +44,9 @@ __device__ __forceinline__ int end_row(const ListArgs& a, int qt) {
 }
 
 // The blocks that any token of a tile has in its list, in order, with the rows of
-// the tokens that take them (a bit each), by a workgroup: a window of the row's blocks at a
-// time, of which each token has a bit for each, so that a block named twice is
-// one.  4,096 tiles of four tokens with 64 blocks each of 512: 12 us.
+// the tokens that take them (a bit each), by a workgroup: a window of the row's
+// blocks at a time, of which each token has a bit for each, so that a block named
+// twice is one.  4,096 tiles of four tokens with 64 blocks each of 512: 12 us.
 // 1,024 threads for rows that a window of 256 does not span: 32 of eight tokens with
 // 96 blocks each of up to 4,096 take 7.5 us, by 256 threads 9.
 template <int kUnionThreads>
@@ -274,8 +274,8 @@ void k_kv4_attend_blocks(ListArgs a) {
   const int64_t len = kv_len_of(a, wk.b), nq = q_len_of(a, wk.b);
   const int row0 = first_row(a, wk.qt), end = end_row(a, wk.qt);
   // the last token sees the most
-  if (visible(a, len, nq, std::min<int64_t>(end, nq * a.group) - 1) == 0 ||
-      nq * a.group <= row0) {
+  const int live = (int)min(nq, a.tokens) * a.group;
+  if (live <= row0 || visible(a, len, nq, min(end, live) - 1) == 0) {
     // no queries: what is split is the join's
     if (a.splits == 1) {
       const int n = min(16, end - row0);

@@ -163,6 +163,23 @@ def test_head_groups_and_scales(gpu, dtype, d, heads, group, t, n, scale):
     assert torch.equal(out, c.attend_blocks(q, sel, table, kv, None, scale))
 
 
+@pytest.mark.parametrize("t,group", [(1, 4), (3, 2), (2, 20)])
+def test_lengths_far_past_the_table(gpu, t, group):
+    """Where a query stands is kv_len - q_len, whatever these are."""
+    c, table, kq, vq, vs = filled(gpu, 2, [150, 90], 1, 64, 32, BF, 72)
+    q = data(gpu, 2, t, group, 64, BF, 73)
+    lens = [150, 90]
+    near = (ints(lens, gpu, torch.int64), ints([t, t], gpu, torch.int64))
+    sel = c.select_blocks(q, table, near[0], near[1], 3, 0, 1)
+    out = c.attend_blocks(q, sel, table, *near)
+    check_blocks(out, q, sel, kq, vq, vs, lens, [t] * 2, BF)
+    # (the same queries as the first t of a row's 2^62 and more)
+    big = 2 ** 62
+    far = (near[0] + big, near[1] + big)
+    assert torch.equal(c.select_blocks(q, table, *far, 3, 0, 1), sel)
+    assert torch.equal(c.attend_blocks(q, sel, table, *far), out)
+
+
 def test_tables_and_pools_of_nothing(gpu):
     from suffixgpu_amd import KV4Cache, PagePool
     q = data(gpu, 2, 3, 4, 64, BF, 80)
