@@ -11,13 +11,16 @@
 // and a selection has one right answer.  The sums are below 2^22 and exact as
 // floats; times the power of two they rank the blocks.
 //
-// Scores are matrix instructions on a few bytes each; what bounds the selection is
-// the choice, vector and scalar instructions that depend on each other.  It is made
-// where the keys are: in LDS and a wave's registers for rows of up to 1,024 blocks (64
-// x 1 tokens over up to 32,768 29 us a call, with the scores in memory and a second
-// launch 54; 64 x 17 over up to 8,192 16 and 50; a prompt's 2,048 over 16,384 40 and
-// 113), in a workgroup's registers past that (one token over 131,072 5.9 + 8.7 us,
-// 4 x 9 with heads of 256 15.8 + 13), and in memory past 16,384 blocks.
+// What bounds it are the steps that follow each other in a workgroup, all of which
+// run at once: the query's packing, the scores (64 x 1 tokens over up to 32,768 read
+// 72 MB of bounds), the choice, of which the search for the least score taken is 2 of
+// 29 us there and 2.5 of 40 for a prompt's 2,048 tokens over 16,384 (vector
+// instructions 52% of the cycles).  It is made where the scores are: in LDS and a
+// wave's registers for rows of up to 1,024 blocks (29 us a call, with the scores in
+// memory and a second launch 54; 64 x 17 over up to 8,192 16 and 50; the prompt 40
+// and 113), in a workgroup's registers past that (one token over 131,072 5.9 + 8.7 us,
+// 4 x 9 with heads of 256 15.8 + 13), and in memory past 16,384 blocks.  Bounds two
+// steps ahead instead of one take registers that leave five waves a SIMD of seven.
 
 #include <algorithm>
 
