@@ -46,9 +46,11 @@ __device__ __forceinline__ int end_row(const ListArgs& a, int qt) {
 // The blocks that any token of a tile has in its list, in order, with the rows of
 // the tokens that take them (a bit each), by a workgroup: a window of the row's
 // blocks at a time, of which each token has a bit for each, so that a block named
-// twice is one.  4,096 tiles of four tokens with 64 blocks each of 512: 12 us.
-// 1,024 threads for rows that a window of 256 does not span: 32 of eight tokens with
-// 96 blocks each of up to 4,096 take 7.5 us, by 256 threads 9.
+// twice is one.
+// 1,024 threads for rows that a window of 256 does not span: 32 tiles of eight tokens
+// with 96 blocks each of up to 4,096 take 7.5 us, by 256 threads 9.  64 where there
+// are many tiles and a window of 64 spans the rows: 4,096 of four tokens with 64 blocks
+// each of 512 take 8 us, by 256 threads 12, but 384 of two tokens with 48 each 0.7 more.
 template <int kUnionThreads>
 __global__ __launch_bounds__(kUnionThreads) void k_kv4_union(ListArgs a) {
   constexpr int kWindow = 8 * kUnionThreads;  // eight blocks a thread
@@ -360,7 +362,10 @@ int launch(const ListArgs& a, hipStream_t stream) {
                        stream, a);
   } else {
     const dim3 tiles((unsigned)(a.batch * a.c.heads * a.q_tiles));
-    if (a.c.positions / kKvBlock <= 2048)
+    const int64_t blocks = a.c.positions / kKvBlock;
+    if (blocks <= 512 && tiles.x >= 2048)
+      hipLaunchKernelGGL(k_kv4_union<64>, tiles, dim3(64), 0, stream, a);
+    else if (blocks <= 2048)
       hipLaunchKernelGGL(k_kv4_union<256>, tiles, dim3(256), 0, stream, a);
     else
       hipLaunchKernelGGL(k_kv4_union<1024>, tiles, dim3(1024), 0, stream, a);
