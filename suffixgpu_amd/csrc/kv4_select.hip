@@ -537,11 +537,15 @@ __global__ __launch_bounds__(kWideThreads) void k_kv4_pick_wide(SelectArgs a) {
   static_assert(kWideWaves == 16, "");
   __shared__ uint32_t of_wave[3][4][kWideWaves];
   __shared__ uint32_t at[kRegs * kWideWaves];  // past the line, and on it << 16
+  __shared__ __align__(16) uint32_t bins[kWideThreads];
+  __shared__ uint32_t line_bin[3], cand[kWave], cands;
   const int tid = threadIdx.x, lane = lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const WideList l(a);
   uint32_t k[kRegs], sure = 0, hi = 0, lo = 0;
   uint32_t n_sure = 0, n_some = 0;
+  bins[tid] = 0;
+  if (tid == 0) cands = 0;
 #pragma unroll
   for (int i = 0; i < kRegs; ++i) {
     const int j = i * kWideThreads + tid;
@@ -602,28 +606,83 @@ __global__ __launch_bounds__(kWideThreads) void k_kv4_pick_wide(SelectArgs a) {
   if (want <= 0) {
     line = 0xffffffffu;
   } else if (some > want) {
-    // (an even number of bits is left)
-    int bit = (31 - __builtin_clz((hi ^ lo) | 1u)) & ~1;
-    line = bit < 30 ? hi >> (bit + 2) << (bit + 2) : 0;
-    bool exact = false;
-    for (; bit >= 0 && !exact; bit -= 2) {
-      const uint32_t step = 1u << bit;
-      int n[3];
-      at_least(line + step, step, n);
-      uint32_t past = 0;
+    const int shift = max(0, 22 - __builtin_clz((hi - lo) | 1u));
 #pragma unroll
-      for (int s = 0; s < 3; ++s) {
-        if (n[s] >= want) past = (uint32_t)(s + 1) * step;
-        exact = exact || n[s] == want;
+    for (int i = 0; i < kRegs; ++i)
+      if (k[i]) atomicAdd(&bins[(k[i] - lo) >> shift], 1u);
+    __syncthreads();
+    if (wave == 0) {
+      // a lane's 16 parts, the largest keys first
+      uint32_t x[16], n = 0;
+      const uint4* p = (const uint4*)bins + (kWave - 1 - lane) * 4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint4 v = p[3 - i];
+        x[4 * i] = v.w;
+        x[4 * i + 1] = v.z;
+        x[4 * i + 2] = v.y;
+        x[4 * i + 3] = v.x;
+        n += v.x + v.y + v.z + v.w;
       }
-      line += past;
+      int upto = (int)(wave_incl_scan(n) - n);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int next = upto + (int)x[i];
+        if (upto < want && next >= want) {
+          line_bin[0] = (uint32_t)(kWideThreads - 1 - lane * 16 - i);
+          line_bin[1] = (uint32_t)upto;
+          line_bin[2] = (uint32_t)next;
+        }
+        upto = next;
+      }
+    }
+    __syncthreads();
+    const uint32_t bin = line_bin[0];
+    const int past = (int)line_bin[1], upto = (int)line_bin[2];
+    line = lo + (bin << shift);
+    bool exact = upto == want;
+    if (!exact && upto - past <= kWave) {
+      // a wave's lanes hold what lies in that part
+#pragma unroll
+      for (int i = 0; i < kRegs; ++i)
+        if (k[i] && (k[i] - lo) >> shift == bin)
+          cand[atomicAdd(&cands, 1u)] = k[i];
+      __syncthreads();
+      const uint32_t x = lane < upto - past ? cand[lane] : 0;
+      int n = upto;
+      for (int bit = shift - 1; bit >= 0 && n != want; --bit) {
+        const uint32_t y = line + (1u << bit);
+        const int c = past + popc(ballot(x >= y));
+        if (c >= want) {
+          line = y;
+          n = c;
+        }
+      }
+      exact = n == want;
+      room = want - past - popc(ballot(x > line));
+    } else if (!exact) {
+      // many equal or nearly equal keys; (an even number of bits is left)
+      for (int bit = (shift - 1) & ~1; bit >= 0 && !exact; bit -= 2) {
+        const uint32_t step = 1u << bit;
+        int n[3];
+        at_least(line + step, step, n);
+        uint32_t more = 0;
+#pragma unroll
+        for (int s = 0; s < 3; ++s) {
+          if (n[s] >= want) more = (uint32_t)(s + 1) * step;
+          exact = exact || n[s] == want;
+        }
+        line += more;
+      }
+      if (!exact) {
+        int n[3];
+        at_least(line + 1, 0, n);
+        room = want - n[0];
+      }
     }
     if (exact) {
       --line;  // those past it now are the wanted ones
-    } else {
-      int n[3];
-      at_least(line + 1, 0, n);
-      room = want - n[0];
+      room = 0;
     }
   }
 #pragma unroll
