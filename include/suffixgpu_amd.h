@@ -742,9 +742,10 @@ int sfx_kv4_bounds_update(const sfx_kv4* cache, const sfx_kv4_bounds* bounds,
  * the same power of two, 1 or more, that leaves 7 bits, halves up, at most 127.
  * selected [batch, tokens, heads, blocks]: positions / 32, ascending, -1 behind
  * them and for what is no query.  1 <= recent, first + recent <= blocks.
- * workspace: sfx_kv4_select_workspace_size bytes (none for tables of up to 1,024
- * blocks, past that 4 for each query token, KV head and block), 16-byte aligned,
- * of any content; calls that may overlap have their own. */
+ * workspace: sfx_kv4_select_workspace_size bytes (none for tables of up to 512
+ * blocks, nor of up to 1,024 and more than 256 lists, otherwise 4 for each list and
+ * block), 16-byte aligned, of any content; calls that may overlap have their
+ * own. */
 size_t sfx_kv4_select_workspace_size(const sfx_kv4* cache, int64_t batch,
                                      int64_t tokens);
 int sfx_kv4_select(const sfx_kv4* cache, const sfx_kv4_bounds* bounds,

@@ -11,16 +11,15 @@
 // and a selection has one right answer.  The sums are below 2^22 and exact as
 // floats; times the power of two they rank the blocks.
 //
-// What bounds it are the steps that follow each other in a workgroup, all of which
-// run at once: the query's packing, the scores (64 x 1 tokens over up to 32,768 read
-// 72 MB of bounds), the choice, of which the search for the least score taken is 2 of
-// 29 us there and 2.5 of 40 for a prompt's 2,048 tokens over 16,384 (vector
-// instructions 52% of the cycles).  It is made where the scores are: in LDS and a
-// wave's registers for rows of up to 1,024 blocks (29 us a call, with the scores in
-// memory and a second launch 54; 64 x 17 over up to 8,192 16 and 50; the prompt 40
-// and 113), in a workgroup's registers past that (one token over 131,072 5.9 + 8.7 us,
-// 4 x 9 with heads of 256 15.8 + 13), and in memory past 16,384 blocks.  Bounds two
-// steps ahead instead of one take registers that leave five waves a SIMD of seven.
+// What bounds it are the steps that follow each other in a workgroup, most of which
+// run at once: packing the query, the scores, the choice (vector instructions issue in
+// half of the cycles); with all rows full, the memory (64 x 1 tokens over 32,768 30 us,
+// 135 MB, 4.5 TB/s).  The choice is made where the scores are: in LDS and a wave's or a
+// workgroup's registers for rows of up to 1,024 blocks (64 x 1 tokens over up to 32,768
+// 26 us a call, with the scores in memory and a second launch 33; 64 x 17 over up to
+// 8,192 16 and 85; a prompt's 2,048 over 16,384 38 and 192), in the registers of a
+// workgroup of a second launch past that (one token over 131,072 11 us, 4 x 9 with heads
+// of 256 24), and in memory past 16,384 blocks.
 
 #include <algorithm>
 
@@ -268,8 +267,11 @@ __device__ __forceinline__ uint32_t score_key(int32_t dot, int unit) {
 // Scores of blocks [blk0, end) of row b and KV head h for its query tokens t0 ..
 // t0 + queries - 1 (packed into sq here, with zeros up to `rows`, a multiple of
 // 16), by a workgroup: put(query, block, keys) of four blocks each.  A wave takes
-// 16 blocks at a time; the next ones, and the places of those after them, are on
-// their way while these are used.
+// 16 blocks at a time, at most 8 times; the next ones are on their way while these
+// are used.  (Two and three ahead give nothing: 64 x 1 tokens 29 us, a prompt 42 and 44
+// instead of 38, as the registers leave fewer waves.  Places read one ahead, instead
+// of all at first, wait for the bounds before them: one token over 32,768 18.0 us, now
+// 16.1.)
 constexpr int kSelectThreads = 512;
 
 template <int D, bool kHalf, class Put>
@@ -281,22 +283,31 @@ __device__ __forceinline__ void score_blocks(
   const int lane = lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int i16 = lane % 16, quad = lane / 16;
-  // (in 32 bits: a pool of 2^31 blocks would be 4 TB)
-  auto place = [&](int blk) {
-    return blk < end ? (int)kv_place(a.c, b, h, blk + i16) : -1;
-  };
-  I4 r[kStep];
-  int unit;
-  auto load = [&](int at) {
-    unit = at < 0 ? kNoPage : a.unit[at];
-    const I4* p =
-        (const I4*)(a.range + (int64_t)(at < 0 ? 0 : at) * (2 * D)) + quad;
-#pragma unroll
-    for (int i = 0; i < kStep; ++i) r[i] = at < 0 ? I4{0, 0, 0, 0} : p[4 * i];
-  };
+  // Places and units of all the wave's blocks, 16 i + j of them in lane 16 (i % 4) +
+  // j: their loads wait for each other once.  (In 32 bits: a pool of 2^31 blocks would
+  // be 4 TB.)
   constexpr int kAll = kSelectWaves * 16;
-  load(place(blk0 + wave * 16));
-  int next = place(blk0 + wave * 16 + kAll);
+  int at[2], unit[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int blk = blk0 + (wave + (4 * i + quad) * kSelectWaves) * 16 + i16;
+    at[i] = blk < end ? (int)kv_place(a.c, b, h, blk) : -1;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) unit[i] = at[i] < 0 ? kNoPage : a.unit[at[i]];
+  auto of_turn = [&](const int (&x)[2], int turn, int j) {
+    return __shfl(turn < 4 ? x[0] : x[1], turn % 4 * 16 + j);
+  };
+  I4 r[2][kStep];
+  auto load = [&](int set, int turn) {
+    const int from = turn < 8 ? of_turn(at, turn, i16) : -1;
+    const I4* p =
+        (const I4*)(a.range + (int64_t)(from < 0 ? 0 : from) * (2 * D)) + quad;
+#pragma unroll
+    for (int i = 0; i < kStep; ++i)
+      r[set][i] = from < 0 ? I4{0, 0, 0, 0} : p[4 * i];
+  };
+  load(0, 0);
   {
     typedef PackQuery<D, kHalf> Pack;
     Pack now;
@@ -314,26 +325,31 @@ __device__ __forceinline__ void score_blocks(
     }
   }
   __syncthreads();
-  for (int blk = blk0 + wave * 16; blk < end; blk += kAll) {
-    I4 now[kStep];
-#pragma unroll
-    for (int i = 0; i < kStep; ++i) now[i] = r[i];
+  int turn = 0, blk = blk0 + wave * 16;
+  auto step = [&](int set) {
+    load(1 - set, turn + 1);
     int us[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) us[e] = __shfl(unit, quad * 4 + e);
-    load(next);
-    next = place(blk + 2 * kAll);
+    for (int e = 0; e < 4; ++e) us[e] = of_turn(unit, turn, quad * 4 + e);
     for (int q0 = 0; q0 < queries; q0 += 16) {
       I4 s = {0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < kStep; ++i)
         s = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-            now[i], *(const I4*)&sq[q0 + i16][i * 64 + quad * 16], s, 0, 0, 0);
+            r[set][i], *(const I4*)&sq[q0 + i16][i * 64 + quad * 16], s, 0, 0,
+            0);
       if (q0 + i16 < queries)
         put(q0 + i16, blk + quad * 4,
             uint4{score_key(s[0], us[0]), score_key(s[1], us[1]),
                   score_key(s[2], us[2]), score_key(s[3], us[3])});
     }
+    blk += kAll;
+    ++turn;
+  };
+  while (blk < end) {
+#pragma unroll
+    for (int set = 0; set < 2; ++set)
+      if (blk < end) step(set);
   }
 }
 
@@ -375,8 +391,9 @@ __global__ __launch_bounds__(kSelectThreads) void k_kv4_scores(SelectArgs a) {
 // kRegs of them in each lane: the least key that is taken, from counts of 64 equal
 // parts of the keys' range and then bit by bit, until as many as are wanted lie past
 // it; then the blocks past it, and those at it while there is room.
-// bins: 64 words of the wave's own.  Bit by bit from the start 64 x 17 tokens take 18.4 us,
-// 2,048 of a prompt 44, with the counts first 16.2 and 40.
+// bins: 64 words of the wave's own.  Bit by bit from the start 64 x 17 tokens take 18.4
+// us, 2,048 of a prompt 44, with the counts first 16.2 and 40; the keys of one part a
+// lane's each, as pick_together has them, changed neither.
 template <int kRegs>
 __device__ __forceinline__ void pick_blocks(int sinks, int recent, int all,
                                             int last, const uint32_t* key,
@@ -456,105 +473,44 @@ __device__ __forceinline__ void pick_blocks(int sinks, int recent, int all,
   for (int i = n + lane; i < all; i += kWave) out[i] = -1;
 }
 
-// Scores and choice at once, where a workgroup holds the keys of its tokens: rows
-// of up to 1,024 blocks.
-constexpr int kSelectTokens = 32;
+// As pick_blocks, by a workgroup with the keys of up to 64 kRegs kPickWaves blocks in
+// its registers.  Among 1,024 equal parts of the keys' range it looks for the one that
+// the line lies in, and the keys of that part, if they are no more than 64, are a
+// lane's each in every wave.  Two bits of the line at a time, a barrier each, one token
+// over 131,072 took 14.7 us and 4 x 9 29.7, now 11.2 and 23.9.
+constexpr int kParts = 1024;
 
-template <int D, bool kHalf>
-__global__ __launch_bounds__(kSelectThreads) void k_kv4_select(SelectArgs a) {
-  constexpr int kPitch = 2 * D + 16;
-  constexpr int kSelectWaves = kSelectThreads / kWave;
-  extern __shared__ __align__(16) char lds[];
-  __shared__ uint32_t bins[kSelectWaves][kWave];
-  // tiles of one row and KV head follow each other on one XCD (32 bits hold all
-  // of these)
-  const uint32_t k = blockIdx.x / 8;
-  const int tile = (int)(k % (uint32_t)a.tiles);
-  const uint32_t bh = k / (uint32_t)a.tiles * 8 + blockIdx.x % 8;
-  if (bh >= (uint32_t)a.batch * (uint32_t)a.c.heads) return;
-  const int64_t b = bh / (uint32_t)a.c.heads;
-  const int h = (int)(bh % (uint32_t)a.c.heads);
-  const int64_t len = kv_len_of(a, b), nq = q_len_of(a, b);
-  const int64_t t0 = (int64_t)tile * a.span;
-  const int tokens = (int)std::min<int64_t>(a.span, a.tokens - t0);
-  const int queries = (int)std::max<int64_t>(
-      0, std::min<int64_t>(tokens, nq - t0));
-  auto sq = (int8_t(*)[kPitch])lds;
-  // (rows 4 banks apart)
-  const int pitch = (int)a.pitch + 4;
-  uint32_t* keys = (uint32_t*)(lds + (a.span + 15) / 16 * 16 * kPitch);
-  const int blocks =
-      queries ? (token_sees(a, len, nq, t0 + queries - 1) + kKvBlock - 1) /
-                    kKvBlock
-              : 0;
-  score_blocks<D, kHalf>(a, b, h, t0, queries, (tokens + 15) / 16 * 16, 0,
-                         blocks, sq, [&](int q, int blk, uint4 key) {
-                           *(uint4*)(keys + q * pitch + blk) = key;
-                         });
-  __syncthreads();
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  for (int i = wave; i < tokens; i += kSelectWaves) {
-    const int last = __builtin_amdgcn_readfirstlane(
-        (token_sees(a, len, nq, t0 + i) + kKvBlock - 1) / kKvBlock - 1);
-    const uint32_t* own = keys + i * pitch;
-    int32_t* out =
-        a.selected + ((b * a.tokens + t0 + i) * a.c.heads + h) * a.want;
-    if (last < 4 * kWave)
-      pick_blocks<4>(a.sinks, a.recent, a.want, last, own, bins[wave], out);
-    else if (last < 8 * kWave)
-      pick_blocks<8>(a.sinks, a.recent, a.want, last, own, bins[wave], out);
-    else
-      pick_blocks<16>(a.sinks, a.recent, a.want, last, own, bins[wave], out);
-  }
-}
-
-// The choice by a workgroup of 1,024 threads, for rows whose keys are in memory.
-constexpr int kWideThreads = 1024;
-constexpr int kWideWaves = kWideThreads / kWave;
-
-struct WideList {
-  int last;
-  const uint32_t* keys;
-  int32_t* out;
-  __device__ __forceinline__ WideList(const SelectArgs& a) {
-    const uint32_t list = blockIdx.x, token = list / (uint32_t)a.c.heads;
-    const uint32_t b = token / (uint32_t)a.tokens;
-    const uint32_t t = token % (uint32_t)a.tokens;
-    const int sees = token_sees(a, kv_len_of(a, b), q_len_of(a, b), t);
-    last = (sees + kKvBlock - 1) / kKvBlock - 1;
-    keys = a.keys + list * a.pitch;
-    out = a.selected + (int64_t)list * a.want;
-  }
+template <int kRegs, int kPickWaves>
+struct PickRoom {
+  uint32_t of_wave[3][4][16];
+  uint32_t at[kRegs * kPickWaves];  // past the line, and on it << 16
+  __align__(16) uint32_t bins[kParts];
+  uint32_t line_bin[3], cand[kWave], cands;
 };
 
-// As pick_blocks, the keys of up to 1,024 kRegs blocks in the workgroup's
-// registers; two bits of the line at a time, as each step is a barrier (a bit at a
-// time, with the scores in shorter pieces, one token over 131,072 took 20 us instead of
-// 16, 4 x 9 36 instead of 28).
-template <int kRegs>
-__global__ __launch_bounds__(kWideThreads) void k_kv4_pick_wide(SelectArgs a) {
-  // (16 waves: a row of a wave's lanes sums up one number of each)
-  static_assert(kWideWaves == 16, "");
-  __shared__ uint32_t of_wave[3][4][kWideWaves];
-  __shared__ uint32_t at[kRegs * kWideWaves];  // past the line, and on it << 16
-  __shared__ __align__(16) uint32_t bins[kWideThreads];
-  __shared__ uint32_t line_bin[3], cand[kWave], cands;
+template <int kRegs, int kPickWaves>
+__device__ __forceinline__ void pick_together(
+    int sinks, int recent, int all, int last, const uint32_t* keys,
+    PickRoom<kRegs, kPickWaves>& lds, int32_t* out) {
+  // (a row of a wave's lanes sums up one number of each wave)
+  static_assert(kPickWaves <= 16, "");
+  constexpr int kThreads = kPickWaves * kWave;
   const int tid = threadIdx.x, lane = lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const WideList l(a);
   uint32_t k[kRegs], sure = 0, hi = 0, lo = 0;
   uint32_t n_sure = 0, n_some = 0;
-  bins[tid] = 0;
-  if (tid == 0) cands = 0;
+#pragma unroll
+  for (int i = tid; i < kParts; i += kThreads) lds.bins[i] = 0;
+  if (tid == 0) lds.cands = 0;
 #pragma unroll
   for (int i = 0; i < kRegs; ++i) {
-    const int j = i * kWideThreads + tid;
-    k[i] = j <= l.last ? l.keys[j] : 0;
+    const int j = i * kThreads + tid;
+    k[i] = j <= last ? keys[j] : 0;
   }
 #pragma unroll
   for (int i = 0; i < kRegs; ++i) {
-    const int j = i * kWideThreads + tid;
-    const bool is = k[i] && (j < a.sinks || j > l.last - a.recent);
+    const int j = i * kThreads + tid;
+    const bool is = k[i] && (j < sinks || j > last - recent);
     n_sure += (uint32_t)popc(ballot(is));
     if (is) {
       sure |= 1u << i;
@@ -567,23 +523,25 @@ __global__ __launch_bounds__(kWideThreads) void k_kv4_pick_wide(SelectArgs a) {
   hi = wave_all_max(hi);
   lo = wave_all_max(lo);
   if (lane == 0) {
-    of_wave[2][0][wave] = n_sure;
-    of_wave[2][1][wave] = n_some;
-    of_wave[2][2][wave] = hi;
-    of_wave[2][3][wave] = lo;
+    lds.of_wave[2][0][wave] = n_sure;
+    lds.of_wave[2][1][wave] = n_some;
+    lds.of_wave[2][2][wave] = hi;
+    lds.of_wave[2][3][wave] = lo;
   }
   __syncthreads();
   auto row_sums = [&](int turn) {
-    return row16_incl_scan(of_wave[turn][lane / 16][lane % 16]);
+    return row16_incl_scan(lane % 16 < kPickWaves
+                               ? lds.of_wave[turn][lane / 16][lane % 16]
+                               : 0);
   };
   auto of_row = [](uint32_t x, int row) {
     return (uint32_t)__builtin_amdgcn_readlane((int)x, 16 * row + 15);
   };
   const uint32_t sums = row_sums(2);
-  const int want = a.want - (int)of_row(sums, 0);
+  const int want = all - (int)of_row(sums, 0);
   const int some = (int)of_row(sums, 1);
-  hi = wave_all_max(lane < kWideWaves ? of_wave[2][2][lane] : 0);
-  lo = 0u - wave_all_max(lane < kWideWaves ? of_wave[2][3][lane] : 0);
+  hi = wave_all_max(lane < kPickWaves ? lds.of_wave[2][2][lane] : 0);
+  lo = 0u - wave_all_max(lane < kPickWaves ? lds.of_wave[2][3][lane] : 0);
   int turn = 0;
   // keys of at least x, x + step, x + 2 step
   auto at_least = [&](uint32_t x, uint32_t step, int (&n)[3]) {
@@ -593,7 +551,7 @@ __global__ __launch_bounds__(kWideThreads) void k_kv4_pick_wide(SelectArgs a) {
 #pragma unroll
       for (int i = 0; i < kRegs; ++i)
         n[s] += popc(ballot(k[i] >= x + s * step));
-      if (lane == 0) of_wave[turn][s][wave] = (uint32_t)n[s];
+      if (lane == 0) lds.of_wave[turn][s][wave] = (uint32_t)n[s];
     }
     __syncthreads();
     const uint32_t sums = row_sums(turn);
@@ -609,12 +567,12 @@ __global__ __launch_bounds__(kWideThreads) void k_kv4_pick_wide(SelectArgs a) {
     const int shift = max(0, 22 - __builtin_clz((hi - lo) | 1u));
 #pragma unroll
     for (int i = 0; i < kRegs; ++i)
-      if (k[i]) atomicAdd(&bins[(k[i] - lo) >> shift], 1u);
+      if (k[i]) atomicAdd(&lds.bins[(k[i] - lo) >> shift], 1u);
     __syncthreads();
     if (wave == 0) {
       // a lane's 16 parts, the largest keys first
       uint32_t x[16], n = 0;
-      const uint4* p = (const uint4*)bins + (kWave - 1 - lane) * 4;
+      const uint4* p = (const uint4*)lds.bins + (kWave - 1 - lane) * 4;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint4 v = p[3 - i];
@@ -629,16 +587,16 @@ __global__ __launch_bounds__(kWideThreads) void k_kv4_pick_wide(SelectArgs a) {
       for (int i = 0; i < 16; ++i) {
         const int next = upto + (int)x[i];
         if (upto < want && next >= want) {
-          line_bin[0] = (uint32_t)(kWideThreads - 1 - lane * 16 - i);
-          line_bin[1] = (uint32_t)upto;
-          line_bin[2] = (uint32_t)next;
+          lds.line_bin[0] = (uint32_t)(kParts - 1 - lane * 16 - i);
+          lds.line_bin[1] = (uint32_t)upto;
+          lds.line_bin[2] = (uint32_t)next;
         }
         upto = next;
       }
     }
     __syncthreads();
-    const uint32_t bin = line_bin[0];
-    const int past = (int)line_bin[1], upto = (int)line_bin[2];
+    const uint32_t bin = lds.line_bin[0];
+    const int past = (int)lds.line_bin[1], upto = (int)lds.line_bin[2];
     line = lo + (bin << shift);
     bool exact = upto == want;
     if (!exact && upto - past <= kWave) {
@@ -646,9 +604,9 @@ __global__ __launch_bounds__(kWideThreads) void k_kv4_pick_wide(SelectArgs a) {
 #pragma unroll
       for (int i = 0; i < kRegs; ++i)
         if (k[i] && (k[i] - lo) >> shift == bin)
-          cand[atomicAdd(&cands, 1u)] = k[i];
+          lds.cand[atomicAdd(&lds.cands, 1u)] = k[i];
       __syncthreads();
-      const uint32_t x = lane < upto - past ? cand[lane] : 0;
+      const uint32_t x = lane < upto - past ? lds.cand[lane] : 0;
       int n = upto;
       for (int bit = shift - 1; bit >= 0 && n != want; --bit) {
         const uint32_t y = line + (1u << bit);
@@ -690,32 +648,134 @@ __global__ __launch_bounds__(kWideThreads) void k_kv4_pick_wide(SelectArgs a) {
     const uint64_t gt = ballot(k[i] > line || (sure >> i & 1));
     const uint64_t eq = ballot(room > 0 && k[i] == line);
     if (lane == 0)
-      at[i * kWideWaves + wave] = (uint32_t)(popc(gt) | popc(eq) << 16);
+      lds.at[i * kPickWaves + wave] = (uint32_t)(popc(gt) | popc(eq) << 16);
   }
   __syncthreads();
   // what comes before each 64, and in all; no sum passes 16 bits
-  uint32_t all = 0;
+  uint32_t sum = 0;
   if (wave == 0) {
-    for (int i0 = 0; i0 < kRegs * kWideWaves; i0 += kWave) {
-      const uint32_t x = at[i0 + lane];
+    for (int i0 = 0; i0 < kRegs * kPickWaves; i0 += kWave) {
+      const bool is = i0 + lane < kRegs * kPickWaves;
+      const uint32_t x = is ? lds.at[i0 + lane] : 0;
       const uint32_t to = wave_incl_scan(x);
-      at[i0 + lane] = all + to - x;
-      all += (uint32_t)__builtin_amdgcn_readlane((int)to, kWave - 1);
+      if (is) lds.at[i0 + lane] = sum + to - x;
+      sum += (uint32_t)__builtin_amdgcn_readlane((int)to, kWave - 1);
     }
-    const int n = (int)(all & 0xffffu) + min((int)(all >> 16), room);
-    for (int i = n + lane; i < a.want; i += kWave) l.out[i] = -1;
+    const int n = (int)(sum & 0xffffu) + min((int)(sum >> 16), room);
+    for (int i = n + lane; i < all; i += kWave) out[i] = -1;
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kRegs; ++i) {
-    const uint32_t before = at[i * kWideWaves + wave];
+    const uint32_t before = lds.at[i * kPickWaves + wave];
     const bool over = k[i] > line || (sure >> i & 1);
     const bool on = room > 0 && k[i] == line;
     const int gt = (int)(before & 0xffffu) + rank_lt(ballot(over));
     const int eq = (int)(before >> 16) + rank_lt(ballot(on));
     if (over || (on && eq < room))
-      l.out[gt + min(eq, room)] = i * kWideThreads + tid;
+      out[gt + min(eq, room)] = i * kThreads + tid;
   }
+}
+
+// Scores and choice at once, where a workgroup holds the keys of its tokens: rows
+// of up to 1,024 blocks.
+constexpr int kSelectTokens = 32;
+constexpr int kSelectBlocks = 1024;
+constexpr int kSelectRegs = kSelectBlocks / kSelectThreads;
+typedef PickRoom<kSelectRegs, kSelectThreads / kWave> SelectRoom;
+
+// kFew: all waves choose for one token after the other, rather than each for its own
+// (64 x 1 tokens over up to 32,768 28.6 and 26.3 us).  A kernel of its own: with both in
+// one the registers leave five waves a SIMD of seven, and a prompt takes 44 us
+// instead of 38.
+template <int D, bool kHalf, bool kFew>
+__global__ __launch_bounds__(kSelectThreads) void k_kv4_select(SelectArgs a) {
+  constexpr int kPitch = 2 * D + 16;
+  constexpr int kSelectWaves = kSelectThreads / kWave;
+  extern __shared__ __align__(16) char lds[];
+  // tiles of one row and KV head follow each other on one XCD (32 bits hold all
+  // of these)
+  const uint32_t k = blockIdx.x / 8;
+  const int tile = (int)(k % (uint32_t)a.tiles);
+  const uint32_t bh = k / (uint32_t)a.tiles * 8 + blockIdx.x % 8;
+  if (bh >= (uint32_t)a.batch * (uint32_t)a.c.heads) return;
+  const int64_t b = bh / (uint32_t)a.c.heads;
+  const int h = (int)(bh % (uint32_t)a.c.heads);
+  const int64_t len = kv_len_of(a, b), nq = q_len_of(a, b);
+  const int64_t t0 = (int64_t)tile * a.span;
+  const int tokens = (int)std::min<int64_t>(a.span, a.tokens - t0);
+  const int queries = (int)std::max<int64_t>(
+      0, std::min<int64_t>(tokens, nq - t0));
+  auto sq = (int8_t(*)[kPitch])lds;
+  // (rows 4 banks apart)
+  const int pitch = (int)a.pitch + 4;
+  uint32_t* keys = (uint32_t*)(lds + (a.span + 15) / 16 * 16 * kPitch);
+  const int blocks =
+      queries ? (token_sees(a, len, nq, t0 + queries - 1) + kKvBlock - 1) /
+                    kKvBlock
+              : 0;
+  score_blocks<D, kHalf>(a, b, h, t0, queries, (tokens + 15) / 16 * 16, 0,
+                         blocks, sq, [&](int q, int blk, uint4 key) {
+                           *(uint4*)(keys + q * pitch + blk) = key;
+                         });
+  __syncthreads();
+  auto last_of = [&](int i) {
+    return __builtin_amdgcn_readfirstlane(
+        (token_sees(a, len, nq, t0 + i) + kKvBlock - 1) / kKvBlock - 1);
+  };
+  auto out_of = [&](int i) {
+    return a.selected + ((b * a.tokens + t0 + i) * a.c.heads + h) * a.want;
+  };
+  if constexpr (kFew) {
+    __shared__ SelectRoom room;
+    for (int i = 0; i < tokens; ++i) {
+      if (i) __syncthreads();
+      pick_together<kSelectRegs, kSelectWaves>(a.sinks, a.recent, a.want,
+                                               last_of(i), keys + i * pitch,
+                                               room, out_of(i));
+    }
+  } else {
+    __shared__ uint32_t bins[kSelectWaves][kWave];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    for (int i = wave; i < tokens; i += kSelectWaves) {
+      const int last = last_of(i);
+      const uint32_t* own = keys + i * pitch;
+      int32_t* out = out_of(i);
+      if (last < 4 * kWave)
+        pick_blocks<4>(a.sinks, a.recent, a.want, last, own, bins[wave], out);
+      else if (last < 8 * kWave)
+        pick_blocks<8>(a.sinks, a.recent, a.want, last, own, bins[wave], out);
+      else
+        pick_blocks<16>(a.sinks, a.recent, a.want, last, own, bins[wave], out);
+    }
+  }
+}
+
+// The choice by a workgroup of 1,024 threads, for rows whose keys are in memory.
+constexpr int kWideThreads = 1024;
+constexpr int kWideWaves = kWideThreads / kWave;
+
+struct WideList {
+  int last;
+  const uint32_t* keys;
+  int32_t* out;
+  __device__ __forceinline__ WideList(const SelectArgs& a) {
+    const uint32_t list = blockIdx.x, token = list / (uint32_t)a.c.heads;
+    const uint32_t b = token / (uint32_t)a.tokens;
+    const uint32_t t = token % (uint32_t)a.tokens;
+    const int sees = token_sees(a, kv_len_of(a, b), q_len_of(a, b), t);
+    last = (sees + kKvBlock - 1) / kKvBlock - 1;
+    keys = a.keys + list * a.pitch;
+    out = a.selected + (int64_t)list * a.want;
+  }
+};
+
+template <int kRegs>
+__global__ __launch_bounds__(kWideThreads) void k_kv4_pick_wide(SelectArgs a) {
+  __shared__ PickRoom<kRegs, kWideWaves> room;
+  const WideList l(a);
+  pick_together<kRegs, kWideWaves>(a.sinks, a.recent, a.want, l.last, l.keys,
+                                   room, l.out);
 }
 
 // The key of block j for what follows: first and recent blocks above all others.
@@ -822,8 +882,15 @@ bool select_ok(const sfx_kv4* c, int64_t batch, int64_t tokens) {
          batch * tokens <= ((int64_t(1) << 22) - 1) / c->heads;
 }
 
-bool held_in_lds(const sfx_kv4* c) {
-  return pitch_of(c) <= 16 * kWave;
+// Whether one launch serves.  With the rows' scores cut into pieces and a second
+// launch for the choice few lists of long rows are chosen sooner: of 1,024 blocks each
+// for one token of one row 14.4 us in one launch, 10.3 in two, of 16 rows 16.9 and
+// 16.8, five tokens of four rows 19.7 and 11.9, 17 of 16 rows 26 and 36; of 512 blocks
+// 10.5 and 10.4, 11.0 and 13.0.
+bool held_in_lds(const sfx_kv4* c, int64_t batch, int64_t tokens) {
+  const int64_t blocks = pitch_of(c);
+  return blocks <= kSelectBlocks / 2 ||
+         (blocks <= kSelectBlocks && batch * tokens * c->heads > 256);
 }
 
 template <int D, bool kHalf>
@@ -839,9 +906,15 @@ int launch_held(SelectArgs a, hipStream_t stream) {
   const int64_t items = (a.batch * a.c.heads + 7) / 8 * 8;
   if (items * a.tiles >= (int64_t(1) << 32) / kSelectThreads)
     return SFX_EINVAL;
-  hipLaunchKernelGGL((k_kv4_select<D, kHalf>),
-                     dim3((unsigned)(items * a.tiles)), dim3(kSelectThreads),
-                     lds, stream, a);
+  const dim3 grid((unsigned)(items * a.tiles)), block(kSelectThreads);
+  // one token, of up to 1,024 blocks, by a wave 18 us, by all of them 14; of up to 256
+  // 7.8 and 8.6
+  if (a.span <= 2 && a.pitch > kSelectBlocks / 4)
+    hipLaunchKernelGGL((k_kv4_select<D, kHalf, true>), grid, block, lds, stream,
+                       a);
+  else
+    hipLaunchKernelGGL((k_kv4_select<D, kHalf, false>), grid, block, lds,
+                       stream, a);
   return (int)hipGetLastError();
 }
 
@@ -874,7 +947,7 @@ int launch_wide(SelectArgs a, hipStream_t stream) {
 
 template <int D, bool kHalf>
 int launch(const SelectArgs& a, const sfx_kv4* cache, hipStream_t stream) {
-  return held_in_lds(cache) ? launch_held<D, kHalf>(a, stream)
+  return held_in_lds(cache, a.batch, a.tokens) ? launch_held<D, kHalf>(a, stream)
                             : launch_wide<D, kHalf>(a, stream);
 }
 
@@ -928,7 +1001,8 @@ extern "C" int sfx_kv4_bounds_update(const sfx_kv4* cache,
 extern "C" size_t sfx_kv4_select_workspace_size(const sfx_kv4* cache,
                                                 int64_t batch,
                                                 int64_t tokens) {
-  if (!select_ok(cache, batch, tokens) || held_in_lds(cache)) return 0;
+  if (!select_ok(cache, batch, tokens) || held_in_lds(cache, batch, tokens))
+    return 0;
   return (size_t)(batch * tokens * cache->heads) * (size_t)pitch_of(cache) * 4;
 }
 

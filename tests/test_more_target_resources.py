@@ -28,7 +28,10 @@ def test_block_kernels_keep_their_waves(tmp_path):
     _check(res, "k_kv4_bounds", 7)
     # by head size, which the mangled name has as the first argument
     for d, waves in ((64, 7), (128, 7), (256, 4)):
-        _check(res, f"k_kv4_selectILi{d}E", waves)
+        for half in (0, 1):
+            _check(res, f"k_kv4_selectILi{d}ELb{half}ELb0E", waves)
+            # (few tokens: two workgroups of eight waves a CU)
+            _check(res, f"k_kv4_selectILi{d}ELb{half}ELb1E", 4)
         _check(res, f"k_kv4_scoresILi{d}E", waves)
     _check(res, "k_kv4_pick_wide", 7)
     _check(res, "k_kv4_pick_far", 8)
