@@ -129,44 +129,51 @@ __device__ __forceinline__ int fresh_thread() {
   return t;
 }
 
-// As each_block, over entries first, first + step, ... below last: block(e) is
-// the block of entry e, negative where there is none, takes(e) the rows that take
-// it.  A block's page id is read a block ahead of its loads.
-template <class B, class Block_, class Takes, class F>
+// A block of a list, negative where there is none, and the rows that take it.
+struct Entry {
+  int blk;
+  uint32_t rows;
+};
+
+// As each_block, over entries first, first + step, ... below last.  An entry is read
+// (as a scalar) a block ahead of its page id, and that a block ahead of the loads.
+template <class B, class Read, class F>
 __device__ __forceinline__ void each_entry(const KvView& c, int64_t b, int h,
                                            int bytes, int first, int step,
-                                           int last, Block_ block, Takes takes,
-                                           F body) {
+                                           int last, Read read, F body) {
   if (first >= last || c.num_pages == 0) return;
   const Scalars ids = (Scalars)(uintptr_t)(c.table + b * c.table_stride);
   const int in_page = (1 << c.page_shift) - 1;
   const uint32_t pages = (uint32_t)min(c.num_pages, int64_t(1) << 31);
-  auto page = [&](int blk) { return blk < 0 ? -1 : ids[blk >> c.page_shift]; };
+  auto page = [&](Entry e) {
+    return e.blk < 0 ? -1 : ids[e.blk >> c.page_shift];
+  };
   auto good = [&](int32_t id) { return (uint32_t)id < pages; };
   // past the last block, and without a page: memory that is there
-  auto at = [&](int32_t id, int blk) {
+  auto at = [&](int32_t id, Entry e) {
     return good(id) ? c.pages + ((((int64_t)id * c.heads + h) << c.page_shift) +
-                                 (blk & in_page)) * bytes
+                                 (e.blk & in_page)) * bytes
                     : c.pages;
   };
+  auto entry = [&](int i) { return read(min(i, last - 1)); };
   B x;
-  int blk = block(first), blk1 = block(min(first + step, last - 1));
-  int32_t id = page(blk), id1 = page(blk1);
-  x.load_k(at(id, blk));
-  x.load_v(at(id, blk));
-  for (int e = first; e < last; e += step) {
-    const char* next = at(id1, blk1);
-    const int blk2 = block(min(e + 2 * step, last - 1));
-    const int32_t id2 = page(blk2);
+  Entry e = entry(first), e1 = entry(first + step), e2 = entry(first + 2 * step);
+  int32_t id = page(e), id1 = page(e1);
+  x.load_k(at(id, e));
+  x.load_v(at(id, e));
+  for (int i = first; i < last; i += step) {
+    const char* next = at(id1, e1);
+    const int32_t id2 = page(e2);
+    const Entry e3 = entry(i + 3 * step);
     if (good(id)) {
-      body(x, blk, takes(e), [&]() { x.load_k(next); },
-           [&]() { x.load_v(next); });
+      body(x, e, [&]() { x.load_k(next); }, [&]() { x.load_v(next); });
     } else {
       x.load_k(next);
       x.load_v(next);
     }
-    blk = blk1;
-    blk1 = blk2;
+    e = e1;
+    e1 = e2;
+    e2 = e3;
     id = id1;
     id1 = id2;
   }
@@ -202,22 +209,21 @@ struct OneList {
   template <class B, class F>
   __device__ __forceinline__ void each(const ListArgs& a, const Work& wk,
                                        int bytes, F body) const {
-    auto block = [&](int e) {
+    auto read = [&](int e) {
       const int x = list[e];
-      if (x < 0 || x >= limit) return -1;
+      if (x < 0 || x >= limit) return Entry{-1, 0};
       if (!ascends) {
         const int32_t* p = (const int32_t*)(uintptr_t)list;
         bool twice = false;
         for (int i = fresh_thread() % kWave; i < e; i += kWave)
           twice |= p[i] == x;
-        if (__any(twice)) return -1;
+        if (__any(twice)) return Entry{-1, 0};
       }
-      return x;
+      return Entry{x, 0};
     };
-    each_entry<B>(a.c, wk.b, wk.h, bytes, first, step, last, block,
-                  [](int) { return 1; },
-                  [&](B& x, int blk, int, auto kdone, auto vdone) {
-                    body(x, blk, AllRows(), kdone, vdone);
+    each_entry<B>(a.c, wk.b, wk.h, bytes, first, step, last, read,
+                  [&](B& x, Entry e, auto kdone, auto vdone) {
+                    body(x, e.blk, AllRows(), kdone, vdone);
                   });
   }
 };
@@ -256,13 +262,14 @@ struct TileList {
   __device__ __forceinline__ void each(const ListArgs& a, const Work& wk,
                                        int bytes, F body) {
     each_entry<B>(a.c, wk.b, wk.h, bytes, first, step, last,
-                  [&](int e) { return entry[2 * e]; },
-                  [&](int e) { return (uint32_t)entry[2 * e + 1]; },
-                  [&](B& x, int blk, uint32_t rows, auto kdone, auto vdone) {
-                    uint64_t mask = rows | rows << 16;
+                  [&](int e) {
+                    return Entry{entry[2 * e], (uint32_t)entry[2 * e + 1]};
+                  },
+                  [&](B& x, Entry e, auto kdone, auto vdone) {
+                    uint64_t mask = e.rows | e.rows << 16;
                     mask |= mask << 32;
                     saw |= mask;
-                    body(x, blk, SomeRows{mask, rows == full}, kdone, vdone);
+                    body(x, e.blk, SomeRows{mask, e.rows == full}, kdone, vdone);
                   });
   }
 };
