@@ -4,9 +4,9 @@
 // them); a row passes over the blocks of the others.  Neighbouring tokens select
 // much the same blocks, each of which is then loaded and converted once.
 //
-// 2,048 tokens of a prompt with 64 blocks each of 512: 156 us and 12 for the unions,
-// which have 84 blocks on average; vector instructions issue in 82% of the cycles,
-// matrix instructions in 29%.  64 x 17 tokens with 32 of 256 37 and 8.  Single tokens
+// 2,048 tokens of a prompt with 64 blocks each of 512: 143 us and 8 for the unions,
+// which have 84 blocks on average; vector instructions issue in 83% of the cycles,
+// matrix instructions in 30%.  64 x 17 tokens with 32 of 256 36 and 7.  Single tokens
 // are bound by memory: 64 with 64 of 1,024 27 us, 145 MB, 5.4 TB/s.
 // Tiles of 32 rows, whose unions are larger (97 blocks), gave 170 us instead of 177 for
 // the prompt, 53 instead of 50 for 64 x 17.  Keys as their 4 bits stand, in products

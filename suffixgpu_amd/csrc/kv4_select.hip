@@ -13,7 +13,7 @@
 //
 // What bounds it are the steps that follow each other in a workgroup, most of which
 // run at once: packing the query, the scores, the choice (vector instructions issue in
-// half of the cycles); with all rows full, the memory (64 x 1 tokens over 32,768 30 us,
+// half of the cycles); of many long rows, the memory (64 x 1 tokens over 32,768 30 us,
 // 135 MB, 4.5 TB/s).  The choice is made where the scores are: in LDS and a wave's or a
 // workgroup's registers for rows of up to 1,024 blocks (64 x 1 tokens over up to 32,768
 // 26 us a call, with the scores in memory and a second launch 33; 64 x 17 over up to
