@@ -10,7 +10,7 @@
 // are bound by memory: 64 with 64 of 1,024 27 us, 145 MB, 5.4 TB/s.
 // Tiles of 32 rows, whose unions are larger (97 blocks), gave 170 us instead of 177 for
 // the prompt, 53 instead of 50 for 64 x 17.  Keys as their 4 bits stand, in products
-// with 8-bit parts of the queries, gave 143 instead of 156, but the matrix instruction
+// with 8-bit parts of the queries, gave 143 instead of 156 in all, but the instruction
 // adds 32 channels to fewer than 24 bits.
 
 #include <algorithm>

@@ -13,12 +13,11 @@
 // Positions without a token leave at once.
 //
 // Memory bounds it where there are no alternatives: 2,048 positions of 128,256
-// bfloat16 logits take 103 us, 5.1 TB/s.  With alternatives it is the vector
-// instructions, 17 a logit with one (116 to 128 us) and 20 with twenty: 256 positions
-// 30 us, 66 MB at 2.2 TB/s, 19 without any.  8,192 logits a workgroup are 32 a lane,
-// which is what stays in registers beside the rest with seven waves a SIMD; for eight
-// the compiler spills.  One position of 32,000 is the latency of the two launches
-// (5.2 + 4.5 us).
+// bfloat16 logits take 96 to 103 us, 5.1 to 5.5 TB/s.  With alternatives it is the
+// vector instructions, 16 a logit with one (112 to 125 us) and 19 with twenty: 256
+// positions 30 us, 66 MB at 2.2 TB/s, 19 without any.  8,192 logits a workgroup are 32 a
+// lane, which is what stays in registers beside the rest with seven or eight waves a
+// SIMD.  One position of 32,000 is the latency of the two launches (5.2 + 4.2 us).
 
 #include <algorithm>
 
@@ -198,12 +197,13 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
     // for all, is put right in the sums.
     if (kTop && DT != SFX_F32) {
       // unpacked again where they are used: kept as floats they would cost the
-      // kernel that also ranks a wave in seven
-      s.forget();
+      // kernel that also ranks a wave in eight
+      if (DT == SFX_F16) s.forget();
+      const typename S::Anew anew;
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[u][e] = s.get(u, e);
+        for (int e = 0; e < E; ++e) x[u][e] = s.get(u, e, anew);
     }
     const float tc = top * c, off = __builtin_fmaf(top, c, -tc);
     float sum = 0.0f, zsum = 0.0f;
@@ -268,7 +268,8 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
     a.part[pos * a.chunks + chunk] = p;
   }
   if (!kTop) return;
-  if (DT != SFX_F32) s.forget();
+  if (DT == SFX_F16) s.forget();
+  const typename S::Anew anew;
   __syncthreads();
   const float line = lds_line;
   int count = 0;
@@ -285,8 +286,8 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
     if (ballot(vtop[u] >= line)) {
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (ballot(s.get(u, e) >= line))
-          offer(s.get(u, e), s.index(u * E + e), true);
+        if (ballot(s.get(u, e, anew) >= line))
+          offer(s.get(u, e, anew), s.index(u * E + e), true);
     }
   }
   if (lane == 0) counts[wave] = count;

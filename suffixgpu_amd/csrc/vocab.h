@@ -111,8 +111,19 @@ struct Share {
     return (float)__builtin_bit_cast(_Float16,
                                      (uint16_t)(e % 2 ? x >> 16 : x));
   }
-  // The compiler shall unpack the elements again where they are next used: the
-  // floats of two uses would not fit beside each other.
+  // As get, by a shift and a mask that the compiler does not know: it unpacks the
+  // element anew, where floats kept from one use to the next would not fit beside
+  // each other.
+  struct Anew {
+    uint32_t shift = 16, mask = 0xffff0000u;
+    __device__ Anew() { asm volatile("" : "+s"(shift), "+s"(mask)); }
+  };
+  __device__ float get(int u, int e, const Anew& by) const {
+    if (DT != SFX_BF16) return get(u, e);
+    const uint32_t q[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+    return __uint_as_float(e % 2 ? q[e / 2] & by.mask : q[e / 2] << by.shift);
+  }
+  // The same for the elements of any type, which costs moves.
   __device__ void forget() {
 #pragma unroll
     for (int u = 0; u < U; ++u)
