@@ -8,7 +8,7 @@
 //
 // The first launch takes 8,192 logits a workgroup, which stay in registers: their
 // largest, R and sum z e^z, and what reaches a number that n of the maxima of its
-// 64 parts reach, and few more: the n largest, and few others.  The second launch
+// 128 parts reach, and few more: the n largest, and few others.  The second launch
 // joins a position's parts and ranks what is left of those.
 // Positions without a token leave at once.
 //
@@ -118,21 +118,23 @@ __device__ __forceinline__ int place_of(const Entry& m, int count) {
   return r;
 }
 
-// A number that n of a wave's lanes reach (at most 64), and few more: by halves,
-// until no more than n + kFew do.
+// A number that n (at most 64) of a wave's 128 numbers x, y reach, and few more: by
+// halves, until no more than n + kFew do.  Of those that are the largest of groups
+// of others, what reaches it is n and few more too: 45 of 8,192 random ones with n = 32
+// (of 64 groups 58, and then and when more than the 64 that a wave ranks).
 constexpr int kFew = 6;
 constexpr int kSpare = 8;  // entries of a list beside the n, which are in no order
 
-__device__ __forceinline__ float reached_by(float x, int n) {
-  const uint32_t k = order_of(x);
-  const uint32_t hi = wave_all_max(k), lo = ~wave_all_max(~k);
+__device__ __forceinline__ float reached_by(float x, float y, int n) {
+  const uint32_t k0 = order_of(x), k1 = order_of(y);
+  const uint32_t hi = wave_all_max(max(k0, k1)), lo = ~wave_all_max(~min(k0, k1));
   int bit = 31 - __builtin_clz((hi ^ lo) | 1u);
   uint32_t line = lo >> bit >> 1 << bit << 1;
   for (; bit >= 0; --bit) {
-    const uint32_t y = line | 1u << bit;
-    const int count = popc(ballot(k >= y));
+    const uint32_t to = line | 1u << bit;
+    const int count = popc(ballot(k0 >= to)) + popc(ballot(k1 >= to));
     if (count >= n) {
-      line = y;
+      line = to;
       if (count <= n + kFew) break;
     }
   }
@@ -145,7 +147,7 @@ template <int DT, bool kTop>
 __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
   using S = Share<DT>;
   constexpr int E = S::E, U = S::U;
-  static_assert(kThreads / 4 == kWave && kWave >= SFX_LOGPROBS_TOP, "");
+  static_assert(kThreads / 2 == 2 * kWave && kWave >= SFX_LOGPROBS_TOP, "");
   const int chunk = blockIdx.x % a.chunks;
   const int64_t pos = blockIdx.x / a.chunks;
   const int64_t b = pos / a.v.positions, j = pos % a.v.positions;
@@ -153,7 +155,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
   if (tok < 0 || tok >= a.v.vocab) return;
   const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id();
   __shared__ Part lds[kWaves];
-  __shared__ float group[kTop ? kWave : 1];  // maxima of four threads' logits
+  __shared__ float group[kTop ? 2 * kWave : 1];  // maxima of two threads' logits
   __shared__ float lds_line;
   __shared__ Entry cand[kTop ? kWaves : 1][kWave];
   __shared__ int counts[kWaves];
@@ -180,9 +182,8 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
   const float mine = top;
   top = wave_max(top);
   if (kTop) {
-    float m = fmaxf(mine, lane_of<0xb1>(mine));  // lane ^ 1
-    m = fmaxf(m, lane_of<0x4e>(m));              // lane ^ 2
-    if (lane % 4 == 0) group[tid / 4] = m;
+    const float m = fmaxf(mine, lane_of<0xb1>(mine));  // lane ^ 1
+    if (lane % 2 == 0) group[tid / 2] = m;
   }
   Part p = {top, 0.0f, 0.0f, 0x7fffffff};
   if (greedy) {
@@ -259,7 +260,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
   const int n = (int)a.v.top;
   if (kTop && wave == 1) {
     // what n groups' maxima reach, so at least n logits, and few more
-    const float y = reached_by(group[lane], n);
+    const float y = reached_by(group[lane], group[lane + kWave], n);
     if (lane == 0) lds_line = y;
   }
   if (tid == 0) {
@@ -352,7 +353,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
 // A position's parts, by a wave.
 //
 // Its n largest logits are among the entries of the parts' lists.  They reach what
-// n of the lanes' largest entries reach, and few others do.
+// n of the largest of the lanes' halves reach, and few others do.
 constexpr int kHeld = 8;  // entries a lane keeps; of more all are read again
 
 template <int DT, bool kTop>
@@ -420,12 +421,14 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogArgs a) {
   }
   if (!kTop) return;
 
-  float most = held[0].x;
+  float most[2] = {held[0].x, held[1].x};
 #pragma unroll
-  for (int i = 1; i < kHeld; ++i) most = fmaxf(most, held[i].x);
-  for (int i = kHeld * kWave + lane; i < all; i += kWave)
-    most = fmaxf(most, in[i].x);
-  const float line = reached_by(most, n);
+  for (int i = 2; i < kHeld; ++i) most[i % 2] = fmaxf(most[i % 2], held[i].x);
+  for (int i0 = kHeld * kWave; i0 < all; i0 += 2 * kWave) {
+    most[0] = fmaxf(most[0], entry(i0 + lane).x);
+    most[1] = fmaxf(most[1], entry(i0 + kWave + lane).x);
+  }
+  const float line = reached_by(most[0], most[1], n);
   __shared__ Entry kept[kWaves][kWave];
   int count = 0;
   auto keep = [&](const Entry& y) {
