@@ -14,8 +14,8 @@
 //
 // Memory bounds it where there are no alternatives: 2,048 positions of 128,256
 // bfloat16 logits take 96 to 103 us, 5.1 to 5.5 TB/s.  With alternatives it is the
-// vector instructions, 16 a logit with one (112 to 125 us) and 19 with twenty: 256
-// positions 30 us, 66 MB at 2.2 TB/s, 19 without any.  8,192 logits a workgroup are 32 a
+// vector instructions, 16 a logit with one (112 to 125 us) and 18 with twenty: 256
+// positions 28.5 us, 66 MB at 2.3 TB/s, 19 without any.  8,192 logits a workgroup are 32 a
 // lane, which is what stays in registers beside the rest with seven or eight waves a
 // SIMD.  One position of 32,000 is the latency of the two launches (5.2 + 4.2 us).
 
@@ -118,6 +118,12 @@ __device__ __forceinline__ int place_of(const Entry& m, int count) {
   return r;
 }
 
+// The next float.
+__device__ __forceinline__ float next_above(float x) {
+  const uint32_t u = __float_as_uint(x == 0.0f ? 0.0f : x);
+  return __uint_as_float(u >> 31 ? u - 1 : u + 1);
+}
+
 // A number that n (at most 64) of a wave's 128 numbers x, y reach, and few more: by
 // halves, until no more than n + kFew do.  Of those that are the largest of groups
 // of others, what reaches it is n and few more too: 45 of 8,192 random ones with n = 32
@@ -158,7 +164,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
   __shared__ float group[kTop ? 2 * kWave : 1];  // maxima of two threads' logits
   __shared__ float lds_line;
   __shared__ Entry cand[kTop ? kWaves : 1][kWave];
-  __shared__ int counts[kWaves];
+  __shared__ int counts[kWaves], ties[1 + U][kWaves];
   const float t = temperature_of(a.v, b);
   const bool greedy = !(t > 0.0f);
   const float c = greedy ? 0.0f : scale_of(t);
@@ -272,14 +278,27 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
   if (DT == SFX_F16) s.forget();
   const typename S::Anew anew;
   __syncthreads();
-  const float line = lds_line;
-  int count = 0;
+  float line = lds_line;
+  int count = 0, all;
   auto offer = [&](float y, int i, bool in) {
     const bool is = in && y >= line && y > kNegInf;
     const uint64_t m = ballot(is);
     const int k = count + rank_lt(m);
     if (is && k < kWave) cand[wave][k] = Entry{y, i};
     count += popc(m);
+  };
+  // whether a wave can rank what was offered
+  auto offered = [&]() {
+    if (lane == 0) counts[wave] = count;
+    __syncthreads();
+    all = 0;
+    bool fits = true;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      fits = fits && counts[w] <= kWave;
+      all += counts[w];
+    }
+    return fits && all <= kWave;
   };
   if (ballot(s.extra >= 0)) offer(s.single, s.extra, s.extra >= 0);
 #pragma unroll
@@ -291,18 +310,67 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
           offer(s.get(u, e, anew), s.index(u * E + e), true);
     }
   }
-  if (lane == 0) counts[wave] = count;
-  __syncthreads();
   const int room = n + kSpare;
   Entry* out = a.entry + (pos * a.chunks + chunk) * room;
-  int all = 0;
-  bool fits = true;
+  bool fits = offered();
+  if (!fits && line > kNegInf) {
+    // Many are equal to the line: what lies past it, and the first of these.  (256
+    // positions of one value, twenty alternatives: 81 us, one after the other 274.)
+    const float tie = line;
+    line = next_above(line);
+    __syncthreads();
+    count = 0;
+    offer(s.single, s.extra, s.extra >= 0);
+#pragma unroll 1
+    for (int u = 0; u < U; ++u) s.again_step(u, offer);
+    fits = offered();
+    if (fits && all < n) {
+      // in the order of their indices: single ones before the vectors (all of
+      // them a wave's), the vectors of each step, wave by wave, single ones
+      const bool equal = s.extra >= 0 && s.single == tie;
+      const uint64_t heads = ballot(equal && s.extra < s.head);
+      const uint64_t tails = ballot(equal && s.extra >= s.head);
+      const int need = n - all;
+      auto equals = [&](int u) {
+        uint32_t c = 0;
+        s.again_step(u, [&](float y, int, bool in) { c += in && y == tie; });
+        return c;
+      };
+#pragma unroll 1
+      for (int u = 0; u < U; ++u) {
+        const uint32_t to = wave_incl_scan(equals(u));
+        if (lane == kWave - 1) ties[1 + u][wave] = (int)to;
+      }
+      if (lane == 0) ties[0][wave] = popc(heads);
+      __syncthreads();
+      line = tie;
+      int before_it = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    fits = fits && counts[w] <= kWave;
-    all += counts[w];
+      for (int w = 0; w < kWaves; ++w) before_it += ties[0][w];
+      offer(s.single, s.extra, (heads >> lane & 1) && rank_lt(heads) < need);
+#pragma unroll 1
+      for (int u = 0; u < U; ++u) {
+        int k = before_it;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          if (w < wave) k += ties[1 + u][w];
+          before_it += ties[1 + u][w];
+        }
+        if (k >= need) continue;
+        const uint32_t c = equals(u);
+        k += (int)(wave_incl_scan(c) - c);
+        s.again_step(u, [&](float y, int i, bool in) {
+          const bool is = in && y == tie;
+          offer(y, i, is && k < need);
+          k += is;
+        });
+      }
+      offer(s.single, s.extra,
+            (tails >> lane & 1) && before_it + rank_lt(tails) < need);
+      fits = offered();
+    }
   }
-  if (fits && all <= kWave) {
+  if (fits) {
     if (wave > 0) return;
     int w = 0, i = lane;
 #pragma unroll
@@ -323,8 +391,8 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
     return;
   }
   if (tid >= n && tid < room) out[tid] = Entry{kNegInf, -1};
-  // Many equal logits: one after the other, the best of what comes after the
-  // last.
+  // Many logits of few groups: one after the other, the best of what comes after
+  // the last.
   Entry last = {__builtin_inff(), -1};
   for (int k = 0; k < n; ++k) {
     Entry best = {kNegInf, 0x7fffffff};
@@ -431,8 +499,8 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogArgs a) {
   const float line = reached_by(most[0], most[1], n);
   __shared__ Entry kept[kWaves][kWave];
   int count = 0;
-  auto keep = [&](const Entry& y) {
-    const bool is = y.at >= 0 && y.x >= line;
+  auto keep = [&](const Entry& y, bool in) {
+    const bool is = in && y.at >= 0;
     const uint64_t m = ballot(is);
     const int at = count + rank_lt(m);
     if (is && at < kWave) kept[wave][at] = y;
@@ -440,8 +508,37 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogArgs a) {
   };
 #pragma unroll
   for (int i = 0; i < kHeld; ++i)
-    if (i * kWave < all) keep(held[i]);
-  for (int i0 = kHeld * kWave; i0 < all; i0 += kWave) keep(entry(i0 + lane));
+    if (i * kWave < all) keep(held[i], held[i].x >= line);
+  for (int i0 = kHeld * kWave; i0 < all; i0 += kWave) {
+    const Entry y = entry(i0 + lane);
+    keep(y, y.x >= line);
+  }
+  if (count > kWave && line > kNegInf) {
+    // Many are equal to the line: those past it, and the first of these.
+    auto each = [&](auto f) {
+#pragma unroll 1
+      for (int i0 = 0; i0 < all; i0 += kWave) f(entry(i0 + lane));
+    };
+    const float past = next_above(line);
+    wave_lds_sync();
+    count = 0;
+    each([&](const Entry& y) { keep(y, y.x >= past); });
+    if (count < n) {
+      // the one with as many before it as are missing (indices are below 2^28)
+      const int need = n - count;
+      int last = 0;
+#pragma unroll 1
+      for (int bit = 27; bit >= 0; --bit) {
+        int c = 0;
+        each([&](const Entry& y) {
+          c += popc(ballot(y.at >= 0 && y.x == line &&
+                           y.at < last + (1 << bit)));
+        });
+        if (c < need) last += 1 << bit;
+      }
+      each([&](const Entry& y) { keep(y, y.x == line && y.at <= last); });
+    }
+  }
   wave_lds_sync();
   Entry best = {kNegInf, -1};  // lane k: the k-th
   if (count <= kWave) {
@@ -453,7 +550,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogArgs a) {
     wave_lds_sync();
     if (lane < min(n, count)) best = kept[wave][lane];
   } else {
-    // Many equal ones: one after the other, the first behind the last.
+    // Many in few of the halves: one after the other, the first behind the last.
     Entry last = {__builtin_inff(), -1};
     for (int k = 0; k < n; ++k) {
       Entry y = {kNegInf, 0x7fffffff};

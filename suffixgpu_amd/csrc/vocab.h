@@ -145,6 +145,18 @@ struct Share {
     }
     if (extra >= 0) f(single, extra);
   }
+  // The same of step u, by all lanes at once: f(x, index, whether there is such
+  // an element).
+  template <class F>
+  __device__ void again_step(int u, F f) const {
+    const int v = first + u * kThreads;
+    T x[E];
+    const uint4 q = v < vecs ? ((const uint4*)body)[v] : uint4{0, 0, 0, 0};
+    __builtin_memcpy(x, &q, 16);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      f(Elem<DT>::get(x[e]), head + v * E + e, v < vecs);
+  }
 };
 
 // Difference to the largest, where infinities may meet; -inf for NaN.
