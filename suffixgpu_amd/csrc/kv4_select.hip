@@ -8,7 +8,7 @@
 // channels: one product of 2 D channels a block, however many heads there are.
 // It is computed in whole numbers (P, N of 7 bits, bounds of 7 bits and a sign in
 // units of a power of two), so it has one value whatever the order of its sums,
-// and a selection has one right answer.  The sums are below 2^22 and exact as
+// and a selection has one right answer.  The sums are below 2^23 and exact as
 // floats; times the power of two they rank the blocks.
 //
 // What bounds it are the steps that follow each other in a workgroup, most of which
@@ -253,15 +253,20 @@ struct PackQuery {
   }
 };
 
-// Order of scores as whole numbers; 0 is no score's.
+// Order of scores as whole numbers; 0 is no score's.  A sum of 2 D products of up to
+// 127^2 has 23 bits, so the last of a float's 24 is nothing but zero: without it all
+// of these are below 2^31, and no line that the choice tries passes 2^32 (a NaN's key is
+// 2^23 below that otherwise, less than the parts of the range that it looks through).
+template <int D>
 __device__ __forceinline__ uint32_t score_key(int32_t dot, int unit) {
+  static_assert(2 * D * 127 * 127 < 1 << 23, "");
   if (unit == kNoPage) return 0;
   const float f = unit == kNanUnit
                       ? __builtin_inff()
                       : (float)dot * __uint_as_float((uint32_t)(unit + 127)
                                                      << 23);
   const uint32_t x = __float_as_uint(f);
-  return x >> 31 ? ~x : x | 0x80000000u;
+  return (x >> 31 ? ~x : x | 0x80000000u) >> 1;
 }
 
 // Scores of blocks [blk0, end) of row b and KV head h for its query tokens t0 ..
@@ -340,8 +345,8 @@ __device__ __forceinline__ void score_blocks(
             0);
       if (q0 + i16 < queries)
         put(q0 + i16, blk + quad * 4,
-            uint4{score_key(s[0], us[0]), score_key(s[1], us[1]),
-                  score_key(s[2], us[2]), score_key(s[3], us[3])});
+            uint4{score_key<D>(s[0], us[0]), score_key<D>(s[1], us[1]),
+                  score_key<D>(s[2], us[2]), score_key<D>(s[3], us[3])});
     }
     blk += kAll;
     ++turn;
