@@ -239,7 +239,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
         }
       }
     };
-    if (fabsf(tc) < 0x1p60f && c < 0x1p60f) {
+    if (fabsf(tc) < 0x1p24f && c < 0x1p60f) {  // (off is at most a half)
       take([&](float y) { return __builtin_fmaf(y, c, -tc); });
       sum = wave_sum(sum);
       zsum = wave_sum(zsum);
@@ -247,7 +247,8 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_scan(LogArgs a) {
       zsum = (zsum - off * sum) * f;
       sum *= f;
     } else {
-      // infinities, and what grows too large: a difference first, by halves
+      // infinities, and what grows too large: a difference first, by halves.  (From
+      // |top c| = 2^32 on 2^-off can be no float, with sums of zero a NaN.)
       const float half = -0.5f * top, c2 = 2.0f * c;
       s.again([&](float y, int) {
         const bool is = y == top;
