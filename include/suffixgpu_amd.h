@@ -745,7 +745,10 @@ int sfx_kv4_bounds_update(const sfx_kv4* cache, const sfx_kv4_bounds* bounds,
  * workspace: sfx_kv4_select_workspace_size bytes (none for tables of up to 512
  * blocks, nor of up to 1,024 and more than 256 lists, otherwise 4 for each list and
  * block), 16-byte aligned, of any content; calls that may overlap have their
- * own. */
+ * own.  A call takes up to 2^24 tokens a row, and with a workspace fewer than
+ * 2^22 lists (batch x tokens x heads); without one fewer than 2^23 tiles of 16
+ * tokens of a row and head (of 11 at least where tables have more than 700
+ * blocks), batch x heads counted up to a multiple of 8. */
 size_t sfx_kv4_select_workspace_size(const sfx_kv4* cache, int64_t batch,
                                      int64_t tokens);
 int sfx_kv4_select(const sfx_kv4* cache, const sfx_kv4_bounds* bounds,

@@ -879,14 +879,6 @@ int64_t pitch_of(const sfx_kv4* c) {
   return (blocks + 15) / 16 * 16;
 }
 
-bool select_ok(const sfx_kv4* c, int64_t batch, int64_t tokens) {
-  KvView v;
-  // the keys' number in 62 bits, lists in a grid's
-  return kv_view(c, &v) && batch >= 0 && batch <= 65535 && tokens >= 0 &&
-         tokens <= (int64_t(1) << 24) &&
-         batch * tokens <= ((int64_t(1) << 22) - 1) / c->heads;
-}
-
 // Whether one launch serves.  With the rows' scores cut into pieces and a second
 // launch for the choice few lists of long rows are chosen sooner: of 1,024 blocks each
 // for one token of one row 14.4 us in one launch, 10.3 in two, of 16 rows 16.9 and
@@ -898,19 +890,35 @@ bool held_in_lds(const sfx_kv4* c, int64_t batch, int64_t tokens) {
          (blocks <= kSelectBlocks && batch * tokens * c->heads > 256);
 }
 
-template <int D, bool kHalf>
-int launch_held(SelectArgs a, hipStream_t stream) {
-  // As many tokens as a workgroup's 64 KB hold keys of; past kSelectTokens in
-  // tiles of 16.
-  const int64_t row = 4 * (a.pitch + 4), packed = 2 * D + 16;
+// In one launch, the tokens of a workgroup: as many as its 64 KB hold keys of; past
+// kSelectTokens in tiles of 16.
+int64_t held_span(const sfx_kv4* c, int64_t tokens) {
+  const int64_t row = 4 * (pitch_of(c) + 4), packed = 2 * c->head_dim + 16;
   const int64_t room = 65536 - kSelectThreads * 4 - kSelectTokens * packed;
-  a.span = (int)std::min<int64_t>(a.tokens <= kSelectTokens ? a.tokens : 16,
-                                  room / row);
+  return std::min<int64_t>(tokens <= kSelectTokens ? tokens : 16, room / row);
+}
+
+bool select_ok(const sfx_kv4* c, int64_t batch, int64_t tokens) {
+  KvView v;
+  if (!kv_view(c, &v) || batch < 0 || batch > 65535 || tokens < 0 ||
+      tokens > (int64_t(1) << 24))
+    return false;
+  if (batch == 0 || tokens == 0) return true;
+  // a grid's threads: of a workgroup for each tile, or for each list
+  if (!held_in_lds(c, batch, tokens))
+    return batch * tokens <= ((int64_t(1) << 22) - 1) / c->heads;
+  const int64_t span = held_span(c, tokens);
+  return (batch * c->heads + 7) / 8 * 8 * ((tokens + span - 1) / span) <
+         (int64_t(1) << 32) / kSelectThreads;
+}
+
+template <int D, bool kHalf>
+int launch_held(SelectArgs a, const sfx_kv4* cache, hipStream_t stream) {
+  a.span = (int)held_span(cache, a.tokens);
   a.tiles = (int)((a.tokens + a.span - 1) / a.span);
-  const size_t lds = (a.span + 15) / 16 * 16 * packed + a.span * row;
+  const size_t lds =
+      (a.span + 15) / 16 * 16 * (2 * D + 16) + a.span * 4 * (a.pitch + 4);
   const int64_t items = (a.batch * a.c.heads + 7) / 8 * 8;
-  if (items * a.tiles >= (int64_t(1) << 32) / kSelectThreads)
-    return SFX_EINVAL;
   const dim3 grid((unsigned)(items * a.tiles)), block(kSelectThreads);
   // one token, of up to 1,024 blocks, by a wave 18 us, by all of them 14; of up to 256
   // 7.8 and 8.6
@@ -952,8 +960,9 @@ int launch_wide(SelectArgs a, hipStream_t stream) {
 
 template <int D, bool kHalf>
 int launch(const SelectArgs& a, const sfx_kv4* cache, hipStream_t stream) {
-  return held_in_lds(cache, a.batch, a.tokens) ? launch_held<D, kHalf>(a, stream)
-                            : launch_wide<D, kHalf>(a, stream);
+  return held_in_lds(cache, a.batch, a.tokens)
+             ? launch_held<D, kHalf>(a, cache, stream)
+             : launch_wide<D, kHalf>(a, stream);
 }
 
 constexpr int64_t kMaxTokens = int64_t(1) << 28;  // the grid's limit

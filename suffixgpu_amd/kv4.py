@@ -305,7 +305,8 @@ class KV4Cache:
         Returns [B, T, num_kv_heads, blocks] int32: block i of a row holds its
         positions 32 i to 32 i + 31; ascending, -1 behind them (and for tokens
         that are no queries).  Whole numbers decide, so the result is the same
-        on any call; their rule is in include/suffixgpu_amd.h."""
+        on any call; their rule, and how many lists a call takes, is in
+        include/suffixgpu_amd.h."""
         self._need_bounds()
         if elsewhere(self.device):
             with torch.cuda.device(self.device):
@@ -329,12 +330,17 @@ class KV4Cache:
         nbytes = L.sfx_kv4_select_workspace_size(view, b, t)
         ws = (torch.empty(nbytes, dtype=torch.uint8, device=self.device)
               if nbytes else None)
-        check(L.sfx_kv4_select(view, self._bounds, qh, b, t, heads,
-                               *keep[0][1:], *keep[1][1:], blocks, first,
-                               recent, out.data_ptr(),
-                               None if ws is None else ws.data_ptr(), nbytes,
-                               stream_of(self.device)),
-              "KV4Cache.select_blocks")
+        rc = L.sfx_kv4_select(view, self._bounds, qh, b, t, heads,
+                              *keep[0][1:], *keep[1][1:], blocks, first,
+                              recent, out.data_ptr(),
+                              None if ws is None else ws.data_ptr(), nbytes,
+                              stream_of(self.device))
+        if rc == _lib.EINVAL:
+            raise SuffixGPUError(
+                f"KV4Cache.select_blocks: {b} x {t} tokens for "
+                f"{heads} query heads on {self.num_kv_heads} KV heads are more "
+                "heads, tokens or lists than a launch takes")
+        check(rc, "KV4Cache.select_blocks")
         return out
 
     def attend_blocks(self, q: torch.Tensor, selected: torch.Tensor,
