@@ -212,7 +212,8 @@ class KV4Cache:
         defaults to head_dim ** -0.5.  Returns [B, T, q_heads, head_dim] in the
         cache's type: zeros for a query that sees nothing and for tokens from
         q_len on.  T = 1 is a decode step, T = k + 1 a verification step, a
-        long T a chunk of a prompt."""
+        long T a chunk of a prompt.  The result has no gradient, whatever q asks
+        for."""
         if elsewhere(self.device):
             with torch.cuda.device(self.device):
                 return self.attend(q, page_table, kv_len, q_len, scale)
@@ -351,7 +352,8 @@ class KV4Cache:
         num_kv_heads, N] int32 (as ``select_blocks`` gives them, or another
         layer's) that each query sees.  Entries may stand in any order; one that
         names no block of the table counts as none, a block that is named twice
-        as one.  Zeros for a query that sees nothing."""
+        as one.  Zeros for a query that sees nothing.  There are no gradients, and
+        queries that ask for them are refused."""
         if elsewhere(self.device):
             with torch.cuda.device(self.device):
                 return self.attend_blocks(q, selected, page_table, kv_len,
@@ -369,6 +371,8 @@ class KV4Cache:
             raise ValueError(f"selected must be a contiguous int32 [{b}, {t}, "
                              f"{self.num_kv_heads}, N] tensor on {self.device}"
                              ", 1 <= N <= 32768")
+        if q.requires_grad and torch.is_grad_enabled():
+            raise ValueError("attend_blocks has no gradient: pass q.detach()")
         n = selected.shape[3]
         view = self._view(page_table, b)
         keep = (self._counts("kv_len", kv_len, b),

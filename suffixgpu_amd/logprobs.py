@@ -43,9 +43,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor,
     logits are above -inf the rest of ``top_tokens`` is -1, of ``top_logprobs``
     -inf; without any, the log probability is -inf and the entropy 0.
 
-    Serves a model; there are no gradients, and logits that ask for them are
-    refused.  No host synchronisation; two launches on the current stream, which
-    may be recorded into a HIP graph."""
+    Serves a model; there are no gradients, and logits or temperatures that ask
+    for them are refused.  No host synchronisation; two launches on the current
+    stream, which may be recorded into a HIP graph."""
     require_gpu(logits, tokens, temperature)
     dev = logits.device
     if elsewhere(dev):
@@ -55,6 +55,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor,
         raise ValueError("logits must be [B, J, V]")
     if logits.requires_grad and torch.is_grad_enabled():
         raise ValueError("token_logprobs has no gradient: pass logits.detach()")
+    if (temperature is not None and temperature.requires_grad
+            and torch.is_grad_enabled()):
+        raise ValueError("token_logprobs has no gradient: pass "
+                         "temperature.detach()")
     b, j, v = logits.shape
     code = _lib.DTYPE_CODES.get(logits.dtype)
     if code is None:
