@@ -717,7 +717,9 @@ int sfx_pages_slots(const sfx_pages* pool, const void* start,
  * count as 127 units); 127: the block holds a NaN.
  * sfx_kv4_bounds_update sets them for the blocks that hold positions start[b]
  * .. start[b] + min(count[b], tokens) - 1, of the tokens up to those; it
- * follows every append. */
+ * follows every append.  Where a row goes on behind these (written again, or out
+ * of order), it is called up to the row's end: a block's bounds do not have the
+ * tokens behind the last one given. */
 typedef struct sfx_kv4_bounds {
     int8_t* range;  /* 16-byte aligned */
     int8_t* unit;

@@ -152,6 +152,12 @@ class KV4Cache:
         [B, T, num_kv_heads, head_dim] at positions ``start[b] + i``, and the
         bounds of the blocks that these lie in, where the cache holds them.
 
+        The bounds take the tokens for the row's last, as they are after a step:
+        what the last block holds behind them (rejected drafts) is in its bounds no
+        longer.  Where a row goes on behind the tokens written, because they are
+        written again or out of order, ``update_bounds`` up to the row's end makes
+        them whole; until then ``select_blocks`` may pass that block over.
+
         A page that one row of a call writes must not be written by another
         row of it.  Infinities and NaN make their 32 channels of a key, or
         their token's values, NaN."""
@@ -272,7 +278,9 @@ class KV4Cache:
     def bounds(self, page_table: torch.Tensor):
         """(least, largest) key [B, blocks, num_kv_heads, head_dim] float32 of
         each block of the rows, as ``select_blocks`` knows them: at most and at
-        least what ``read`` gives.  Blocks without a page: zeros; with a NaN: NaN."""
+        least what ``read`` gives, up to the last position of the block that the
+        latest ``append`` or ``update_bounds`` of it had.  Blocks without a page:
+        zeros; with a NaN: NaN."""
         self._need_bounds()
         view = self._view(page_table, page_table.shape[0])
         b, w = page_table.shape
