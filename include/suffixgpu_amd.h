@@ -693,15 +693,17 @@ typedef struct sfx_pages {
  * from the top of the stack, the first row first, while there are any of those
  * that were free when the call began; rows that shrink give back their last
  * pages, which are free from the next call on (the first row's first on top).
- * So lengths put back as they were put the pages back as well.  room [n]: the
- * tokens that each row's pages hold. */
+ * So lengths put back as they were put the pages back as well, where no row then
+ * had fewer than its length asks for.  room [n]: the tokens that each row's pages
+ * hold. */
 int sfx_pages_resize(const sfx_pages* pool, const void* lengths,
                      int32_t lengths_is64, int64_t n, int32_t* room,
                      hipStream_t stream);
 
 /* slots [n, tokens]: where position start[r] + i of row r lies, page id *
  * page_size + position % page_size, for i < count[r] (all without it); -1 where
- * the row holds no page, and from count on. */
+ * the row holds no page, from count on, and in all of a row whose start is
+ * negative. */
 int sfx_pages_slots(const sfx_pages* pool, const void* start,
                     int32_t start_is64, const void* count, int32_t count_is64,
                     int64_t n, int64_t tokens, int64_t* slots,

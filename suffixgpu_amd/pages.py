@@ -88,7 +88,8 @@ class PagePool:
         are the rows from n on.  A row that grows takes pages that were free when
         the call began, the first row first: where they run out, rows have fewer.
         A row that shrinks gives back its last pages, free from the next call on.
-        Lengths put back as they were before a call put the pages back as well.
+        Lengths put back as they were before a call put the pages back as well,
+        where no row then had fewer than its length asks for.
 
         Returns room [n] int32: the tokens that each row's pages hold."""
         if elsewhere(self.device):
@@ -110,7 +111,8 @@ class PagePool:
               count: torch.Tensor | None = None) -> torch.Tensor:
         """Where positions ``start[r] + i``, i < ``tokens``, of rows 0 .. n - 1
         lie: page id * page_size + position % page_size, [n, tokens] int64; -1
-        where a row holds no page, and for i >= ``count[r]``.  An index into the
+        where a row holds no page, for i >= ``count[r]``, and in all of a row whose
+        start is negative (as one that is not in use has it).  An index into the
         tokens of a cache of such pages (``KV4Cache`` takes ``table`` itself)."""
         if elsewhere(self.device):
             with torch.cuda.device(self.device):
