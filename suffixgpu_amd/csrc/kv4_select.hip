@@ -13,13 +13,14 @@
 //
 // What bounds it are the steps that follow each other in a workgroup, most of which
 // run at once: packing the query, the scores, the choice (vector instructions issue in
-// half of the cycles); of many long rows, the memory (64 x 1 tokens over 32,768 30 us,
-// 135 MB, 4.5 TB/s).  The choice is made where the scores are: in LDS and a wave's or a
-// workgroup's registers for rows of up to 1,024 blocks (64 x 1 tokens over up to 32,768
-// 26 us a call, with the scores in memory and a second launch 33; 64 x 17 over up to
-// 8,192 16 and 85; a prompt's 2,048 over 16,384 38 and 192), in the registers of a
+// half of the cycles); of many long rows, the memory (64 x 1 tokens over 32,768 each
+// 30.6 us, 135 MB, 4.4 TB/s; over 16,384 to 32,768 26 us, 110 MB).  The choice is made
+// where the scores are: in LDS and a wave's or a workgroup's registers for rows of up to
+// 1,024 blocks (the 26 us, with the scores in memory and a second launch 33; 64 x 17 over
+// up to 8,192 16 and 85; a prompt's 2,048 over 16,384 38 and 192), in the registers of a
 // workgroup of a second launch past that (one token over 131,072 11 us, 4 x 9 with heads
-// of 256 24), and in memory past 16,384 blocks.
+// of 256 24), and in memory past 16,384 blocks (one token over 1,048,576 87 us, eight of
+// them 189, 539 MB).
 
 #include <algorithm>
 
@@ -791,7 +792,8 @@ __device__ __forceinline__ uint32_t ranked(const SelectArgs& a, uint32_t key,
 }
 
 // Rows of any length: the keys stay in memory, and four passes narrow the line
-// down by 8 bits each.
+// down by 8 bits each.  (71 us for a list of 32,768 blocks: a workgroup's loads, of
+// which few are under way at a time.)
 __global__ __launch_bounds__(kWideThreads) void k_kv4_pick_far(SelectArgs a) {
   __shared__ int hist[256];
   __shared__ int sums[kWideWaves];

@@ -13,7 +13,8 @@
 // Positions without a token leave at once.
 //
 // Memory bounds it where there are no alternatives: 2,048 positions of 128,256
-// bfloat16 logits take 96 to 103 us, 5.1 to 5.5 TB/s.  With alternatives it is the
+// bfloat16 logits take 96 to 103 us, 5.1 to 5.5 TB/s; float32 logits also with a few
+// (64 x 17 positions with five 105 us, 5.3 TB/s).  With alternatives it is the
 // vector instructions, 16 a logit with one (112 to 125 us) and 18 with twenty: 256
 // positions 28.5 us, 66 MB at 2.3 TB/s, 19 without any.  8,192 logits a workgroup are 32 a
 // lane, which is what stays in registers beside the rest with seven or eight waves a
